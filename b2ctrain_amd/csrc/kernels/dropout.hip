@@ -1,0 +1,75 @@
+// Dropout with a mask that is formed from a counter and never stored (b2c_hip_dropout).
+#include "dense.h"
+
+namespace b2c {
+namespace dev {
+namespace {
+
+// One thread to a counter: eight elements, which may cross the end of a row. `flat`: rows follow each other
+// without a gap in every matrix, and all start on 16 bytes.
+template <typename T, bool FLAT>
+__global__ __launch_bounds__(256) void dropout_kernel(const T* x, int64_t ldx, const T* r, int64_t ldr, T* y, int64_t ldy,
+                                                      uint64_t n, uint32_t cols, Drop d) {
+  const uint64_t q = (uint64_t)blockIdx.x * 256 + threadIdx.x, e = q * 8;
+  if (e >= n) return;
+  Philox4 w{};
+  if (d.threshold) w = philox(q, d.stream, d.seed);
+  if (FLAT && e + 8 <= n) {
+    const vec<T, 8> a = *reinterpret_cast<const vec<T, 8>*>(x + e);
+    vec<T, 8> b{};
+    if (r) b = *reinterpret_cast<const vec<T, 8>*>(r + e);
+    vec<T, 8> o;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      float v = kept(w, j, d.threshold) ? (float)a[j] * d.scale : 0.f;
+      if (r) v += (float)b[j];
+      o[j] = (T)v;
+    }
+    *reinterpret_cast<vec<T, 8>*>(y + e) = o;
+    return;
+  }
+  uint64_t m = e / cols;
+  uint32_t c = (uint32_t)(e - m * cols);
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    if (e + j >= n) break;
+    float v = kept(w, j, d.threshold) ? (float)x[m * ldx + c] * d.scale : 0.f;
+    if (r) v += (float)r[m * ldr + c];
+    y[m * ldy + c] = (T)v;
+    if (++c == cols) c = 0, m++;
+  }
+}
+
+bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+template <typename T>
+int launch(const b2c_dropout_args* a, const Drop& d, hipStream_t stream) {
+  const uint64_t n = (uint64_t)a->rows * (uint64_t)a->cols, groups = (n + 7) / 8, blocks = (groups + 255) / 256;
+  const bool flat = (a->rows == 1 || (a->ldx == a->cols && a->ldy == a->cols && (!a->residual || a->ldr == a->cols))) &&
+                    on16(a->x) && on16(a->y) && on16(a->residual);
+  const T *x = (const T*)a->x, *r = (const T*)a->residual;
+  auto kernel = flat ? dropout_kernel<T, true> : dropout_kernel<T, false>;
+  kernel<<<dim3((unsigned)blocks), 256, 0, stream>>>(x, a->ldx, r, a->ldr, (T*)a->y, a->ldy, n, (uint32_t)a->cols, d);
+  return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace dev
+}  // namespace b2c
+
+extern "C" int b2c_hip_dropout(const b2c_dropout_args* a, hipStream_t stream) {
+  using namespace b2c::dev;
+  Drop d;
+  if (!a || a->rows < 0 || a->cols < 1 || a->cols > 0x7fffffff || !drop_of(a->p, a->seed, a->stream, &d))
+    return hipErrorInvalidValue;
+  if (a->rows && (uint64_t)a->rows > ((uint64_t)1 << 41) / (uint64_t)a->cols) return hipErrorInvalidValue;
+  const size_t size = a->dtype == B2C_F32 ? 4 : 2;
+  if (a->dtype != B2C_F32 && a->dtype != B2C_F16 && a->dtype != B2C_BF16) return hipErrorInvalidValue;
+  if (a->rows == 0) return hipSuccess;
+  if (!good(a->x, a->ldx, a->cols, size) || !good(a->y, a->ldy, a->cols, size) ||
+      (a->residual && !good(a->residual, a->ldr, a->cols, size)))
+    return hipErrorInvalidValue;
+  if (a->dtype == B2C_F32) return launch<float>(a, d, stream);
+  if (a->dtype == B2C_F16) return launch<f16>(a, d, stream);
+  return launch<bf16>(a, d, stream);
+}

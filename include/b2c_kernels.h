@@ -559,6 +559,144 @@ typedef struct b2c_ply_encode_args {
 } b2c_ply_encode_args;
 int b2c_hip_ply_encode(const b2c_ply_encode_args* a, hipStream_t stream);
 
+/* ---- dense operators of a learned head (no reference counterpart: the reference's appearance MLP has its own kernels) ----
+ * Matrices are row-major with a distance between rows ("ld", in elements, at least the columns). Pointers need the
+ * alignment of their element only; rows that start on 16 bytes, with a multiple of 8 columns (16 for 8-bit), are read
+ * fastest. Sums are held in 32 bits. Every entry checks its arguments and returns hipErrorInvalidValue before any launch
+ * when they do not fit; rows = 0 is valid. Workspaces need 16-byte alignment; what they hold before a call does not
+ * matter. Inputs and outputs may not overlap except where an entry says so. Results do not depend on the order in which
+ * workgroups run. */
+enum { B2C_F32 = 0, B2C_F16 = 1, B2C_BF16 = 2 };
+enum { B2C_ACT_SILU = 0, B2C_ACT_GELU = 1, B2C_ACT_RELU = 2 }; /* g / (1 + e^-g); g (1 + erf(g / sqrt 2)) / 2; max(g, 0) */
+
+/* y = residual + keep * x * s over a [rows][cols] matrix. Element e = row * cols + col is kept iff its 16 random bits are
+ * at least T = floor(65536 p + 1/2); s = 65536 / (65536 - T). The bits are those of Philox4x32-10 (J. Salmon, M. Moraes,
+ * R. Dror, D. Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011) under the key `seed` at the counter
+ * (e >> 3, stream), e & 7 counting the eight 16-bit fields from the lowest: they depend on e, seed and stream alone, so
+ * the backward pass is this entry on the gradient with the same p, seed and stream and no residual. A dropped value counts
+ * as 0 whatever it is. y may be x or residual themselves (same pointer and ld). */
+typedef struct b2c_dropout_args {
+  int64_t rows, cols;
+  int dtype;            /* of x, residual and y: B2C_F32, B2C_F16 or B2C_BF16 */
+  float p;              /* 0 <= p, and T < 65536 */
+  uint64_t seed, stream;
+  const void* x;
+  int64_t ldx;
+  const void* residual; /* or NULL */
+  int64_t ldr;
+  void* y;
+  int64_t ldy;
+} b2c_dropout_args;
+int b2c_hip_dropout(const b2c_dropout_args* a, hipStream_t stream);
+
+/* The gated feed-forward block: g = x w_gate^T, u = x w_up^T, h = act(g) u, y = residual + dropout(h w_down^T), dropout
+ * as in b2c_hip_dropout over [rows][d_out]. h is rounded to dtype between the two products. With `saved` set, g and u
+ * are kept there (rounded to dtype) for the backward pass. */
+typedef struct b2c_ffn_args {
+  int64_t rows;
+  int d_in, d_hidden, d_out;
+  int dtype, act;       /* dtype of every matrix: B2C_F16 or B2C_BF16 */
+  float p;              /* dropout, as above; 0: none */
+  uint64_t seed, stream;
+  const void* x;        /* [rows][d_in] */
+  int64_t ldx;
+  const void* w_gate;   /* [d_hidden][d_in] */
+  const void* w_up;
+  int64_t ld_in;        /* of w_gate and w_up */
+  const void* w_down;   /* [d_out][d_hidden] */
+  int64_t ld_out;
+  const void* residual; /* [rows][d_out] or NULL; may be y */
+  int64_t ldr;
+  void* y;              /* [rows][d_out] */
+  int64_t ldy;
+  void* saved;          /* b2c_ffn_saved_bytes, or NULL: no backward pass will follow */
+  void* workspace;      /* b2c_ffn_workspace_bytes; not needed after the call */
+  size_t workspace_bytes;
+} b2c_ffn_args;
+/* Sizes for a's shapes, type and alignment (pointers are looked at, not read); 0 with invalid arguments, and a saved
+ * size of 0 where the backward pass recomputes g and u (saved may then be NULL). */
+size_t b2c_ffn_saved_bytes(const b2c_ffn_args* a);
+size_t b2c_ffn_workspace_bytes(const b2c_ffn_args* a);
+int b2c_hip_ffn_forward(const b2c_ffn_args* a, hipStream_t stream);
+
+/* Its gradients. `fwd` holds the forward call's arguments (y, residual and workspace are not used); the residual's
+ * gradient is dy itself. Outputs that are NULL are not formed. */
+typedef struct b2c_ffn_grad_args {
+  b2c_ffn_args fwd;
+  const void* dy;       /* [rows][d_out], dtype */
+  int64_t lddy;
+  void* dx;             /* [rows][d_in], dtype */
+  int64_t lddx;
+  int grad_dtype;       /* of the weights' gradients: fwd.dtype or B2C_F32 */
+  int accumulate;       /* add to the weights' gradients (B2C_F32 only) instead of overwriting them */
+  void* dw_gate;        /* [d_hidden][d_in] */
+  void* dw_up;
+  int64_t ld_din;       /* of dw_gate and dw_up */
+  void* dw_down;        /* [d_out][d_hidden] */
+  int64_t ld_dout;
+  void* workspace;      /* b2c_ffn_grad_workspace_bytes; not needed after the call */
+  size_t workspace_bytes;
+} b2c_ffn_grad_args;
+size_t b2c_ffn_grad_workspace_bytes(const b2c_ffn_grad_args* a);
+int b2c_hip_ffn_backward(const b2c_ffn_grad_args* a, hipStream_t stream);
+
+/* 8-bit rows: scale[i] = max |x[i][j]| / 127 and q[i][j] = x[i][j] / scale[i], rounded to nearest even, both in single
+ * precision. A row of zeros gets scale 0; a row with an infinity or NaN gets scale NaN and zeros. Columns cols .. ldq - 1
+ * of q are set to 0 up to the next multiple of 16. For weights, rows are output channels. */
+typedef struct b2c_quantize_args {
+  int64_t rows, cols;
+  int dtype;            /* of x: B2C_F32, B2C_F16 or B2C_BF16 */
+  const void* x;
+  int64_t ldx;
+  int8_t* q;            /* [rows][ldq] */
+  int64_t ldq;
+  float* scale;         /* [rows] */
+} b2c_quantize_args;
+int b2c_hip_quantize_rows(const b2c_quantize_args* a, hipStream_t stream);
+
+/* y[i][j] = sum_k qx[i][k] w[j][k] * sx[i] * w_scale[j], with x quantised by rows as above within the call and the sum
+ * exact in 32-bit integers (d_in up to 131072). */
+typedef struct b2c_i8_linear_args {
+  int64_t rows;
+  int d_in, d_out;
+  int dtype;            /* of x and y: B2C_F32, B2C_F16 or B2C_BF16 */
+  const void* x;        /* [rows][d_in] */
+  int64_t ldx;
+  const int8_t* w;      /* [d_out][d_in], values -127 .. 127 */
+  int64_t ldw;
+  const float* w_scale; /* [d_out] */
+  void* y;              /* [rows][d_out] */
+  int64_t ldy;
+  void* workspace;      /* b2c_i8_linear_workspace_bytes */
+  size_t workspace_bytes;
+} b2c_i8_linear_args;
+size_t b2c_i8_linear_workspace_bytes(const b2c_i8_linear_args* a);
+int b2c_hip_i8_linear(const b2c_i8_linear_args* a, hipStream_t stream);
+
+/* The feed-forward block with every product in 8-bit integers: g, u by the products of the quantised x, h = act(g) u in
+ * single precision, quantised by rows again, then the down product. No dropout: this form answers, it does not train. */
+typedef struct b2c_i8_ffn_args {
+  int64_t rows;
+  int d_in, d_hidden, d_out;
+  int dtype, act;       /* dtype of x and y */
+  const void* x;
+  int64_t ldx;
+  const int8_t* w_gate; /* [d_hidden][d_in] */
+  const int8_t* w_up;
+  int64_t ld_in;
+  const float* s_gate;  /* [d_hidden] */
+  const float* s_up;
+  const int8_t* w_down; /* [d_out][d_hidden] */
+  int64_t ld_out;
+  const float* s_down;  /* [d_out] */
+  void* y;
+  int64_t ldy;
+  void* workspace;      /* b2c_i8_ffn_workspace_bytes */
+  size_t workspace_bytes;
+} b2c_i8_ffn_args;
+size_t b2c_i8_ffn_workspace_bytes(const b2c_i8_ffn_args* a);
+int b2c_hip_i8_ffn(const b2c_i8_ffn_args* a, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
