@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <algorithm>
 #include <type_traits>
 
 #include "b2c_kernels.h"
@@ -69,16 +70,16 @@ __device__ __forceinline__ void act_grad(float g, float& a, float& d) {
   }
 }
 
-// W neighbouring values of row m from column n on, of which those from `cols` on do not exist. `wide`: rows
-// start on 16 bytes.
+// W neighbouring values of row m from column n on, of which those from `cols` on do not exist. Whole vectors go in
+// one access whatever their alignment, which costs the device nothing but the extra line that they may touch.
 template <int W, typename T>
-__device__ __forceinline__ void put(T* base, int64_t ld, int64_t m, int n, int cols, bool wide, const float (&v)[W]) {
+__device__ __forceinline__ void put(T* base, int64_t ld, int64_t m, int n, int cols, const float (&v)[W]) {
   T* p = base + m * ld + n;
-  if (wide && n + W <= cols) {
+  if (n + W <= cols) {
     vec<T, W> t;
 #pragma unroll
     for (int j = 0; j < W; j++) t[j] = (T)v[j];
-    *reinterpret_cast<vec<T, W>*>(p) = t;
+    __builtin_memcpy(p, &t, sizeof(t));
   } else {
 #pragma unroll
     for (int j = 0; j < W; j++)
@@ -86,10 +87,11 @@ __device__ __forceinline__ void put(T* base, int64_t ld, int64_t m, int n, int c
   }
 }
 template <int W, typename T>
-__device__ __forceinline__ void get(const T* base, int64_t ld, int64_t m, int n, int cols, bool wide, float (&v)[W]) {
+__device__ __forceinline__ void get(const T* base, int64_t ld, int64_t m, int n, int cols, float (&v)[W]) {
   const T* p = base + m * ld + n;
-  if (wide && n + W <= cols) {
-    const vec<T, W> t = *reinterpret_cast<const vec<T, W>*>(p);
+  if (n + W <= cols) {
+    vec<T, W> t;
+    __builtin_memcpy(&t, p, sizeof(t));
 #pragma unroll
     for (int j = 0; j < W; j++) v[j] = (float)t[j];
   } else {
@@ -98,7 +100,7 @@ __device__ __forceinline__ void get(const T* base, int64_t ld, int64_t m, int n,
   }
 }
 
-// ---- epilogues: row m of out, columns n .. n + W - 1 ------------------------------------------------------
+// ---- epilogues: row m of out, columns n .. n + W - 1 (the first argument is a part, see Parts) ------------------------------------------------------
 // The block's inner widths are stored at a pitch of fp columns, a multiple of 64 >= f; columns f .. fp - 1 hold
 // zeros, so that a later product may run over them.
 
@@ -110,17 +112,17 @@ struct GateOut {
   int64_t fp;
   int f;
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int n, const float (&g)[W], const float (&u)[W]) const {
+  __device__ __forceinline__ void operator()(uint32_t, int64_t m, int n, const float (&g)[W], const float (&u)[W]) const {
     float v[W];
 #pragma unroll
     for (int j = 0; j < W; j++) v[j] = n + j < f ? act<ACT>(g[j]) * u[j] : 0.f;
-    put<W>(h, fp, m, n, (int)fp, true, v);
+    put<W>(h, fp, m, n, (int)fp, v);
     if (saved) {
       float a[W], b[W];
 #pragma unroll
       for (int j = 0; j < W; j++) a[j] = n + j < f ? g[j] : 0.f, b[j] = n + j < f ? u[j] : 0.f;
-      put<W>(saved, 2 * fp, m, n, (int)fp, true, a);
-      put<W>(saved + fp, 2 * fp, m, n, (int)fp, true, b);
+      put<W>(saved, 2 * fp, m, n, (int)fp, a);
+      put<W>(saved + fp, 2 * fp, m, n, (int)fp, b);
     }
   }
 };
@@ -133,10 +135,9 @@ struct RowsOut {
   const T* r;  // or null
   int64_t ldr;
   int cols;
-  bool wide_y, wide_r;
   Drop drop;
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int n, const float (&acc)[W]) const {
+  __device__ __forceinline__ void operator()(uint32_t, int64_t m, int n, const float (&acc)[W]) const {
     float v[W];
 #pragma unroll
     for (int j = 0; j < W; j++) v[j] = acc[j];
@@ -150,11 +151,11 @@ struct RowsOut {
     }
     if (r) {
       float t[W];
-      get<W>(r, ldr, m, n, cols, wide_r, t);
+      get<W>(r, ldr, m, n, cols, t);
 #pragma unroll
       for (int j = 0; j < W; j++) v[j] += t[j];
     }
-    put<W>(y, ldy, m, n, cols, wide_y, v);
+    put<W>(y, ldy, m, n, cols, v);
   }
 };
 
@@ -168,23 +169,25 @@ struct GateBack {
   T* dgu;          // [m][2 fp]: dg, then du
   int64_t fp;
   int f;
+  float scale;  // dropout's: dz enters the products as dy where it is kept, which needs no rounding
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int n, const float (&dh)[W]) const {
+  __device__ __forceinline__ void operator()(uint32_t, int64_t m, int n, const float (&dh)[W]) const {
     float g[W], u[W], v[W];
-    get<W>(saved, 2 * fp, m, n, (int)fp, true, g);
-    get<W>(saved + fp, 2 * fp, m, n, (int)fp, true, u);
+    get<W>(saved, 2 * fp, m, n, (int)fp, g);
+    get<W>(saved + fp, 2 * fp, m, n, (int)fp, u);
 #pragma unroll
     for (int j = 0; j < W; j++) {
       float a, d;
       act_grad<ACT>(g[j], a, d);
       const bool in = n + j < f;
       v[j] = in ? a * u[j] : 0.f;
-      g[j] = in ? dh[j] * u[j] * d : 0.f;
-      u[j] = in ? dh[j] * a : 0.f;
+      const float s = dh[j] * scale;
+      g[j] = in ? s * u[j] * d : 0.f;
+      u[j] = in ? s * a : 0.f;
     }
-    if (h) put<W>(h, fp, m, n, (int)fp, true, v);
-    put<W>(dgu, 2 * fp, m, n, (int)fp, true, g);
-    put<W>(dgu + fp, 2 * fp, m, n, (int)fp, true, u);
+    if (h) put<W>(h, fp, m, n, (int)fp, v);
+    put<W>(dgu, 2 * fp, m, n, (int)fp, g);
+    put<W>(dgu + fp, 2 * fp, m, n, (int)fp, u);
   }
 };
 
@@ -196,25 +199,26 @@ struct WeightOut {
   void* b;
   int64_t ld;
   int rows, second, cols;
-  bool f32, add, wide;
+  bool f32, add;
+  float scale;
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int n, const float (&acc)[W]) const {
+  __device__ __forceinline__ void operator()(uint32_t, int64_t m, int n, const float (&acc)[W]) const {
     void* to = m < rows ? a : (m >= second && m < second + rows ? b : nullptr);
     if (!to) return;
     if (m >= rows) m -= second;
-    if (f32) {
-      float v[W];
+    float v[W];
 #pragma unroll
-      for (int j = 0; j < W; j++) v[j] = acc[j];
+    for (int j = 0; j < W; j++) v[j] = acc[j] * scale;
+    if (f32) {
       if (add) {
         float t[W];
-        get<W>((const float*)to, ld, m, n, cols, wide, t);
+        get<W>((const float*)to, ld, m, n, cols, t);
 #pragma unroll
         for (int j = 0; j < W; j++) v[j] += t[j];
       }
-      put<W>((float*)to, ld, m, n, cols, wide, v);
+      put<W>((float*)to, ld, m, n, cols, v);
     } else {
-      put<W>((T*)to, ld, m, n, cols, wide, acc);
+      put<W>((T*)to, ld, m, n, cols, v);
     }
   }
 };
@@ -226,14 +230,13 @@ struct ScaledOut {
   int64_t ldy;
   const float *sx, *sw;
   int cols;
-  bool wide;
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int n, const int (&acc)[W]) const {
+  __device__ __forceinline__ void operator()(uint32_t, int64_t m, int n, const int (&acc)[W]) const {
     const float s = sx[m];
     float v[W];
 #pragma unroll
     for (int j = 0; j < W; j++) v[j] = (float)acc[j] * s * sw[n + j < cols ? n + j : cols - 1];
-    put<W>(y, ldy, m, n, cols, wide, v);
+    put<W>(y, ldy, m, n, cols, v);
   }
 };
 // and h = act(g) u from them, in single precision: its rounding to 8 bits, which follows, goes by the row's
@@ -245,7 +248,7 @@ struct ScaledGate {
   int64_t fp;
   int f;
   template <int W>
-  __device__ __forceinline__ void operator()(int64_t m, int n, const int (&g)[W], const int (&u)[W]) const {
+  __device__ __forceinline__ void operator()(uint32_t, int64_t m, int n, const int (&g)[W], const int (&u)[W]) const {
     const float s = sx[m];
     float v[W];
 #pragma unroll
@@ -253,7 +256,7 @@ struct ScaledGate {
       const int c = n + j < f ? n + j : f - 1;
       v[j] = n + j < f ? act<ACT>((float)g[j] * s * sg[c]) * ((float)u[j] * s * su[c]) : 0.f;
     }
-    put<W>(h, fp, m, n, (int)fp, true, v);
+    put<W>(h, fp, m, n, (int)fp, v);
   }
 };
 
@@ -262,9 +265,6 @@ struct ScaledGate {
 // A matrix that a call reads or writes: present, on its element's alignment, rows at least as far apart as wide.
 inline bool good(const void* p, int64_t ld, int64_t cols, size_t size) {
   return p && reinterpret_cast<uintptr_t>(p) % size == 0 && ld >= cols;
-}
-inline bool wide(const void* p, int64_t ld, size_t size) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (int64_t)size % 16 == 0;
 }
 // Dropout's constants from p; false where p is outside its range.
 inline bool drop_of(float p, uint64_t seed, uint64_t stream, Drop* d) {
@@ -275,8 +275,6 @@ inline bool drop_of(float p, uint64_t seed, uint64_t stream, Drop* d) {
   return true;
 }
 
-// ---- a product ---------------------------------------------------------------------------------------------
-
 // One operand of a product over k: element (i, k) is p[i ld + k], or p[k ld + i] where it is transposed.
 template <typename T>
 struct Side {
@@ -284,87 +282,19 @@ struct Side {
   int64_t ld;
 };
 
-// out[m][n] = sum_k Q[m][k] P[n][k] by 64x64 tiles, 32 bytes x 2 of k a step, any alignment. DUAL: P2 runs beside
-// P with the same Q (gate and up). A second segment (q2, p2, k2 > 0) continues the sum.
-template <typename T, bool PT, bool QT, bool DUAL, typename Epi>
-__global__ __launch_bounds__(256) void product_kernel(Side<T> q, Side<T> p, Side<T> q2, Side<T> p2, int64_t M, int N,
-                                                      int64_t K, int64_t K2, int tiles_n, Epi epi) {
-  constexpr int V = Elem<T>::N, BK = 4 * V, PAD = V, BM = 64, BN = 64;
-  using Acc = typename Elem<T>::Acc;
-  using A = vec<T, V>;
-  __shared__ alignas(16) T sq[BM][BK + PAD];
-  __shared__ alignas(16) T sp[DUAL ? 2 : 1][BN][BK + PAD];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * BM;
-  const int n0 = (int)(blockIdx.x % tiles_n) * BN;
-  Acc acc[DUAL ? 2 : 1][2][2] = {};
-  const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
+inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-  auto stage = [&](const Side<T>& s, bool trans, int64_t i0, int64_t I, int64_t k0, int64_t kn, T(*dst)[BK + PAD]) {
-    if (!trans) {
-      const int r = t >> 2, c = (t & 3) * V;
-      const int64_t i = i0 + r;
-#pragma unroll
-      for (int j = 0; j < V; j++) dst[r][c + j] = i < I && k0 + c + j < kn ? s.p[i * s.ld + k0 + c + j] : (T)0;
-    } else {
-      const int r = t & 63;
-      const int64_t i = i0 + r;
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        const int c = (t >> 6) * V + j;
-        dst[r][c] = i < I && k0 + c < kn ? s.p[(k0 + c) * s.ld + i] : (T)0;
-      }
-    }
-  };
-  for (int seg = 0; seg < 2; seg++) {
-    const Side<T>&Q = seg ? q2 : q, &P = seg && !DUAL ? p2 : p;
-    const int64_t kn = seg ? K2 : K;
-    for (int64_t k0 = 0; k0 < kn; k0 += BK) {
-      __syncthreads();
-      stage(Q, QT, m0, M, k0, kn, sq);
-      stage(P, PT, n0, N, k0, kn, sp[0]);
-      if constexpr (DUAL) stage(p2, PT, n0, N, k0, kn, sp[1]);
-      __syncthreads();
-      const int row = lane & 15, kk = (lane >> 4) * V;
-      A fq[2];
-#pragma unroll
-      for (int i = 0; i < 2; i++) fq[i] = *reinterpret_cast<const A*>(&sq[wm + i * 16 + row][kk]);
-#pragma unroll
-      for (int d = 0; d < (DUAL ? 2 : 1); d++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const A fp = *reinterpret_cast<const A*>(&sp[d][wn + j * 16 + row][kk]);
-#pragma unroll
-          for (int i = 0; i < 2; i++) acc[d][i][j] = mfma(fp, fq[i], acc[d][i][j]);
-        }
-    }
+// A workspace handed out in pieces; without a base it only counts.
+struct Room {
+  char* base;
+  size_t used = 0;
+  template <typename T>
+  T* take(int64_t n) {
+    T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += (size_t)up(n * (int64_t)sizeof(T), 256);
+    return p;
   }
-#pragma unroll
-  for (int i = 0; i < 2; i++)
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const int64_t m = m0 + wm + i * 16 + (lane & 15);
-      const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-      if (m >= M || n >= N) continue;
-      using S = std::remove_reference_t<decltype(acc[0][0][0][0])>;
-      S a[4], b[4];
-#pragma unroll
-      for (int r = 0; r < 4; r++) a[r] = acc[0][i][j][r], b[r] = acc[DUAL ? 1 : 0][i][j][r];
-      if constexpr (DUAL) epi.template operator()<4>(m, n, a, b);
-      else epi.template operator()<4>(m, n, a);
-    }
-}
-
-template <typename T, bool PT, bool QT, bool DUAL, typename Epi>
-int product(Side<T> q, Side<T> p, Side<T> q2, Side<T> p2, int64_t M, int64_t N, int64_t K, int64_t K2, const Epi& epi,
-            hipStream_t stream) {
-  if (M <= 0 || N <= 0) return hipSuccess;
-  const int64_t tn = (N + 63) / 64, tm = (M + 63) / 64;
-  if (tn * tm > 0x7fffffff) return hipErrorInvalidValue;
-  product_kernel<T, PT, QT, DUAL, Epi>
-      <<<dim3((unsigned)(tm * tn)), 256, 0, stream>>>(q, p, q2, p2, M, (int)N, K, K2, (int)tn, epi);
-  return hipGetLastError();
-}
+};
 
 }  // namespace dev
 }  // namespace b2c

@@ -1,0 +1,323 @@
+// The tiled matrix product behind the dense operators: out[m][n] = sum_k Q[m][k] P[n][k], with an epilogue.
+//
+// A workgroup computes BM x BN of out in steps of 128 bytes of k (64 values of 16 bits, 128 of 8). Both operands'
+// next step is copied from memory to LDS by the buffer unit itself while the current one is multiplied: two
+// buffers, one barrier a step, no registers in between. A copy instruction writes 64 pieces of 16 bytes in lane order,
+// so any rearrangement is done on the side of the addresses it reads:
+//   - rows along k ("plain" operand, element (i, k) at p[i ld + k]): row i's eight pieces are stored at
+//     (piece ^ i & 7), so that the sixteen rows that a matrix instruction's lanes read lie in different banks;
+//     rows of P are permuted so that a lane ends up with 4 x (tiles of its wave) neighbouring columns of out;
+//   - rows along i ("transposed", element (i, k) at p[k ld + i]): stored as they are, the pieces of row k at
+//     (piece ^ 2 key(k)), and read with the transposing LDS load, which hands lane l of each sixteen the four
+//     values that column l has in four rows.
+// Pieces beyond an operand's edge are read as zeros: their lanes are given an offset outside the buffer's range.
+#pragma once
+#include "dense.h"
+
+namespace b2c {
+namespace dev {
+
+constexpr uint32_t kOutside = 0x80000000u;  // an offset beyond every buffer range used here (2 GiB)
+
+// 16 bytes a lane from base + offset to LDS at `lds` + 16 lane. In assembly, since the compiler would wait for
+// every copy in flight before each LDS read; the kernel waits once a step.
+__device__ __forceinline__ void copy_to_lds(const void* base, uint32_t offset, uint32_t lds) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const vec<uint32_t, 4> rsrc = {(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, kOutside, 0x00020000u};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc)
+               : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ vec<T, 8> join(vec<short, 4> a, vec<short, 4> b) {
+  return __builtin_bit_cast(vec<T, 8>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ vec<short, 4> read_transposed(const char* lds) {
+  using L = __attribute__((address_space(3))) vec<short, 4>;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(lds));
+}
+
+// Operand of a tile: R rows of i from i0 on, of I; `trans` as above. Rows k of K.
+template <typename T, int R, int THREADS, bool TRANS>
+struct Tile {
+  static constexpr int V = Elem<T>::N, BK = 128 / sizeof(T);
+  static constexpr int BYTES = R * 128, COPIES = BYTES / (THREADS * 16);
+  static constexpr int PIECES = TRANS ? R / V : 8;  // of a stored row
+  static constexpr int key_of(int k) { return k & (PIECES / 2 - 1); }
+  static_assert(COPIES >= 1 && COPIES * THREADS * 16 == BYTES);
+  uint32_t off[COPIES];
+  int kpos[TRANS ? COPIES : 1];  // this lane's k within a step
+
+  // `row_of`: which row of the operand is stored at LDS row r (plain operands)
+  template <typename RowOf>
+  __device__ __forceinline__ void init(int64_t ld, int64_t i0, int64_t I, int wave, int lane, RowOf row_of) {
+#pragma unroll
+    for (int j = 0; j < COPIES; j++) {
+      const uint32_t piece = (uint32_t)((wave * COPIES + j) * 64 + lane);
+      const int r = (int)(piece / PIECES), s = (int)(piece % PIECES);
+      if constexpr (!TRANS) {
+        const int64_t i = (int64_t)row_of(r);
+        kpos[0] = (s ^ (r & 7)) * V;
+        off[j] = i0 + i < I ? (uint32_t)((i * ld + kpos[0]) * (int64_t)sizeof(T)) : kOutside;
+      } else {
+        const int key = key_of(r & 3 | (r >> 3 & 1) << 2), c = (s ^ key << 1) * V;
+        kpos[j] = r;
+        off[j] = i0 + c < I ? (uint32_t)(((int64_t)r * ld + c) * (int64_t)sizeof(T)) : kOutside;
+      }
+    }
+  }
+  // Starts the copies of the step whose first k is k0; `base`: element (i0, k0).
+  __device__ __forceinline__ void copy(int j, const void* base, uint32_t lds, int wave, int left) const {
+    const uint32_t o = kpos[TRANS ? j : 0] < left ? off[j] : kOutside;
+    copy_to_lds(base, o, lds + (uint32_t)((wave * COPIES + j) * 1024));
+  }
+};
+
+// The 16 x (16 bytes of k) fragments of a wave's rows w0 .. in an operand's LDS tile.
+template <typename T, int R, bool TRANS>
+struct Fragments {
+  static constexpr int V = Elem<T>::N;
+  int base;       // plain: byte offset of (row l % 16, piece 0)
+  int sw;         // plain: this lane's row & 7
+  int q, key, col;
+  __device__ __forceinline__ void init(int w0, int lane) {
+    q = lane >> 4;
+    if constexpr (!TRANS) {
+      base = (w0 + (lane & 15)) * 128;
+      sw = lane & 7;
+    } else {
+      const int i = lane & 15;
+      key = ((i >> 2) | (q & 1) << 2) & (R / V / 2 - 1);
+      base = (q * 8 + (i >> 2)) * (R * 2) + (i & 1) * 8;
+      col = w0 / 8 + (i >> 1 & 1);
+    }
+  }
+  // Tile t (16 rows), half kk of the step.
+  __device__ __forceinline__ vec<T, V> get(const char* lds, int t, int kk) const {
+    if constexpr (!TRANS) {
+      return *reinterpret_cast<const vec<T, V>*>(lds + base + t * 2048 + ((kk * 4 + q) ^ sw) * 16);
+    } else {
+      const char* p = lds + base + ((col + t * 2) ^ key << 1) * 16 + kk * 32 * (R * 2);
+      return join<T>(read_transposed(p), read_transposed(p + 4 * (R * 2)));
+    }
+  }
+};
+
+// Tile id -> (m tile, n tile): each of the eight dies works on a run of neighbouring tiles, and a run goes down
+// `group` m tiles before the next n tile, so that a die's cache holds both operands' rows for a while.
+__device__ __forceinline__ void place(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t group, uint32_t& tm,
+                                      uint32_t& tn) {
+  const uint32_t total = tiles_m * tiles_n, die = id % 8, per = total / 8, more = total % 8;
+  const uint32_t t = die * per + (die < more ? die : more) + id / 8;
+  const uint32_t g = t / (group * tiles_n), first = g * group;
+  const uint32_t rows = tiles_m - first < group ? tiles_m - first : group, r = t - g * group * tiles_n;
+  tn = r / rows;
+  tm = first + r - tn * rows;
+}
+
+// A product: operands p, q (and with TWO, after K values of k, p2, q2 for K2 more, rows as far apart), or with DUAL two
+// products that share q (p the gate's weights, p2 the up projection's; the epilogue gets both).
+template <typename T>
+struct Product {
+  Side<T> q, p, q2, p2;
+  int64_t M, N, K, K2;
+  int64_t q_lim, p_lim;  // how far m and n may be read in the operands; what lies beyond counts as zeros
+};
+
+template <typename T, bool PT, bool QT, bool DUAL, bool TWO, int WAVES_M, int WAVES_N, int WM, int WN, typename Epi>
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Product<T> a, int tiles_m, int tiles_n, int parts,
+                                                                     Epi epi) {
+  constexpr int THREADS = WAVES_M * WAVES_N * 64, BM = WAVES_M * WM, BN = WAVES_N * WN;
+  constexpr bool AHEAD = THREADS == 512;
+  constexpr int MT = WM / 16, NT = WN / 16, COLS = DUAL ? BN / 2 : BN;  // columns of out in a tile
+  using Acc = typename Elem<T>::Acc;
+  using TQ = Tile<T, BM, THREADS, QT>;
+  using TP = Tile<T, BN, THREADS, PT>;
+  static_assert(!DUAL || (!PT && !TWO));
+  constexpr int STEP = TQ::BYTES + TP::BYTES, BK = TQ::BK;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STEP];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t tiles = (uint32_t)tiles_m * tiles_n, part = blockIdx.x / tiles;
+  uint32_t tm, tn;
+  place(blockIdx.x - part * tiles, tiles_m, tiles_n, 4, tm, tn);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * COLS;
+  const int wm = wave % WAVES_M * WM, wb = wave / WAVES_M, wn = wb * WN;
+
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  const int steps1 = (int)((a.K + BK - 1) / BK), all = steps1 + (TWO ? (int)((a.K2 + BK - 1) / BK) : 0);
+  const int begin = (int)((int64_t)all * part / parts), steps = (int)((int64_t)all * (part + 1) / parts) - begin;
+
+  TQ cq;
+  TP cp;
+  auto q_row = [](uint32_t r) { return r; };
+  auto p_row = [](uint32_t r) {  // LDS row t 16 + q 4 + r of a wave's block holds column q (4 tiles) + 4 t + r
+    const uint32_t b = r / WN, t = r % WN / 16, q = r % 16 / 4, x = r % 4;
+    if constexpr (DUAL) return b * (WN / 2) + q * (2 * NT) + t % (NT / 2) * 4 + x;
+    else return b * WN + q * (4 * NT) + t * 4 + x;
+  };
+  const T *pq = nullptr, *pp = nullptr, *pu = nullptr;
+  int left = 0;
+  auto enter = [&](int seg, int step) {  // a segment's step
+    const Side<T>&Q = seg ? a.q2 : a.q, &P = seg && !DUAL ? a.p2 : a.p;
+    pq = Q.p + (QT ? m0 : m0 * Q.ld);
+    pp = P.p + (PT ? n0 : n0 * P.ld);
+    if constexpr (DUAL) pu = a.p2.p + n0 * a.p2.ld;
+    left = (int)(seg ? a.K2 : a.K) - step * BK;
+    pq += QT ? (int64_t)step * BK * a.q.ld : step * BK;
+    pp += PT ? (int64_t)step * BK * a.p.ld : step * BK;
+    if constexpr (DUAL) pu += step * BK;
+    cq.init(Q.ld, m0, a.q_lim, wave, lane, q_row);
+    cp.init(P.ld, n0, a.p_lim, wave, lane, p_row);
+  };
+  constexpr int COPIES = TQ::COPIES + TP::COPIES;
+  auto copy = [&](int s, int j) {  // copy j of step s; beyond the last step `left` makes it one of zeros
+    const uint32_t to = lds0 + (uint32_t)(s & 1) * STEP;
+    if (j < TQ::COPIES) {
+      cq.copy(j, pq, to, wave, left);
+    } else {
+      j -= TQ::COPIES;
+      const T* base = pp;
+      if constexpr (DUAL) {  // eight LDS rows a copy, all of one of the two
+        const int r = (wave * TP::COPIES + j) * 8;
+        base = r % WN >= WN / 2 ? pu : pp;
+      }
+      cp.copy(j, base, to + TQ::BYTES, wave, left);
+    }
+  };
+  auto advance = [&](int s) {  // from step s to the next
+    left -= BK;
+    if (TWO && begin + s + 1 == steps1) {
+      enter(1, 0);
+    } else {
+      pq += QT ? BK * a.q.ld : BK;
+      pp += PT ? BK * a.p.ld : BK;
+      if constexpr (DUAL) pu += BK;
+    }
+  };
+  auto start = [&](int s) {
+#pragma unroll
+    for (int j = 0; j < COPIES; j++) copy(s, j);
+    advance(s);
+  };
+
+  Fragments<T, BM, QT> fq;
+  Fragments<T, BN, PT> fp;
+  fq.init(wm, lane);
+  fp.init(wn, lane);
+  Acc acc[NT][MT] = {};
+  using F = vec<T, TQ::V>;
+  F q0[MT], p0[NT], q1[MT], p1[NT];
+  auto read = [&](int s, int kk, F(&q)[MT], F(&p)[NT]) {
+    const char* at = lds + (s & 1) * STEP;
+#pragma unroll
+    for (int t = 0; t < NT; t++) p[t] = fp.get(at + TQ::BYTES, t, kk);
+#pragma unroll
+    for (int t = 0; t < MT; t++) q[t] = fq.get(at, t, kk);
+  };
+  auto multiply = [&](const F(&q)[MT], const F(&p)[NT]) {
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) acc[j][i] = mfma(p[j], q[i], acc[j][i]);
+  };
+  auto landed = [] {  // this wave's copies are in LDS and its reads done; then everybody's
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // Multiplies one half's fragments while those of another are read from buffer `at`, spread over the first three
+  // quarters, and with COPY the copies of step s are started, spread too: a wave issues in order, and the address unit
+  // takes 16 cycles for each copy, so eight waves' copies in a row would hold up all of them for a thousand cycles.
+  auto half = [&](const F(&q)[MT], const F(&p)[NT], F(&qn)[MT], F(&pn)[NT], const char* at, int kk, auto with_copies, int s) {
+    constexpr int READS = MT + NT, SLOTS = MT * 3 / 4;
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+      if constexpr (decltype(with_copies)::value) {
+#pragma unroll
+        for (int j = COPIES * i / MT; j < COPIES * (i + 1) / MT; j++) copy(s, j);
+      }
+      if (i < SLOTS) {
+#pragma unroll
+        for (int j = READS * i / SLOTS; j < READS * (i + 1) / SLOTS; j++) {
+          if (j < NT) pn[j] = fp.get(at + TQ::BYTES, j, kk);
+          else qn[j - NT] = fq.get(at, j - NT, kk);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NT; j++) acc[j][i] = mfma(p[j], q[i], acc[j][i]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // A step in two halves of k. While one half is multiplied the next is read into registers, across the steps too:
+  // the barrier stands between the halves, where nothing of the current buffer is left to read, so the copies of
+  // the step after next can start there, and have a whole step's time to land.
+  if constexpr (AHEAD) {
+    if (steps) {
+      TWO && begin >= steps1 ? enter(1, begin - steps1) : enter(0, begin);
+      start(0);
+      landed();
+      start(1);
+      read(0, 0, q0, p0);
+    }
+    for (int s = 0; s < steps; s++) {
+      half(q0, p0, q1, p1, lds + (s & 1) * STEP, 1, std::false_type{}, 0);
+      landed();
+      // after the last step the reads get what is there, unused
+      half(q1, p1, q0, p0, lds + ((s + 1) & 1) * STEP, 0, std::true_type{}, s + 2);
+      advance(s + 2);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup
+  } else {
+    if (steps) {
+      TWO && begin >= steps1 ? enter(1, begin - steps1) : enter(0, begin);
+      start(0);
+    }
+    for (int s = 0; s < steps; s++) {
+      landed();
+      if (s + 1 < steps) start(s + 1);
+      read(s, 0, q0, p0);
+      multiply(q0, p0);
+      read(s, 1, q1, p1);
+      multiply(q1, p1);
+    }
+  }
+
+  using S = std::remove_reference_t<decltype(acc[0][0][0])>;
+  const int lq = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < MT; i++) {
+    const int64_t m = m0 + wm + i * 16 + (lane & 15);
+    if (m >= a.M) continue;
+    if constexpr (DUAL) {
+      constexpr int W = 2 * NT;
+      const int64_t n = n0 + wb * (WN / 2) + lq * W;
+      S g[W], u[W];
+#pragma unroll
+      for (int j = 0; j < W; j++) g[j] = acc[j / 4][i][j % 4], u[j] = acc[NT / 2 + j / 4][i][j % 4];
+      if (n < a.N) epi.template operator()<W>(part, m, (int)n, g, u);
+    } else if constexpr (!PT) {
+      constexpr int W = NT >= 2 ? 8 : 4;
+#pragma unroll
+      for (int h = 0; h < 4 * NT / W; h++) {
+        const int64_t n = n0 + wn + lq * 4 * NT + h * W;
+        S v[W];
+#pragma unroll
+        for (int j = 0; j < W; j++) v[j] = acc[h * (W / 4) + j / 4][i][j % 4];
+        if (n < a.N) epi.template operator()<W>(part, m, (int)n, v);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        const int64_t n = n0 + wn + t * 16 + lq * 4;
+        S v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = acc[t][i][j];
+        if (n < a.N) epi.template operator()<4>(part, m, (int)n, v);
+      }
+    }
+  }
+}
+
+}  // namespace dev
+}  // namespace b2c

@@ -1,15 +1,13 @@
 // The gated feed-forward block and its gradients (b2c_hip_ffn_forward, b2c_hip_ffn_backward).
-#include "dense.h"
+#include "dense_product.h"
 
 namespace b2c {
 namespace dev {
 namespace {
 
-int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
-
 bool sizes_ok(const b2c_ffn_args* a, Drop* d) {
   const int most = 1 << 24;
-  return a && a->rows >= 0 && a->rows <= ((int64_t)1 << 31) && a->d_in >= 1 && a->d_in <= most && a->d_hidden >= 1 &&
+  return a && a->rows >= 0 && a->rows <= (1 << 30) && a->d_in >= 1 && a->d_in <= most && a->d_hidden >= 1 &&
          a->d_hidden <= most && a->d_out >= 1 && a->d_out <= most && (a->dtype == B2C_F16 || a->dtype == B2C_BF16) &&
          a->act >= B2C_ACT_SILU && a->act <= B2C_ACT_RELU && drop_of(a->p, a->seed, a->stream, d);
 }
@@ -17,60 +15,177 @@ bool room_ok(const void* p, size_t have, size_t need) {
   return have >= need && (need == 0 || (p && reinterpret_cast<uintptr_t>(p) % 16 == 0));
 }
 
+// A matrix copied to rows that start on 16 bytes, `pitch` values apart, zeros in the columns from `cols` up to
+// the next multiple of 8; where dropout is given, zeros in the place of what it drops too. Eight values a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* x, int64_t ldx, int64_t rows, int cols, T* to, int64_t pitch,
+                                                   uint32_t groups, Drop d) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, m = t / groups;
+  if (m >= rows) return;
+  const int n = (int)(t - m * groups) * 8;
+  const T* p = x + m * ldx + n;
+  vec<T, 8> v{};
+  if (n + 8 <= cols) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (n + j < cols) v[j] = p[j];
+  }
+  if (d.threshold) {
+    const uint64_t e = (uint64_t)m * cols + n;
+    const uint32_t keep = kept4(d, e) | kept4(d, e + 4) << 4;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (!(keep >> j & 1)) v[j] = (T)0.f;
+  }
+  *reinterpret_cast<vec<T, 8>*>(to + m * pitch + n) = v;
+}
+template <typename T>
+int pack(Side<T> from, int64_t rows, int cols, T* to, int64_t pitch, const Drop& d, hipStream_t stream) {
+  const int64_t groups = up(cols, 8) / 8, blocks = up(rows * groups, 256) / 256;
+  if (blocks == 0) return hipSuccess;
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  pack_kernel<T><<<dim3((unsigned)blocks), 256, 0, stream>>>(from.p, from.ld, rows, cols, to, pitch, (uint32_t)groups, d);
+  return hipGetLastError();
+}
+
+// Whether the tiles' copies can read a matrix where it is: rows on 16 bytes, whole pieces of 8 columns, and 256 rows
+// within the 2 GiB that a copy's offset spans.
+bool direct(const void* p, int64_t ld, int64_t cols) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && cols % 8 == 0 && ld < ((int64_t)1 << 21);
+}
+
+// An operand: where it is, or its packed copy.
+template <typename T>
+struct Operand {
+  Side<T> from;
+  int64_t rows;
+  int cols;
+  T* copy = nullptr;
+  int64_t pitch = 0;
+  Drop drop{};
+  void place(Room& room, bool straight) {
+    if (straight) return;
+    pitch = up(cols, 64);
+    copy = room.take<T>(rows * pitch);
+  }
+  Side<T> side() const { return pitch ? Side<T>{copy, pitch} : from; }
+  int make(hipStream_t stream) const { return pitch ? pack(from, rows, cols, copy, pitch, drop, stream) : hipSuccess; }
+};
+
+// The steps of 64 values that a sum over k takes.
+int64_t steps_of(int64_t k) { return up(k, 64) / 64; }
+
+// What a forward pass needs beside its matrices.
+template <typename T>
+struct ForwardPlan {
+  int64_t fp;
+  T* h;
+  Operand<T> x, wg, wu, wd;
+  Way gate, down;
+  void* sums;
+  ForwardPlan(const b2c_ffn_args* a, Room& room) {
+    const int64_t M = a->rows;
+    fp = up(a->d_hidden, 64);
+    h = room.take<T>(M * fp);
+    gate = choose(M, fp, steps_of(a->d_in), true, true);
+    down = choose(M, a->d_out, steps_of(a->d_hidden), false, true);
+    x = {{(const T*)a->x, a->ldx}, M, a->d_in};
+    wg = {{(const T*)a->w_gate, a->ld_in}, a->d_hidden, a->d_in};
+    wu = {{(const T*)a->w_up, a->ld_in}, a->d_hidden, a->d_in};
+    wd = {{(const T*)a->w_down, a->ld_out}, a->d_out, a->d_hidden};
+    if (gate.tile != FEW_ROWS) {  // all or none along d_in: a copy's zeros beyond the last column meet zeros
+      x.place(room, direct(a->x, a->ldx, a->d_in));
+      const bool in = direct(a->w_gate, a->ld_in, a->d_in) && direct(a->w_up, a->ld_in, a->d_in);
+      wg.place(room, in);
+      wu.place(room, in);
+      wd.place(room, direct(a->w_down, a->ld_out, a->d_hidden));
+    }
+    sums = room.take<char>(std::max(gate.sums, down.sums));
+  }
+};
+
 template <typename T, int ACT>
 int forward(const b2c_ffn_args* a, const Drop& d, hipStream_t stream) {
-  const int64_t fp = up64(a->d_hidden);
-  T* h = (T*)a->workspace;
-  GateOut<T, ACT> gate{h, (T*)a->saved, fp, a->d_hidden};
-  const Side<T> x{(const T*)a->x, a->ldx};
-  int rc = product<T, false, false, true>(x, {(const T*)a->w_gate, a->ld_in}, x, {(const T*)a->w_up, a->ld_in}, a->rows,
-                                          a->d_hidden, a->d_in, 0, gate, stream);
-  if (rc) return rc;
-  RowsOut<T> out{(T*)a->y, a->ldy, (const T*)a->residual, a->ldr, a->d_out, wide(a->y, a->ldy, 2),
-                 wide(a->residual, a->ldr, 2), d};
-  return product<T, false, false, false>(Side<T>{h, fp}, {(const T*)a->w_down, a->ld_out}, {}, {}, a->rows, a->d_out,
-                                         a->d_hidden, 0, out, stream);
+  Room room{(char*)a->workspace};
+  const ForwardPlan<T> p(a, room);
+  int rc;
+  if ((rc = p.x.make(stream)) || (rc = p.wg.make(stream)) || (rc = p.wu.make(stream)) || (rc = p.wd.make(stream))) return rc;
+  const GateOut<T, ACT> gate{p.h, (T*)a->saved, p.fp, a->d_hidden};
+  Product<T> in{p.x.side(), p.wg.side(), {}, p.wu.side(), a->rows, p.fp, a->d_in, 0, a->rows, a->d_hidden};
+  if ((rc = product<T, false, false, true, false>(in, p.gate, p.sums, gate, stream))) return rc;
+  const RowsOut<T> out{(T*)a->y, a->ldy, (const T*)a->residual, a->ldr, a->d_out, d};
+  Product<T> down{{p.h, p.fp}, p.wd.side(), {}, {}, a->rows, a->d_out, a->d_hidden, 0, a->rows, a->d_out};
+  return product<T, false, false, false, false>(down, p.down, p.sums, out, stream);
 }
+
+template <typename T>
+struct BackwardPlan {
+  int64_t fp;
+  T *h, *dgu;
+  Operand<T> x, wg, wu, wd, dz;
+  Way back, down, in, dx;
+  void* sums;
+  BackwardPlan(const b2c_ffn_grad_args* b, const Drop& d, Room& room) {
+    const b2c_ffn_args* a = &b->fwd;
+    const int64_t M = a->rows;
+    fp = up(a->d_hidden, 64);
+    dgu = room.take<T>(M * 2 * fp);
+    h = room.take<T>(M * fp);
+    back = choose(M, fp, steps_of(a->d_out), false, false);
+    down = choose(a->d_out, a->d_hidden, steps_of(M), false, false);
+    in = choose(fp + a->d_hidden, a->d_in, steps_of(M), false, false);
+    dx = choose(M, a->d_in, 2 * steps_of(a->d_hidden), false, false);
+    x = {{(const T*)a->x, a->ldx}, M, a->d_in};
+    wg = {{(const T*)a->w_gate, a->ld_in}, a->d_hidden, a->d_in};
+    wu = {{(const T*)a->w_up, a->ld_in}, a->d_hidden, a->d_in};
+    wd = {{(const T*)a->w_down, a->ld_out}, a->d_out, a->d_hidden};
+    dz = {{(const T*)b->dy, b->lddy}, M, a->d_out};
+    dz.drop = d;
+    if (b->dw_gate || b->dw_up) x.place(room, direct(a->x, a->ldx, a->d_in));
+    if (b->dx) {
+      const bool in = direct(a->w_gate, a->ld_in, a->d_in) && direct(a->w_up, a->ld_in, a->d_in);
+      wg.place(room, in);
+      wu.place(room, in);
+    }
+    wd.place(room, direct(a->w_down, a->ld_out, a->d_hidden));
+    dz.place(room, !d.threshold && direct(b->dy, b->lddy, a->d_out));
+    sums = room.take<char>(std::max(std::max(back.sums, down.sums), std::max(in.sums, dx.sums)));
+  }
+};
 
 template <typename T, int ACT>
 int backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream) {
   const b2c_ffn_args* a = &b->fwd;
-  const int64_t fp = up64(a->d_hidden), op = up64(a->d_out), M = a->rows;
-  T* dgu = (T*)b->workspace;
-  T* h = dgu + M * 2 * fp;
-  T* dz = h + M * fp;
-  Side<T> dy{(const T*)b->dy, b->lddy};
+  Room room{(char*)b->workspace};
+  const BackwardPlan<T> p(b, d, room);
+  const int64_t fp = p.fp, M = a->rows;
+  const float scale = d.threshold ? d.scale : 1.f;
   int rc;
-  if (d.threshold && M) {
-    b2c_dropout_args da{M, a->d_out, a->dtype, a->p, a->seed, a->stream, b->dy, b->lddy, nullptr, 0, dz, op};
-    if ((rc = b2c_hip_dropout(&da, stream))) return rc;
-    dy = {dz, op};
-  }
-  const bool inner = b->dx || b->dw_gate || b->dw_up;
-  const Side<T> wd{(const T*)a->w_down, a->ld_out};
-  if (inner || b->dw_down) {
-    GateBack<T, ACT> back{(const T*)a->saved, b->dw_down ? h : nullptr, dgu, fp, a->d_hidden};
-    if ((rc = product<T, true, false, false>(dy, wd, {}, {}, M, a->d_hidden, a->d_out, 0, back, stream))) return rc;
-  }
-  const size_t gs = b->grad_dtype == B2C_F32 ? 4 : 2;
+  if (!b->dx && !b->dw_gate && !b->dw_up && !b->dw_down) return hipSuccess;
+  if (M && ((rc = p.x.make(stream)) || (rc = p.wg.make(stream)) || (rc = p.wu.make(stream)) || (rc = p.wd.make(stream)) ||
+            (rc = p.dz.make(stream))))
+    return rc;
+  const Side<T> dz = p.dz.side(), x = p.x.side(), dgu{p.dgu, 2 * fp};
+  const GateBack<T, ACT> back{(const T*)a->saved, p.h, p.dgu, fp, a->d_hidden, scale};
+  const Product<T> dh{dz, p.wd.side(), {}, {}, M, fp, a->d_out, 0, M, a->d_hidden};
+  if ((rc = product<T, true, false, false, false>(dh, p.back, p.sums, back, stream))) return rc;
   const bool f32 = b->grad_dtype == B2C_F32, add = b->accumulate != 0;
   if (b->dw_down) {
-    WeightOut<T> out{b->dw_down, nullptr, b->ld_dout, a->d_out, 0, a->d_hidden, f32, add, wide(b->dw_down, b->ld_dout, gs)};
-    if ((rc = product<T, true, true, false>(dy, Side<T>{h, fp}, {}, {}, a->d_out, a->d_hidden, M, 0, out, stream))) return rc;
+    const WeightOut<T> out{b->dw_down, nullptr, b->ld_dout, a->d_out, 0, a->d_hidden, f32, add, scale};
+    const Product<T> dw{dz, {p.h, fp}, {}, {}, a->d_out, a->d_hidden, M, 0, a->d_out, a->d_hidden};
+    if ((rc = product<T, true, true, false, false>(dw, p.down, p.sums, out, stream))) return rc;
   }
   if (b->dw_gate || b->dw_up) {
-    WeightOut<T> out{b->dw_gate, b->dw_up, b->ld_din, a->d_hidden, (int)fp, a->d_in, f32, add,
-                     wide(b->dw_gate, b->ld_din, gs) && wide(b->dw_up, b->ld_din, gs)};
-    if ((rc = product<T, true, true, false>(Side<T>{dgu, 2 * fp}, Side<T>{(const T*)a->x, a->ldx}, {}, {}, fp + a->d_hidden,
-                                            a->d_in, M, 0, out, stream)))
-      return rc;
+    const WeightOut<T> out{b->dw_gate, b->dw_up, b->ld_din, a->d_hidden, (int)fp, a->d_in, f32, add, 1.f};
+    const Product<T> dw{dgu, x, {}, {}, fp + a->d_hidden, a->d_in, M, 0, fp + a->d_hidden, a->d_in};
+    if ((rc = product<T, true, true, false, false>(dw, p.in, p.sums, out, stream))) return rc;
   }
   if (b->dx) {
-    RowsOut<T> out{(T*)b->dx, b->lddx, nullptr, 0, a->d_in, wide(b->dx, b->lddx, 2), false, {}};
-    if ((rc = product<T, true, false, false>(Side<T>{dgu, 2 * fp}, Side<T>{(const T*)a->w_gate, a->ld_in},
-                                             Side<T>{dgu + fp, 2 * fp}, Side<T>{(const T*)a->w_up, a->ld_in}, M, a->d_in,
-                                             a->d_hidden, a->d_hidden, out, stream)))
-      return rc;
+    const RowsOut<T> out{(T*)b->dx, b->lddx, nullptr, 0, a->d_in, {}};
+    const Product<T> dx{dgu, p.wg.side(), {p.dgu + fp, 2 * fp}, p.wu.side(), M, a->d_in, a->d_hidden, a->d_hidden, M, a->d_in};
+    if ((rc = product<T, true, false, false, true>(dx, p.dx, p.sums, out, stream))) return rc;
   }
   return hipSuccess;
 }
@@ -96,11 +211,14 @@ using namespace b2c::dev;
 
 extern "C" size_t b2c_ffn_saved_bytes(const b2c_ffn_args* a) {
   Drop d;
-  return sizes_ok(a, &d) ? (size_t)a->rows * 2 * up64(a->d_hidden) * 2 : 0;
+  return sizes_ok(a, &d) ? (size_t)a->rows * 2 * up(a->d_hidden, 64) * 2 : 0;
 }
 extern "C" size_t b2c_ffn_workspace_bytes(const b2c_ffn_args* a) {
   Drop d;
-  return sizes_ok(a, &d) ? (size_t)a->rows * up64(a->d_hidden) * 2 : 0;
+  if (!sizes_ok(a, &d) || a->rows == 0) return 0;
+  Room room{nullptr};
+  ForwardPlan<bf16>(a, room);  // both types have the same size
+  return room.used;
 }
 extern "C" int b2c_hip_ffn_forward(const b2c_ffn_args* a, hipStream_t stream) {
   Drop d;
@@ -117,7 +235,9 @@ extern "C" int b2c_hip_ffn_forward(const b2c_ffn_args* a, hipStream_t stream) {
 extern "C" size_t b2c_ffn_grad_workspace_bytes(const b2c_ffn_grad_args* b) {
   Drop d;
   if (!b || !sizes_ok(&b->fwd, &d)) return 0;
-  return (size_t)b->fwd.rows * (3 * up64(b->fwd.d_hidden) + (d.threshold ? up64(b->fwd.d_out) : 0)) * 2;
+  Room room{nullptr};
+  BackwardPlan<bf16>(b, d, room);
+  return room.used;
 }
 extern "C" int b2c_hip_ffn_backward(const b2c_ffn_grad_args* b, hipStream_t stream) {
   Drop d;
@@ -132,9 +252,9 @@ extern "C" int b2c_hip_ffn_backward(const b2c_ffn_grad_args* b, hipStream_t stre
   if (a->rows) {
     if (!good(a->x, a->ldx, a->d_in, 2) || !good(a->w_gate, a->ld_in, a->d_in, 2) || !good(a->w_up, a->ld_in, a->d_in, 2) ||
         !good(a->w_down, a->ld_out, a->d_hidden, 2) || !good(b->dy, b->lddy, a->d_out, 2) ||
-        (b->dx && !good(b->dx, b->lddx, a->d_in, 2)) || !a->saved || reinterpret_cast<uintptr_t>(a->saved) % 16 ||
-        !room_ok(b->workspace, b->workspace_bytes, b2c_ffn_grad_workspace_bytes(b)))
+        (b->dx && !good(b->dx, b->lddx, a->d_in, 2)) || !a->saved || reinterpret_cast<uintptr_t>(a->saved) % 16)
       return hipErrorInvalidValue;
   }
+  if (!room_ok(b->workspace, b->workspace_bytes, b2c_ffn_grad_workspace_bytes(b))) return hipErrorInvalidValue;
   return a->dtype == B2C_F16 ? backward<f16>(b, d, stream) : backward<bf16>(b, d, stream);
 }

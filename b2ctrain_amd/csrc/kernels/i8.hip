@@ -1,12 +1,10 @@
 // Products in 8-bit integers with a scale for each row and each channel (b2c_hip_quantize_rows, b2c_hip_i8_linear,
 // b2c_hip_i8_ffn).
-#include "dense.h"
+#include "dense_product.h"
 
 namespace b2c {
 namespace dev {
 namespace {
-
-int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
 
 // A row to a workgroup, in two passes over it: the largest magnitude, then the values. A row's columns from
 // cols to `pad` become 0.
@@ -60,27 +58,108 @@ bool sizes_ok(const b2c_i8_ffn_args* a) {
   return a && a->rows >= 0 && a->rows <= 0x7fffffff && a->d_in >= 1 && a->d_in <= MOST && a->d_hidden >= 1 && a->d_hidden <= MOST && a->d_out >= 1 &&
          a->d_out <= (1 << 24) && type_ok(a->dtype) && a->act >= B2C_ACT_SILU && a->act <= B2C_ACT_RELU;
 }
-size_t up16(size_t v) { return (v + 15) / 16 * 16; }
+
+// Weights in 8 bits as the products read them: in place where rows start on 16 bytes (columns beyond the last meet zeros of
+// the quantised rows), else copied to rows that do. A few rows read them anywhere.
+__global__ __launch_bounds__(256) void pack_kernel(const int8_t* w, int64_t ldw, int64_t rows, int cols, int8_t* to,
+                                                   int64_t pitch, uint32_t groups) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, m = t / groups;
+  if (m >= rows) return;
+  const int n = (int)(t - m * groups) * 16;
+  const int8_t* p = w + m * ldw + n;
+  vec<int8_t, 16> v{};
+  if (n + 16 <= cols) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+      if (n + j < cols) v[j] = p[j];
+  }
+  *reinterpret_cast<vec<int8_t, 16>*>(to + m * pitch + n) = v;
+}
+struct Weights {
+  Side<int8_t> from;
+  int64_t rows;
+  int cols;
+  int8_t* copy = nullptr;
+  int64_t pitch = 0;
+  void place(Room& room, bool few) {
+    if (few || (reinterpret_cast<uintptr_t>(from.p) % 16 == 0 && from.ld % 16 == 0 && cols % 16 == 0 && from.ld < (1 << 22))) return;
+    pitch = up(cols, 128);
+    copy = room.take<int8_t>(rows * pitch);
+  }
+  Side<int8_t> side() const { return pitch ? Side<int8_t>{copy, pitch} : from; }
+  int make(hipStream_t stream) const {
+    if (!pitch) return hipSuccess;
+    const int64_t groups = up(cols, 16) / 16, blocks = up(rows * groups, 256) / 256;
+    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+    pack_kernel<<<dim3((unsigned)blocks), 256, 0, stream>>>(from.p, from.ld, rows, cols, copy, pitch, (uint32_t)groups);
+    return hipGetLastError();
+  }
+};
+int64_t steps_of(int64_t k) { return up(k, 128) / 128; }
+
+struct LinearPlan {
+  int64_t kp;
+  int8_t* q;
+  float* sx;
+  Weights w;
+  Way way;
+  void* sums;
+  LinearPlan(const b2c_i8_linear_args* a, Room& room) {
+    kp = up(a->d_in, 128);
+    q = room.take<int8_t>(a->rows * kp);
+    sx = room.take<float>(a->rows);
+    way = choose(a->rows, a->d_out, steps_of(a->d_in), false, true);
+    w = {{a->w, a->ldw}, a->d_out, a->d_in};
+    w.place(room, way.tile == FEW_ROWS);
+    sums = room.take<char>(way.sums);
+  }
+};
+struct BlockPlan {
+  int64_t kp, fp;
+  float *h, *s;  // s: of x's rows, then of h's
+  int8_t *qx, *qh;
+  Weights wg, wu, wd;
+  Way gate, down;
+  void* sums;
+  BlockPlan(const b2c_i8_ffn_args* a, Room& room) {
+    kp = up(a->d_in, 128);
+    fp = up(a->d_hidden, 128);
+    h = room.take<float>(a->rows * fp);
+    qh = room.take<int8_t>(a->rows * fp);
+    qx = room.take<int8_t>(a->rows * kp);
+    s = room.take<float>(a->rows);
+    gate = choose(a->rows, a->d_hidden, steps_of(a->d_in), true, true);
+    down = choose(a->rows, a->d_out, steps_of(a->d_hidden), false, true);
+    const bool few = gate.tile == FEW_ROWS;
+    wg = {{a->w_gate, a->ld_in}, a->d_hidden, a->d_in};
+    wu = {{a->w_up, a->ld_in}, a->d_hidden, a->d_in};
+    wd = {{a->w_down, a->ld_out}, a->d_out, a->d_hidden};
+    wg.place(room, few);
+    wu.place(room, few);
+    wd.place(room, few);
+    sums = room.take<char>(std::max(gate.sums, down.sums));
+  }
+};
 
 template <typename T>
-int linear_out(const int8_t* q, int64_t ldq, const float* sx, const int8_t* w, int64_t ldw, const float* sw, int64_t rows,
-               int d_out, int d_in, void* y, int64_t ldy, hipStream_t stream) {
-  ScaledOut<T> out{(T*)y, ldy, sx, sw, d_out, wide(y, ldy, sizeof(T))};
-  return product<int8_t, false, false, false>(Side<int8_t>{q, ldq}, Side<int8_t>{w, ldw}, {}, {}, rows, d_out, d_in, 0, out,
-                                              stream);
+int scaled(const Product<int8_t>& p, const Way& way, void* sums, const float* sx, const float* sw, void* y, int64_t ldy,
+           hipStream_t stream) {
+  const ScaledOut<T> out{(T*)y, ldy, sx, sw, (int)p.N};
+  return product<int8_t, false, false, false, false>(p, way, sums, out, stream);
 }
-int linear(const int8_t* q, int64_t ldq, const float* sx, const int8_t* w, int64_t ldw, const float* sw, int64_t rows,
-           int d_out, int d_in, int dtype, void* y, int64_t ldy, hipStream_t stream) {
-  if (dtype == B2C_F32) return linear_out<float>(q, ldq, sx, w, ldw, sw, rows, d_out, d_in, y, ldy, stream);
-  if (dtype == B2C_F16) return linear_out<f16>(q, ldq, sx, w, ldw, sw, rows, d_out, d_in, y, ldy, stream);
-  return linear_out<bf16>(q, ldq, sx, w, ldw, sw, rows, d_out, d_in, y, ldy, stream);
+int scaled(const Product<int8_t>& p, const Way& way, void* sums, const float* sx, const float* sw, int dtype, void* y,
+           int64_t ldy, hipStream_t stream) {
+  if (dtype == B2C_F32) return scaled<float>(p, way, sums, sx, sw, y, ldy, stream);
+  if (dtype == B2C_F16) return scaled<f16>(p, way, sums, sx, sw, y, ldy, stream);
+  return scaled<bf16>(p, way, sums, sx, sw, y, ldy, stream);
 }
 template <int ACT>
-int gated(const int8_t* q, int64_t ldq, const float* sx, const b2c_i8_ffn_args* a, float* h, int64_t fp, hipStream_t stream) {
-  ScaledGate<ACT> out{h, sx, a->s_gate, a->s_up, fp, a->d_hidden};
-  const Side<int8_t> x{q, ldq};
-  return product<int8_t, false, false, true>(x, {a->w_gate, a->ld_in}, x, {a->w_up, a->ld_in}, a->rows, a->d_hidden, a->d_in,
-                                             0, out, stream);
+int gated(const BlockPlan& p, const b2c_i8_ffn_args* a, hipStream_t stream) {
+  const ScaledGate<ACT> out{p.h, p.s, a->s_gate, a->s_up, p.fp, a->d_hidden};
+  const Product<int8_t> in{{p.qx, p.kp}, p.wg.side(), {}, p.wu.side(), a->rows, a->d_hidden, a->d_in, 0, a->rows, a->d_hidden};
+  return product<int8_t, false, false, true, false>(in, p.gate, p.sums, out, stream);
 }
 
 }  // namespace
@@ -98,7 +177,10 @@ extern "C" int b2c_hip_quantize_rows(const b2c_quantize_args* a, hipStream_t str
 }
 
 extern "C" size_t b2c_i8_linear_workspace_bytes(const b2c_i8_linear_args* a) {
-  return sizes_ok(a) ? (size_t)a->rows * up64(a->d_in) + up16((size_t)a->rows * 4) : 0;
+  if (!sizes_ok(a) || a->rows == 0) return 0;
+  Room room{nullptr};
+  LinearPlan(a, room);
+  return room.used;
 }
 extern "C" int b2c_hip_i8_linear(const b2c_i8_linear_args* a, hipStream_t stream) {
   if (!sizes_ok(a)) return hipErrorInvalidValue;
@@ -107,17 +189,19 @@ extern "C" int b2c_hip_i8_linear(const b2c_i8_linear_args* a, hipStream_t stream
       !good(a->y, a->ldy, a->d_out, size_of(a->dtype)) ||
       !room_ok(a->workspace, a->workspace_bytes, b2c_i8_linear_workspace_bytes(a)))
     return hipErrorInvalidValue;
-  const int64_t kp = up64(a->d_in);
-  int8_t* q = (int8_t*)a->workspace;
-  float* sx = (float*)(q + a->rows * kp);
-  const int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, q, kp, sx, stream);
-  if (rc) return rc;
-  return linear(q, kp, sx, a->w, a->ldw, a->w_scale, a->rows, a->d_out, a->d_in, a->dtype, a->y, a->ldy, stream);
+  Room room{(char*)a->workspace};
+  const LinearPlan p(a, room);
+  int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.q, p.kp, p.sx, stream);
+  if (rc || (rc = p.w.make(stream))) return rc;
+  const Product<int8_t> out{{p.q, p.kp}, p.w.side(), {}, {}, a->rows, a->d_out, a->d_in, 0, a->rows, a->d_out};
+  return scaled(out, p.way, p.sums, p.sx, a->w_scale, a->dtype, a->y, a->ldy, stream);
 }
 
 extern "C" size_t b2c_i8_ffn_workspace_bytes(const b2c_i8_ffn_args* a) {
-  if (!sizes_ok(a)) return 0;
-  return (size_t)a->rows * (up64(a->d_in) + up64(a->d_hidden) * 5) + up16((size_t)a->rows * 4);
+  if (!sizes_ok(a) || a->rows == 0) return 0;
+  Room room{nullptr};
+  BlockPlan(a, room);
+  return room.used;
 }
 extern "C" int b2c_hip_i8_ffn(const b2c_i8_ffn_args* a, hipStream_t stream) {
   if (!sizes_ok(a)) return hipErrorInvalidValue;
@@ -127,18 +211,15 @@ extern "C" int b2c_hip_i8_ffn(const b2c_i8_ffn_args* a, hipStream_t stream) {
       !good(a->s_up, 1, 1, 4) || !good(a->s_down, 1, 1, 4) || !good(a->y, a->ldy, a->d_out, size_of(a->dtype)) ||
       !room_ok(a->workspace, a->workspace_bytes, b2c_i8_ffn_workspace_bytes(a)))
     return hipErrorInvalidValue;
-  const int64_t kp = up64(a->d_in), fp = up64(a->d_hidden);
-  float* h = (float*)a->workspace;
-  int8_t* qh = (int8_t*)(h + a->rows * fp);
-  int8_t* qx = qh + a->rows * fp;
-  float* s = (float*)(qx + a->rows * kp);  // of x's rows, then of h's
-  int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, qx, kp, s, stream);
+  Room room{(char*)a->workspace};
+  const BlockPlan p(a, room);
+  int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.qx, p.kp, p.s, stream);
+  if (rc || (rc = p.wg.make(stream)) || (rc = p.wu.make(stream)) || (rc = p.wd.make(stream))) return rc;
+  if (a->act == B2C_ACT_SILU) rc = gated<B2C_ACT_SILU>(p, a, stream);
+  else if (a->act == B2C_ACT_GELU) rc = gated<B2C_ACT_GELU>(p, a, stream);
+  else rc = gated<B2C_ACT_RELU>(p, a, stream);
   if (rc) return rc;
-  if (a->act == B2C_ACT_SILU) rc = gated<B2C_ACT_SILU>(qx, kp, s, a, h, fp, stream);
-  else if (a->act == B2C_ACT_GELU) rc = gated<B2C_ACT_GELU>(qx, kp, s, a, h, fp, stream);
-  else rc = gated<B2C_ACT_RELU>(qx, kp, s, a, h, fp, stream);
-  if (rc) return rc;
-  rc = quantize(h, fp, B2C_F32, a->rows, a->d_hidden, qh, fp, s, stream);
-  if (rc) return rc;
-  return linear(qh, fp, s, a->w_down, a->ld_out, a->s_down, a->rows, a->d_out, a->d_hidden, a->dtype, a->y, a->ldy, stream);
+  if ((rc = quantize(p.h, p.fp, B2C_F32, a->rows, a->d_hidden, p.qh, p.fp, p.s, stream))) return rc;
+  const Product<int8_t> out{{p.qh, p.fp}, p.wd.side(), {}, {}, a->rows, a->d_out, a->d_hidden, 0, a->rows, a->d_out};
+  return scaled(out, p.down, p.sums, p.s, a->s_down, a->dtype, a->y, a->ldy, stream);
 }
