@@ -142,12 +142,11 @@ struct RowsOut {
 #pragma unroll
     for (int j = 0; j < W; j++) v[j] = acc[j];
     if (drop.threshold) {
+      static_assert(W == 4 || W == 8);
+      const uint64_t e = (uint64_t)m * cols + n;
+      const uint32_t k = W == 8 ? kept8(drop, e) : kept4(drop, e);
 #pragma unroll
-      for (int j = 0; j < W; j += 4) {
-        const uint32_t k = kept4(drop, (uint64_t)m * cols + n + j);
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[j + i] = k >> i & 1 ? v[j + i] * drop.scale : 0.f;
-      }
+      for (int j = 0; j < W; j++) v[j] = k >> j & 1 ? v[j] * drop.scale : 0.f;
     }
     if (r) {
       float t[W];

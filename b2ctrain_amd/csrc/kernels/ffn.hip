@@ -1,8 +1,18 @@
 // The gated feed-forward block and its gradients (b2c_hip_ffn_forward, b2c_hip_ffn_backward).
-#include "dense_product.h"
+#include "ffn_head.h"
 
 namespace b2c {
 namespace dev {
+
+template <>
+int head_forward<f16>(const b2c_ffn_args*, const Drop&, hipStream_t);
+template <>
+int head_forward<bf16>(const b2c_ffn_args*, const Drop&, hipStream_t);
+template <>
+int head_backward<f16>(const b2c_ffn_grad_args*, const Drop&, hipStream_t);
+template <>
+int head_backward<bf16>(const b2c_ffn_grad_args*, const Drop&, hipStream_t);
+
 namespace {
 
 bool sizes_ok(const b2c_ffn_args* a, Drop* d) {
@@ -33,8 +43,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* x, int64_t ldx, int6
       if (n + j < cols) v[j] = p[j];
   }
   if (d.threshold) {
-    const uint64_t e = (uint64_t)m * cols + n;
-    const uint32_t keep = kept4(d, e) | kept4(d, e + 4) << 4;
+    const uint32_t keep = kept8(d, (uint64_t)m * cols + n);
 #pragma unroll
     for (int j = 0; j < 8; j++)
       if (!(keep >> j & 1)) v[j] = (T)0.f;
@@ -192,12 +201,14 @@ int backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream) {
 
 template <typename T>
 int forward(const b2c_ffn_args* a, const Drop& d, hipStream_t s) {
+  if (is_head(a)) return head_forward<T>(a, d, s);
   if (a->act == B2C_ACT_SILU) return forward<T, B2C_ACT_SILU>(a, d, s);
   if (a->act == B2C_ACT_GELU) return forward<T, B2C_ACT_GELU>(a, d, s);
   return forward<T, B2C_ACT_RELU>(a, d, s);
 }
 template <typename T>
 int backward(const b2c_ffn_grad_args* a, const Drop& d, hipStream_t s) {
+  if (is_head(&a->fwd)) return head_backward<T>(a, d, s);
   if (a->fwd.act == B2C_ACT_SILU) return backward<T, B2C_ACT_SILU>(a, d, s);
   if (a->fwd.act == B2C_ACT_GELU) return backward<T, B2C_ACT_GELU>(a, d, s);
   return backward<T, B2C_ACT_RELU>(a, d, s);
@@ -211,13 +222,14 @@ using namespace b2c::dev;
 
 extern "C" size_t b2c_ffn_saved_bytes(const b2c_ffn_args* a) {
   Drop d;
-  return sizes_ok(a, &d) ? (size_t)a->rows * 2 * up(a->d_hidden, 64) * 2 : 0;
+  return sizes_ok(a, &d) && !is_head(a) ? (size_t)a->rows * 2 * up(a->d_hidden, 64) * 2 : 0;
 }
 extern "C" size_t b2c_ffn_workspace_bytes(const b2c_ffn_args* a) {
   Drop d;
   if (!sizes_ok(a, &d) || a->rows == 0) return 0;
   Room room{nullptr};
-  ForwardPlan<bf16>(a, room);  // both types have the same size
+  if (is_head(a)) HeadPlan<bf16>(a, nullptr, room);  // both types have the same size
+  else ForwardPlan<bf16>(a, room);
   return room.used;
 }
 extern "C" int b2c_hip_ffn_forward(const b2c_ffn_args* a, hipStream_t stream) {
@@ -236,7 +248,8 @@ extern "C" size_t b2c_ffn_grad_workspace_bytes(const b2c_ffn_grad_args* b) {
   Drop d;
   if (!b || !sizes_ok(&b->fwd, &d)) return 0;
   Room room{nullptr};
-  BackwardPlan<bf16>(b, d, room);
+  if (is_head(&b->fwd)) HeadPlan<bf16>(&b->fwd, b, room);
+  else BackwardPlan<bf16>(b, d, room);
   return room.used;
 }
 extern "C" int b2c_hip_ffn_backward(const b2c_ffn_grad_args* b, hipStream_t stream) {
@@ -252,7 +265,8 @@ extern "C" int b2c_hip_ffn_backward(const b2c_ffn_grad_args* b, hipStream_t stre
   if (a->rows) {
     if (!good(a->x, a->ldx, a->d_in, 2) || !good(a->w_gate, a->ld_in, a->d_in, 2) || !good(a->w_up, a->ld_in, a->d_in, 2) ||
         !good(a->w_down, a->ld_out, a->d_hidden, 2) || !good(b->dy, b->lddy, a->d_out, 2) ||
-        (b->dx && !good(b->dx, b->lddx, a->d_in, 2)) || !a->saved || reinterpret_cast<uintptr_t>(a->saved) % 16)
+        (b->dx && !good(b->dx, b->lddx, a->d_in, 2)) || (!a->saved && !is_head(a)) ||
+        reinterpret_cast<uintptr_t>(a->saved) % 16)
       return hipErrorInvalidValue;
   }
   if (!room_ok(b->workspace, b->workspace_bytes, b2c_ffn_grad_workspace_bytes(b))) return hipErrorInvalidValue;

@@ -57,5 +57,20 @@ __device__ __forceinline__ uint32_t kept4(const Drop& d, uint64_t e) {
   return m >> o & 15u;
 }
 
+// The same of elements e .. e + 7, as eight bits.
+__device__ __forceinline__ uint32_t kept8(const Drop& d, uint64_t e) {
+  const int o = (int)(e & 7);
+  Philox4 w = philox(e >> 3, d.stream, d.seed);
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) m |= (uint32_t)kept(w, j, d.threshold) << j;
+  if (o) {
+    w = philox((e >> 3) + 1, d.stream, d.seed);
+#pragma unroll
+    for (int j = 0; j < 8; j++) m |= (uint32_t)kept(w, j, d.threshold) << (8 + j);
+  }
+  return m >> o & 255u;
+}
+
 }  // namespace dev
 }  // namespace b2c
