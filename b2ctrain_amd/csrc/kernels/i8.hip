@@ -1,48 +1,99 @@
 // Products in 8-bit integers with a scale for each row and each channel (b2c_hip_quantize_rows, b2c_hip_i8_linear,
 // b2c_hip_i8_ffn).
 #include "dense_product.h"
+#include "i8_head.h"
+#include "i8_quant.h"
 
 namespace b2c {
 namespace dev {
 namespace {
 
-// A row to a workgroup, in two passes over it: the largest magnitude, then the values. A row's columns from
-// cols to `pad` become 0.
-template <typename T>
-__global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t ldx, int64_t cols, int8_t* q, int64_t ldq,
-                                                       int64_t pad, float* scale) {
-  __shared__ float part[4];
-  const int64_t m = blockIdx.x;
-  const T* row = x + m * ldx;
-  float top = 0.f;
-  for (int64_t j = threadIdx.x; j < cols; j += 256) {
-    const float v = fabsf((float)row[j]);
-    top = v <= top ? top : v;  // a NaN stays in `top`: it is not <= anything
-    if (v != v) top = INFINITY;
-  }
+// THREADS threads to a row, sixteen values each at a time. What they read first they keep (up to HELD times sixteen), so that a
+// row is read once; the rest of a longer row is read again. A row's columns from cols to the next multiple of 16 become 0.
+template <typename T, int THREADS, int HELD>
+__global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q,
+                                                       int64_t ldq, float* scale) {
+  __shared__ uint32_t part[4];
+  const int t = threadIdx.x % THREADS;
+  const int64_t m = (int64_t)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
+  const bool there = m < rows;
+  const T* row = x + (there ? m : 0) * ldx;
+  auto load = [&](int64_t k) {
+    vec<T, 16> v{};
+    if (there && k + 16 <= cols) {
+      __builtin_memcpy(&v, row + k, sizeof(v));
+    } else if (there && k < cols) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-  const bool fine = top < INFINITY;
-  const float s = fine ? top / 127.f : NAN;
-  if (threadIdx.x == 0) scale[m] = s;
-  for (int64_t j = threadIdx.x; j < pad; j += 256) {
-    int v = 0;
-    if (j < cols && fine && s > 0.f) v = (int)rintf((float)row[j] / s);
-    q[m * ldq + j] = (int8_t)(v > 127 ? 127 : (v < -127 ? -127 : v));
+      for (int j = 0; j < 16; j++)
+        if (k + j < cols) v[j] = row[k + j];
+    }
+    return v;
+  };
+  uint32_t top = 0;
+  auto highest = [&](const vec<T, 16>& v) {
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      const uint32_t b = magnitude((float)v[j]);
+      top = b > top ? b : top;
+    }
+  };
+  vec<T, 16> held[HELD];
+#pragma unroll
+  for (int h = 0; h < HELD; h++) {
+    held[h] = load((int64_t)(h * THREADS + t) * 16);
+    highest(held[h]);
   }
+  for (int64_t k = (int64_t)(HELD * THREADS + t) * 16; k < cols; k += THREADS * 16) highest(load(k));
+#pragma unroll
+  for (int o = 1; o < THREADS && o < 64; o *= 2) {
+    const uint32_t b = __shfl_xor(top, o);
+    top = b > top ? b : top;
+  }
+  if constexpr (THREADS > 64) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; w++) top = part[w] > top ? part[w] : top;
+  }
+  const RowScale s(top);
+  if (there && t == 0) scale[m] = s.scale;
+  auto write = [&](int64_t k, const vec<T, 16>& v) {
+    if (!there || k >= cols) return;
+    vec<uint32_t, 4> b;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      b[j] = bytes4(s((float)v[4 * j]), s((float)v[4 * j + 1]), s((float)v[4 * j + 2]), s((float)v[4 * j + 3]));
+    int8_t* to = q + m * ldq + k;
+    if (k + 16 <= ldq) {
+      __builtin_memcpy(to, &b, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (k + j < ldq) to[j] = (int8_t)(b[j / 4] >> (j % 4 * 8));
+    }
+  };
+#pragma unroll
+  for (int h = 0; h < HELD; h++) write((int64_t)(h * THREADS + t) * 16, held[h]);
+  for (int64_t k = (int64_t)(HELD * THREADS + t) * 16; k < cols; k += THREADS * 16) write(k, load(k));
 }
 
+// Four lanes a row up to 128 columns, sixteen up to 1024, a wave or a workgroup beyond: whole rows in registers, and as few idle
+// lanes as that allows (four waves a row of 64 took 600 us for a million of them).
+template <typename T>
+int quantize(const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq, float* scale, hipStream_t stream) {
+  auto grid = [&](int threads) { return dim3((unsigned)(up(rows, 256 / threads) / (256 / threads))); };
+  constexpr int H = sizeof(T) == 4 ? 2 : 4;
+  if (cols <= 128) quantize_kernel<T, 4, 2><<<grid(4), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
+  else if (cols <= 1024) quantize_kernel<T, 16, H><<<grid(16), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
+  else if (cols <= 4096 && rows >= 2048) quantize_kernel<T, 64, H><<<grid(64), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
+  else quantize_kernel<T, 256, H><<<grid(256), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
+  return hipGetLastError();
+}
 int quantize(const void* x, int64_t ldx, int dtype, int64_t rows, int64_t cols, int8_t* q, int64_t ldq, float* scale,
              hipStream_t stream) {
-  const int64_t pad = ldq < (cols + 15) / 16 * 16 ? ldq : (cols + 15) / 16 * 16;
-  const dim3 grid((unsigned)rows);
-  if (dtype == B2C_F32) quantize_kernel<float><<<grid, 256, 0, stream>>>((const float*)x, ldx, cols, q, ldq, pad, scale);
-  else if (dtype == B2C_F16) quantize_kernel<f16><<<grid, 256, 0, stream>>>((const f16*)x, ldx, cols, q, ldq, pad, scale);
-  else quantize_kernel<bf16><<<grid, 256, 0, stream>>>((const bf16*)x, ldx, cols, q, ldq, pad, scale);
-  return hipGetLastError();
+  if (dtype == B2C_F32) return quantize((const float*)x, ldx, rows, cols, q, ldq, scale, stream);
+  if (dtype == B2C_F16) return quantize((const f16*)x, ldx, rows, cols, q, ldq, scale, stream);
+  return quantize((const bf16*)x, ldx, rows, cols, q, ldq, scale, stream);
 }
 
 bool type_ok(int t) { return t == B2C_F32 || t == B2C_F16 || t == B2C_BF16; }
@@ -199,6 +250,7 @@ extern "C" int b2c_hip_i8_linear(const b2c_i8_linear_args* a, hipStream_t stream
 
 extern "C" size_t b2c_i8_ffn_workspace_bytes(const b2c_i8_ffn_args* a) {
   if (!sizes_ok(a) || a->rows == 0) return 0;
+  if (is_i8_head(a)) return i8_head_bytes(a);
   Room room{nullptr};
   BlockPlan(a, room);
   return room.used;
@@ -211,6 +263,7 @@ extern "C" int b2c_hip_i8_ffn(const b2c_i8_ffn_args* a, hipStream_t stream) {
       !good(a->s_up, 1, 1, 4) || !good(a->s_down, 1, 1, 4) || !good(a->y, a->ldy, a->d_out, size_of(a->dtype)) ||
       !room_ok(a->workspace, a->workspace_bytes, b2c_i8_ffn_workspace_bytes(a)))
     return hipErrorInvalidValue;
+  if (is_i8_head(a)) return i8_head(a, stream);
   Room room{(char*)a->workspace};
   const BlockPlan p(a, room);
   int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.qx, p.kp, p.s, stream);

@@ -1,0 +1,190 @@
+// The 8-bit block where it is narrow (at most 128 wide, all weights in LDS) and its rows many: a trained head over the
+// splats of a scene, in one pass over x. A wave takes 16 rows from x to y: it quantises them, multiplies them by the
+// gate's and the up projection's weights from LDS, keeps the whole row of h in registers (its largest value is needed
+// before the first of them can be rounded), rounds it and multiplies it by the down weights. As in the 16-bit head, the rows
+// of the weights are dealt out so that a lane's accumulators are the next instruction's operand: hidden unit
+// 16 (l / 16) + 4 t + r of each 64 for accumulator r of tile t. Bound by the arithmetic on h, about 25 instructions a value.
+#include "i8_head.h"
+#include "i8_quant.h"
+
+namespace b2c {
+namespace dev {
+namespace {
+
+constexpr int head_fragments(int ki) { return 12 * ki; }  // of 64 hidden units: g (t, k), u (t, k), down (o tile)
+
+template <int KI>
+__global__ __launch_bounds__(256) void fragments_kernel(b2c_i8_ffn_args a, int chunks, int8_t* out) {
+  const int t = blockIdx.x * 256 + threadIdx.x, lane = t & 63, i = lane & 15, q = lane >> 4, all = t >> 6;
+  const int c = all / head_fragments(KI), f = all % head_fragments(KI);
+  if (c >= chunks) return;
+  vec<int8_t, 16> v{};
+  if (f < 8 * KI) {
+    const int8_t* w = f < 4 * KI ? a.w_gate : a.w_up;
+    const int tile = f % (4 * KI) / KI, h = c * 64 + (i >> 2) * 16 + tile * 4 + (i & 3), k = f % KI * 64 + q * 16;
+    if (h < a.d_hidden)
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (k + j < a.d_in) v[j] = w[h * a.ld_in + k + j];
+  } else {
+    const int o = (i >> 2) * (16 * KI) + (f - 8 * KI) * 4 + (i & 3), k = c * 64 + q * 16;
+    if (o < a.d_out)
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (k + j < a.d_hidden) v[j] = a.w_down[o * a.ld_out + k + j];
+  }
+  *reinterpret_cast<vec<int8_t, 16>*>(out + (int64_t)t * 16) = v;
+}
+
+// Sixteen values of row m from column k on, as floats; zeros beyond the ends.
+template <typename T>
+__device__ __forceinline__ void sixteen(const void* x, int64_t ld, int64_t m, int64_t M, int k, int K, float (&v)[16]) {
+  const T* p = (const T*)x + m * ld + k;
+  if (m < M && k + 16 <= K) {
+    vec<T, 16> t;
+    __builtin_memcpy(&t, p, sizeof(t));
+#pragma unroll
+    for (int j = 0; j < 16; j++) v[j] = (float)t[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; j++) v[j] = m < M && k + j < K ? (float)p[j] : 0.f;
+  }
+}
+
+__device__ __forceinline__ uint32_t over_row(uint32_t top) {  // of the four lanes that share a row
+  const uint32_t a = __shfl_xor(top, 16), b = top > a ? top : a, c = __shfl_xor(b, 32);
+  return b > c ? b : c;
+}
+
+template <int ACT, int KI, int NC>
+__global__ __launch_bounds__(512) void head_kernel(b2c_i8_ffn_args a, const int8_t* frags, int chunks) {
+  constexpr int N = head_fragments(KI), OT = 4 * KI;
+  using A = vec<int8_t, 16>;
+  __shared__ A w[NC * N][64];
+  __shared__ f32x4 sg[NC * 16], su[NC * 16], sd[KI * 16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q4 = lane >> 4;
+  for (int f = wave; f < NC * N; f += 8) w[f][lane] = f < chunks * N ? *reinterpret_cast<const A*>(frags + ((int64_t)f * 64 + lane) * 16) : A{};
+  for (int j = threadIdx.x; j < NC * 64; j += 512) {
+    ((float*)sg)[j] = j < a.d_hidden ? a.s_gate[j] : 0.f;
+    ((float*)su)[j] = j < a.d_hidden ? a.s_up[j] : 0.f;
+    if (j < KI * 64) ((float*)sd)[j] = j < a.d_out ? a.s_down[j] : 0.f;
+  }
+  if (NC < KI)
+    for (int j = NC * 64 + threadIdx.x; j < KI * 64; j += 512) ((float*)sd)[j] = j < a.d_out ? a.s_down[j] : 0.f;
+  __syncthreads();
+  const int64_t M = a.rows, tiles = (M + 15) / 16;
+  for (int64_t tile = (int64_t)blockIdx.x * 8 + wave; tile < tiles; tile += (int64_t)gridDim.x * 8) {
+    const int64_t m = tile * 16 + (lane & 15);
+    float x[KI][16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < KI; k++) {
+      if (a.dtype == B2C_BF16) sixteen<bf16>(a.x, a.ldx, m, M, k * 64 + q4 * 16, a.d_in, x[k]);
+      else if (a.dtype == B2C_F16) sixteen<f16>(a.x, a.ldx, m, M, k * 64 + q4 * 16, a.d_in, x[k]);
+      else sixteen<float>(a.x, a.ldx, m, M, k * 64 + q4 * 16, a.d_in, x[k]);
+#pragma unroll
+      for (int j = 0; j < 16; j++) top = magnitude(x[k][j]) > top ? magnitude(x[k][j]) : top;
+    }
+    const RowScale rx(over_row(top));
+    i32x4 qx[KI];
+#pragma unroll
+    for (int k = 0; k < KI; k++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) qx[k][j] = (int)bytes4(rx(x[k][4 * j]), rx(x[k][4 * j + 1]), rx(x[k][4 * j + 2]), rx(x[k][4 * j + 3]));
+
+    float h[NC][16];
+    top = 0;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      asm volatile("" ::: "memory");  // the weights stay in LDS: held over the loop, they would fill the registers
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        i32x4 g = {}, u = {};
+#pragma unroll
+        for (int k = 0; k < KI; k++) {
+          g = mfma(w[c * N + t * KI + k][lane], __builtin_bit_cast(A, qx[k]), g);
+          u = mfma(w[c * N + (4 + t) * KI + k][lane], __builtin_bit_cast(A, qx[k]), u);
+        }
+        const f32x4 a4 = sg[c * 16 + q4 * 4 + t], b4 = su[c * 16 + q4 * 4 + t];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float v = act<ACT>((float)g[r] * rx.scale * a4[r]) * ((float)u[r] * rx.scale * b4[r]);
+          h[c][t * 4 + r] = v;
+          top = magnitude(v) > top ? magnitude(v) : top;
+        }
+      }
+    }
+    const RowScale rh(over_row(top));
+    i32x4 y[OT] = {};
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      asm volatile("" ::: "memory");
+      i32x4 qh;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        uint32_t b[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) b[r] = rh(h[c][4 * j + r]);
+        qh[j] = (int)bytes4(b[0], b[1], b[2], b[3]);
+      }
+#pragma unroll
+      for (int t = 0; t < OT; t++) y[t] = mfma(w[c * N + 8 * KI + t][lane], __builtin_bit_cast(A, qh), y[t]);
+    }
+    if (m >= M) continue;
+#pragma unroll
+    for (int t = 0; t < OT; t += 2) {
+      const int n = q4 * (16 * KI) + t * 4;
+      if (n >= a.d_out) continue;
+      const f32x4 a4 = sd[n / 4], b4 = sd[n / 4 + 1];
+      float v[8];
+#pragma unroll
+      for (int r = 0; r < 4; r++) v[r] = (float)y[t][r] * rh.scale * a4[r], v[4 + r] = (float)y[t + 1][r] * rh.scale * b4[r];
+      if (a.dtype == B2C_BF16) put<8>((bf16*)a.y, a.ldy, m, n, a.d_out, v);
+      else if (a.dtype == B2C_F16) put<8>((f16*)a.y, a.ldy, m, n, a.d_out, v);
+      else put<8>((float*)a.y, a.ldy, m, n, a.d_out, v);
+    }
+  }
+}
+
+int chunks_of(const b2c_i8_ffn_args* a) { return (int)up(a->d_hidden, 64) / 64; }
+int width_of(const b2c_i8_ffn_args* a) { return std::max(a->d_in, a->d_out) <= 64 ? 1 : 2; }
+
+template <int ACT, int KI, int NC>
+int launch(const b2c_i8_ffn_args* a, const int8_t* frags, hipStream_t stream) {
+  const int64_t groups = up(a->rows, 128) / 128;
+  const int held = NC * KI <= 4 ? 2 : 1;  // workgroups that a compute unit holds, by LDS and registers
+  head_kernel<ACT, KI, NC><<<dim3((unsigned)std::min<int64_t>(groups, 256 * held)), 512, 0, stream>>>(*a, frags, chunks_of(a));
+  return hipGetLastError();
+}
+template <int ACT, int KI>
+int launch(const b2c_i8_ffn_args* a, const int8_t* frags, hipStream_t stream) {
+  const int c = chunks_of(a);
+  if (c <= 2) return launch<ACT, KI, 2>(a, frags, stream);
+  if (c <= 4) return launch<ACT, KI, 4>(a, frags, stream);
+  if (KI == 2 || c <= 6) return launch<ACT, KI, 6>(a, frags, stream);
+  if constexpr (KI == 1) return launch<ACT, 1, 8>(a, frags, stream);
+  return hipErrorInvalidValue;
+}
+template <int KI>
+int run(const b2c_i8_ffn_args* a, int8_t* frags, hipStream_t stream) {
+  const int n = chunks_of(a) * head_fragments(KI);
+  fragments_kernel<KI><<<dim3((unsigned)up(n, 4) / 4), 256, 0, stream>>>(*a, chunks_of(a), frags);
+  const int rc = hipGetLastError();
+  if (rc) return rc;
+  if (a->act == B2C_ACT_SILU) return launch<B2C_ACT_SILU, KI>(a, frags, stream);
+  if (a->act == B2C_ACT_GELU) return launch<B2C_ACT_GELU, KI>(a, frags, stream);
+  return launch<B2C_ACT_RELU, KI>(a, frags, stream);
+}
+
+}  // namespace
+
+bool is_i8_head(const b2c_i8_ffn_args* a) {
+  return a->rows > kI8HeadRows && a->d_in <= 128 && a->d_out <= 128 && chunks_of(a) <= (width_of(a) == 1 ? 8 : 6);
+}
+size_t i8_head_bytes(const b2c_i8_ffn_args* a) { return (size_t)chunks_of(a) * head_fragments(width_of(a)) * 1024; }
+int i8_head(const b2c_i8_ffn_args* a, hipStream_t stream) {
+  return width_of(a) == 1 ? run<1>(a, (int8_t*)a->workspace, stream) : run<2>(a, (int8_t*)a->workspace, stream);
+}
+
+}  // namespace dev
+}  // namespace b2c
