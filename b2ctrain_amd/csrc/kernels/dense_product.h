@@ -68,7 +68,7 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Product<T> a, Epi epi) {
   Acc acc[PL][MT] = {};
   auto load = [&](const Side<T>& s, int64_t i, bool there, int k) {
     A v{};
-    if (!there) return v;
+    if (!there || k >= K) return v;
     const T* p = s.p + i * s.ld + k;
     if (k + V <= K) {
       __builtin_memcpy(&v, p, 16);
@@ -78,22 +78,31 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Product<T> a, Epi epi) {
     }
     return v;
   };
-  for (int k0 = wave * RUN; k0 < K; k0 += 8 * RUN) {
-    A p[PL][4], x[MT][4];
+  A p[2][PL][4], x[2][MT][4];
+  auto fetch = [&](int b, int k0) {  // the run from k0 on; beyond K it is zeros and reads nothing
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       const int k = k0 + (c * 4 + q4) * V;
-      p[0][c] = load(a.p, n, n < a.p_lim, k);
-      if constexpr (DUAL) p[1][c] = load(a.p2, n, n < a.p_lim, k);
+      p[b][0][c] = load(a.p, n, n < a.p_lim, k);
+      if constexpr (DUAL) p[b][1][c] = load(a.p2, n, n < a.p_lim, k);
 #pragma unroll
-      for (int i = 0; i < MT; i++) x[i][c] = load(a.q, i * 16 + row, i * 16 + row < a.M, k);
+      for (int i = 0; i < MT; i++) x[b][i][c] = load(a.q, i * 16 + row, i * 16 + row < a.M, k);
     }
+  };
+  auto multiply = [&](int b) {
 #pragma unroll
     for (int c = 0; c < 4; c++)
 #pragma unroll
       for (int i = 0; i < MT; i++)
 #pragma unroll
-        for (int d = 0; d < PL; d++) acc[d][i] = mfma(p[d][c], x[i][c], acc[d][i]);
+        for (int d = 0; d < PL; d++) acc[d][i] = mfma(p[b][d][c], x[b][i][c], acc[d][i]);
+  };
+  fetch(0, wave * RUN);
+  for (int k0 = wave * RUN; k0 < K; k0 += 16 * RUN) {  // a run ahead of the one at work
+    fetch(1, k0 + 8 * RUN);
+    multiply(0);
+    fetch(0, k0 + 16 * RUN);
+    multiply(1);
   }
 #pragma unroll
   for (int d = 0; d < PL; d++)
@@ -130,13 +139,16 @@ struct Way {
   size_t sums;  // bytes of workspace for the parts
 };
 
-// What a product of these sizes costs by each tile, in microseconds, from the measured time of a step of 128 bytes of k:
-// a compute unit holds one 256x256 tile (1.65 us a step), two of 128x128 (0.51 each side by side, 0.9 alone) or five of
-// 64x64 (0.19, 0.58): a large tile reads less, small ones keep more compute units at work when there are few. Where
-// even those do not fill the device, k is split, for a write and a read of the sums.
+// What a product of these sizes costs by each tile, in microseconds, from measured times: a step of 128 bytes of k takes a
+// compute unit 1.58 us for a 256x256 tile, 0.51 each for two of 128x128 side by side (0.82 for one alone), 0.2 each for five of 64x64
+// (0.51 alone), beside a launch, a first copy and an epilogue of 6, 3.7 and 2.9. A large tile reads less, small ones keep
+// more compute units at work when there are few: 4096 x 4096 x 4096 takes 106, 133 and 210 us, 1037 x 2752 x 1000 takes 28, 14
+// and 14, 512 x 512 x 512 takes 16, 7 and 5. Where even the small ones leave the device idle, k is split, for a write and a
+// read of the sums.
 inline Way choose(int64_t M, int64_t N, int64_t steps, bool dual, bool may_be_few) {
   if (may_be_few && M <= kFewRows) return {FEW_ROWS, 1, 0};
-  static const struct { int side; double wide, alone; int held; } tiles[3] = {{256, 1.65, 1.65, 1}, {128, 0.51, 0.9, 2}, {64, 0.19, 0.58, 5}};
+  static const struct { int side; double wide, alone, fixed; int held; } tiles[3] = {
+      {256, 1.58, 1.45, 6.0, 1}, {128, 0.51, 0.82, 3.7, 2}, {64, 0.2, 0.51, 2.9, 5}};
   Way best{TILE_64, 1, 0};
   double least = 1e30;
   const int64_t ld = up(N, 8);
@@ -148,7 +160,7 @@ inline Way choose(int64_t M, int64_t N, int64_t steps, bool dual, bool may_be_fe
       if (parts > 1 && (steps / parts < 4 || sums > 256e6)) break;
       const int64_t all = count * parts;
       const double step = std::max(tiles[t].wide * (double)up(all, 256) / 256, tiles[t].alone * (double)up(all, 256 * tiles[t].held) / (256 * tiles[t].held));
-      const double us = step * ((double)steps / parts + 4) + (parts > 1 ? 4 + 2 * sums / 3.5e6 : 0);
+      const double us = tiles[t].fixed + step * std::max(1.0, (double)steps / parts) + (parts > 1 ? 4 + 2 * sums / 3.5e6 : 0);
       if (us < least) least = us, best = {t, parts, parts > 1 ? (size_t)sums : 0};
     }
   }
@@ -164,7 +176,7 @@ int launch_tiles(const Product<T>& a, int parts, const Epi& epi, hipStream_t str
   if constexpr (SIDE == 256)
     tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 128, 64><<<grid, 512, 0, stream>>>(a, (int)tm, (int)tn, parts, epi);
   else if constexpr (SIDE == 128)
-    tile_kernel<T, PT, QT, DUAL, TWO, 2, 2, 64, 64><<<grid, 256, 0, stream>>>(a, (int)tm, (int)tn, parts, epi);
+    tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 64, 32><<<grid, 512, 0, stream>>>(a, (int)tm, (int)tn, parts, epi);
   else
     tile_kernel<T, PT, QT, DUAL, TWO, 2, 2, 32, 32><<<grid, 256, 0, stream>>>(a, (int)tm, (int)tn, parts, epi);
   return hipGetLastError();

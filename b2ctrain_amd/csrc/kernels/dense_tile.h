@@ -6,7 +6,6 @@
 // so any rearrangement is done on the side of the addresses it reads:
 //   - rows along k ("plain" operand, element (i, k) at p[i ld + k]): row i's eight pieces are stored at
 //     (piece ^ i & 7), so that the sixteen rows that a matrix instruction's lanes read lie in different banks;
-//     rows of P are permuted so that a lane ends up with 4 x (tiles of its wave) neighbouring columns of out;
 //   - rows along i ("transposed", element (i, k) at p[k ld + i]): stored as they are, the pieces of row k at
 //     (piece ^ 2 key(k)), and read with the transposing LDS load, which hands lane l of each sixteen the four
 //     values that column l has in four rows.
@@ -128,7 +127,7 @@ template <typename T, bool PT, bool QT, bool DUAL, bool TWO, int WAVES_M, int WA
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Product<T> a, int tiles_m, int tiles_n, int parts,
                                                                      Epi epi) {
   constexpr int THREADS = WAVES_M * WAVES_N * 64, BM = WAVES_M * WM, BN = WAVES_N * WN;
-  constexpr bool AHEAD = THREADS == 512;
+  constexpr bool AHEAD = WAVES_M * WAVES_N == 8;
   constexpr int MT = WM / 16, NT = WN / 16, COLS = DUAL ? BN / 2 : BN;  // columns of out in a tile
   using Acc = typename Elem<T>::Acc;
   using TQ = Tile<T, BM, THREADS, QT>;
@@ -151,10 +150,9 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Product<T> 
   TQ cq;
   TP cp;
   auto q_row = [](uint32_t r) { return r; };
-  auto p_row = [](uint32_t r) {  // LDS row t 16 + q 4 + r of a wave's block holds column q (4 tiles) + 4 t + r
-    const uint32_t b = r / WN, t = r % WN / 16, q = r % 16 / 4, x = r % 4;
-    if constexpr (DUAL) return b * (WN / 2) + q * (2 * NT) + t % (NT / 2) * 4 + x;
-    else return b * WN + q * (4 * NT) + t * 4 + x;
+  auto p_row = [](uint32_t r) {  // DUAL: a wave's block of rows is half gate, half up
+    if constexpr (DUAL) return r / WN * (WN / 2) + r % (WN / 2);
+    else return r;
   };
   const T *pq = nullptr, *pp = nullptr, *pu = nullptr;
   int left = 0;
@@ -209,7 +207,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Product<T> 
   using F = vec<T, TQ::V>;
   F q0[MT], p0[NT], q1[MT], p1[NT];
   auto read = [&](int s, int kk, F(&q)[MT], F(&p)[NT]) {
-    const char* at = lds + (s & 1) * STEP;
+    const char* at = lds + (uint32_t)(s & 1) * STEP;
 #pragma unroll
     for (int t = 0; t < NT; t++) p[t] = fp.get(at + TQ::BYTES, t, kk);
 #pragma unroll
@@ -249,12 +247,12 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Product<T> 
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // A step in two halves of k. While one half is multiplied the next is read into registers, across the steps too:
-  // the barrier stands between the halves, where nothing of the current buffer is left to read, so the copies of
-  // the step after next can start there, and have a whole step's time to land.
+  if (steps) TWO && begin >= steps1 ? enter(1, begin - steps1) : enter(0, begin);
   if constexpr (AHEAD) {
+    // A step in two halves of k. While one half is multiplied the next is read into registers, across the steps too: the
+    // barrier stands between the halves, where nothing of the current buffer is left to read, so the copies of the step
+    // after next can start there, and have a whole step's time to land.
     if (steps) {
-      TWO && begin >= steps1 ? enter(1, begin - steps1) : enter(0, begin);
       start(0);
       landed();
       start(1);
@@ -267,53 +265,48 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Product<T> 
       half(q1, p1, q0, p0, lds + ((s + 1) & 1) * STEP, 0, std::true_type{}, s + 2);
       advance(s + 2);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup
   } else {
-    if (steps) {
-      TWO && begin >= steps1 ? enter(1, begin - steps1) : enter(0, begin);
-      start(0);
-    }
+    // Small tiles: five workgroups a compute unit fill each other's waits. (More than one step on its way gains nothing:
+    // 25 us with one, two or three of them for 1037 x 1000 x 2744.)
+    if (steps) start(0);
     for (int s = 0; s < steps; s++) {
       landed();
-      if (s + 1 < steps) start(s + 1);
+      start(s + 1);
       read(s, 0, q0, p0);
       multiply(q0, p0);
       read(s, 1, q1, p1);
       multiply(q1, p1);
     }
   }
+  landed();  // no copy may outlive the workgroup, and everybody's reads are done
 
+  // The epilogue's values pass through LDS, 16 rows of a wave at a time, so that it gets eight neighbouring columns a lane and
+  // eight lanes a row: whole lines where it reads and writes. A wave has its own piece of LDS and waits for nobody.
   using S = std::remove_reference_t<decltype(acc[0][0][0])>;
+  constexpr int PITCH = WN + 4;  // values between rows: sixteen rows' pieces in different banks
+  constexpr int LANES = (DUAL ? WN / 2 : WN) / 8, ROWS = 64 / LANES;
+  static_assert(sizeof(S) * PITCH * 16 * WAVES_M * WAVES_N <= 2 * STEP && ROWS * LANES == 64);
+  S* turn = reinterpret_cast<S*>(lds) + wave * (16 * PITCH);
   const int lq = lane >> 4;
 #pragma unroll
   for (int i = 0; i < MT; i++) {
-    const int64_t m = m0 + wm + i * 16 + (lane & 15);
-    if (m >= a.M) continue;
-    if constexpr (DUAL) {
-      constexpr int W = 2 * NT;
-      const int64_t n = n0 + wb * (WN / 2) + lq * W;
-      S g[W], u[W];
 #pragma unroll
-      for (int j = 0; j < W; j++) g[j] = acc[j / 4][i][j % 4], u[j] = acc[NT / 2 + j / 4][i][j % 4];
-      if (n < a.N) epi.template operator()<W>(part, m, (int)n, g, u);
-    } else if constexpr (!PT) {
-      constexpr int W = NT >= 2 ? 8 : 4;
+    for (int t = 0; t < NT; t++) *reinterpret_cast<Acc*>(turn + (lane & 15) * PITCH + t * 16 + lq * 4) = acc[t][i];
 #pragma unroll
-      for (int h = 0; h < 4 * NT / W; h++) {
-        const int64_t n = n0 + wn + lq * 4 * NT + h * W;
-        S v[W];
+    for (int h = 0; h < 16; h += ROWS) {
+      const int row = h + lane / LANES, col = lane % LANES * 8;
+      const int64_t m = m0 + wm + i * 16 + row;
+      if (row >= 16 || m >= a.M) continue;
+      const S* v = turn + row * PITCH + col;
+      S g[8], u[8];
 #pragma unroll
-        for (int j = 0; j < W; j++) v[j] = acc[h * (W / 4) + j / 4][i][j % 4];
-        if (n < a.N) epi.template operator()<W>(part, m, (int)n, v);
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        const int64_t n = n0 + wn + t * 16 + lq * 4;
-        S v[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = acc[t][i][j];
-        if (n < a.N) epi.template operator()<4>(part, m, (int)n, v);
+      for (int j = 0; j < 8; j++) g[j] = v[j], u[j] = DUAL ? v[WN / 2 + j] : S(0);
+      if constexpr (DUAL) {
+        const int64_t n = n0 + wb * (WN / 2) + col;
+        if (n < a.N) epi.template operator()<8>(part, m, (int)n, g, u);
+      } else {
+        const int64_t n = n0 + wn + col;
+        if (n < a.N) epi.template operator()<8>(part, m, (int)n, g);
       }
     }
   }
