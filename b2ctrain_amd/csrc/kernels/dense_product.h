@@ -3,51 +3,59 @@
 #pragma once
 #include "dense_tile.h"
 
+#include <initializer_list>
+
 namespace b2c {
 namespace dev {
 
 // ---- a long k in parts -------------------------------------------------------------------------------------
 
-// Sums of a part of k, kept whole: value (part, plane, m, n) at ((part planes + plane) M + m) ld + n.
-template <typename S>
+// Sums of parts of k, tile by tile: value (plane, m, n) of workgroup w at ((w planes + plane) rows + m % rows) cols + n % cols,
+// in single precision, or in integers, which stay exact.
+template <typename S, int ROWS, int COLS, int PLANES>
 struct Parts {
   S* sums;
-  int64_t M, ld;
-  int planes;
+  __device__ __forceinline__ S* at(uint32_t w, int plane, int64_t m, int n) const {
+    return sums + (((int64_t)w * PLANES + plane) * ROWS + m % ROWS) * COLS + n % COLS;
+  }
   template <int W>
-  __device__ __forceinline__ void store(int64_t plane, int64_t m, int n, const S (&v)[W]) const {
+  __device__ __forceinline__ void store(S* to, const S (&v)[W]) const {
     vec<S, W> t;
 #pragma unroll
     for (int j = 0; j < W; j++) t[j] = v[j];
-    *reinterpret_cast<vec<S, W>*>(sums + (plane * M + m) * ld + n) = t;
+    *reinterpret_cast<vec<S, W>*>(to) = t;
   }
   template <int W>
-  __device__ __forceinline__ void operator()(uint32_t part, int64_t m, int n, const S (&v)[W]) const {
-    store<W>((int64_t)part * planes, m, n, v);
+  __device__ __forceinline__ void operator()(uint32_t w, int64_t m, int n, const S (&v)[W]) const {
+    store<W>(at(w, 0, m, n), v);
   }
   template <int W>
-  __device__ __forceinline__ void operator()(uint32_t part, int64_t m, int n, const S (&g)[W], const S (&u)[W]) const {
-    store<W>((int64_t)part * planes, m, n, g);
-    store<W>((int64_t)part * planes + 1, m, n, u);
+  __device__ __forceinline__ void operator()(uint32_t w, int64_t m, int n, const S (&g)[W], const S (&u)[W]) const {
+    store<W>(at(w, 0, m, n), g);
+    store<W>(at(w, 1, m, n), u);
   }
 };
 
 // Adds the parts in their order and finishes them with the product's epilogue, eight columns a thread.
-template <typename S, bool DUAL, typename Epi>
-__global__ __launch_bounds__(256) void join_kernel(Parts<S> p, int64_t M, uint32_t groups, int N, int parts, Epi epi) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, m = t / groups;
-  if (m >= M) return;
-  const int n = (int)(t - m * groups) * 8;
-  S v[DUAL ? 2 : 1][8] = {};
+template <typename T, bool DUAL, int ROWS, int COLS, typename S, typename Epi, int NJ>
+__global__ __launch_bounds__(256) void join_kernel(Jobs<T, Epi, NJ> jobs, uint32_t first, uint32_t count, int parts, S* sums) {
+  constexpr int PL = DUAL ? 2 : 1, BLOCKS = ROWS * COLS / 2048;
+  const Parts<S, ROWS, COLS, PL> p{sums};
+  const uint32_t slot = blockIdx.x / BLOCKS, v0 = (blockIdx.x % BLOCKS * 256 + threadIdx.x) * 8;
+  uint32_t tm, tn;
+  const int job = find<Jobs<T, Epi, NJ>, NJ>(jobs, first + tile_of(slot, count), tm, tn);
+  const int64_t m = (int64_t)tm * ROWS + v0 / COLS, n = (int64_t)tn * COLS + v0 % COLS;
+  if (m >= jobs.product[job].M || n >= jobs.product[job].N) return;
+  S v[PL][8] = {};
   for (int part = 0; part < parts; part++)
 #pragma unroll
-    for (int d = 0; d < (DUAL ? 2 : 1); d++) {
-      const S* from = p.sums + (((int64_t)part * p.planes + d) * p.M + m) * p.ld + n;
+    for (int d = 0; d < PL; d++) {
+      const vec<S, 8> t = *reinterpret_cast<const vec<S, 8>*>(p.at(part * count + slot, d, m, (int)n));
 #pragma unroll
-      for (int j = 0; j < 8; j++) v[d][j] += from[j];
+      for (int j = 0; j < 8; j++) v[d][j] += t[j];
     }
-  if constexpr (DUAL) epi.template operator()<8>(0u, m, n, v[0], v[1]);
-  else epi.template operator()<8>(0u, m, n, v[0]);
+  if constexpr (DUAL) jobs.epi[job].template operator()<8>(0u, m, (int)n, v[0], v[1]);
+  else jobs.epi[job].template operator()<8>(0u, m, (int)n, v[0]);
 }
 
 // ---- a few rows --------------------------------------------------------------------------------------------
@@ -133,83 +141,113 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Product<T> a, Epi epi) {
 enum { TILE_256, TILE_128, TILE_64, FEW_ROWS };
 constexpr int64_t kFewRows = 32;
 
+// Tiles of one size; the first `whole` of them each by one workgroup, the rest by `parts`, through `sums` bytes of workspace.
 struct Way {
   int tile;
+  int64_t whole, rest;
   int parts;
-  size_t sums;  // bytes of workspace for the parts
+  size_t sums;
+};
+struct Extent {
+  int64_t M, N;
 };
 
-// What a product of these sizes costs by each tile, in microseconds, from measured times: a step of 128 bytes of k takes a
-// compute unit 1.58 us for a 256x256 tile, 0.51 each for two of 128x128 side by side (0.82 for one alone), 0.2 each for five of 64x64
-// (0.51 alone), beside a launch, a first copy and an epilogue of 6, 3.7 and 2.9. A large tile reads less, small ones keep
-// more compute units at work when there are few: 4096 x 4096 x 4096 takes 106, 133 and 210 us, 1037 x 2752 x 1000 takes 28, 14
-// and 14, 512 x 512 x 512 takes 16, 7 and 5. Where even the small ones leave the device idle, k is split, for a write and a
-// read of the sums.
-inline Way choose(int64_t M, int64_t N, int64_t steps, bool dual, bool may_be_few) {
-  if (may_be_few && M <= kFewRows) return {FEW_ROWS, 1, 0};
+// What a product of these sizes costs by each tile, in microseconds, from times measured warm: a step of 128 bytes of k takes
+// a compute unit 1.43 us for a 256x256 tile when all are busy (1.1 alone), 0.46 each for two of 128x128 side by side (0.63
+// alone), 0.18 each for five of 64x64 (0.45 alone), beside a launch, a first copy and an epilogue of 5.9, 3.8 and 3.6. A large
+// tile reads less, small ones keep more compute units at work when there are few: 4096 x 4096 x 4096 takes 100, 125 and 191 us,
+// 1037 x 2752 x 1000 takes 27, 14 and 13. Tiles beyond the last full round of compute units, or all where there are too few,
+// may be split over k, for a write and a read of their sums.
+inline Way choose(std::initializer_list<Extent> jobs, int64_t steps, bool dual, bool may_be_few) {
+  if (may_be_few && jobs.begin()->M <= kFewRows) return {FEW_ROWS, 0, 0, 1, 0};
   static const struct { int side; double wide, alone, fixed; int held; } tiles[3] = {
-      {256, 1.58, 1.45, 6.0, 1}, {128, 0.51, 0.82, 3.7, 2}, {64, 0.2, 0.51, 2.9, 5}};
-  Way best{TILE_64, 1, 0};
+      {256, 1.43, 1.1, 5.9, 1}, {128, 0.46, 0.63, 3.8, 2}, {64, 0.18, 0.45, 3.6, 5}};
+  Way best{TILE_64, 0, 0, 1, 0};
   double least = 1e30;
-  const int64_t ld = up(N, 8);
   for (int t = 0; t < 3; t++) {
-    const int64_t cols = dual ? tiles[t].side / 2 : tiles[t].side;
-    const int64_t count = up(M, tiles[t].side) / tiles[t].side * (up(N, cols) / cols);
-    for (int parts = 1; parts <= 64; parts *= 2) {
-      const double sums = 4.0 * parts * (dual ? 2 : 1) * M * ld;
-      if (parts > 1 && (steps / parts < 4 || sums > 256e6)) break;
-      const int64_t all = count * parts;
-      const double step = std::max(tiles[t].wide * (double)up(all, 256) / 256, tiles[t].alone * (double)up(all, 256 * tiles[t].held) / (256 * tiles[t].held));
-      const double us = tiles[t].fixed + step * std::max(1.0, (double)steps / parts) + (parts > 1 ? 4 + 2 * sums / 3.5e6 : 0);
-      if (us < least) least = us, best = {t, parts, parts > 1 ? (size_t)sums : 0};
+    const auto& k = tiles[t];
+    const int64_t cols = dual ? k.side / 2 : k.side;
+    int64_t count = 0;
+    for (const Extent& e : jobs) count += up(e.M, k.side) / k.side * (up(e.N, cols) / cols);
+    auto time = [&](int64_t n, double st) {
+      return std::max(k.wide * (double)(up(n, 256) / 256), k.alone * (double)(up(n, 256 * k.held) / (256 * k.held))) * st;
+    };
+    const double all = k.fixed + time(count, (double)std::max<int64_t>(steps, 1));
+    if (all < least) least = all, best = {t, count, 0, 1, 0};
+    for (const int64_t whole : {(int64_t)0, count / 256 * 256, count / (256 * k.held) * (256 * k.held)}) {
+      const int64_t rest = count - whole;
+      for (int parts = 2; parts <= 64 && rest > 0; parts++) {
+        const double sums = 4.0 * parts * (double)rest * k.side * k.side;
+        if (steps / parts < 4 || sums > 256e6) break;
+        const double us = (whole ? k.fixed + time(whole, (double)steps) : 0) + k.fixed + time(rest * parts, (double)steps / parts) + 4 + 2 * sums / 3.5e6;
+        if (us < least) least = us, best = {t, whole, rest, parts, (size_t)sums};
+      }
     }
   }
   return best;
 }
 
-template <typename T, bool PT, bool QT, bool DUAL, bool TWO, int SIDE, typename Epi>
-int launch_tiles(const Product<T>& a, int parts, const Epi& epi, hipStream_t stream) {
-  constexpr int COLS = DUAL ? SIDE / 2 : SIDE;
-  const int64_t tm = up(a.M, SIDE) / SIDE, tn = up(a.N, COLS) / COLS;
-  if (tm * tn * parts > 0x7fffffff) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)(tm * tn * parts));
+template <typename T, bool PT, bool QT, bool DUAL, bool TWO, int SIDE, typename Epi, int NJ>
+int launch_tiles(const Jobs<T, Epi, NJ>& jobs, int64_t first, int64_t count, int parts, hipStream_t stream) {
+  if (count <= 0) return hipSuccess;
+  if (count * parts > 0x7fffffff) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)(count * parts));
   if constexpr (SIDE == 256)
-    tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 128, 64><<<grid, 512, 0, stream>>>(a, (int)tm, (int)tn, parts, epi);
+    tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 128, 64><<<grid, 512, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
   else if constexpr (SIDE == 128)
-    tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 64, 32><<<grid, 512, 0, stream>>>(a, (int)tm, (int)tn, parts, epi);
+    tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 64, 32><<<grid, 512, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
   else
-    tile_kernel<T, PT, QT, DUAL, TWO, 2, 2, 32, 32><<<grid, 256, 0, stream>>>(a, (int)tm, (int)tn, parts, epi);
+    tile_kernel<T, PT, QT, DUAL, TWO, 2, 2, 32, 32><<<grid, 256, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
   return hipGetLastError();
 }
 
-template <typename T, bool PT, bool QT, bool DUAL, bool TWO, typename Epi>
-int tiles(const Product<T>& a, int tile, int parts, const Epi& epi, hipStream_t stream) {
-  if (tile == TILE_256) return launch_tiles<T, PT, QT, DUAL, TWO, 256>(a, parts, epi, stream);
-  if (tile == TILE_128) return launch_tiles<T, PT, QT, DUAL, TWO, 128>(a, parts, epi, stream);
-  return launch_tiles<T, PT, QT, DUAL, TWO, 64>(a, parts, epi, stream);
+template <typename T, bool PT, bool QT, bool DUAL, bool TWO, int SIDE, typename Epi, int NJ>
+int run_tiles(Jobs<T, Epi, NJ>& jobs, const Way& way, void* sums, hipStream_t stream) {
+  constexpr int COLS = DUAL ? SIDE / 2 : SIDE;
+  for (int j = 0; j < NJ; j++) {
+    jobs.tiles_m[j] = (uint32_t)(up(jobs.product[j].M, SIDE) / SIDE);
+    jobs.tiles_n[j] = (uint32_t)(up(jobs.product[j].N, COLS) / COLS);
+  }
+  int rc = launch_tiles<T, PT, QT, DUAL, TWO, SIDE>(jobs, 0, way.whole, 1, stream);
+  if (rc || way.rest == 0) return rc;
+  using S = std::conditional_t<std::is_same_v<T, int8_t>, int, float>;
+  using P = Parts<S, SIDE, COLS, DUAL ? 2 : 1>;
+  Jobs<T, P, NJ> parts{};
+  for (int j = 0; j < NJ; j++) {
+    parts.product[j] = jobs.product[j];
+    parts.epi[j] = P{(S*)sums};
+    parts.tiles_m[j] = jobs.tiles_m[j];
+    parts.tiles_n[j] = jobs.tiles_n[j];
+  }
+  rc = launch_tiles<T, PT, QT, DUAL, TWO, SIDE>(parts, way.whole, way.rest, way.parts, stream);
+  if (rc) return rc;
+  join_kernel<T, DUAL, SIDE, COLS, S><<<dim3((unsigned)(way.rest * (SIDE * COLS / 2048))), 256, 0, stream>>>(
+      jobs, (uint32_t)way.whole, (uint32_t)way.rest, way.parts, (S*)sums);
+  return hipGetLastError();
 }
 
-// Carries out `a` the way that choose() gave; `sums`: its workspace.
-template <typename T, bool PT, bool QT, bool DUAL, bool TWO, typename Epi>
-int product(const Product<T>& a, const Way& way, void* sums, const Epi& epi, hipStream_t stream) {
-  if (a.M <= 0 || a.N <= 0) return hipSuccess;
+// Carries the jobs out the way that choose() gave for their extents; `sums`: its workspace.
+template <typename T, bool PT, bool QT, bool DUAL, bool TWO, typename Epi, int NJ>
+int products(Jobs<T, Epi, NJ>& jobs, const Way& way, void* sums, hipStream_t stream) {
+  for (int j = 0; j < NJ; j++)
+    if (jobs.product[j].M <= 0 || jobs.product[j].N <= 0) return hipSuccess;
   if constexpr (!PT && !QT && !TWO) {
     if (way.tile == FEW_ROWS) {
+      const Product<T>& a = jobs.product[0];
       const dim3 grid((unsigned)(up(a.N, 16) / 16));
-      if (a.M <= 16) few_rows_kernel<T, DUAL, 1><<<grid, 512, 0, stream>>>(a, epi);
-      else few_rows_kernel<T, DUAL, 2><<<grid, 512, 0, stream>>>(a, epi);
+      if (a.M <= 16) few_rows_kernel<T, DUAL, 1><<<grid, 512, 0, stream>>>(a, jobs.epi[0]);
+      else few_rows_kernel<T, DUAL, 2><<<grid, 512, 0, stream>>>(a, jobs.epi[0]);
       return hipGetLastError();
     }
   }
-  if (way.parts == 1) return tiles<T, PT, QT, DUAL, TWO>(a, way.tile, 1, epi, stream);
-  using S = std::conditional_t<std::is_same_v<T, int8_t>, int, float>;
-  const Parts<S> p{(S*)sums, a.M, up(a.N, 8), DUAL ? 2 : 1};
-  const int rc = tiles<T, PT, QT, DUAL, TWO>(a, way.tile, way.parts, p, stream);
-  if (rc) return rc;
-  const int64_t groups = up(a.N, 8) / 8, blocks = up(a.M * groups, 256) / 256;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-  join_kernel<S, DUAL><<<dim3((unsigned)blocks), 256, 0, stream>>>(p, a.M, (uint32_t)groups, (int)a.N, way.parts, epi);
-  return hipGetLastError();
+  if (way.tile == TILE_256) return run_tiles<T, PT, QT, DUAL, TWO, 256>(jobs, way, sums, stream);
+  if (way.tile == TILE_128) return run_tiles<T, PT, QT, DUAL, TWO, 128>(jobs, way, sums, stream);
+  return run_tiles<T, PT, QT, DUAL, TWO, 64>(jobs, way, sums, stream);
+}
+template <typename T, bool PT, bool QT, bool DUAL, bool TWO, typename Epi>
+int product(const Product<T>& a, const Way& way, void* sums, const Epi& epi, hipStream_t stream) {
+  Jobs<T, Epi, 1> one{{a}, {epi}, {0}, {0}};
+  return products<T, PT, QT, DUAL, TWO>(one, way, sums, stream);
 }
 
 }  // namespace dev

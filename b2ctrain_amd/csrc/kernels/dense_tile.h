@@ -102,12 +102,15 @@ struct Fragments {
   }
 };
 
-// Tile id -> (m tile, n tile): each of the eight dies works on a run of neighbouring tiles, and a run goes down
-// `group` m tiles before the next n tile, so that a die's cache holds both operands' rows for a while.
-__device__ __forceinline__ void place(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t group, uint32_t& tm,
-                                      uint32_t& tn) {
-  const uint32_t total = tiles_m * tiles_n, die = id % 8, per = total / 8, more = total % 8;
-  const uint32_t t = die * per + (die < more ? die : more) + id / 8;
+// Which of `count` neighbouring tiles workgroup `slot` takes: workgroups go to the eight dies in turn, and each die takes a run.
+__device__ __forceinline__ uint32_t tile_of(uint32_t slot, uint32_t count) {
+  const uint32_t die = slot % 8, per = count / 8, more = count % 8;
+  return die * per + (die < more ? die : more) + slot / 8;
+}
+// Tile t -> (m tile, n tile): down four m tiles before the next n tile, so that a die's cache holds both operands' rows for a
+// while.
+__device__ __forceinline__ void place(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
+  constexpr uint32_t group = 4;
   const uint32_t g = t / (group * tiles_n), first = g * group;
   const uint32_t rows = tiles_m - first < group ? tiles_m - first : group, r = t - g * group * tiles_n;
   tn = r / rows;
@@ -123,9 +126,31 @@ struct Product {
   int64_t q_lim, p_lim;  // how far m and n may be read in the operands; what lies beyond counts as zeros
 };
 
-template <typename T, bool PT, bool QT, bool DUAL, bool TWO, int WAVES_M, int WAVES_N, int WM, int WN, typename Epi>
-__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Product<T> a, int tiles_m, int tiles_n, int parts,
-                                                                     Epi epi) {
+// One or two products of a kind, to be carried out together; the second's tiles follow the first's.
+template <typename T, typename Epi, int N>
+struct Jobs {
+  Product<T> product[N];
+  Epi epi[N];
+  uint32_t tiles_m[N], tiles_n[N];
+};
+
+// Tile t of the jobs: which job's, and where in it.
+template <typename J, int N>
+__device__ __forceinline__ int find(const J& jobs, uint32_t t, uint32_t& tm, uint32_t& tn) {
+  int job = 0;
+  if constexpr (N == 2) {
+    const uint32_t first = jobs.tiles_m[0] * jobs.tiles_n[0];
+    if (t >= first) job = 1, t -= first;
+  }
+  place(t, jobs.tiles_m[job], jobs.tiles_n[job], tm, tn);
+  return job;
+}
+
+// Tiles first .. first + count - 1 of the jobs, each in `parts` parts of its k: workgroup part count + slot. The epilogue is
+// told the workgroup too.
+template <typename T, bool PT, bool QT, bool DUAL, bool TWO, int WAVES_M, int WAVES_N, int WM, int WN, typename Epi, int NJ>
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Jobs<T, Epi, NJ> jobs, uint32_t first, uint32_t count,
+                                                                     int parts) {
   constexpr int THREADS = WAVES_M * WAVES_N * 64, BM = WAVES_M * WM, BN = WAVES_N * WN;
   constexpr bool AHEAD = WAVES_M * WAVES_N == 8;
   constexpr int MT = WM / 16, NT = WN / 16, COLS = DUAL ? BN / 2 : BN;  // columns of out in a tile
@@ -137,9 +162,11 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Product<T> 
   __shared__ __attribute__((aligned(1024))) char lds[2 * STEP];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t tiles = (uint32_t)tiles_m * tiles_n, part = blockIdx.x / tiles;
+  const uint32_t part = blockIdx.x / count;
   uint32_t tm, tn;
-  place(blockIdx.x - part * tiles, tiles_m, tiles_n, 4, tm, tn);
+  const int job = find<Jobs<T, Epi, NJ>, NJ>(jobs, first + tile_of(blockIdx.x - part * count, count), tm, tn);
+  const Product<T>& a = jobs.product[job];
+  const Epi& epi = jobs.epi[job];
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * COLS;
   const int wm = wave % WAVES_M * WM, wb = wave / WAVES_M, wn = wb * WN;
 
@@ -303,10 +330,10 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Product<T> 
       for (int j = 0; j < 8; j++) g[j] = v[j], u[j] = DUAL ? v[WN / 2 + j] : S(0);
       if constexpr (DUAL) {
         const int64_t n = n0 + wb * (WN / 2) + col;
-        if (n < a.N) epi.template operator()<8>(part, m, (int)n, g, u);
+        if (n < a.N) epi.template operator()<8>(blockIdx.x, m, (int)n, g, u);
       } else {
         const int64_t n = n0 + wn + col;
-        if (n < a.N) epi.template operator()<8>(part, m, (int)n, g);
+        if (n < a.N) epi.template operator()<8>(blockIdx.x, m, (int)n, g);
       }
     }
   }

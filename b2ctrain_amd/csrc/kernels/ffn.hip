@@ -98,8 +98,8 @@ struct ForwardPlan {
     const int64_t M = a->rows;
     fp = up(a->d_hidden, 64);
     h = room.take<T>(M * fp);
-    gate = choose(M, fp, steps_of(a->d_in), true, true);
-    down = choose(M, a->d_out, steps_of(a->d_hidden), false, true);
+    gate = choose({{M, fp}}, steps_of(a->d_in), true, true);
+    down = choose({{M, a->d_out}}, steps_of(a->d_hidden), false, true);
     x = {{(const T*)a->x, a->ldx}, M, a->d_in};
     wg = {{(const T*)a->w_gate, a->ld_in}, a->d_hidden, a->d_in};
     wu = {{(const T*)a->w_up, a->ld_in}, a->d_hidden, a->d_in};
@@ -134,7 +134,7 @@ struct BackwardPlan {
   int64_t fp;
   T *h, *dgu;
   Operand<T> x, wg, wu, wd, dz;
-  Way back, down, in, dx;
+  Way back, dw, dx;
   void* sums;
   BackwardPlan(const b2c_ffn_grad_args* b, const Drop& d, Room& room) {
     const b2c_ffn_args* a = &b->fwd;
@@ -142,10 +142,13 @@ struct BackwardPlan {
     fp = up(a->d_hidden, 64);
     dgu = room.take<T>(M * 2 * fp);
     h = room.take<T>(M * fp);
-    back = choose(M, fp, steps_of(a->d_out), false, false);
-    down = choose(a->d_out, a->d_hidden, steps_of(M), false, false);
-    in = choose(fp + a->d_hidden, a->d_in, steps_of(M), false, false);
-    dx = choose(M, a->d_in, 2 * steps_of(a->d_hidden), false, false);
+    back = choose({{M, fp}}, steps_of(a->d_out), false, false);
+    const Extent in{fp + a->d_hidden, a->d_in}, down{a->d_out, a->d_hidden};
+    const int64_t k = steps_of(M);
+    dw = b->dw_down && (b->dw_gate || b->dw_up) ? choose({in, down}, k, false, false)
+         : b->dw_down                           ? choose({down}, k, false, false)
+                                                : choose({in}, k, false, false);
+    dx = choose({{M, a->d_in}}, 2 * steps_of(a->d_hidden), false, false);
     x = {{(const T*)a->x, a->ldx}, M, a->d_in};
     wg = {{(const T*)a->w_gate, a->ld_in}, a->d_hidden, a->d_in};
     wu = {{(const T*)a->w_up, a->ld_in}, a->d_hidden, a->d_in};
@@ -160,7 +163,7 @@ struct BackwardPlan {
     }
     wd.place(room, direct(a->w_down, a->ld_out, a->d_hidden));
     dz.place(room, !d.threshold && direct(b->dy, b->lddy, a->d_out));
-    sums = room.take<char>(std::max(std::max(back.sums, down.sums), std::max(in.sums, dx.sums)));
+    sums = room.take<char>(std::max(back.sums, std::max(dw.sums, dx.sums)));
   }
 };
 
@@ -181,16 +184,20 @@ int backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream) {
   const Product<T> dh{dz, p.wd.side(), {}, {}, M, fp, a->d_out, 0, M, a->d_hidden};
   if ((rc = product<T, true, false, false, false>(dh, p.back, p.sums, back, stream))) return rc;
   const bool f32 = b->grad_dtype == B2C_F32, add = b->accumulate != 0;
-  if (b->dw_down) {
-    const WeightOut<T> out{b->dw_down, nullptr, b->ld_dout, a->d_out, 0, a->d_hidden, f32, add, scale};
-    const Product<T> dw{dz, {p.h, fp}, {}, {}, a->d_out, a->d_hidden, M, 0, a->d_out, a->d_hidden};
-    if ((rc = product<T, true, true, false, false>(dw, p.down, p.sums, out, stream))) return rc;
+  const bool in = b->dw_gate || b->dw_up;
+  const WeightOut<T> to_in{b->dw_gate, b->dw_up, b->ld_din, a->d_hidden, (int)fp, a->d_in, f32, add, 1.f};
+  const WeightOut<T> to_down{b->dw_down, nullptr, b->ld_dout, a->d_out, 0, a->d_hidden, f32, add, scale};
+  const Product<T> dwi{dgu, x, {}, {}, fp + a->d_hidden, a->d_in, M, 0, fp + a->d_hidden, a->d_in};
+  const Product<T> dwd{dz, {p.h, fp}, {}, {}, a->d_out, a->d_hidden, M, 0, a->d_out, a->d_hidden};
+  if (in && b->dw_down) {  // together: one launch, and fewer compute units without work in its last round
+    Jobs<T, WeightOut<T>, 2> both{{dwi, dwd}, {to_in, to_down}, {}, {}};
+    rc = products<T, true, true, false, false>(both, p.dw, p.sums, stream);
+  } else if (in) {
+    rc = product<T, true, true, false, false>(dwi, p.dw, p.sums, to_in, stream);
+  } else if (b->dw_down) {
+    rc = product<T, true, true, false, false>(dwd, p.dw, p.sums, to_down, stream);
   }
-  if (b->dw_gate || b->dw_up) {
-    const WeightOut<T> out{b->dw_gate, b->dw_up, b->ld_din, a->d_hidden, (int)fp, a->d_in, f32, add, 1.f};
-    const Product<T> dw{dgu, x, {}, {}, fp + a->d_hidden, a->d_in, M, 0, fp + a->d_hidden, a->d_in};
-    if ((rc = product<T, true, true, false, false>(dw, p.in, p.sums, out, stream))) return rc;
-  }
+  if (rc) return rc;
   if (b->dx) {
     const RowsOut<T> out{(T*)b->dx, b->lddx, nullptr, 0, a->d_in, {}};
     const Product<T> dx{dgu, p.wg.side(), {p.dgu + fp, 2 * fp}, p.wu.side(), M, a->d_in, a->d_hidden, a->d_hidden, M, a->d_in};

@@ -161,7 +161,7 @@ struct LinearPlan {
     kp = up(a->d_in, 128);
     q = room.take<int8_t>(a->rows * kp);
     sx = room.take<float>(a->rows);
-    way = choose(a->rows, a->d_out, steps_of(a->d_in), false, true);
+    way = choose({{a->rows, a->d_out}}, steps_of(a->d_in), false, true);
     w = {{a->w, a->ldw}, a->d_out, a->d_in};
     w.place(room, way.tile == FEW_ROWS);
     sums = room.take<char>(way.sums);
@@ -181,8 +181,8 @@ struct BlockPlan {
     qh = room.take<int8_t>(a->rows * fp);
     qx = room.take<int8_t>(a->rows * kp);
     s = room.take<float>(a->rows);
-    gate = choose(a->rows, a->d_hidden, steps_of(a->d_in), true, true);
-    down = choose(a->rows, a->d_out, steps_of(a->d_hidden), false, true);
+    gate = choose({{a->rows, a->d_hidden}}, steps_of(a->d_in), true, true);
+    down = choose({{a->rows, a->d_out}}, steps_of(a->d_hidden), false, true);
     const bool few = gate.tile == FEW_ROWS;
     wg = {{a->w_gate, a->ld_in}, a->d_hidden, a->d_in};
     wu = {{a->w_up, a->ld_in}, a->d_hidden, a->d_in};
