@@ -159,7 +159,7 @@ struct RowsOut {
     if (drop.threshold) {
       static_assert(W == 4 || W == 8);
       const uint64_t e = (uint64_t)m * cols + n;
-      const uint32_t k = W == 8 ? kept8(drop, e) : kept4(drop, e);
+      const uint32_t k = kept_bits<W>(drop, e);
 #pragma unroll
       for (int j = 0; j < W; j++) v[j] = k >> j & 1 ? v[j] * drop.scale : 0.f;
     }

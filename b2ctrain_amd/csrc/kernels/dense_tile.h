@@ -319,7 +319,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Jobs<T, Epi
   for (int i = 0; i < MT; i++) {
 #pragma unroll
     for (int t = 0; t < NT; t++) *reinterpret_cast<Acc*>(turn + (lane & 15) * PITCH + t * 16 + lq * 4) = acc[t][i];
-#pragma unroll
+#pragma unroll 1
     for (int h = 0; h < 16; h += ROWS) {
       const int row = h + lane / LANES, col = lane % LANES * 8;
       const int64_t m = m0 + wm + i * 16 + row;

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* x, int64_t ldx, int6
       if (n + j < cols) v[j] = p[j];
   }
   if (d.threshold) {
-    const uint32_t keep = kept8(d, (uint64_t)m * cols + n);
+    const uint32_t keep = kept_bits<8>(d, (uint64_t)m * cols + n);
 #pragma unroll
     for (int j = 0; j < 8; j++)
       if (!(keep >> j & 1)) v[j] = (T)0.f;

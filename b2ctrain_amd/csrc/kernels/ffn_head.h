@@ -96,7 +96,7 @@ template <typename T>
 __device__ __forceinline__ vec<T, 8> eight_kept(const T* p, int64_t ld, int64_t m, int64_t M, int k, int K, const Drop& d) {
   vec<T, 8> v = eight(p, ld, m, M, k, K);
   if (d.threshold && m < M && k < K) {
-    const uint32_t keep = kept8(d, (uint64_t)m * K + k);
+    const uint32_t keep = kept_bits<8>(d, (uint64_t)m * K + k);
 #pragma unroll
     for (int j = 0; j < 8; j++)
       if (!(keep >> j & 1)) v[j] = (T)0.f;

@@ -42,34 +42,21 @@ __device__ __forceinline__ bool kept(const Philox4& w, int j, uint32_t threshold
   return ((w.w[j >> 1] >> ((j & 1) * 16)) & 0xffffu) >= threshold;
 }
 
-// Which of elements e .. e + 3 are kept, as four bits: one counter where e & 7 <= 4, else two.
-__device__ __forceinline__ uint32_t kept4(const Drop& d, uint64_t e) {
+// Which of elements e .. e + N - 1 are kept (N at most 8), as bits: they lie in one counter's fields or in two neighbouring
+// counters'. One copy of the rounds, run once or twice.
+template <int N>
+__device__ __forceinline__ uint32_t kept_bits(const Drop& d, uint64_t e) {
   const int o = (int)(e & 7);
-  Philox4 w = philox(e >> 3, d.stream, d.seed);
   uint32_t m = 0;
+#pragma unroll 1
+  for (int i = 0; i <= (o + N > 8); i++) {
+    const Philox4 w = philox((e >> 3) + i, d.stream, d.seed);
+    uint32_t b = 0;
 #pragma unroll
-  for (int j = 0; j < 8; j++) m |= (uint32_t)kept(w, j, d.threshold) << j;
-  if (o > 4) {
-    w = philox((e >> 3) + 1, d.stream, d.seed);
-#pragma unroll
-    for (int j = 0; j < 4; j++) m |= (uint32_t)kept(w, j, d.threshold) << (8 + j);
+    for (int j = 0; j < 8; j++) b |= (uint32_t)kept(w, j, d.threshold) << j;
+    m |= b << (8 * i);
   }
-  return m >> o & 15u;
-}
-
-// The same of elements e .. e + 7, as eight bits.
-__device__ __forceinline__ uint32_t kept8(const Drop& d, uint64_t e) {
-  const int o = (int)(e & 7);
-  Philox4 w = philox(e >> 3, d.stream, d.seed);
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; j++) m |= (uint32_t)kept(w, j, d.threshold) << j;
-  if (o) {
-    w = philox((e >> 3) + 1, d.stream, d.seed);
-#pragma unroll
-    for (int j = 0; j < 8; j++) m |= (uint32_t)kept(w, j, d.threshold) << (8 + j);
-  }
-  return m >> o & 255u;
+  return m >> o;
 }
 
 }  // namespace dev
