@@ -369,7 +369,7 @@ inline int head_steps(const b2c_ffn_args* a) {
 }
 
 // How the weights' gradients are shared out: tiles of 16 hidden units a wave, workgroups of eight waves along the hidden
-// units, parts of the rows: 512 workgroups in all, two for each compute unit.
+// units, parts of the rows: 256 workgroups in all, one for each compute unit, which its registers fill (512 took 679 us where 256 take 661).
 struct HeadSplit {
   int ht, blocks, parts;
   int64_t chunks;
@@ -377,7 +377,7 @@ struct HeadSplit {
     chunks = up(a->d_hidden, 16) / 16;
     ht = head_steps(a) <= 2 && up(a->d_hidden, 256) == up(a->d_hidden, 128) ? 2 : 1;
     blocks = (int)(up(chunks, 8 * ht) / (8 * ht));
-    parts = (int)std::max<int64_t>(1, std::min<int64_t>(up(a->rows, 64) / 64, 512 / blocks));
+    parts = (int)std::max<int64_t>(1, std::min<int64_t>(up(a->rows, 64) / 64, 256 / blocks));
   }
   int64_t sums(int ks) const { return (int64_t)parts * 3 * chunks * 16 * 32 * ks; }
 };
@@ -412,13 +412,16 @@ int make_fragments(const b2c_ffn_args* a, int64_t chunks, T* to, hipStream_t str
   return hipGetLastError();
 }
 
-// Eight waves of several row tiles each where that still gives every compute unit a workgroup, else four waves of one.
+// Four waves of two row tiles each (of one where the widths fill the registers) where that gives every compute unit its three
+// workgroups, else of one. A training step of 1M rows of 64-256-64 took 756 us with eight waves of four tiles, 729 with four of
+// four, 690 with four of two: what counts is that a compute unit's workgroups are out of step, so that one's matrix
+// instructions meet another's arithmetic.
 template <typename T, int ACT, int USE, int KS>
 int head_rows(const HeadRows<T>& rows, const T* frags, int chunks, const RowsOut<T>& out, hipStream_t stream) {
-  constexpr int RT = KS == 4 ? 2 : 4;
-  const int64_t many = up(rows.M, 128 * RT) / (128 * RT), few = up(rows.M, 64) / 64;
-  if (many >= 256) head_rows_kernel<T, ACT, USE, KS, RT, 8><<<dim3((unsigned)many), 512, 0, stream>>>(rows, frags, chunks, out);
-  else head_rows_kernel<T, ACT, USE, KS, 1, 4><<<dim3((unsigned)few), 256, 0, stream>>>(rows, frags, chunks, out);
+  constexpr int RT = KS == 4 ? 1 : 2;
+  const int64_t many = up(rows.M, 64 * RT) / (64 * RT), few = up(rows.M, 64) / 64;
+  if (RT == 1 || many < 768) head_rows_kernel<T, ACT, USE, KS, 1, 4><<<dim3((unsigned)few), 256, 0, stream>>>(rows, frags, chunks, out);
+  else head_rows_kernel<T, ACT, USE, KS, RT, 4><<<dim3((unsigned)many), 256, 0, stream>>>(rows, frags, chunks, out);
   return hipGetLastError();
 }
 
