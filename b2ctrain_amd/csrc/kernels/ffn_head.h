@@ -69,11 +69,17 @@ __device__ __forceinline__ vec<T, 8> fragment(const HeadWeights<T>& w, int c, in
   return v;
 }
 
-template <typename T, int USE, int KS>
-__global__ __launch_bounds__(256) void fragments_kernel(HeadWeights<T> w, int chunks, T* out) {
-  const int t = blockIdx.x * 256 + threadIdx.x, lane = t & 63, f = t >> 6, n = fragments(USE, KS);
-  if (f >= chunks * n) return;
-  *reinterpret_cast<vec<T, 8>*>(out + (int64_t)t * 8) = fragment<T, USE, KS>(w, f / n, f % n, lane);
+// A use's fragments, and with BOTH also those of FOR_DW, behind them.
+template <typename T, int USE, bool BOTH, int KS>
+__global__ __launch_bounds__(256) void fragments_kernel(HeadWeights<T> w, int chunks, T* out, int chunks_dw, T* out_dw) {
+  const int lane = threadIdx.x & 63, n = fragments(USE, KS), all = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (all < chunks * n) {
+    *reinterpret_cast<vec<T, 8>*>(out + ((int64_t)all * 64 + lane) * 8) = fragment<T, USE, KS>(w, all / n, all % n, lane);
+  } else if constexpr (BOTH) {
+    const int f = all - chunks * n, nd = fragments(FOR_DW, KS);
+    if (f < chunks_dw * nd)
+      *reinterpret_cast<vec<T, 8>*>(out_dw + ((int64_t)f * 64 + lane) * 8) = fragment<T, FOR_DW, KS>(w, f / nd, f % nd, lane);
+  }
 }
 
 // Eight values of a row from column k on, zeros beyond the row's or the matrix's end.
@@ -113,6 +119,7 @@ struct HeadRows {
   int64_t M;
   int D, F, O;
   Drop drop;
+  T* kept;  // FOR_DX: dy with dropout's zeros is left here for the weights' gradients, rows 32 KS apart; or null
 };
 
 // Rows by waves: y (USE = FOR_Y), or the gradient of x. RT tiles of 16 rows a wave; the chunks' fragments pass through two
@@ -142,6 +149,14 @@ __global__ __launch_bounds__(WAVES * 64) void head_rows_kernel(HeadRows<T> a, co
       x[r][k] = eight(a.x, a.ldx, m0 + r * 16, a.M, k * 32 + q4 * 8, a.D);
       if constexpr (USE == FOR_DX) dz[r][k] = eight_kept(a.dy, a.lddy, m0 + r * 16, a.M, k * 32 + q4 * 8, a.O, a.drop);
     }
+  if constexpr (USE == FOR_DX) {
+    if (a.kept)
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+          if (m0 + r * 16 < a.M) *reinterpret_cast<F8*>(a.kept + (m0 + r * 16) * (32 * KS) + k * 32 + q4 * 8) = dz[r][k];
+  }
   f32x4 acc[RT][OT] = {};
   const float scale = a.drop.scale;
   for (int c = 0; c < chunks; c++) {
@@ -328,22 +343,22 @@ __global__ __launch_bounds__(WAVES * 64) void head_weights_kernel(HeadRows<T> a,
   }
 }
 
-// Adds the parts in their order and writes the gradients: four columns a thread, eight threads to them, each for every
-// eighth part.
+// Adds the parts in a fixed order and writes the gradients: four columns a thread, 32 threads to them, each for every 32nd
+// part.
 template <typename T>
 __global__ __launch_bounds__(256) void head_join_kernel(const float* sums, int64_t hidden, int wide, int parts, int F, int D, int O,
                                                         WeightOut<T> in, WeightOut<T> down) {
-  __shared__ f32x4 some[8][32];
-  const int64_t plane = hidden * wide, at = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 4;
-  const int g = threadIdx.x >> 5;
+  __shared__ f32x4 some[32][8];
+  const int64_t plane = hidden * wide, at = ((int64_t)blockIdx.x * 8 + (threadIdx.x & 7)) * 4;
+  const int g = threadIdx.x >> 3;
   f32x4 v = {};
-  if (at < 3 * plane)
-    for (int p = g; p < parts; p += 8) v += *reinterpret_cast<const f32x4*>(sums + (int64_t)p * 3 * plane + at);
-  some[g][threadIdx.x & 31] = v;
+#pragma unroll 8
+  for (int p = g; p < parts; p += 32) v += *reinterpret_cast<const f32x4*>(sums + (int64_t)p * 3 * plane + at);
+  some[g][threadIdx.x & 7] = v;
   __syncthreads();
-  if (g || at >= 3 * plane) return;
+  if (g) return;
 #pragma unroll
-  for (int j = 1; j < 8; j++) v += some[j][threadIdx.x];
+  for (int j = 1; j < 32; j++) v += some[j][threadIdx.x];
   const int which = (int)(at / plane), h = (int)((at - which * plane) / wide), n = (int)((at - which * plane) % wide);
   if (h >= F) return;
   float o[4] = {v[0], v[1], v[2], v[3]};
@@ -368,16 +383,18 @@ inline int head_steps(const b2c_ffn_args* a) {
   return n == 3 ? 4 : n;
 }
 
-// How the weights' gradients are shared out: tiles of 16 hidden units a wave, workgroups of eight waves along the hidden
-// units, parts of the rows: 256 workgroups in all, one for each compute unit, which its registers fill (512 took 679 us where 256 take 661).
+// How the weights' gradients are shared out: tiles of 16 hidden units a wave (two where the registers take them), workgroups
+// of eight waves along the hidden units (four where there are few), parts of the rows: as many workgroups as the compute
+// units hold (a step of 1M rows of 64-256-64 took 679 us with 512 where 256 take 661).
 struct HeadSplit {
-  int ht, blocks, parts;
+  int ht, waves, blocks, parts;
   int64_t chunks;
   HeadSplit(const b2c_ffn_args* a) {
     chunks = up(a->d_hidden, 16) / 16;
     ht = head_steps(a) <= 2 && up(a->d_hidden, 256) == up(a->d_hidden, 128) ? 2 : 1;
-    blocks = (int)(up(chunks, 8 * ht) / (8 * ht));
-    parts = (int)std::max<int64_t>(1, std::min<int64_t>(up(a->rows, 64) / 64, 256 / blocks));
+    waves = chunks <= 4 ? 4 : 8;
+    blocks = (int)(up(chunks, waves * ht) / (waves * ht));
+    parts = (int)std::max<int64_t>(1, std::min<int64_t>(up(a->rows, 64) / 64, (waves == 4 ? 768 : 256) / blocks));
   }
   int64_t sums(int ks) const { return (int64_t)parts * 3 * chunks * 16 * 32 * ks; }
 };
@@ -385,8 +402,8 @@ struct HeadSplit {
 template <typename T>
 struct HeadPlan {
   int ks, chunks;  // of 32 hidden units
-  T *for_y, *for_dx, *for_dw;
-  float* sums;
+  T *for_y = nullptr, *for_dx = nullptr, *for_dw = nullptr, *kept = nullptr;
+  float* sums = nullptr;
   HeadPlan(const b2c_ffn_args* a, const b2c_ffn_grad_args* b, Room& room) {
     ks = head_steps(a);
     chunks = (int)(up(a->d_hidden, 32) / 32);
@@ -399,16 +416,17 @@ struct HeadPlan {
     if (b->dw_gate || b->dw_up || b->dw_down) {
       for_dw = room.take<T>(split.chunks * fragments(FOR_DW, ks) * 512);
       sums = room.take<float>(split.sums(ks));
+      if (b->dx && b->fwd.p > 0.f) kept = room.take<T>(a->rows * 32 * ks);
     }
   }
 };
 
-template <typename T, int USE, int KS>
-int make_fragments(const b2c_ffn_args* a, int64_t chunks, T* to, hipStream_t stream) {
+template <typename T, int USE, bool BOTH, int KS>
+int make_fragments(const b2c_ffn_args* a, int64_t chunks, T* to, int64_t chunks_dw, T* to_dw, hipStream_t stream) {
   const HeadWeights<T> w{(const T*)a->w_gate, (const T*)a->w_up, (const T*)a->w_down, a->ld_in, a->ld_out, a->d_in, a->d_hidden, a->d_out};
-  const int64_t blocks = up(chunks * fragments(USE, KS) * 64, 256) / 256;
+  const int64_t blocks = up(chunks * fragments(USE, KS) + (BOTH ? chunks_dw * fragments(FOR_DW, KS) : 0), 4) / 4;
   if (blocks > 0x7fffff) return hipErrorInvalidValue;
-  fragments_kernel<T, USE, KS><<<dim3((unsigned)blocks), 256, 0, stream>>>(w, (int)chunks, to);
+  fragments_kernel<T, USE, BOTH, KS><<<dim3((unsigned)blocks), 256, 0, stream>>>(w, (int)chunks, to, (int)chunks_dw, to_dw);
   return hipGetLastError();
 }
 
@@ -429,9 +447,9 @@ template <typename T, int ACT, int KS>
 int head_forward(const b2c_ffn_args* a, const Drop& d, hipStream_t stream) {
   Room room{(char*)a->workspace};
   const HeadPlan<T> p(a, nullptr, room);
-  const int rc = make_fragments<T, FOR_Y, KS>(a, p.chunks, p.for_y, stream);
+  const int rc = make_fragments<T, FOR_Y, false, KS>(a, p.chunks, p.for_y, 0, nullptr, stream);
   if (rc) return rc;
-  const HeadRows<T> rows{(const T*)a->x, a->ldx, nullptr, 0, a->rows, a->d_in, a->d_hidden, a->d_out, {}};
+  const HeadRows<T> rows{(const T*)a->x, a->ldx, nullptr, 0, a->rows, a->d_in, a->d_hidden, a->d_out, {}, nullptr};
   const RowsOut<T> out{(T*)a->y, a->ldy, (const T*)a->residual, a->ldr, a->d_out, d};
   return head_rows<T, ACT, FOR_Y, KS>(rows, p.for_y, p.chunks, out, stream);
 }
@@ -441,20 +459,31 @@ int head_backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream)
   const b2c_ffn_args* a = &b->fwd;
   Room room{(char*)b->workspace};
   const HeadPlan<T> p(a, b, room);
-  HeadRows<T> rows{(const T*)a->x, a->ldx, (const T*)b->dy, b->lddy, a->rows, a->d_in, a->d_hidden, a->d_out, d};
+  HeadRows<T> rows{(const T*)a->x, a->ldx, (const T*)b->dy, b->lddy, a->rows, a->d_in, a->d_hidden, a->d_out, d, p.kept};
   rows.drop.scale = d.threshold ? d.scale : 1.f;
-  int rc;
+  const bool weights = b->dw_gate || b->dw_up || b->dw_down;
+  const HeadSplit split(a);
+  int rc = hipSuccess;
   if (b->dx) {
-    if ((rc = make_fragments<T, FOR_DX, KS>(a, p.chunks, p.for_dx, stream))) return rc;
+    rc = weights ? make_fragments<T, FOR_DX, true, KS>(a, p.chunks, p.for_dx, split.chunks, p.for_dw, stream)
+                 : make_fragments<T, FOR_DX, false, KS>(a, p.chunks, p.for_dx, 0, nullptr, stream);
+    if (rc) return rc;
     const RowsOut<T> out{(T*)b->dx, b->lddx, nullptr, 0, a->d_in, {}};
     if ((rc = head_rows<T, ACT, FOR_DX, KS>(rows, p.for_dx, p.chunks, out, stream))) return rc;
+  } else if (weights) {
+    if ((rc = make_fragments<T, FOR_DW, false, KS>(a, split.chunks, p.for_dw, 0, nullptr, stream))) return rc;
   }
-  if (!b->dw_gate && !b->dw_up && !b->dw_down) return hipSuccess;
-  const HeadSplit split(a);
-  if ((rc = make_fragments<T, FOR_DW, KS>(a, split.chunks, p.for_dw, stream))) return rc;
+  if (!weights) return hipSuccess;
+  if (p.kept) {  // dropout's bits cost as much as a third of a pass over the rows
+    rows.dy = p.kept;
+    rows.lddy = 32 * KS;
+    rows.drop.threshold = 0;
+  }
   const dim3 grid((unsigned)split.blocks, (unsigned)split.parts);
   const int chunks = (int)split.chunks;
-  if constexpr (KS <= 2) {
+  if (split.waves == 4) {
+    head_weights_kernel<T, ACT, KS, 1, 4><<<grid, 256, 0, stream>>>(rows, p.for_dw, chunks, p.sums);
+  } else if constexpr (KS <= 2) {
     if (split.ht == 2) head_weights_kernel<T, ACT, KS, 2, 8><<<grid, 512, 0, stream>>>(rows, p.for_dw, chunks, p.sums);
     else head_weights_kernel<T, ACT, KS, 1, 8><<<grid, 512, 0, stream>>>(rows, p.for_dw, chunks, p.sums);
   } else {
@@ -464,7 +493,7 @@ int head_backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream)
   const bool f32 = b->grad_dtype == B2C_F32, add = b->accumulate != 0;
   const WeightOut<T> in{b->dw_gate, b->dw_up, b->ld_din, a->d_hidden, a->d_hidden, a->d_in, f32, add, 1.f};
   const WeightOut<T> down{b->dw_down, nullptr, b->ld_dout, a->d_out, 0, a->d_hidden, f32, add, rows.drop.scale};
-  const int64_t hidden = split.chunks * 16, blocks = up(3 * hidden * 32 * KS, 128) / 128;
+  const int64_t hidden = split.chunks * 16, blocks = 3 * hidden * KS;
   head_join_kernel<T><<<dim3((unsigned)blocks), 256, 0, stream>>>(p.sums, hidden, 32 * KS, split.parts, a->d_hidden, a->d_in, a->d_out, in,
                                                                   down);
   return hipGetLastError();
