@@ -3,6 +3,7 @@
 #pragma once
 #include "dense_tile.h"
 
+#include <cmath>
 #include <initializer_list>
 
 namespace b2c {
@@ -152,34 +153,52 @@ struct Extent {
   int64_t M, N;
 };
 
-// What a product of these sizes costs by each tile, in microseconds, from times measured warm: a step of 128 bytes of k takes
-// a compute unit 1.43 us for a 256x256 tile when all are busy (1.1 alone), 0.46 each for two of 128x128 side by side (0.63
-// alone), 0.18 each for five of 64x64 (0.45 alone), beside a launch, a first copy and an epilogue of 5.9, 3.8 and 3.6. A large
-// tile reads less, small ones keep more compute units at work when there are few: 4096 x 4096 x 4096 takes 100, 125 and 191 us,
-// 1037 x 2752 x 1000 takes 27, 14 and 13. Tiles beyond the last full round of compute units, or all where there are too few,
-// may be split over k, for a write and a read of their sums.
-inline Way choose(std::initializer_list<Extent> jobs, int64_t steps, bool dual, bool may_be_few) {
+// What `n` tiles of a size cost over `steps` steps of 128 bytes of k, in microseconds, fitted to 360 products of 64 to 8000 rows,
+// 256 to 5504 columns and 256 to 5504 values of k, timed warm:
+//   256x256, one a compute unit: a step takes 1.04 with half of them busy, 1.43 with all; 8 a round for its start and end.
+//   128x128: 0.36 where a compute unit has one (four buffers), 0.9 for a round of two in each.
+//   64x64: 0.27 up to one each, 0.4 up to two (three buffers), then 0.2 for each of several side by side.
+// A large tile reads less, small ones keep more compute units at work when there are few: 4096 x 4096 x 4096 takes 100, 125 and
+// 191 us, 1000 x 1024 x 1024 takes 25, 10 and 10.
+inline double tile_time(int tile, int64_t n, double steps) {
+  const double each = (double)n / 256;
+  if (tile == TILE_256) {
+    const double part = each - std::floor(each);
+    return (1.43 * std::floor(each) + (part > 0 ? 1.04 + 0.39 * std::max(0.0, 2 * part - 1) : 0)) * steps + 8 * std::ceil(each);
+  }
+  if (tile == TILE_128) {
+    if (n <= 256) return 0.365 * steps + 4.4;
+    const double part = (each / 2 - std::floor(each / 2)) * 2;
+    return (0.9 * std::floor(each / 2) + (part > 0 ? 0.64 + 0.26 * std::max(0.0, part - 1) : 0)) * steps + 3 + 3.2 * std::ceil(each / 2);
+  }
+  return (n <= 512 ? 0.265 + 0.14 * std::max(0.0, each - 1) : 0.2 * each) * steps + 3.1 + 0.35 * each;
+}
+
+// The cheapest way for products of these extents, `steps` long. Tiles beyond the last full round of compute units, or all of them
+// where there are too few, may be split over k, for a write and a read of their sums at 5 TB/s. `moved`: bytes that the
+// epilogue reads and writes for each value of out; a compute unit's only tile does nothing beside them, several hide them.
+inline Way choose(std::initializer_list<Extent> jobs, int64_t steps, bool dual, bool may_be_few, int moved = 2) {
   if (may_be_few && jobs.begin()->M <= kFewRows) return {FEW_ROWS, 0, 0, 1, 0};
-  static const struct { int side; double wide, alone, fixed; int held; } tiles[3] = {
-      {256, 1.43, 1.1, 5.9, 1}, {128, 0.46, 0.63, 3.8, 2}, {64, 0.18, 0.45, 3.6, 5}};
   Way best{TILE_64, 0, 0, 1, 0};
   double least = 1e30;
   for (int t = 0; t < 3; t++) {
-    const auto& k = tiles[t];
-    const int64_t cols = dual ? k.side / 2 : k.side;
+    const int64_t side = t == TILE_256 ? 256 : t == TILE_128 ? 128 : 64, cols = dual ? side / 2 : side;
+    const int64_t full = t == TILE_256 ? 256 : t == TILE_128 ? 512 : 1280;
     int64_t count = 0;
-    for (const Extent& e : jobs) count += up(e.M, k.side) / k.side * (up(e.N, cols) / cols);
-    auto time = [&](int64_t n, double st) {
-      return std::max(k.wide * (double)(up(n, 256) / 256), k.alone * (double)(up(n, 256 * k.held) / (256 * k.held))) * st;
-    };
-    const double all = k.fixed + time(count, (double)std::max<int64_t>(steps, 1));
+    double values = 0;
+    for (const Extent& e : jobs) {
+      count += up(e.M, side) / side * (up(e.N, cols) / cols);
+      values += (double)e.M * (double)e.N;
+    }
+    const double end = values * (moved - 2) / 4.5e6 * (t == TILE_256 ? 1.0 : t == TILE_128 ? 0.5 : 0.3);
+    const double all = tile_time(t, count, (double)steps) + end;
     if (all < least) least = all, best = {t, count, 0, 1, 0};
-    for (const int64_t whole : {(int64_t)0, count / 256 * 256, count / (256 * k.held) * (256 * k.held)}) {
+    for (const int64_t whole : {(int64_t)0, count / full * full}) {
       const int64_t rest = count - whole;
       for (int parts = 2; parts <= 64 && rest > 0; parts++) {
-        const double sums = 4.0 * parts * (double)rest * k.side * k.side;
-        if (steps / parts < 4 || sums > 256e6) break;
-        const double us = (whole ? k.fixed + time(whole, (double)steps) : 0) + k.fixed + time(rest * parts, (double)steps / parts) + 4 + 2 * sums / 3.5e6;
+        const double sums = 4.0 * parts * (double)rest * (double)(side * side);
+        if (steps / parts < 3 || sums > 256e6) break;
+        const double us = (whole ? tile_time(t, whole, (double)steps) : 0) + tile_time(t, rest * parts, (double)((steps + parts - 1) / parts)) + 3 + 2 * sums / 5e6 + end;
         if (us < least) least = us, best = {t, whole, rest, parts, (size_t)sums};
       }
     }
@@ -193,11 +212,18 @@ int launch_tiles(const Jobs<T, Epi, NJ>& jobs, int64_t first, int64_t count, int
   if (count * parts > 0x7fffffff) return hipErrorInvalidValue;
   const dim3 grid((unsigned)(count * parts));
   if constexpr (SIDE == 256)
-    tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 128, 64><<<grid, 512, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
-  else if constexpr (SIDE == 128)
-    tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 64, 32><<<grid, 512, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
-  else
-    tile_kernel<T, PT, QT, DUAL, TWO, 2, 2, 32, 32><<<grid, 256, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
+    tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 128, 64, 2><<<grid, 512, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
+  else if constexpr (SIDE == 128) {
+    if (count * parts <= 256)
+      tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 64, 32, 4><<<grid, 512, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
+    else
+      tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 64, 32, 2><<<grid, 512, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
+  } else {
+    if (count * parts <= 512)
+      tile_kernel<T, PT, QT, DUAL, TWO, 2, 2, 32, 32, 3><<<grid, 256, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
+    else
+      tile_kernel<T, PT, QT, DUAL, TWO, 2, 2, 32, 32, 2><<<grid, 256, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
+  }
   return hipGetLastError();
 }
 

@@ -148,7 +148,7 @@ __device__ __forceinline__ int find(const J& jobs, uint32_t t, uint32_t& tm, uin
 
 // Tiles first .. first + count - 1 of the jobs, each in `parts` parts of its k: workgroup part count + slot. The epilogue is
 // told the workgroup too.
-template <typename T, bool PT, bool QT, bool DUAL, bool TWO, int WAVES_M, int WAVES_N, int WM, int WN, typename Epi, int NJ>
+template <typename T, bool PT, bool QT, bool DUAL, bool TWO, int WAVES_M, int WAVES_N, int WM, int WN, int STAGES, typename Epi, int NJ>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Jobs<T, Epi, NJ> jobs, uint32_t first, uint32_t count,
                                                                      int parts) {
   constexpr int THREADS = WAVES_M * WAVES_N * 64, BM = WAVES_M * WM, BN = WAVES_N * WN;
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Jobs<T, Epi
   using TP = Tile<T, BN, THREADS, PT>;
   static_assert(!DUAL || (!PT && !TWO));
   constexpr int STEP = TQ::BYTES + TP::BYTES, BK = TQ::BK;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * STEP];
+  __shared__ __attribute__((aligned(1024))) char lds[STAGES * STEP];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t part = blockIdx.x / count;
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Jobs<T, Epi
   };
   constexpr int COPIES = TQ::COPIES + TP::COPIES;
   auto copy = [&](int s, int j) {  // copy j of step s; beyond the last step `left` makes it one of zeros
-    const uint32_t to = lds0 + (uint32_t)(s & 1) * STEP;
+    const uint32_t to = lds0 + (uint32_t)s % STAGES * STEP;
     if (j < TQ::COPIES) {
       cq.copy(j, pq, to, wave, left);
     } else {
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Jobs<T, Epi
   using F = vec<T, TQ::V>;
   F q0[MT], p0[NT], q1[MT], p1[NT];
   auto read = [&](int s, int kk, F(&q)[MT], F(&p)[NT]) {
-    const char* at = lds + (uint32_t)(s & 1) * STEP;
+    const char* at = lds + (uint32_t)s % STAGES * STEP;
 #pragma unroll
     for (int t = 0; t < NT; t++) p[t] = fp.get(at + TQ::BYTES, t, kk);
 #pragma unroll
@@ -246,11 +246,15 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Jobs<T, Epi
 #pragma unroll
       for (int j = 0; j < NT; j++) acc[j][i] = mfma(p[j], q[i], acc[j][i]);
   };
-  auto landed = [] {  // this wave's copies are in LDS and its reads done; then everybody's
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  // This wave's copies are in LDS, but for those of the last LATER steps, and its reads done; then everybody's.
+  auto landed = [](auto later) {
+    constexpr int n = decltype(later)::value * COPIES;
+    static_assert(n < 64);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
+  using All = std::integral_constant<int, 0>;
   // Multiplies one half's fragments while those of another are read from buffer `at`, spread over the first three
   // quarters, and with COPY the copies of step s are started, spread too: a wave issues in order, and the address unit
   // takes 16 cycles for each copy, so eight waves' copies in a row would hold up all of them for a thousand cycles.
@@ -275,44 +279,48 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void tile_kernel(Jobs<T, Epi
     }
   };
   if (steps) TWO && begin >= steps1 ? enter(1, begin - steps1) : enter(0, begin);
+  // Where a compute unit has several workgroups they fill each other's waits, and one step ahead is enough; where it has one,
+  // what a step reads comes from beyond the die's cache and takes longer than a step, so two steps are on their way. The number
+  // of copies on their way is counted, so beyond the last step they go on, reading nothing.
   if constexpr (AHEAD) {
     // A step in two halves of k. While one half is multiplied the next is read into registers, across the steps too: the
     // barrier stands between the halves, where nothing of the current buffer is left to read, so the copies of the step
-    // after next can start there, and have a whole step's time to land.
+    // that will use it next can start there.
     if (steps) {
-      start(0);
-      landed();
-      start(1);
+#pragma unroll
+      for (int s = 0; s < STAGES; s++) start(s);
+      landed(std::integral_constant<int, STAGES - 1>{});
       read(0, 0, q0, p0);
     }
     for (int s = 0; s < steps; s++) {
-      half(q0, p0, q1, p1, lds + (s & 1) * STEP, 1, std::false_type{}, 0);
-      landed();
+      half(q0, p0, q1, p1, lds + (uint32_t)s % STAGES * STEP, 1, std::false_type{}, 0);
+      landed(std::integral_constant<int, STAGES - 2>{});
       // after the last step the reads get what is there, unused
-      half(q1, p1, q0, p0, lds + ((s + 1) & 1) * STEP, 0, std::true_type{}, s + 2);
-      advance(s + 2);
+      half(q1, p1, q0, p0, lds + (uint32_t)(s + 1) % STAGES * STEP, 0, std::true_type{}, s + STAGES);
+      advance(s + STAGES);
     }
   } else {
-    // Small tiles: five workgroups a compute unit fill each other's waits. (More than one step on its way gains nothing:
-    // 25 us with one, two or three of them for 1037 x 1000 x 2744.)
-    if (steps) start(0);
+    // The copies of step s + STAGES - 1 go where step s - 1 was, which everybody has left at the barrier.
+    if (steps)
+#pragma unroll
+      for (int s = 0; s < STAGES - 1; s++) start(s);
     for (int s = 0; s < steps; s++) {
-      landed();
-      start(s + 1);
+      landed(std::integral_constant<int, STAGES - 2>{});
+      start(s + STAGES - 1);
       read(s, 0, q0, p0);
       multiply(q0, p0);
       read(s, 1, q1, p1);
       multiply(q1, p1);
     }
   }
-  landed();  // no copy may outlive the workgroup, and everybody's reads are done
+  landed(All{});  // no copy may outlive the workgroup, and everybody's reads are done
 
   // The epilogue's values pass through LDS, 16 rows of a wave at a time, so that it gets eight neighbouring columns a lane and
   // eight lanes a row: whole lines where it reads and writes. A wave has its own piece of LDS and waits for nobody.
   using S = std::remove_reference_t<decltype(acc[0][0][0])>;
   constexpr int PITCH = WN + 4;  // values between rows: sixteen rows' pieces in different banks
   constexpr int LANES = (DUAL ? WN / 2 : WN) / 8, ROWS = 64 / LANES;
-  static_assert(sizeof(S) * PITCH * 16 * WAVES_M * WAVES_N <= 2 * STEP && ROWS * LANES == 64);
+  static_assert(sizeof(S) * PITCH * 16 * WAVES_M * WAVES_N <= STAGES * STEP && ROWS * LANES == 64);
   S* turn = reinterpret_cast<S*>(lds) + wave * (16 * PITCH);
   const int lq = lane >> 4;
 #pragma unroll

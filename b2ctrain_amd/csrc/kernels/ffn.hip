@@ -98,7 +98,7 @@ struct ForwardPlan {
     const int64_t M = a->rows;
     fp = up(a->d_hidden, 64);
     h = room.take<T>(M * fp);
-    gate = choose({{M, fp}}, steps_of(a->d_in), true, true);
+    gate = choose({{M, fp}}, steps_of(a->d_in), true, true, a->saved ? 6 : 2);
     down = choose({{M, a->d_out}}, steps_of(a->d_hidden), false, true);
     x = {{(const T*)a->x, a->ldx}, M, a->d_in};
     wg = {{(const T*)a->w_gate, a->ld_in}, a->d_hidden, a->d_in};
@@ -142,7 +142,7 @@ struct BackwardPlan {
     fp = up(a->d_hidden, 64);
     dgu = room.take<T>(M * 2 * fp);
     h = room.take<T>(M * fp);
-    back = choose({{M, fp}}, steps_of(a->d_out), false, false);
+    back = choose({{M, fp}}, steps_of(a->d_out), false, false, 10);
     const Extent in{fp + a->d_hidden, a->d_in}, down{a->d_out, a->d_hidden};
     const int64_t k = steps_of(M);
     dw = b->dw_down && (b->dw_gate || b->dw_up) ? choose({in, down}, k, false, false)
