@@ -176,7 +176,7 @@ inline double tile_time(int tile, int64_t n, double steps) {
 
 // The cheapest way for products of these extents, `steps` long. Tiles beyond the last full round of compute units, or all of them
 // where there are too few, may be split over k, for a write and a read of their sums at 5 TB/s. `moved`: bytes that the
-// epilogue reads and writes for each value of out; a compute unit's only tile does nothing beside them, several hide them.
+// epilogue reads and writes for each value of out; several tiles in a compute unit hide a little of them.
 inline Way choose(std::initializer_list<Extent> jobs, int64_t steps, bool dual, bool may_be_few, int moved = 2) {
   if (may_be_few && jobs.begin()->M <= kFewRows) return {FEW_ROWS, 0, 0, 1, 0};
   Way best{TILE_64, 0, 0, 1, 0};
@@ -190,7 +190,7 @@ inline Way choose(std::initializer_list<Extent> jobs, int64_t steps, bool dual, 
       count += up(e.M, side) / side * (up(e.N, cols) / cols);
       values += (double)e.M * (double)e.N;
     }
-    const double end = values * (moved - 2) / 4.5e6 * (t == TILE_256 ? 1.0 : t == TILE_128 ? 0.5 : 0.3);
+    const double end = values * (moved - 2) / 4.5e6 * (t == TILE_256 ? 0.55 : t == TILE_128 ? 0.5 : 0.4);
     const double all = tile_time(t, count, (double)steps) + end;
     if (all < least) least = all, best = {t, count, 0, 1, 0};
     for (const int64_t whole : {(int64_t)0, count / full * full}) {

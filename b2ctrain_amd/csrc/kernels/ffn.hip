@@ -25,37 +25,63 @@ bool room_ok(const void* p, size_t have, size_t need) {
   return have >= need && (need == 0 || (p && reinterpret_cast<uintptr_t>(p) % 16 == 0));
 }
 
-// A matrix copied to rows that start on 16 bytes, `pitch` values apart, zeros in the columns from `cols` up to
-// the next multiple of 8; where dropout is given, zeros in the place of what it drops too. Eight values a thread.
+// Matrices copied to rows that start on 16 bytes, `pitch` values apart, zeros in the columns from `cols` up to the next
+// multiple of 8; where dropout is given, zeros in the place of what it drops too. Eight values a thread; all of a call's
+// copies in one launch.
 template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* x, int64_t ldx, int64_t rows, int cols, T* to, int64_t pitch,
-                                                   uint32_t groups, Drop d) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, m = t / groups;
-  if (m >= rows) return;
-  const int n = (int)(t - m * groups) * 8;
-  const T* p = x + m * ldx + n;
+struct Pack {
+  Side<T> from;
+  T* to;
+  int64_t rows, pitch;
+  int cols;
+  uint32_t groups, blocks;
+  Drop drop;
+};
+template <typename T>
+struct Packs {
+  Pack<T> of[5];
+  int n = 0;
+  void add(const Side<T>& from, int64_t rows, int cols, T* to, int64_t pitch, const Drop& d) {
+    const int64_t groups = up(cols, 8) / 8;
+    of[n++] = {from, to, rows, pitch, cols, (uint32_t)groups, (uint32_t)(up(rows * groups, 256) / 256), d};
+  }
+};
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(Packs<T> all) {
+  uint32_t block = blockIdx.x;
+  int i = 0;
+  while (block >= all.of[i].blocks) block -= all.of[i++].blocks;
+  const Pack<T>& p = all.of[i];
+  const int64_t t = (int64_t)block * 256 + threadIdx.x, m = t / p.groups;
+  if (m >= p.rows) return;
+  const int n = (int)(t - m * p.groups) * 8;
+  const T* from = p.from.p + m * p.from.ld + n;
   vec<T, 8> v{};
-  if (n + 8 <= cols) {
-    __builtin_memcpy(&v, p, 16);
+  if (n + 8 <= p.cols) {
+    __builtin_memcpy(&v, from, 16);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; j++)
-      if (n + j < cols) v[j] = p[j];
+      if (n + j < p.cols) v[j] = from[j];
   }
-  if (d.threshold) {
-    const uint32_t keep = kept_bits<8>(d, (uint64_t)m * cols + n);
+  if (p.drop.threshold) {
+    const uint32_t keep = kept_bits<8>(p.drop, (uint64_t)m * p.cols + n);
 #pragma unroll
     for (int j = 0; j < 8; j++)
       if (!(keep >> j & 1)) v[j] = (T)0.f;
   }
-  *reinterpret_cast<vec<T, 8>*>(to + m * pitch + n) = v;
+  *reinterpret_cast<vec<T, 8>*>(p.to + m * p.pitch + n) = v;
 }
 template <typename T>
-int pack(Side<T> from, int64_t rows, int cols, T* to, int64_t pitch, const Drop& d, hipStream_t stream) {
-  const int64_t groups = up(cols, 8) / 8, blocks = up(rows * groups, 256) / 256;
+int make(const Packs<T>& all, hipStream_t stream) {
+  int64_t blocks = 0;
+  for (int i = 0; i < all.n; i++) {
+    blocks += all.of[i].blocks;
+    if (up(all.of[i].rows * all.of[i].groups, 256) / 256 > 0x7fffffff) return hipErrorInvalidValue;
+  }
   if (blocks == 0) return hipSuccess;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-  pack_kernel<T><<<dim3((unsigned)blocks), 256, 0, stream>>>(from.p, from.ld, rows, cols, to, pitch, (uint32_t)groups, d);
+  pack_kernel<T><<<dim3((unsigned)blocks), 256, 0, stream>>>(all);
   return hipGetLastError();
 }
 
@@ -80,7 +106,9 @@ struct Operand {
     copy = room.take<T>(rows * pitch);
   }
   Side<T> side() const { return pitch ? Side<T>{copy, pitch} : from; }
-  int make(hipStream_t stream) const { return pitch ? pack(from, rows, cols, copy, pitch, drop, stream) : hipSuccess; }
+  void add_to(Packs<T>& all) const {
+    if (pitch) all.add(from, rows, cols, copy, pitch, drop);
+  }
 };
 
 // The steps of 64 values that a sum over k takes.
@@ -120,7 +148,9 @@ int forward(const b2c_ffn_args* a, const Drop& d, hipStream_t stream) {
   Room room{(char*)a->workspace};
   const ForwardPlan<T> p(a, room);
   int rc;
-  if ((rc = p.x.make(stream)) || (rc = p.wg.make(stream)) || (rc = p.wu.make(stream)) || (rc = p.wd.make(stream))) return rc;
+  Packs<T> packs;
+  for (const Operand<T>* o : {&p.x, &p.wg, &p.wu, &p.wd}) o->add_to(packs);
+  if ((rc = make(packs, stream))) return rc;
   const GateOut<T, ACT> gate{p.h, (T*)a->saved, p.fp, a->d_hidden};
   Product<T> in{p.x.side(), p.wg.side(), {}, p.wu.side(), a->rows, p.fp, a->d_in, 0, a->rows, a->d_hidden};
   if ((rc = product<T, false, false, true, false>(in, p.gate, p.sums, gate, stream))) return rc;
@@ -176,9 +206,11 @@ int backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream) {
   const float scale = d.threshold ? d.scale : 1.f;
   int rc;
   if (!b->dx && !b->dw_gate && !b->dw_up && !b->dw_down) return hipSuccess;
-  if (M && ((rc = p.x.make(stream)) || (rc = p.wg.make(stream)) || (rc = p.wu.make(stream)) || (rc = p.wd.make(stream)) ||
-            (rc = p.dz.make(stream))))
-    return rc;
+  if (M) {
+    Packs<T> packs;
+    for (const Operand<T>* o : {&p.x, &p.wg, &p.wu, &p.wd, &p.dz}) o->add_to(packs);
+    if ((rc = make(packs, stream))) return rc;
+  }
   const Side<T> dz = p.dz.side(), x = p.x.side(), dgu{p.dgu, 2 * fp};
   const GateBack<T, ACT> back{(const T*)a->saved, p.h, p.dgu, fp, a->d_hidden, scale};
   const Product<T> dh{dz, p.wd.side(), {}, {}, M, fp, a->d_out, 0, M, a->d_hidden};

@@ -8,6 +8,40 @@ namespace b2c {
 namespace dev {
 namespace {
 
+// Weights in 8 bits as the products read them: in place where rows start on 16 bytes (columns beyond the last meet zeros of
+// the quantised rows), else copied to rows that do, all of a call's in one launch. A few rows read them anywhere.
+struct Copy {
+  const int8_t* from;
+  int64_t ld, rows, pitch;
+  int8_t* to;
+  int cols;
+  uint32_t groups, blocks;
+};
+struct Copies {
+  Copy of[3];
+  int n = 0;
+  uint32_t blocks = 0;
+};
+__global__ __launch_bounds__(256) void copies_kernel(Copies all) {
+  uint32_t block = blockIdx.x;
+  int i = 0;
+  while (block >= all.of[i].blocks) block -= all.of[i++].blocks;
+  const Copy& c = all.of[i];
+  const int64_t t = (int64_t)block * 256 + threadIdx.x, m = t / c.groups;
+  if (m >= c.rows) return;
+  const int n = (int)(t - m * c.groups) * 16;
+  const int8_t* p = c.from + m * c.ld + n;
+  vec<int8_t, 16> v{};
+  if (n + 16 <= c.cols) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+      if (n + j < c.cols) v[j] = p[j];
+  }
+  *reinterpret_cast<vec<int8_t, 16>*>(c.to + m * c.pitch + n) = v;
+}
+
 // THREADS threads to a row, sixteen values each at a time. What they read first they keep (up to HELD times sixteen), so that a
 // row is read once; the rest of a longer row is read again. A row's columns from cols to the next multiple of 16 become 0.
 template <typename T, int THREADS, int HELD>
@@ -110,24 +144,6 @@ bool sizes_ok(const b2c_i8_ffn_args* a) {
          a->d_out <= (1 << 24) && type_ok(a->dtype) && a->act >= B2C_ACT_SILU && a->act <= B2C_ACT_RELU;
 }
 
-// Weights in 8 bits as the products read them: in place where rows start on 16 bytes (columns beyond the last meet zeros of
-// the quantised rows), else copied to rows that do. A few rows read them anywhere.
-__global__ __launch_bounds__(256) void pack_kernel(const int8_t* w, int64_t ldw, int64_t rows, int cols, int8_t* to,
-                                                   int64_t pitch, uint32_t groups) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, m = t / groups;
-  if (m >= rows) return;
-  const int n = (int)(t - m * groups) * 16;
-  const int8_t* p = w + m * ldw + n;
-  vec<int8_t, 16> v{};
-  if (n + 16 <= cols) {
-    __builtin_memcpy(&v, p, 16);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; j++)
-      if (n + j < cols) v[j] = p[j];
-  }
-  *reinterpret_cast<vec<int8_t, 16>*>(to + m * pitch + n) = v;
-}
 struct Weights {
   Side<int8_t> from;
   int64_t rows;
@@ -140,14 +156,18 @@ struct Weights {
     copy = room.take<int8_t>(rows * pitch);
   }
   Side<int8_t> side() const { return pitch ? Side<int8_t>{copy, pitch} : from; }
-  int make(hipStream_t stream) const {
-    if (!pitch) return hipSuccess;
-    const int64_t groups = up(cols, 16) / 16, blocks = up(rows * groups, 256) / 256;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    pack_kernel<<<dim3((unsigned)blocks), 256, 0, stream>>>(from.p, from.ld, rows, cols, copy, pitch, (uint32_t)groups);
-    return hipGetLastError();
+  void add_to(Copies& all) const {
+    if (!pitch) return;
+    const int64_t groups = up(cols, 16) / 16, blocks = up(rows * groups, 256) / 256;  // at most 2^24 rows of 8192 groups
+    all.of[all.n++] = {from.p, from.ld, rows, pitch, copy, cols, (uint32_t)groups, (uint32_t)blocks};
+    all.blocks += (uint32_t)blocks;
   }
 };
+int make(const Copies& all, hipStream_t stream) {
+  if (all.blocks == 0) return hipSuccess;
+  copies_kernel<<<dim3(all.blocks), 256, 0, stream>>>(all);
+  return hipGetLastError();
+}
 int64_t steps_of(int64_t k) { return up(k, 128) / 128; }
 
 struct LinearPlan {
@@ -242,8 +262,10 @@ extern "C" int b2c_hip_i8_linear(const b2c_i8_linear_args* a, hipStream_t stream
     return hipErrorInvalidValue;
   Room room{(char*)a->workspace};
   const LinearPlan p(a, room);
+  Copies copies;
+  p.w.add_to(copies);
   int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.q, p.kp, p.sx, stream);
-  if (rc || (rc = p.w.make(stream))) return rc;
+  if (rc || (rc = make(copies, stream))) return rc;
   const Product<int8_t> out{{p.q, p.kp}, p.w.side(), {}, {}, a->rows, a->d_out, a->d_in, 0, a->rows, a->d_out};
   return scaled(out, p.way, p.sums, p.sx, a->w_scale, a->dtype, a->y, a->ldy, stream);
 }
@@ -266,8 +288,10 @@ extern "C" int b2c_hip_i8_ffn(const b2c_i8_ffn_args* a, hipStream_t stream) {
   if (is_i8_head(a)) return i8_head(a, stream);
   Room room{(char*)a->workspace};
   const BlockPlan p(a, room);
+  Copies copies;
+  for (const Weights* w : {&p.wg, &p.wu, &p.wd}) w->add_to(copies);
   int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.qx, p.kp, p.s, stream);
-  if (rc || (rc = p.wg.make(stream)) || (rc = p.wu.make(stream)) || (rc = p.wd.make(stream))) return rc;
+  if (rc || (rc = make(copies, stream))) return rc;
   if (a->act == B2C_ACT_SILU) rc = gated<B2C_ACT_SILU>(p, a, stream);
   else if (a->act == B2C_ACT_GELU) rc = gated<B2C_ACT_GELU>(p, a, stream);
   else rc = gated<B2C_ACT_RELU>(p, a, stream);
