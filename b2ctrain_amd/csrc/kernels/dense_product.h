@@ -140,7 +140,9 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Product<T> a, Epi epi) {
 // ---- the choice --------------------------------------------------------------------------------------------
 
 enum { TILE_256, TILE_128, TILE_64, FEW_ROWS };
-constexpr int64_t kFewRows = 32;
+// Up to 8 rows by the kernel for a few, up to 32 where the tiles would need the weights copied first: 16 rows of a 4096-11264
+// block take 78 us that way and 66 by tiles, one row 54.
+inline bool few_rows(int64_t M, bool straight) { return M <= 8 || (M <= 32 && !straight); }
 
 // Tiles of one size; the first `whole` of them each by one workgroup, the rest by `parts`, through `sums` bytes of workspace.
 struct Way {
@@ -177,8 +179,8 @@ inline double tile_time(int tile, int64_t n, double steps) {
 // The cheapest way for products of these extents, `steps` long. Tiles beyond the last full round of compute units, or all of them
 // where there are too few, may be split over k, for a write and a read of their sums at 5 TB/s. `moved`: bytes that the
 // epilogue reads and writes for each value of out; several tiles in a compute unit hide a little of them.
-inline Way choose(std::initializer_list<Extent> jobs, int64_t steps, bool dual, bool may_be_few, int moved = 2) {
-  if (may_be_few && jobs.begin()->M <= kFewRows) return {FEW_ROWS, 0, 0, 1, 0};
+inline Way choose(std::initializer_list<Extent> jobs, int64_t steps, bool dual, bool few, int moved = 2) {
+  if (few) return {FEW_ROWS, 0, 0, 1, 0};
   Way best{TILE_64, 0, 0, 1, 0};
   double least = 1e30;
   for (int t = 0; t < 3; t++) {

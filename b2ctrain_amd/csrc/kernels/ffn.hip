@@ -126,18 +126,19 @@ struct ForwardPlan {
     const int64_t M = a->rows;
     fp = up(a->d_hidden, 64);
     h = room.take<T>(M * fp);
-    gate = choose({{M, fp}}, steps_of(a->d_in), true, true, a->saved ? 6 : 2);
-    down = choose({{M, a->d_out}}, steps_of(a->d_hidden), false, true);
+    const bool in = direct(a->w_gate, a->ld_in, a->d_in) && direct(a->w_up, a->ld_in, a->d_in);
+    const bool out = direct(a->w_down, a->ld_out, a->d_hidden), few = few_rows(M, in && out);
+    gate = choose({{M, fp}}, steps_of(a->d_in), true, few, a->saved ? 6 : 2);
+    down = choose({{M, a->d_out}}, steps_of(a->d_hidden), false, few);
     x = {{(const T*)a->x, a->ldx}, M, a->d_in};
     wg = {{(const T*)a->w_gate, a->ld_in}, a->d_hidden, a->d_in};
     wu = {{(const T*)a->w_up, a->ld_in}, a->d_hidden, a->d_in};
     wd = {{(const T*)a->w_down, a->ld_out}, a->d_out, a->d_hidden};
-    if (gate.tile != FEW_ROWS) {  // all or none along d_in: a copy's zeros beyond the last column meet zeros
+    if (!few) {  // all or none along d_in: a copy's zeros beyond the last column meet zeros
       x.place(room, direct(a->x, a->ldx, a->d_in));
-      const bool in = direct(a->w_gate, a->ld_in, a->d_in) && direct(a->w_up, a->ld_in, a->d_in);
       wg.place(room, in);
       wu.place(room, in);
-      wd.place(room, direct(a->w_down, a->ld_out, a->d_hidden));
+      wd.place(room, out);
     }
     sums = room.take<char>(std::max(gate.sums, down.sums));
   }

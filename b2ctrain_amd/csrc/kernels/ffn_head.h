@@ -377,7 +377,7 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float* sums, int64
 // ---- host --------------------------------------------------------------------------------------------------
 
 // Whether a block is such a head. Its rows are more than a few, since the weights are rearranged in each call.
-inline bool is_head(const b2c_ffn_args* a) { return a->rows > kFewRows && a->d_in <= 128 && a->d_out <= 128; }
+inline bool is_head(const b2c_ffn_args* a) { return a->rows > 32 && a->d_in <= 128 && a->d_out <= 128; }
 inline int head_steps(const b2c_ffn_args* a) {
   const int n = (int)(up(std::max(a->d_in, a->d_out), 32) / 32);
   return n == 3 ? 4 : n;

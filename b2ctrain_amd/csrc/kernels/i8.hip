@@ -150,8 +150,11 @@ struct Weights {
   int cols;
   int8_t* copy = nullptr;
   int64_t pitch = 0;
+  bool straight() const {
+    return reinterpret_cast<uintptr_t>(from.p) % 16 == 0 && from.ld % 16 == 0 && cols % 16 == 0 && from.ld < (1 << 22);
+  }
   void place(Room& room, bool few) {
-    if (few || (reinterpret_cast<uintptr_t>(from.p) % 16 == 0 && from.ld % 16 == 0 && cols % 16 == 0 && from.ld < (1 << 22))) return;
+    if (few || straight()) return;
     pitch = up(cols, 128);
     copy = room.take<int8_t>(rows * pitch);
   }
@@ -181,9 +184,10 @@ struct LinearPlan {
     kp = up(a->d_in, 128);
     q = room.take<int8_t>(a->rows * kp);
     sx = room.take<float>(a->rows);
-    way = choose({{a->rows, a->d_out}}, steps_of(a->d_in), false, true);
     w = {{a->w, a->ldw}, a->d_out, a->d_in};
-    w.place(room, way.tile == FEW_ROWS);
+    const bool few = few_rows(a->rows, w.straight());
+    way = choose({{a->rows, a->d_out}}, steps_of(a->d_in), false, few);
+    w.place(room, few);
     sums = room.take<char>(way.sums);
   }
 };
@@ -201,12 +205,12 @@ struct BlockPlan {
     qh = room.take<int8_t>(a->rows * fp);
     qx = room.take<int8_t>(a->rows * kp);
     s = room.take<float>(a->rows);
-    gate = choose({{a->rows, a->d_hidden}}, steps_of(a->d_in), true, true);
-    down = choose({{a->rows, a->d_out}}, steps_of(a->d_hidden), false, true);
-    const bool few = gate.tile == FEW_ROWS;
     wg = {{a->w_gate, a->ld_in}, a->d_hidden, a->d_in};
     wu = {{a->w_up, a->ld_in}, a->d_hidden, a->d_in};
     wd = {{a->w_down, a->ld_out}, a->d_out, a->d_hidden};
+    const bool few = few_rows(a->rows, wg.straight() && wu.straight() && wd.straight());
+    gate = choose({{a->rows, a->d_hidden}}, steps_of(a->d_in), true, few, 4);
+    down = choose({{a->rows, a->d_out}}, steps_of(a->d_hidden), false, few);
     wg.place(room, few);
     wu.place(room, few);
     wd.place(room, few);
@@ -248,7 +252,7 @@ extern "C" int b2c_hip_quantize_rows(const b2c_quantize_args* a, hipStream_t str
 }
 
 extern "C" size_t b2c_i8_linear_workspace_bytes(const b2c_i8_linear_args* a) {
-  if (!sizes_ok(a) || a->rows == 0) return 0;
+  if (!sizes_ok(a) || a->rows == 0 || is_i8_narrow(a)) return 0;
   Room room{nullptr};
   LinearPlan(a, room);
   return room.used;
@@ -260,6 +264,7 @@ extern "C" int b2c_hip_i8_linear(const b2c_i8_linear_args* a, hipStream_t stream
       !good(a->y, a->ldy, a->d_out, size_of(a->dtype)) ||
       !room_ok(a->workspace, a->workspace_bytes, b2c_i8_linear_workspace_bytes(a)))
     return hipErrorInvalidValue;
+  if (is_i8_narrow(a)) return i8_narrow(a, stream);
   Room room{(char*)a->workspace};
   const LinearPlan p(a, room);
   Copies copies;

@@ -56,6 +56,33 @@ __device__ __forceinline__ uint32_t over_row(uint32_t top) {  // of the four lan
   return b > c ? b : c;
 }
 
+// Row m of x in 8 bits, as the matrix instruction's operand (lane group q4 holds values 16 q4 .. of each 64), and its scale.
+template <int KI>
+__device__ __forceinline__ RowScale row_in_bytes(const void* x, int64_t ldx, int dtype, int64_t m, int64_t M, int K, int q4,
+                                                 i32x4 (&q)[KI]) {
+  float v[KI][16];
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < KI; k++) {
+    if (dtype == B2C_BF16) sixteen<bf16>(x, ldx, m, M, k * 64 + q4 * 16, K, v[k]);
+    else if (dtype == B2C_F16) sixteen<f16>(x, ldx, m, M, k * 64 + q4 * 16, K, v[k]);
+    else sixteen<float>(x, ldx, m, M, k * 64 + q4 * 16, K, v[k]);
+#pragma unroll
+    for (int j = 0; j < 16; j++) top = magnitude(v[k][j]) > top ? magnitude(v[k][j]) : top;
+  }
+  const RowScale s(over_row(top));
+#pragma unroll
+  for (int k = 0; k < KI; k++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) q[k][j] = (int)bytes4(s(v[k][4 * j]), s(v[k][4 * j + 1]), s(v[k][4 * j + 2]), s(v[k][4 * j + 3]));
+  return s;
+}
+__device__ __forceinline__ void put_as(int dtype, void* y, int64_t ldy, int64_t m, int n, int cols, const float (&v)[8]) {
+  if (dtype == B2C_BF16) put<8>((bf16*)y, ldy, m, n, cols, v);
+  else if (dtype == B2C_F16) put<8>((f16*)y, ldy, m, n, cols, v);
+  else put<8>((float*)y, ldy, m, n, cols, v);
+}
+
 template <int ACT, int KI, int NC>
 __global__ __launch_bounds__(512) void head_kernel(b2c_i8_ffn_args a, const int8_t* frags, int chunks) {
   constexpr int N = head_fragments(KI), OT = 4 * KI;
@@ -75,25 +102,11 @@ __global__ __launch_bounds__(512) void head_kernel(b2c_i8_ffn_args a, const int8
   const int64_t M = a.rows, tiles = (M + 15) / 16;
   for (int64_t tile = (int64_t)blockIdx.x * 8 + wave; tile < tiles; tile += (int64_t)gridDim.x * 8) {
     const int64_t m = tile * 16 + (lane & 15);
-    float x[KI][16];
-    uint32_t top = 0;
-#pragma unroll
-    for (int k = 0; k < KI; k++) {
-      if (a.dtype == B2C_BF16) sixteen<bf16>(a.x, a.ldx, m, M, k * 64 + q4 * 16, a.d_in, x[k]);
-      else if (a.dtype == B2C_F16) sixteen<f16>(a.x, a.ldx, m, M, k * 64 + q4 * 16, a.d_in, x[k]);
-      else sixteen<float>(a.x, a.ldx, m, M, k * 64 + q4 * 16, a.d_in, x[k]);
-#pragma unroll
-      for (int j = 0; j < 16; j++) top = magnitude(x[k][j]) > top ? magnitude(x[k][j]) : top;
-    }
-    const RowScale rx(over_row(top));
     i32x4 qx[KI];
-#pragma unroll
-    for (int k = 0; k < KI; k++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) qx[k][j] = (int)bytes4(rx(x[k][4 * j]), rx(x[k][4 * j + 1]), rx(x[k][4 * j + 2]), rx(x[k][4 * j + 3]));
+    const RowScale rx = row_in_bytes<KI>(a.x, a.ldx, a.dtype, m, M, a.d_in, q4, qx);
 
     float h[NC][16];
-    top = 0;
+    uint32_t top = 0;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
       asm volatile("" ::: "memory");  // the weights stay in LDS: held over the loop, they would fill the registers
@@ -108,13 +121,14 @@ __global__ __launch_bounds__(512) void head_kernel(b2c_i8_ffn_args a, const int8
         const f32x4 a4 = sg[c * 16 + q4 * 4 + t], b4 = su[c * 16 + q4 * 4 + t];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          const float v = act<ACT>((float)g[r] * rx.scale * a4[r]) * ((float)u[r] * rx.scale * b4[r]);
+          const float v = act<ACT>((float)g[r] * (rx.scale * a4[r])) * ((float)u[r] * b4[r]);  // x's scale of u follows below
           h[c][t * 4 + r] = v;
           top = magnitude(v) > top ? magnitude(v) : top;
         }
       }
     }
     const RowScale rh(over_row(top));
+    const float sh = rh.scale * rx.scale;
     i32x4 y[OT] = {};
 #pragma unroll
     for (int c = 0; c < NC; c++) {
@@ -124,7 +138,7 @@ __global__ __launch_bounds__(512) void head_kernel(b2c_i8_ffn_args a, const int8
       for (int j = 0; j < 4; j++) {
         uint32_t b[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) b[r] = rh(h[c][4 * j + r]);
+        for (int r = 0; r < 4; r++) b[r] = rh.near(h[c][4 * j + r]);
         qh[j] = (int)bytes4(b[0], b[1], b[2], b[3]);
       }
 #pragma unroll
@@ -138,10 +152,58 @@ __global__ __launch_bounds__(512) void head_kernel(b2c_i8_ffn_args a, const int8
       const f32x4 a4 = sd[n / 4], b4 = sd[n / 4 + 1];
       float v[8];
 #pragma unroll
-      for (int r = 0; r < 4; r++) v[r] = (float)y[t][r] * rh.scale * a4[r], v[4 + r] = (float)y[t + 1][r] * rh.scale * b4[r];
-      if (a.dtype == B2C_BF16) put<8>((bf16*)a.y, a.ldy, m, n, a.d_out, v);
-      else if (a.dtype == B2C_F16) put<8>((f16*)a.y, a.ldy, m, n, a.d_out, v);
-      else put<8>((float*)a.y, a.ldy, m, n, a.d_out, v);
+      for (int r = 0; r < 4; r++) v[r] = (float)y[t][r] * sh * a4[r], v[4 + r] = (float)y[t + 1][r] * sh * b4[r];
+      put_as(a.dtype, a.y, a.ldy, m, n, a.d_out, v);
+    }
+  }
+}
+
+// The same for one layer: 16 rows of x to a wave, quantised in registers, times weights that all lie in LDS. Bound by memory: what
+// a tile of 128 outputs would do in one step of k is over before its copies could be hidden.
+template <int KI>
+__global__ __launch_bounds__(512) void linear_kernel(b2c_i8_linear_args a, int chunks) {
+  using A = vec<int8_t, 16>;
+  extern __shared__ __attribute__((aligned(1024))) char room[];
+  A(*w)[64] = reinterpret_cast<A(*)[64]>(room);  // fragment 4 KI c + KI t + k: outputs 64 c + 16 (i / 4) + 4 t + i % 4
+  float* sw = reinterpret_cast<float*>(room + (size_t)chunks * 4 * KI * 1024);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q4 = lane >> 4, i = lane & 15;
+  for (int f = wave; f < chunks * 4 * KI; f += 8) {
+    const int o = f / (4 * KI) * 64 + (i >> 2) * 16 + f % (4 * KI) / KI * 4 + (i & 3), k = f % KI * 64 + q4 * 16;
+    A v{};
+    if (o < a.d_out) {
+      const int8_t* p = a.w + o * a.ldw + k;
+      if (k + 16 <= a.d_in) {
+        __builtin_memcpy(&v, p, 16);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+          if (k + j < a.d_in) v[j] = p[j];
+      }
+    }
+    w[f][lane] = v;
+  }
+  for (int j = threadIdx.x; j < chunks * 64; j += 512) sw[j] = j < a.d_out ? a.w_scale[j] : 0.f;
+  __syncthreads();
+  const int64_t M = a.rows, tiles = (M + 15) / 16;
+  for (int64_t tile = (int64_t)blockIdx.x * 8 + wave; tile < tiles; tile += (int64_t)gridDim.x * 8) {
+    const int64_t m = tile * 16 + i;
+    i32x4 qx[KI];
+    const RowScale rx = row_in_bytes<KI>(a.x, a.ldx, a.dtype, m, M, a.d_in, q4, qx);
+    for (int c = 0; c < chunks; c++) {
+      i32x4 y[4] = {};
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int k = 0; k < KI; k++) y[t] = mfma(w[c * 4 * KI + t * KI + k][lane], __builtin_bit_cast(A, qx[k]), y[t]);
+      const int n = c * 64 + q4 * 16;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if (m >= M || n + h * 8 >= a.d_out) continue;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = (float)y[h * 2 + j / 4][j % 4] * (rx.scale * sw[n + h * 8 + j]);
+        put_as(a.dtype, a.y, a.ldy, m, n + h * 8, a.d_out, v);
+      }
     }
   }
 }
@@ -176,6 +238,11 @@ int run(const b2c_i8_ffn_args* a, int8_t* frags, hipStream_t stream) {
   return launch<B2C_ACT_RELU, KI>(a, frags, stream);
 }
 
+constexpr int64_t kRoom = 64 << 10;  // of LDS for a layer's weights, so that a compute unit holds two workgroups
+int64_t linear_room(const b2c_i8_linear_args* a) {
+  return up(a->d_out, 64) / 64 * (4 * (a->d_in <= 64 ? 1 : 2) * 1024 + 256);
+}
+
 }  // namespace
 
 bool is_i8_head(const b2c_i8_ffn_args* a) {
@@ -184,6 +251,16 @@ bool is_i8_head(const b2c_i8_ffn_args* a) {
 size_t i8_head_bytes(const b2c_i8_ffn_args* a) { return (size_t)chunks_of(a) * head_fragments(width_of(a)) * 1024; }
 int i8_head(const b2c_i8_ffn_args* a, hipStream_t stream) {
   return width_of(a) == 1 ? run<1>(a, (int8_t*)a->workspace, stream) : run<2>(a, (int8_t*)a->workspace, stream);
+}
+
+
+bool is_i8_narrow(const b2c_i8_linear_args* a) { return a->rows > kI8HeadRows && a->d_in <= 128 && linear_room(a) <= kRoom; }
+int i8_narrow(const b2c_i8_linear_args* a, hipStream_t stream) {
+  const int chunks = (int)(up(a->d_out, 64) / 64);
+  const dim3 grid((unsigned)std::min<int64_t>(up(a->rows, 128) / 128, 512));
+  if (a->d_in <= 64) linear_kernel<1><<<grid, 512, (size_t)linear_room(a), stream>>>(*a, chunks);
+  else linear_kernel<2><<<grid, 512, (size_t)linear_room(a), stream>>>(*a, chunks);
+  return hipGetLastError();
 }
 
 }  // namespace dev
