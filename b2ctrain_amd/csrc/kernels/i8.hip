@@ -130,6 +130,136 @@ int quantize(const void* x, int64_t ldx, int dtype, int64_t rows, int64_t cols, 
   return quantize((const bf16*)x, ldx, rows, cols, q, ldq, scale, stream);
 }
 
+// A few rows of a product, quantised on the way: every workgroup takes all of x (at most kHeld values, which the caches hand
+// out) to LDS in 8 bits, while the first of its weights are on their way, and then streams 16 rows of the weights (DUAL: of
+// each of the two), every eighth 256-byte run a wave. One launch less than quantising first: 4096 -> 4096 for one row takes
+// 7 us where two launches take 10.
+constexpr int kHeld = 32768, kHeldRows = 8;
+inline bool held(int64_t rows, int64_t cols) { return rows <= kHeldRows && rows * up(cols, 16) <= kHeld; }
+
+template <typename TX, bool DUAL, typename Epi>
+__global__ __launch_bounds__(512) void quantised_rows_kernel(const TX* x, int64_t ldx, Product<int8_t> a, Epi epi) {
+  constexpr int PL = DUAL ? 2 : 1, RUN = 256;
+  using A = vec<int8_t, 16>;
+  __shared__ __attribute__((aligned(16))) int8_t qx[kHeld];
+  __shared__ uint32_t tops[8][kHeldRows];
+  __shared__ float scales[kHeldRows];
+  __shared__ i32x4 sums[8][PL][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, q4 = lane >> 4;
+  const int64_t n = (int64_t)blockIdx.x * 16 + row;
+  const int K = (int)a.K, M = (int)a.M, pitch = (K + 15) / 16 * 16;
+  auto load = [&](const Side<int8_t>& s, int k) {
+    A v{};
+    if (n >= a.p_lim || k >= K) return v;
+    const int8_t* p = s.p + n * s.ld + k;
+    if (k + 16 <= K) {
+      __builtin_memcpy(&v, p, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (k + j < K) v[j] = p[j];
+    }
+    return v;
+  };
+  A p[2][PL][4];
+  auto fetch = [&](int b, int k0) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      p[b][0][c] = load(a.p, k0 + (c * 4 + q4) * 16);
+      if constexpr (DUAL) p[b][1][c] = load(a.p2, k0 + (c * 4 + q4) * 16);
+    }
+  };
+  fetch(0, wave * RUN);
+
+  auto values = [&](int m, int k) {
+    vec<TX, 16> v{};
+    const TX* from = x + m * ldx + k;
+    if (k + 16 <= K) {
+      __builtin_memcpy(&v, from, sizeof(v));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (k + j < K) v[j] = from[j];
+    }
+    return v;
+  };
+  for (int m = 0; m < M; m++) {
+    uint32_t top = 0;
+    for (int k = (int)threadIdx.x * 16; k < K; k += 512 * 16) {
+      const vec<TX, 16> v = values(m, k);
+#pragma unroll
+      for (int j = 0; j < 16; j++) top = magnitude((float)v[j]) > top ? magnitude((float)v[j]) : top;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const uint32_t b = __shfl_xor(top, o);
+      top = b > top ? b : top;
+    }
+    if (lane == 0) tops[wave][m] = top;
+  }
+  __syncthreads();
+  for (int m = 0; m < M; m++) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int w = 0; w < 8; w++) top = tops[w][m] > top ? tops[w][m] : top;
+    const RowScale s(top);
+    if (threadIdx.x == 0) scales[m] = s.scale;
+    for (int k = (int)threadIdx.x * 16; k < K; k += 512 * 16) {
+      const vec<TX, 16> v = values(m, k);
+      vec<uint32_t, 4> b;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        b[j] = bytes4(s((float)v[4 * j]), s((float)v[4 * j + 1]), s((float)v[4 * j + 2]), s((float)v[4 * j + 3]));
+      *reinterpret_cast<vec<uint32_t, 4>*>(qx + m * pitch + k) = b;
+    }
+  }
+  __syncthreads();
+
+  i32x4 acc[PL] = {};
+  auto multiply = [&](int b, int k0) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const int k = k0 + (c * 4 + q4) * 16;
+      const A v = row < M && k < K ? *reinterpret_cast<const A*>(qx + row * pitch + k) : A{};
+#pragma unroll
+      for (int d = 0; d < PL; d++) acc[d] = mfma(p[b][d][c], v, acc[d]);
+    }
+  };
+  for (int k0 = wave * RUN; k0 < K; k0 += 16 * RUN) {
+    fetch(1, k0 + 8 * RUN);
+    multiply(0, k0);
+    fetch(0, k0 + 16 * RUN);
+    multiply(1, k0 + 8 * RUN);
+  }
+#pragma unroll
+  for (int d = 0; d < PL; d++) sums[wave][d][lane] = acc[d];
+  __syncthreads();
+  if (wave) return;
+  i32x4 v[PL];
+#pragma unroll
+  for (int d = 0; d < PL; d++) {
+    v[d] = sums[0][d][lane];
+#pragma unroll
+    for (int w = 1; w < 8; w++) v[d] += sums[w][d][lane];
+  }
+  const int n4 = (int)blockIdx.x * 16 + q4 * 4;
+  if (row >= M || n4 >= a.N) return;
+  epi.sx = scales;
+  int g[4], u[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) g[j] = v[0][j], u[j] = v[PL - 1][j];
+  if constexpr (DUAL) epi.template operator()<4>(0u, row, n4, g, u);
+  else epi.template operator()<4>(0u, row, n4, g);
+}
+template <bool DUAL, typename Epi>
+int quantised_rows(const void* x, int64_t ldx, int dtype, const Product<int8_t>& a, const Epi& epi, hipStream_t stream) {
+  const dim3 grid((unsigned)(up(a.N, 16) / 16));
+  if (dtype == B2C_F32) quantised_rows_kernel<float, DUAL><<<grid, 512, 0, stream>>>((const float*)x, ldx, a, epi);
+  else if (dtype == B2C_F16) quantised_rows_kernel<f16, DUAL><<<grid, 512, 0, stream>>>((const f16*)x, ldx, a, epi);
+  else quantised_rows_kernel<bf16, DUAL><<<grid, 512, 0, stream>>>((const bf16*)x, ldx, a, epi);
+  return hipGetLastError();
+}
+
 bool type_ok(int t) { return t == B2C_F32 || t == B2C_F16 || t == B2C_BF16; }
 size_t size_of(int t) { return t == B2C_F32 ? 4 : 2; }
 bool room_ok(const void* p, size_t have, size_t need) {
@@ -218,22 +348,30 @@ struct BlockPlan {
   }
 };
 
+// x, ldx, type: where the rows still have to be quantised (held()), else null
+struct Raw {
+  const void* x;
+  int64_t ldx;
+  int dtype;
+};
 template <typename T>
 int scaled(const Product<int8_t>& p, const Way& way, void* sums, const float* sx, const float* sw, void* y, int64_t ldy,
-           hipStream_t stream) {
+           const Raw& raw, hipStream_t stream) {
   const ScaledOut<T> out{(T*)y, ldy, sx, sw, (int)p.N};
+  if (raw.x) return quantised_rows<false>(raw.x, raw.ldx, raw.dtype, p, out, stream);
   return product<int8_t, false, false, false, false>(p, way, sums, out, stream);
 }
 int scaled(const Product<int8_t>& p, const Way& way, void* sums, const float* sx, const float* sw, int dtype, void* y,
-           int64_t ldy, hipStream_t stream) {
-  if (dtype == B2C_F32) return scaled<float>(p, way, sums, sx, sw, y, ldy, stream);
-  if (dtype == B2C_F16) return scaled<f16>(p, way, sums, sx, sw, y, ldy, stream);
-  return scaled<bf16>(p, way, sums, sx, sw, y, ldy, stream);
+           int64_t ldy, const Raw& raw, hipStream_t stream) {
+  if (dtype == B2C_F32) return scaled<float>(p, way, sums, sx, sw, y, ldy, raw, stream);
+  if (dtype == B2C_F16) return scaled<f16>(p, way, sums, sx, sw, y, ldy, raw, stream);
+  return scaled<bf16>(p, way, sums, sx, sw, y, ldy, raw, stream);
 }
 template <int ACT>
-int gated(const BlockPlan& p, const b2c_i8_ffn_args* a, hipStream_t stream) {
+int gated(const BlockPlan& p, const b2c_i8_ffn_args* a, const Raw& raw, hipStream_t stream) {
   const ScaledGate<ACT> out{p.h, p.s, a->s_gate, a->s_up, p.fp, a->d_hidden};
   const Product<int8_t> in{{p.qx, p.kp}, p.wg.side(), {}, p.wu.side(), a->rows, a->d_hidden, a->d_in, 0, a->rows, a->d_hidden};
+  if (raw.x) return quantised_rows<true>(raw.x, raw.ldx, raw.dtype, in, out, stream);
   return product<int8_t, false, false, true, false>(in, p.gate, p.sums, out, stream);
 }
 
@@ -267,12 +405,17 @@ extern "C" int b2c_hip_i8_linear(const b2c_i8_linear_args* a, hipStream_t stream
   if (is_i8_narrow(a)) return i8_narrow(a, stream);
   Room room{(char*)a->workspace};
   const LinearPlan p(a, room);
-  Copies copies;
-  p.w.add_to(copies);
-  int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.q, p.kp, p.sx, stream);
-  if (rc || (rc = make(copies, stream))) return rc;
   const Product<int8_t> out{{p.q, p.kp}, p.w.side(), {}, {}, a->rows, a->d_out, a->d_in, 0, a->rows, a->d_out};
-  return scaled(out, p.way, p.sums, p.sx, a->w_scale, a->dtype, a->y, a->ldy, stream);
+  Raw raw{};
+  if (p.way.tile == FEW_ROWS && held(a->rows, a->d_in)) {
+    raw = {a->x, a->ldx, a->dtype};
+  } else {
+    Copies copies;
+    p.w.add_to(copies);
+    int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.q, p.kp, p.sx, stream);
+    if (rc || (rc = make(copies, stream))) return rc;
+  }
+  return scaled(out, p.way, p.sums, p.sx, a->w_scale, a->dtype, a->y, a->ldy, raw, stream);
 }
 
 extern "C" size_t b2c_i8_ffn_workspace_bytes(const b2c_i8_ffn_args* a) {
@@ -293,15 +436,23 @@ extern "C" int b2c_hip_i8_ffn(const b2c_i8_ffn_args* a, hipStream_t stream) {
   if (is_i8_head(a)) return i8_head(a, stream);
   Room room{(char*)a->workspace};
   const BlockPlan p(a, room);
-  Copies copies;
-  for (const Weights* w : {&p.wg, &p.wu, &p.wd}) w->add_to(copies);
-  int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.qx, p.kp, p.s, stream);
-  if (rc || (rc = make(copies, stream))) return rc;
-  if (a->act == B2C_ACT_SILU) rc = gated<B2C_ACT_SILU>(p, a, stream);
-  else if (a->act == B2C_ACT_GELU) rc = gated<B2C_ACT_GELU>(p, a, stream);
-  else rc = gated<B2C_ACT_RELU>(p, a, stream);
+  int rc = hipSuccess;
+  Raw raw{};
+  if (p.gate.tile == FEW_ROWS && held(a->rows, a->d_in)) {
+    raw = {a->x, a->ldx, a->dtype};
+  } else {
+    Copies copies;
+    for (const Weights* w : {&p.wg, &p.wu, &p.wd}) w->add_to(copies);
+    rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.qx, p.kp, p.s, stream);
+    if (rc || (rc = make(copies, stream))) return rc;
+  }
+  if (a->act == B2C_ACT_SILU) rc = gated<B2C_ACT_SILU>(p, a, raw, stream);
+  else if (a->act == B2C_ACT_GELU) rc = gated<B2C_ACT_GELU>(p, a, raw, stream);
+  else rc = gated<B2C_ACT_RELU>(p, a, raw, stream);
   if (rc) return rc;
-  if ((rc = quantize(p.h, p.fp, B2C_F32, a->rows, a->d_hidden, p.qh, p.fp, p.s, stream))) return rc;
+  raw = {};
+  if (p.down.tile == FEW_ROWS && held(a->rows, a->d_hidden)) raw = {p.h, p.fp, B2C_F32};
+  else if ((rc = quantize(p.h, p.fp, B2C_F32, a->rows, a->d_hidden, p.qh, p.fp, p.s, stream))) return rc;
   const Product<int8_t> out{{p.qh, p.fp}, p.wd.side(), {}, {}, a->rows, a->d_out, a->d_hidden, 0, a->rows, a->d_out};
-  return scaled(out, p.down, p.sums, p.s, a->s_down, a->dtype, a->y, a->ldy, stream);
+  return scaled(out, p.down, p.sums, p.s, a->s_down, a->dtype, a->y, a->ldy, raw, stream);
 }
