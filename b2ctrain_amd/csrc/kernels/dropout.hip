@@ -53,19 +53,40 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* x, int64_t ldx, cons
     for (int j = 0; j < 8; j++) bits |= (uint32_t)kept(w, j, d.threshold) << j;
   }
   const uint32_t down = 64 / cols, right = 64 % cols;
-  uint64_t m = (first + lane) / cols;
+  const uint64_t m = (first + lane) / cols;
   uint32_t c = (uint32_t)((first + lane) - m * cols);
+  // Places advance by sums: a product m ld for each element took longer than the memory does.
+  int64_t px = (int64_t)m * ldx + c, pr = (int64_t)m * ldr + c, py = (int64_t)m * ldy + c;
+  const int64_t dx = (int64_t)down * ldx + right, dr = (int64_t)down * ldr + right, dy = (int64_t)down * ldy + right;
+  // All loads first and without conditions (a last, partial wave reads its first element again for those that are not there): one
+  // at a time, each store holds up the next load, which it might be the source of.
+  const bool whole = first + 512 <= n;
+  float v[8], add[8];
+  int64_t to[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const bool there = whole || first + j * 64 + lane < n;
+    const int64_t m0 = (int64_t)(first / cols), c0 = (int64_t)(first - (uint64_t)m0 * cols);
+    v[j] = (float)x[there ? px : m0 * ldx + c0];
+    add[j] = r ? (float)r[there ? pr : m0 * ldr + c0] : 0.f;
+    to[j] = there ? py : -1;
+    c += right;
+    px += dx;
+    pr += dr;
+    py += dy;
+    if (c >= cols) {
+      c -= cols;
+      px += ldx - (int64_t)cols;
+      pr += ldr - (int64_t)cols;
+      py += ldy - (int64_t)cols;
+    }
+  }
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     const bool keep = __shfl(bits, j * 8 + (lane >> 3)) >> (lane & 7) & 1;
-    if (first + j * 64 + lane < n) {
-      float v = keep ? (float)x[m * ldx + c] * d.scale : 0.f;
-      if (r) v += (float)r[m * ldr + c];
-      y[m * ldy + c] = (T)v;
-    }
-    m += down;
-    c += right;
-    if (c >= cols) c -= cols, m++;
+    float o = keep ? v[j] * d.scale : 0.f;
+    if (r) o += add[j];
+    if (to[j] >= 0) y[to[j]] = (T)o;
   }
 }
 
