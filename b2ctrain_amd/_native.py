@@ -129,6 +129,8 @@ EXPORTS = [
     "b2c_png_decode", "b2c_image_decode", "b2c_image_resample", "b2c_dataset_load", "b2c_dataset_destroy", "b2c_dataset_count", "b2c_dataset_view_info",
     "b2c_dataset_view_read", "b2c_dataset_view_upload", "b2c_dataset_points", "b2c_dataset_summary",
     # dense operators (nn.py)
+    "b2c_dense_create", "b2c_dense_destroy", "b2c_dropout", "b2c_feed_forward", "b2c_feed_forward_backward",
+    "b2c_quantize_rows", "b2c_i8_linear", "b2c_i8_feed_forward",
     "b2c_hip_dropout", "b2c_ffn_saved_bytes", "b2c_ffn_workspace_bytes", "b2c_hip_ffn_forward",
     "b2c_ffn_grad_workspace_bytes", "b2c_hip_ffn_backward", "b2c_hip_quantize_rows", "b2c_i8_linear_workspace_bytes",
     "b2c_hip_i8_linear", "b2c_i8_ffn_workspace_bytes", "b2c_hip_i8_ffn",

@@ -8,6 +8,7 @@
 #include <string>
 
 #include "b2c/dataset.h"
+#include "b2c/dense.h"
 #include "b2c/evidence.h"
 #include "b2c/loss.h"
 #include "b2c/optim.h"
@@ -27,6 +28,10 @@ struct b2c_ctx {
   int n = 0;
   int degree = 0;
   hipEvent_t ev[8] = {};
+};
+
+struct b2c_dense {
+  b2c::DenseCtx ctx;
 };
 
 struct b2c_dataset {
@@ -858,6 +863,41 @@ int b2c_train_step(b2c_ctx* c, b2c_model* m, const b2c_view* v, const b2c_render
 int b2c_train_step_adam(b2c_ctx* c, b2c_model* m, const b2c_view* v, const b2c_render_opts* ro,
                         const b2c_loss_opts* lo, int mode, const b2c_adam_opts* a, b2c_step_times* times) {
   return train_step(c, m, v, ro, lo, mode, 0, a, times);
+}
+
+b2c_dense* b2c_dense_create(void) {
+  b2c_dense* d = nullptr;
+  guarded([&] { d = new b2c_dense; });
+  return d;
+}
+void b2c_dense_destroy(b2c_dense* d) { delete d; }
+
+extern "C++" {
+namespace {
+template <typename Args>
+const Args& given(const Args* a, const char* what) {
+  if (!a) throw std::runtime_error(std::string(what) + ": null argument");
+  return *a;
+}
+}  // namespace
+}
+int b2c_dropout(const b2c_dropout_args* a, void* stream) {
+  return guarded([&] { b2c::dropout(given(a, "dropout"), (hipStream_t)stream); });
+}
+int b2c_feed_forward(b2c_dense* d, const b2c_ffn_args* a, int train, void* stream) {
+  return guarded([&] { b2c::feed_forward(d->ctx, given(a, "feed_forward"), train != 0, (hipStream_t)stream); });
+}
+int b2c_feed_forward_backward(b2c_dense* d, const b2c_ffn_grad_args* a, void* stream) {
+  return guarded([&] { b2c::feed_forward_backward(d->ctx, given(a, "feed_forward_backward"), (hipStream_t)stream); });
+}
+int b2c_quantize_rows(const b2c_quantize_args* a, void* stream) {
+  return guarded([&] { b2c::quantize_rows(given(a, "quantize_rows"), (hipStream_t)stream); });
+}
+int b2c_i8_linear(b2c_dense* d, const b2c_i8_linear_args* a, void* stream) {
+  return guarded([&] { b2c::i8_linear(d->ctx, given(a, "i8_linear"), (hipStream_t)stream); });
+}
+int b2c_i8_feed_forward(b2c_dense* d, const b2c_i8_ffn_args* a, void* stream) {
+  return guarded([&] { b2c::i8_feed_forward(d->ctx, given(a, "i8_feed_forward"), (hipStream_t)stream); });
 }
 
 }  // extern "C"

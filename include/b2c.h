@@ -270,6 +270,20 @@ int b2c_train_step(b2c_ctx* c, b2c_model* m, const b2c_view* v, const b2c_render
 int b2c_train_step_adam(b2c_ctx* c, b2c_model* m, const b2c_view* v, const b2c_render_opts* ro,
                         const b2c_loss_opts* lo, int mode, const b2c_adam_opts* a, b2c_step_times* times);
 
+/* ---- dense operators of a learned head (b2c/dense.h; the argument structs are b2c_kernels.h's) ----
+ * A b2c_dense handle keeps one block's workspace, and between its passes what the backward pass needs: the workspace and saved
+ * fields of the structs are filled in here. stream: a hipStream_t (b2c_ctx_stream), NULL for the default stream. The calls
+ * return before the work is done. Device memory is the caller's (b2c_device_upload). */
+typedef struct b2c_dense b2c_dense;
+b2c_dense* b2c_dense_create(void);
+void b2c_dense_destroy(b2c_dense* d);
+int b2c_dropout(const b2c_dropout_args* a, void* stream);
+int b2c_feed_forward(b2c_dense* d, const b2c_ffn_args* a, int train, void* stream);
+int b2c_feed_forward_backward(b2c_dense* d, const b2c_ffn_grad_args* a, void* stream);
+int b2c_quantize_rows(const b2c_quantize_args* a, void* stream);
+int b2c_i8_linear(b2c_dense* d, const b2c_i8_linear_args* a, void* stream);
+int b2c_i8_feed_forward(b2c_dense* d, const b2c_i8_ffn_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
