@@ -73,7 +73,7 @@ __device__ __forceinline__ void act_grad(float g, float& a, float& d) {
   if constexpr (ACT == B2C_ACT_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.f + __expf(-g));
     a = g * s;
-    d = s * (1.f + g * (1.f - s));
+    d = fmaf(a, 1.f - s, s);
   } else if constexpr (ACT == B2C_ACT_GELU) {
     float cdf, bell;
     normal(g, cdf, bell);

@@ -158,7 +158,6 @@ __global__ __launch_bounds__(WAVES * 64) void head_rows_kernel(HeadRows<T> a, co
           if (m0 + r * 16 < a.M) *reinterpret_cast<F8*>(a.kept + (m0 + r * 16) * (32 * KS) + k * 32 + q4 * 8) = dz[r][k];
   }
   f32x4 acc[RT][OT] = {};
-  const float scale = a.drop.scale;
   for (int c = 0; c < chunks; c++) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -192,7 +191,7 @@ __global__ __launch_bounds__(WAVES * 64) void head_rows_kernel(HeadRows<T> a, co
           } else {
             float av, dv;
             act_grad<ACT>(gv, av, dv);
-            const float s = dh[r][j / 4][j % 4] * scale;
+            const float s = dh[r][j / 4][j % 4];  // dropout's scale follows at the end
             h[r][j] = (T)(s * uv * dv);
             du[r][j] = (T)(s * av);
           }
@@ -219,7 +218,7 @@ __global__ __launch_bounds__(WAVES * 64) void head_rows_kernel(HeadRows<T> a, co
       const int n = q4 * 8 * KS + h * 8;
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = acc[r][2 * h + j / 4][j % 4];
+      for (int j = 0; j < 8; j++) v[j] = USE == FOR_DX ? acc[r][2 * h + j / 4][j % 4] * a.drop.scale : acc[r][2 * h + j / 4][j % 4];
       if (n < out.cols) out.template operator()<8>(0u, m, n, v);
     }
   }
@@ -249,7 +248,6 @@ __global__ __launch_bounds__(WAVES * 64) void head_weights_kernel(HeadRows<T> a,
     }
   const int64_t tiles = (a.M + R - 1) / R;
   const int64_t first = tiles * blockIdx.y / gridDim.y, last = tiles * (blockIdx.y + 1) / gridDim.y;
-  const float scale = a.drop.scale;
   f32x4 sg[HT][OT] = {}, su[HT][OT] = {}, sd[HT][OT] = {};
 
   F8 next_x[PIECES], next_dz[PIECES];
@@ -312,7 +310,7 @@ __global__ __launch_bounds__(WAVES * 64) void head_weights_kernel(HeadRows<T> a,
           const float uv = u[j / 4][t][j % 4];
           float av, dv;
           act_grad<ACT>(g[j / 4][t][j % 4], av, dv);
-          const float s = dh[j / 4][t][j % 4] * scale;
+          const float s = dh[j / 4][t][j % 4];  // dropout's scale follows when the parts are added
           h[t][j] = (T)(av * uv);
           dg[t][j] = (T)(s * uv * dv);
           du[t][j] = (T)(s * av);
@@ -491,7 +489,7 @@ int head_backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream)
   }
   if ((rc = hipGetLastError())) return rc;
   const bool f32 = b->grad_dtype == B2C_F32, add = b->accumulate != 0;
-  const WeightOut<T> in{b->dw_gate, b->dw_up, b->ld_din, a->d_hidden, a->d_hidden, a->d_in, f32, add, 1.f};
+  const WeightOut<T> in{b->dw_gate, b->dw_up, b->ld_din, a->d_hidden, a->d_hidden, a->d_in, f32, add, rows.drop.scale};
   const WeightOut<T> down{b->dw_down, nullptr, b->ld_dout, a->d_out, 0, a->d_hidden, f32, add, rows.drop.scale};
   const int64_t hidden = split.chunks * 16, blocks = 3 * hidden * KS;
   head_join_kernel<T><<<dim3((unsigned)blocks), 256, 0, stream>>>(p.sums, hidden, 32 * KS, split.parts, a->d_hidden, a->d_in, a->d_out, in,
