@@ -228,7 +228,7 @@ __global__ __launch_bounds__(WAVES * 64) void head_rows_kernel(HeadRows<T> a, co
 // tiles of 64, x beside dz (dropout applied), each row's 16-byte pieces at (piece ^ row & 7) of its 128-byte blocks.
 // sums: [part][3][chunks 16][32 KS]: dWg, dWu, dWd transposed.
 template <typename T, int ACT, int KS, int HT, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void head_weights_kernel(HeadRows<T> a, const T* frags, int chunks, float* sums) {
+__global__ __launch_bounds__(WAVES * 64, KS == 1 && WAVES == 4 ? 4 : 1) void head_weights_kernel(HeadRows<T> a, const T* frags, int chunks, float* sums) {
   constexpr int KB = (KS + 1) / 2, R = 64, PIECES = R * 8 * KB / (WAVES * 64), OT = 2 * KS;
   static_assert(PIECES * WAVES * 64 == R * 8 * KB);
   using F8 = vec<T, 8>;
@@ -383,7 +383,8 @@ inline int head_steps(const b2c_ffn_args* a) {
 
 // How the weights' gradients are shared out: tiles of 16 hidden units a wave (two where the registers take them), workgroups
 // of eight waves along the hidden units (four where there are few), parts of the rows: as many workgroups as the compute
-// units hold (a step of 1M rows of 64-256-64 took 679 us with 512 where 256 take 661).
+// units hold: one of eight waves (a step of 1M rows of 64-256-64 took 679 us with 512 where 256 take 661), four of four waves
+// (600k rows of 16-32-16 took 93 us with 768 of them, 84 with 1024).
 struct HeadSplit {
   int ht, waves, blocks, parts;
   int64_t chunks;
@@ -392,7 +393,7 @@ struct HeadSplit {
     ht = head_steps(a) <= 2 && up(a->d_hidden, 256) == up(a->d_hidden, 128) ? 2 : 1;
     waves = chunks <= 4 ? 4 : 8;
     blocks = (int)(up(chunks, waves * ht) / (waves * ht));
-    parts = (int)std::max<int64_t>(1, std::min<int64_t>(up(a->rows, 64) / 64, (waves == 4 ? 768 : 256) / blocks));
+    parts = (int)std::max<int64_t>(1, std::min<int64_t>(up(a->rows, 64) / 64, (waves == 4 ? 1024 : 256) / blocks));
   }
   int64_t sums(int ks) const { return (int64_t)parts * 3 * chunks * 16 * 32 * ks; }
 };
