@@ -114,6 +114,12 @@ struct Operand {
 // The steps of 64 values that a sum over k takes.
 int64_t steps_of(int64_t k) { return up(k, 64) / 64; }
 
+// The inner activations that a forward pass keeps for the down weights' gradient: behind its factors.
+template <typename T>
+T* kept_h(const b2c_ffn_args* a) {
+  return (T*)a->saved + a->rows * 2 * up(a->d_hidden, 64);
+}
+
 // What a forward pass needs beside its matrices.
 template <typename T>
 struct ForwardPlan {
@@ -125,7 +131,7 @@ struct ForwardPlan {
   ForwardPlan(const b2c_ffn_args* a, Room& room) {
     const int64_t M = a->rows;
     fp = up(a->d_hidden, 64);
-    h = room.take<T>(M * fp);
+    h = a->saved ? kept_h<T>(a) : room.take<T>(M * fp);
     const bool in = direct(a->w_gate, a->ld_in, a->d_in) && direct(a->w_up, a->ld_in, a->d_in);
     const bool out = direct(a->w_down, a->ld_out, a->d_hidden), few = few_rows(M, in && out);
     gate = choose({{M, fp}}, steps_of(a->d_in), true, few, a->saved ? 6 : 2);
@@ -163,7 +169,7 @@ int forward(const b2c_ffn_args* a, const Drop& d, hipStream_t stream) {
 template <typename T>
 struct BackwardPlan {
   int64_t fp;
-  T *h, *dgu;
+  T* dgu;
   Operand<T> x, wg, wu, wd, dz;
   Way back, dw, dx;
   void* sums;
@@ -172,8 +178,7 @@ struct BackwardPlan {
     const int64_t M = a->rows;
     fp = up(a->d_hidden, 64);
     dgu = room.take<T>(M * 2 * fp);
-    h = room.take<T>(M * fp);
-    back = choose({{M, fp}}, steps_of(a->d_out), false, false, 10);
+    back = choose({{M, fp}}, steps_of(a->d_out), false, false, 8);
     const Extent in{fp + a->d_hidden, a->d_in}, down{a->d_out, a->d_hidden};
     const int64_t k = steps_of(M);
     dw = b->dw_down && (b->dw_gate || b->dw_up) ? choose({in, down}, k, false, false)
@@ -198,8 +203,8 @@ struct BackwardPlan {
   }
 };
 
-template <typename T, int ACT>
-int backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream) {
+template <typename T>
+int block_backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream) {
   const b2c_ffn_args* a = &b->fwd;
   Room room{(char*)b->workspace};
   const BackwardPlan<T> p(b, d, room);
@@ -213,7 +218,7 @@ int backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream) {
     if ((rc = make(packs, stream))) return rc;
   }
   const Side<T> dz = p.dz.side(), x = p.x.side(), dgu{p.dgu, 2 * fp};
-  const GateBack<T, ACT> back{(const T*)a->saved, p.h, p.dgu, fp, a->d_hidden, scale};
+  const GateBack<T> back{(const T*)a->saved, p.dgu, fp, a->d_hidden, scale};
   const Product<T> dh{dz, p.wd.side(), {}, {}, M, fp, a->d_out, 0, M, a->d_hidden};
   if ((rc = product<T, true, false, false, false>(dh, p.back, p.sums, back, stream))) return rc;
   const bool f32 = b->grad_dtype == B2C_F32, add = b->accumulate != 0;
@@ -221,7 +226,7 @@ int backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream) {
   const WeightOut<T> to_in{b->dw_gate, b->dw_up, b->ld_din, a->d_hidden, (int)fp, a->d_in, f32, add, 1.f};
   const WeightOut<T> to_down{b->dw_down, nullptr, b->ld_dout, a->d_out, 0, a->d_hidden, f32, add, scale};
   const Product<T> dwi{dgu, x, {}, {}, fp + a->d_hidden, a->d_in, M, 0, fp + a->d_hidden, a->d_in};
-  const Product<T> dwd{dz, {p.h, fp}, {}, {}, a->d_out, a->d_hidden, M, 0, a->d_out, a->d_hidden};
+  const Product<T> dwd{dz, {kept_h<T>(a), fp}, {}, {}, a->d_out, a->d_hidden, M, 0, a->d_out, a->d_hidden};
   if (in && b->dw_down) {  // together: one launch, and fewer compute units without work in its last round
     Jobs<T, WeightOut<T>, 2> both{{dwi, dwd}, {to_in, to_down}, {}, {}};
     rc = products<T, true, true, false, false>(both, p.dw, p.sums, stream);
@@ -249,9 +254,7 @@ int forward(const b2c_ffn_args* a, const Drop& d, hipStream_t s) {
 template <typename T>
 int backward(const b2c_ffn_grad_args* a, const Drop& d, hipStream_t s) {
   if (is_head(&a->fwd)) return head_backward<T>(a, d, s);
-  if (a->fwd.act == B2C_ACT_SILU) return backward<T, B2C_ACT_SILU>(a, d, s);
-  if (a->fwd.act == B2C_ACT_GELU) return backward<T, B2C_ACT_GELU>(a, d, s);
-  return backward<T, B2C_ACT_RELU>(a, d, s);
+  return block_backward<T>(a, d, s);
 }
 
 }  // namespace
@@ -262,7 +265,7 @@ using namespace b2c::dev;
 
 extern "C" size_t b2c_ffn_saved_bytes(const b2c_ffn_args* a) {
   Drop d;
-  return sizes_ok(a, &d) && !is_head(a) ? (size_t)a->rows * 2 * up(a->d_hidden, 64) * 2 : 0;
+  return sizes_ok(a, &d) && !is_head(a) ? (size_t)a->rows * 3 * up(a->d_hidden, 64) * 2 : 0;
 }
 extern "C" size_t b2c_ffn_workspace_bytes(const b2c_ffn_args* a) {
   Drop d;
