@@ -64,7 +64,8 @@ __global__ __launch_bounds__(256) void join_kernel(Jobs<T, Epi, NJ> jobs, uint32
 // At most 16 MT rows of q against P: bound by reading P once. A workgroup takes 16 rows of P (DUAL: of each of the
 // two), its eight waves every eighth 256-byte run of k; P goes from memory straight into the matrix instruction's
 // registers, sixteen bytes of a row a lane, and q, which every workgroup reads again, comes from the caches. The
-// eight sums meet in LDS and are added in a fixed order. No alignment is asked for.
+// eight sums meet in LDS and are added in a fixed order. No alignment is asked for. One row of a 4096-11264 block: gate and up
+// 37 us (4.9 TB/s of weights), down 21 (4.4).
 template <typename T, bool DUAL, int MT, typename Epi>
 __global__ __launch_bounds__(512) void few_rows_kernel(Product<T> a, Epi epi) {
   constexpr int V = Elem<T>::N, PL = DUAL ? 2 : 1, RUN = 16 * V;

@@ -2,7 +2,7 @@
 //
 // A workgroup computes BM x BN of out in steps of 128 bytes of k (64 values of 16 bits, 128 of 8). Both operands'
 // next step is copied from memory to LDS by the buffer unit itself while the current one is multiplied: two
-// buffers, one barrier a step, no registers in between. A copy instruction writes 64 pieces of 16 bytes in lane order,
+// to four buffers, one barrier a step, no registers in between. A copy instruction writes 64 pieces of 16 bytes in lane order,
 // so any rearrangement is done on the side of the addresses it reads:
 //   - rows along k ("plain" operand, element (i, k) at p[i ld + k]): row i's eight pieces are stored at
 //     (piece ^ i & 7), so that the sixteen rows that a matrix instruction's lanes read lie in different banks;
@@ -10,6 +10,9 @@
 //     (piece ^ 2 key(k)), and read with the transposing LDS load, which hands lane l of each sixteen the four
 //     values that column l has in four rows.
 // Pieces beyond an operand's edge are read as zeros: their lanes are given an offset outside the buffer's range.
+//
+// Bound by the matrix instructions and, over a long run, by the clock that their power leaves: 4096 x 4096 x 11264 with tiles
+// of 256x256 takes 257 us in bfloat16 (1.47 PFLOP/s), 138 in 8 bits (2.73 POP/s); 272 within a 4096-11264 block's pass.
 #pragma once
 #include "dense.h"
 

@@ -6,8 +6,8 @@ namespace dev {
 namespace {
 
 // Rows that follow each other without a gap in every matrix, all on 16 bytes: a thread takes the eight elements of a counter
-// in one access. Bound by memory: 8192 x 4096 in bfloat16 with a residual, and its gradient, 63 us, 5.3 TB/s, which is what
-// a copy reaches.
+// in one access. Bound by memory: 8192 x 4096 in bfloat16 with a residual, and its gradient, 62 us, 5.4 TB/s; a copy
+// of 0.5 GiB reaches 5.3.
 template <typename T>
 __global__ __launch_bounds__(256) void flat_kernel(const T* x, const T* r, T* y, uint64_t n, Drop d) {
   const uint64_t q = (uint64_t)blockIdx.x * 256 + threadIdx.x, e = q * 8;
@@ -38,7 +38,8 @@ __global__ __launch_bounds__(256) void flat_kernel(const T* x, const T* r, T* y,
 }
 
 // Any rows: a wave takes 512 elements in their order, lane l first forms the bits of the l-th counter of them and then
-// moves elements l, l + 64, ..., neighbouring lanes neighbouring elements, fetching their bits from the lane that has them.
+// moves elements l, l + 64, ..., neighbouring lanes neighbouring elements, fetching their bits from the lane that has them. Bound by
+// memory: 333333 x 45 in single precision, rows three apart, and its gradient, 50 us, 4.8 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void rows_kernel(const T* x, int64_t ldx, const T* r, int64_t ldr, T* y, int64_t ldy, uint64_t n,
                                                    uint32_t cols, Drop d) {
