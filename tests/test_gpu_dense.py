@@ -1,5 +1,7 @@
 """The dense operators on the GPU against their restatement in 64 bits (dense_util.py), which also says how far a kernel that
 sums in single precision and rounds where the documentation says may be off, value by value."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -266,6 +268,74 @@ def test_runs_repeat_bit_for_bit_on_a_stream():
         assert all(np.array_equal(a, b) for a, b in zip(*got))
     finally:
         L.b2c_ctx_destroy(ctx)
+
+
+class Graph:
+    """What `work(stream)` launches, recorded once."""
+
+    def __init__(self, stream, work):
+        self.hip, self.stream, self.exec = C.CDLL("libamdhip64.so.7"), C.c_void_p(stream), C.c_void_p()  # the library's own copy
+        graph = C.c_void_p()
+        self.check(self.hip.hipStreamBeginCapture(self.stream, 1))  # this thread's calls
+        work(stream)
+        self.check(self.hip.hipStreamEndCapture(self.stream, C.byref(graph)))
+        self.check(self.hip.hipGraphInstantiate(C.byref(self.exec), graph, None, None, C.c_size_t(0)))
+        self.check(self.hip.hipGraphDestroy(graph))
+
+    @staticmethod
+    def check(rc):
+        assert rc == 0, f"hipError {rc}"
+
+    def replay(self):
+        self.check(self.hip.hipGraphLaunch(self.exec, self.stream))
+        self.check(self.hip.hipStreamSynchronize(self.stream))
+
+    def close(self):
+        self.check(self.hip.hipGraphExecDestroy(self.exec))
+
+
+@pytest.mark.parametrize("rows,di,f,do,pad", [(5, 200, 100, 56, 0), (129, 200, 330, 136, 3), (3000, 64, 256, 64, 0), (300, 512, 1032, 512, 0)])
+def test_a_recorded_step_replays(rows, di, f, do, pad):
+    """Dropout, the block with its gradients and its 8-bit form from a recorded graph, between passes with another mask."""
+    emit(f"graph {rows} x {di}-{f}-{do} pad {pad}")
+    v, h = make(rows, di, f, do, BF16, 9, pad, 0)
+    g, space = np.random.default_rng(rows), U.Space()
+    x, y, z = [U.Held(None, BF16, pad, 0, rows, n) for n in (di, do, do)]
+    out = {k: U.Held(None, BF16, pad, 0, a, b) for k, a, b in (("dx", rows, di), ("dw_gate", f, di), ("dw_up", f, di), ("dw_down", do, f))}
+    drop = nn.Dropout(h["x"].matrix, x.matrix, 0.25, 3, 0)
+    ff = nn.FeedForward(x.matrix, h["wg"].matrix, h["wu"].matrix, h["wd"].matrix, y.matrix, p=0.3, seed=1, train=True, room=space)
+    ff.gradients(h["dy"].matrix, **{k: o.matrix for k, o in out.items()}, room=space)
+    hw = [U.Held(g.integers(-127, 128, s).astype(np.int8), nn.I8, pad) for s in ((f, di), (f, di), (do, f))]
+    hs = [U.Held(np.full((n, 1), 0.01, np.float32), F32) for n in (f, f, do)]
+    i8 = nn.I8FeedForward(x.matrix, hw[0].matrix, hs[0].matrix, hw[1].matrix, hs[1].matrix, hw[2].matrix, hs[2].matrix, z.matrix, room=space)
+
+    def step(mask, stream):
+        drop.set_stream_id(mask)
+        ff.set_stream_id(mask)
+        drop.run(stream)
+        ff.forward(stream)
+        ff.backward(stream)
+        i8.run(stream)
+
+    L = _native.lib()
+    ctx = L.b2c_ctx_create()
+    try:
+        s = L.b2c_ctx_stream(ctx)
+        results = lambda: [o.get() for o in (x, y, z, *out.values())]  # noqa: E731
+        step(0, s)
+        assert L.b2c_ctx_synchronize(ctx) == 0
+        want = results()
+        graph = Graph(s, lambda stream: step(0, stream))
+        for _ in range(3):
+            step(1, s)
+            assert L.b2c_ctx_synchronize(ctx) == 0
+            assert not any(np.array_equal(a, b) for a, b in zip(want, results()))
+            graph.replay()
+            assert all(np.array_equal(a, b) for a, b in zip(want, results()))
+        graph.close()
+    finally:
+        L.b2c_ctx_destroy(ctx)
+    space.check()
 
 
 # ---- 8 bits ------------------------------------------------------------------------------------------------
