@@ -131,7 +131,8 @@ struct ForwardPlan {
   ForwardPlan(const b2c_ffn_args* a, Room& room) {
     const int64_t M = a->rows;
     fp = up(a->d_hidden, 64);
-    h = a->saved ? kept_h<T>(a) : room.take<T>(M * fp);
+    h = room.take<T>(M * fp);  // with `saved` too, where it stays unused: a call without it may follow in the same workspace
+    if (a->saved) h = kept_h<T>(a);
     const bool in = direct(a->w_gate, a->ld_in, a->d_in) && direct(a->w_up, a->ld_in, a->d_in);
     const bool out = direct(a->w_down, a->ld_out, a->d_hidden), few = few_rows(M, in && out);
     gate = choose({{M, fp}}, steps_of(a->d_in), true, few, a->saved ? 6 : 2);
