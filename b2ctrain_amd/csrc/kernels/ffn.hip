@@ -16,7 +16,7 @@ int head_backward<bf16>(const b2c_ffn_grad_args*, const Drop&, hipStream_t);
 namespace {
 
 bool sizes_ok(const b2c_ffn_args* a, Drop* d) {
-  const int most = 1 << 24;
+  const int most = 1 << 20;  // 256 rows of two such widths span 1 GiB: the copies to LDS have offsets of 31 bits
   return a && a->rows >= 0 && a->rows <= (1 << 30) && a->d_in >= 1 && a->d_in <= most && a->d_hidden >= 1 &&
          a->d_hidden <= most && a->d_out >= 1 && a->d_out <= most && (a->dtype == B2C_F16 || a->dtype == B2C_BF16) &&
          a->act >= B2C_ACT_SILU && a->act <= B2C_ACT_RELU && drop_of(a->p, a->seed, a->stream, d);

@@ -112,6 +112,17 @@ def test_forward_launcher_refuses(kw):
     assert refused(nn._lib().b2c_hip_ffn_forward, f.args, **kw)
 
 
+@pytest.mark.parametrize("width", ["d_in", "d_hidden", "d_out"])
+def test_launchers_refuse_widths_beyond_their_offsets(width):
+    """256 rows of 2^22 16-bit values are the 2 GiB that a copy's offset spans, and a gradient's rows hold two widths."""
+    wide = {width: (1 << 20) + 1, "ldx": 1 << 21, "ld_in": 1 << 21, "ld_out": 1 << 21, "ldy": 1 << 21, "workspace_bytes": 1 << 62}
+    assert refused(nn._lib().b2c_hip_ffn_forward, ffn().args, **wide)
+    f = ffn()
+    f.gradients(M(8, 24), dx=M(8, 16), dw_gate=M(32, 16), dw_up=M(32, 16), dw_down=M(24, 32), room=Room())
+    ld = {k: 1 << 21 for k in ("lddy", "lddx", "ld_din", "ld_dout")}
+    assert refused(nn._lib().b2c_hip_ffn_backward, f.grad, **{"fwd__" + k: v for k, v in wide.items()}, **ld, workspace_bytes=1 << 62)
+
+
 @pytest.mark.parametrize("kw", [
     dict(fwd__rows=-1), dict(dy=None), dict(lddy=23), dict(lddx=15), dict(grad_dtype=1), dict(accumulate=1),
     dict(ld_din=15), dict(ld_dout=31), dict(workspace=None), dict(workspace_bytes=16), dict(fwd__act=9),
