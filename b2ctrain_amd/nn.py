@@ -269,11 +269,18 @@ class FeedForward:
 
 
 class QuantizeRows:
-    """q, scale = x in 8 bits by rows; b2c_hip_quantize_rows. For weights [outputs, inputs], rows are channels."""
+    """q, scale = x in 8 bits by rows; b2c_hip_quantize_rows. For weights [outputs, inputs], rows are channels. Where q's rows are
+    further apart than wide, the columns between them become 0 up to the next multiple of 16: a view has to leave room for
+    them in its own rows."""
 
     def __init__(self, x, q, scale):
         x = _floating(matrix(x, "x"), "x")
         q = matrix(q, "q", x.rows, x.cols, I8)
+        if hasattr(q.keep, "untyped_storage"):
+            wide, first = min(-(-q.cols // 16) * 16, q.ld), q.keep.storage_offset()
+            ends = first + (q.rows - 1) * q.ld + wide
+            if q.rows and wide > q.cols and (first % q.ld + wide > q.ld or ends > q.keep.untyped_storage().nbytes()):
+                raise ValueError("q: its last columns have no room for the zeros up to the next multiple of 16")
         self._keep = (x, q, scale)
         self.args = QuantizeArgs(rows=x.rows, cols=x.cols, dtype=x.dtype, x=x.ptr, ldx=x.ld, q=q.ptr, ldq=q.ld,
                                  scale=_vector(scale, "scale", x.rows))

@@ -642,7 +642,7 @@ int b2c_hip_ffn_backward(const b2c_ffn_grad_args* a, hipStream_t stream);
 
 /* 8-bit rows: scale[i] = max |x[i][j]| / 127 and q[i][j] = x[i][j] / scale[i], rounded to nearest even, both in single
  * precision. A row of zeros gets scale 0; a row with an infinity or NaN gets scale NaN and zeros. Columns cols .. ldq - 1
- * of q are set to 0 up to the next multiple of 16. For weights, rows are output channels. */
+ * of q are set to 0 up to the next multiple of 16, those of the last row too. For weights, rows are output channels. */
 typedef struct b2c_quantize_args {
   int64_t rows, cols;
   int dtype;            /* of x: B2C_F32, B2C_F16 or B2C_BF16 */

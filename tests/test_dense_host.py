@@ -135,6 +135,40 @@ def test_backward_launcher_refuses(kw):
     assert refused(nn._lib().b2c_hip_ffn_backward, f.grad, **kw)
 
 
+class View:
+    """What QuantizeRows asks of a tensor: rows x cols bytes, rows ld apart, `first` bytes into a storage of `size`."""
+
+    def __init__(self, rows, cols, ld, first, size):
+        self.shape, self.dtype, self._ld, self._first, self._size = (rows, cols), "torch.int8", ld, first, size
+
+    def stride(self, i):
+        return 1 if i else self._ld
+
+    def data_ptr(self):
+        return ADDRESS + self._first
+
+    def storage_offset(self):
+        return self._first
+
+    def untyped_storage(self):
+        return self
+
+    def nbytes(self):
+        return self._size
+
+
+@pytest.mark.parametrize("rows,cols,ld,first,size,fits", [
+    (4, 5, 5, 0, 20, True), (4, 16, 40, 24, 160, True), (4, 10, 16, 0, 64, True), (4, 10, 16, 6, 64, False), (4, 20, 40, 0, 152, True),
+    (4, 20, 40, 0, 140, False), (4, 20, 40, 16, 160, False), (1, 5, 5, 59, 64, True)])
+def test_quantize_rows_keeps_to_the_rows_of_a_view(rows, cols, ld, first, size, fits):
+    plan = lambda: nn.QuantizeRows(M(rows, cols), View(rows, cols, ld, first, size), nn.Matrix(ADDRESS, rows, 1, 1, nn.F32))  # noqa: E731
+    if fits:
+        plan()
+    else:
+        with pytest.raises(ValueError, match="room"):
+            plan()
+
+
 def test_other_launchers_refuse():
     L = nn._lib()
     d = lambda: nn.Dropout(M(4, 5), M(4, 5), 0.1, 1, 2)  # noqa: E731
