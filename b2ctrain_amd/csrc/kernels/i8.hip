@@ -9,7 +9,7 @@ namespace dev {
 namespace {
 
 // Weights in 8 bits as the products read them: in place where rows start on 16 bytes (columns beyond the last meet zeros of
-// the quantised rows), else copied to rows that do, all of a call's in one launch. A few rows read them anywhere.
+// the quantised rows), else copied to rows that do, in the launch that quantises x. A few rows read them anywhere.
 struct Copy {
   const int8_t* from;
   int64_t ld, rows, pitch;
@@ -18,15 +18,11 @@ struct Copy {
   uint32_t groups, blocks;
 };
 struct Copies {
-  Copy of[3];
+  Copy of[3]{};
   int n = 0;
   uint32_t blocks = 0;
 };
-__global__ __launch_bounds__(256) void copies_kernel(Copies all) {
-  uint32_t block = blockIdx.x;
-  int i = 0;
-  while (block >= all.of[i].blocks) block -= all.of[i++].blocks;
-  const Copy& c = all.of[i];
+__device__ __forceinline__ void copy_block(const Copy& c, uint32_t block) {
   const int64_t t = (int64_t)block * 256 + threadIdx.x, m = t / c.groups;
   if (m >= c.rows) return;
   const int n = (int)(t - m * c.groups) * 16;
@@ -45,10 +41,23 @@ __global__ __launch_bounds__(256) void copies_kernel(Copies all) {
 // THREADS threads to a row, sixteen values each at a time. What they read first they keep (up to HELD times sixteen), so that a
 // row is read once; the rest of a longer row is read again. A row's columns from cols to the next multiple of 16 become 0.
 // Bound by memory: 4096 x 11264 in single precision 39 us, 5.9 TB/s, most of which the last-level cache gives.
-template <typename T, int THREADS, int HELD>
+// The workgroups from `own` on make a call's copies of weights: in a launch of their own they cost 1333 rows of 2050 -> 5001
+// three of 33 us. Where there are none, a kernel that takes Nothing: each launch with the larger arguments costs half a
+// microsecond more (1000 rows of 1024-2816: 37.2 us with two of them, 36.6 without).
+struct Nothing {};
+template <typename T, int THREADS, int HELD, typename With>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q,
-                                                       int64_t ldq, float* scale) {
+                                                       int64_t ldq, float* scale, uint32_t own, With copies) {
   __shared__ uint32_t part[4];
+  if constexpr (std::is_same_v<With, Copies>) {
+    if (blockIdx.x >= own) {  // each with an index of its own: for a variable one the compiler puts them into scratch memory
+      const uint32_t b = blockIdx.x - own, b1 = copies.of[0].blocks, b2 = b1 + copies.of[1].blocks;
+      if (b < b1) copy_block(copies.of[0], b);
+      else if (b < b2) copy_block(copies.of[1], b - b1);
+      else copy_block(copies.of[2], b - b2);
+      return;
+    }
+  }
   const int t = threadIdx.x % THREADS;
   const int64_t m = (int64_t)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
   const bool there = m < rows;
@@ -115,20 +124,28 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t ldx, 
 // Four lanes a row up to 128 columns, sixteen up to 1024, a wave or a workgroup beyond: whole rows in registers, and as few idle
 // lanes as that allows (four waves a row of 64 took 600 us for a million of them).
 template <typename T>
-int quantize(const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq, float* scale, hipStream_t stream) {
-  auto grid = [&](int threads) { return dim3((unsigned)(up(rows, 256 / threads) / (256 / threads))); };
+int quantize(const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq, float* scale, const Copies& copies,
+             hipStream_t stream) {
   constexpr int H = sizeof(T) == 4 ? 2 : 4;
-  if (cols <= 128) quantize_kernel<T, 4, 2><<<grid(4), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
-  else if (cols <= 1024) quantize_kernel<T, 16, H><<<grid(16), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
-  else if (cols <= 4096 && rows >= 2048) quantize_kernel<T, 64, H><<<grid(64), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
-  else quantize_kernel<T, 256, H><<<grid(256), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale);
-  return hipGetLastError();
+  auto run = [&](auto threads, auto held) {
+    constexpr int N = decltype(threads)::value;
+    const uint32_t own = (uint32_t)(up(rows, 256 / N) / (256 / N));
+    constexpr int HELD = decltype(held)::value;
+    if (copies.blocks) quantize_kernel<T, N, HELD><<<dim3(own + copies.blocks), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale, own, copies);
+    else quantize_kernel<T, N, HELD><<<dim3(own), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale, own, Nothing{});
+    return hipGetLastError();
+  };
+  using std::integral_constant;
+  if (cols <= 128) return run(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+  if (cols <= 1024) return run(integral_constant<int, 16>{}, integral_constant<int, H>{});
+  if (cols <= 4096 && rows >= 2048) return run(integral_constant<int, 64>{}, integral_constant<int, H>{});
+  return run(integral_constant<int, 256>{}, integral_constant<int, H>{});
 }
 int quantize(const void* x, int64_t ldx, int dtype, int64_t rows, int64_t cols, int8_t* q, int64_t ldq, float* scale,
-             hipStream_t stream) {
-  if (dtype == B2C_F32) return quantize((const float*)x, ldx, rows, cols, q, ldq, scale, stream);
-  if (dtype == B2C_F16) return quantize((const f16*)x, ldx, rows, cols, q, ldq, scale, stream);
-  return quantize((const bf16*)x, ldx, rows, cols, q, ldq, scale, stream);
+             hipStream_t stream, const Copies& copies = {}) {
+  if (dtype == B2C_F32) return quantize((const float*)x, ldx, rows, cols, q, ldq, scale, copies, stream);
+  if (dtype == B2C_F16) return quantize((const f16*)x, ldx, rows, cols, q, ldq, scale, copies, stream);
+  return quantize((const bf16*)x, ldx, rows, cols, q, ldq, scale, copies, stream);
 }
 
 // A few rows of a product, quantised on the way: every workgroup takes all of x (at most kHeld values, which the caches hand
@@ -297,11 +314,6 @@ struct Weights {
     all.blocks += (uint32_t)blocks;
   }
 };
-int make(const Copies& all, hipStream_t stream) {
-  if (all.blocks == 0) return hipSuccess;
-  copies_kernel<<<dim3(all.blocks), 256, 0, stream>>>(all);
-  return hipGetLastError();
-}
 int64_t steps_of(int64_t k) { return up(k, 128) / 128; }
 
 struct LinearPlan {
@@ -413,8 +425,8 @@ extern "C" int b2c_hip_i8_linear(const b2c_i8_linear_args* a, hipStream_t stream
   } else {
     Copies copies;
     p.w.add_to(copies);
-    int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.q, p.kp, p.sx, stream);
-    if (rc || (rc = make(copies, stream))) return rc;
+    const int rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.q, p.kp, p.sx, stream, copies);
+    if (rc) return rc;
   }
   return scaled(out, p.way, p.sums, p.sx, a->w_scale, a->dtype, a->y, a->ldy, raw, stream);
 }
@@ -444,8 +456,8 @@ extern "C" int b2c_hip_i8_ffn(const b2c_i8_ffn_args* a, hipStream_t stream) {
   } else {
     Copies copies;
     for (const Weights* w : {&p.wg, &p.wu, &p.wd}) w->add_to(copies);
-    rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.qx, p.kp, p.s, stream);
-    if (rc || (rc = make(copies, stream))) return rc;
+    rc = quantize(a->x, a->ldx, a->dtype, a->rows, a->d_in, p.qx, p.kp, p.s, stream, copies);
+    if (rc) return rc;
   }
   if (a->act == B2C_ACT_SILU) rc = gated<B2C_ACT_SILU>(p, a, raw, stream);
   else if (a->act == B2C_ACT_GELU) rc = gated<B2C_ACT_GELU>(p, a, raw, stream);
