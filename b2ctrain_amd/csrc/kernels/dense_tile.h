@@ -121,7 +121,7 @@ __device__ __forceinline__ void place(uint32_t t, uint32_t tiles_m, uint32_t til
 }
 
 // A product: operands p, q (and with TWO, after K values of k, p2, q2 for K2 more, rows as far apart), or with DUAL two
-// products that share q (p the gate's weights, p2 the up projection's; the epilogue gets both).
+// products that share q (p the gate's weights, p2 the up projection's, rows as far apart; the epilogue gets both).
 template <typename T>
 struct Product {
   Side<T> q, p, q2, p2;

@@ -301,8 +301,8 @@ struct Weights {
   bool straight() const {
     return reinterpret_cast<uintptr_t>(from.p) % 16 == 0 && from.ld % 16 == 0 && cols % 16 == 0 && from.ld < (1 << 22);
   }
-  void place(Room& room, bool few) {
-    if (few || straight()) return;
+  void place(Room& room, bool stay) {
+    if (stay) return;
     pitch = up(cols, 128);
     copy = room.take<int8_t>(rows * pitch);
   }
@@ -330,7 +330,7 @@ struct LinearPlan {
     w = {{a->w, a->ldw}, a->d_out, a->d_in};
     const bool few = few_rows(a->rows, w.straight());
     way = choose({{a->rows, a->d_out}}, steps_of(a->d_in), false, few);
-    w.place(room, few);
+    w.place(room, few || w.straight());
     sums = room.take<char>(way.sums);
   }
 };
@@ -351,12 +351,13 @@ struct BlockPlan {
     wg = {{a->w_gate, a->ld_in}, a->d_hidden, a->d_in};
     wu = {{a->w_up, a->ld_in}, a->d_hidden, a->d_in};
     wd = {{a->w_down, a->ld_out}, a->d_out, a->d_hidden};
-    const bool few = few_rows(a->rows, wg.straight() && wu.straight() && wd.straight());
+    const bool in = wg.straight() && wu.straight();  // both or none: the tiles read them with one distance between rows
+    const bool few = few_rows(a->rows, in && wd.straight());
     gate = choose({{a->rows, a->d_hidden}}, steps_of(a->d_in), true, few, 4);
     down = choose({{a->rows, a->d_out}}, steps_of(a->d_hidden), false, few);
-    wg.place(room, few);
-    wu.place(room, few);
-    wd.place(room, few);
+    wg.place(room, few || in);
+    wu.place(room, few || in);
+    wd.place(room, few || wd.straight());
     sums = room.take<char>(std::max(gate.sums, down.sums));
   }
 };

@@ -1,0 +1,45 @@
+"""Calls of the dense operators that differ from the usual ones in one thing: an alignment, a buffer's place, a size at the end of
+its range; against their restatement in 64 bits (dense_util.py)."""
+import numpy as np
+import pytest
+
+from b2ctrain_amd import nn
+from tests import dense_util as U
+from tests.gpu_harness import emit
+from tests.test_gpu_dense import close
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = nn.F32, nn.F16, nn.BF16
+
+
+def i8_block(x, ws, ss, name):
+    """y of the 8-bit block, and which values of h lie within single precision's rounding of the middle between two steps: each may
+    move y by one step of its row."""
+    dense = lambda q, s, w, sw: (q.astype(np.float64) @ w.T.astype(np.float64)) * s[:, None].astype(np.float64) * sw[:, 0].astype(np.float64)  # noqa: E731
+    q, sx = U.quantised(x)
+    up = dense(q, sx, ws[1], ss[1])
+    h = U.act(name, dense(q, sx, ws[0], ss[0]))[0] * up
+    top = abs(h).max(axis=1, keepdims=True)
+    step = top / 127
+    safe = np.where(step > 0, step, 1)
+    t = np.where(step > 0, h / safe, 0)
+    unsure = abs(t - np.floor(t) - 0.5) <= 2.0 ** -20 * (abs(h) + abs(up) + top) / safe
+    want = (np.rint(t) @ ws[2].T.astype(np.float64)) * step * ss[2][:, 0].astype(np.float64)
+    return want, (unsure @ abs(ws[2]).T.astype(np.float64)) * step * ss[2][:, 0]
+
+
+@pytest.mark.parametrize("rows,di,f,do,pad", [(64, 144, 256, 144, 0), (64, 256, 320, 256, 16), (200, 48, 1040, 48, 0), (20, 144, 256, 144, 0)])
+@pytest.mark.parametrize("gate,up,down", [(0, 8, 0), (8, 0, 0), (8, 3, 8), (0, 0, 5)])
+def test_i8_block_of_weights_aligned_differently(rows, di, f, do, pad, gate, up, down):
+    emit(f"i8 block {rows} x {di}-{f}-{do} pad {pad}, weights {gate}, {up}, {down} bytes off")
+    g = np.random.default_rng(rows + di)
+    x = U.rounded(g.standard_normal((rows, di)), BF16)
+    ws = [g.integers(-127, 128, s).astype(np.int8) for s in ((f, di), (f, di), (do, f))]
+    ss = [(np.exp(g.uniform(-0.5, 0.5, (n, 1))) / 73 / np.sqrt(k)).astype(np.float32) for n, k in ((f, di), (f, di), (do, f))]
+    hx, y, space = U.Held(x, BF16), U.Held(None, BF16, rows=rows, cols=do), U.Space()
+    hw, hs = [U.Held(w, nn.I8, pad, shift) for w, shift in zip(ws, (gate, up, down))], [U.Held(s, F32) for s in ss]
+    nn.I8FeedForward(hx.matrix, hw[0].matrix, hs[0].matrix, hw[1].matrix, hs[1].matrix, hw[2].matrix, hs[2].matrix, y.matrix, room=space).run()
+    want, slack = i8_block(x, ws, ss, "silu")
+    close("y", y.get(), want, (U.UNIT[BF16] + 2.0 ** -19) * abs(want) + slack + 1e-30)
+    space.check()
