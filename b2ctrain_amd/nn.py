@@ -3,7 +3,7 @@ products in 8-bit integers (include/b2c_kernels.h, "dense operators").
 
 An operator is planned once for its matrices and then run on a HIP stream as often as wanted: the plan holds the
 launcher's argument struct, and allocates nothing but through `room`, a function that the caller gives (bytes -> an
-object with `data_ptr()`; in a torch program ``lambda n: torch.empty(n, dtype=torch.uint8, device="cuda")``). A matrix is
+object with `data_ptr()` or `ptr`; in a torch program ``lambda n: torch.empty(n, dtype=torch.uint8, device="cuda")``). A matrix is
 a two-dimensional torch tensor whose columns lie next to each other, or a ``Matrix`` over any device pointer. Plans keep
 what they point at alive. Streams are the integer handle of a HIP stream (0: the default stream), and the caller orders
 work on different streams, as for every launcher.
@@ -127,14 +127,22 @@ def matrix(what, name, rows=None, cols=None, dtype=None):
 
 
 def _vector(what, name, n):
-    """The pointer of n single-precision values."""
+    """The pointer of n single-precision values on the GPU."""
     if isinstance(what, Matrix):
-        if what.dtype != F32 or what.rows * what.cols != n:
-            raise ValueError(f"{name}: {n} single-precision values are wanted")
-        return what.ptr
-    if tuple(what.shape) != (n,) or str(what.dtype) != "torch.float32" or (n > 1 and what.stride(0) != 1):
+        m, fits = what, what.rows * what.cols == n and (what.rows <= 1 or what.ld == what.cols)
+    else:
+        try:
+            fits = tuple(what.shape) == (n,) and (n <= 1 or what.stride(0) == 1)
+            if getattr(what, "is_cuda", True) is False:
+                raise ValueError(f"{name}: is not on the GPU")
+            m = Matrix(what.data_ptr(), n, 1, 1, NAMES.get(str(what.dtype).replace("torch.", "")), keep=what)
+        except AttributeError:
+            raise ValueError(f"{name}: {n} single-precision values are wanted, got {type(what).__name__}") from None
+    if m.dtype != F32 or not fits:
         raise ValueError(f"{name}: {n} single-precision values next to each other are wanted")
-    return what.data_ptr()
+    if n and not m.ptr:
+        raise ValueError(f"{name}: a null pointer")
+    return m.ptr
 
 
 def _floating(m, name, types=(F32, F16, BF16)):
@@ -169,7 +177,10 @@ def _get_room(room, n, what):
     if room is None:
         raise ValueError(f"{what}: needs {n} bytes of workspace: give `room`")
     b = room(n)
-    return b, b.data_ptr() if hasattr(b, "data_ptr") else b.ptr
+    at = b.data_ptr() if hasattr(b, "data_ptr") else getattr(b, "ptr", None)
+    if not at or getattr(b, "is_cuda", True) is False or getattr(b, "nbytes", n) < n:
+        raise ValueError(f"{what}: `room` has to give {n} bytes of workspace on the GPU")
+    return b, at
 
 
 class Dropout:

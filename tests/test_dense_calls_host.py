@@ -3,6 +3,7 @@ its range. What can be seen of them without a GPU."""
 import ctypes as C
 
 import pytest
+import torch
 
 from b2ctrain_amd import nn
 from tests.test_dense_host import ADDRESS, M, Room
@@ -21,3 +22,41 @@ def test_i8_block_copies_both_input_weights_or_none(rows, di, f, ld, pitch):
         return p.args.workspace_bytes
 
     assert room(0, 8) == room(8, 0) == room(8, 8) == room(0, 0) + 2 * f * pitch
+
+
+def linear(scale, room=Room()):
+    return nn.I8Linear(M(4, 5), M(6, 5, nn.I8), scale, M(4, 6), room=room)
+
+
+@pytest.mark.parametrize("scale", [
+    torch.ones(6), nn.Matrix(ADDRESS, 6, 1, 9, nn.F32), nn.Matrix(ADDRESS, 2, 3, 4, nn.F32), nn.Matrix(0, 6, 1, 1, nn.F32),
+    nn.Matrix(ADDRESS, 6, 1, 1, nn.BF16), 3, None, [1.0] * 6], ids=str)
+def test_scales_have_to_lie_on_the_gpu_next_to_each_other(scale):
+    with pytest.raises(ValueError, match="scale"):
+        linear(scale)
+    with pytest.raises(ValueError, match="scale"):
+        nn.QuantizeRows(M(6, 5), M(6, 5, nn.I8), scale)
+    for at in range(3):
+        s = [scale if i == at else column(6) for i in range(3)]
+        with pytest.raises(ValueError, match="s_"):
+            nn.I8FeedForward(M(4, 5), M(6, 5, nn.I8), s[0], M(6, 5, nn.I8), s[1], M(6, 6, nn.I8), s[2], M(4, 6), room=Room())
+
+
+def test_scales_that_are_taken():
+    for scale in (column(6), nn.Matrix(ADDRESS, 1, 6, 6, nn.F32), nn.Matrix(ADDRESS, 1, 6, 20, nn.F32), nn.Matrix(ADDRESS, 2, 3, 3, nn.F32)):
+        assert linear(scale).args.w_scale == ADDRESS
+
+
+def test_workspace_has_to_lie_on_the_gpu_and_be_large_enough():
+    need = linear(column(6)).args.workspace_bytes
+
+    class Bytes(Room):
+        is_cuda = True
+
+        def __init__(self, nbytes):
+            self.nbytes = nbytes
+
+    linear(column(6), lambda n: Bytes(n))
+    for room in (lambda n: torch.empty(n, dtype=torch.uint8), lambda n: Bytes(need - 1), lambda n: None, lambda n: bytearray(n)):
+        with pytest.raises(ValueError, match="workspace"):
+            linear(column(6), room)
