@@ -18,6 +18,12 @@ void give_workspace(DenseCtx& ctx, Args& a, size_t bytes, hipStream_t stream) {
   a.workspace_bytes = ctx.workspace.bytes();
 }
 
+// Whether what a forward pass kept is what the gradients of `b` need.
+bool same_call(const b2c_ffn_args& a, const b2c_ffn_args& b) {
+  return a.rows == b.rows && a.d_in == b.d_in && a.d_hidden == b.d_hidden && a.d_out == b.d_out && a.dtype == b.dtype && a.act == b.act &&
+         a.p == b.p && a.seed == b.seed && a.stream == b.stream;
+}
+
 }  // namespace
 
 void dropout(const b2c_dropout_args& a, hipStream_t stream) { done(b2c_hip_dropout(&a, stream), "dropout"); }
@@ -25,16 +31,18 @@ void dropout(const b2c_dropout_args& a, hipStream_t stream) { done(b2c_hip_dropo
 void feed_forward(DenseCtx& ctx, b2c_ffn_args a, bool train, hipStream_t stream) {
   a.saved = nullptr;
   if (train) {
+    ctx.kept.rows = -1;  // until the call has succeeded
     ctx.saved.reserve(b2c_ffn_saved_bytes(&a), false, stream);
     a.saved = ctx.saved.ptr;
   }
   give_workspace(ctx, a, b2c_ffn_workspace_bytes(&a), stream);
   done(b2c_hip_ffn_forward(&a, stream), "feed_forward");
+  if (train) ctx.kept = a;
 }
 
 void feed_forward_backward(DenseCtx& ctx, b2c_ffn_grad_args a, hipStream_t stream) {
-  if (b2c_ffn_saved_bytes(&a.fwd) > ctx.saved.bytes())
-    throw std::runtime_error("feed_forward_backward: no forward pass of these sizes was kept on this context");
+  if (b2c_ffn_saved_bytes(&a.fwd) && !same_call(ctx.kept, a.fwd))
+    throw std::runtime_error("feed_forward_backward: no forward pass of these sizes, type, activation and mask was kept on this context");
   a.fwd.saved = ctx.saved.ptr;
   give_workspace(ctx, a, b2c_ffn_grad_workspace_bytes(&a), stream);
   done(b2c_hip_ffn_backward(&a, stream), "feed_forward_backward");

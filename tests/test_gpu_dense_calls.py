@@ -1,9 +1,11 @@
 """Calls of the dense operators that differ from the usual ones in one thing: an alignment, a buffer's place, a size at the end of
 its range; against their restatement in 64 bits (dense_util.py)."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
-from b2ctrain_amd import nn
+from b2ctrain_amd import _native, nn
 from tests import dense_util as U
 from tests.gpu_harness import emit
 from tests.test_gpu_dense import close
@@ -42,4 +44,62 @@ def test_i8_block_of_weights_aligned_differently(rows, di, f, do, pad, gate, up,
     nn.I8FeedForward(hx.matrix, hw[0].matrix, hs[0].matrix, hw[1].matrix, hs[1].matrix, hw[2].matrix, hs[2].matrix, y.matrix, room=space).run()
     want, slack = i8_block(x, ws, ss, "silu")
     close("y", y.get(), want, (U.UNIT[BF16] + 2.0 ** -19) * abs(want) + slack + 1e-30)
+    space.check()
+
+
+class Handle:
+    """A b2c_dense handle with the C entries that the tests call."""
+
+    def __init__(self):
+        self.L = _native.lib()
+        for name, args in (("b2c_feed_forward", [C.c_void_p, C.POINTER(nn.FfnArgs), C.c_int, C.c_void_p]),
+                           ("b2c_feed_forward_backward", [C.c_void_p, C.POINTER(nn.FfnGradArgs), C.c_void_p])):
+            getattr(self.L, name).argtypes = args
+        self.L.b2c_dense_create.restype = C.c_void_p
+        self.L.b2c_dense_destroy.argtypes = [C.c_void_p]
+        self.ptr = self.L.b2c_dense_create()
+
+    def forward(self, ff, train=1):
+        return self.L.b2c_feed_forward(self.ptr, C.byref(ff.args), train, None)
+
+    def backward(self, ff):
+        return self.L.b2c_feed_forward_backward(self.ptr, C.byref(ff.grad), None)
+
+    def close(self):
+        self.L.b2c_dense_destroy(self.ptr)
+
+
+def test_a_handle_refuses_gradients_of_another_forward_pass():
+    """What the handle kept is of one call: gradients of smaller sizes, another type, activation or mask are refused, though they
+    would fit what is there."""
+    g = np.random.default_rng(1)
+    space, held, d = U.Space(), [], Handle()
+
+    def block(rows, di=200, f=330, dtype=BF16, **kw):
+        h = [U.Held(g.standard_normal(s) * 0.1, dtype) for s in ((rows, di), (f, di), (f, di), (di, f), (rows, di))]
+        out = [U.Held(None, dtype, rows=a, cols=b) for a, b in ((rows, di), (rows, di), (f, di))]
+        held.extend(h + out)
+        x, wg, wu, wd, dy = (m.matrix for m in h)
+        y, dx, dw = (m.matrix for m in out)
+        ff = nn.FeedForward(x, wg, wu, wd, y, **{"p": 0.2, "seed": 3, "train": True, "room": space, **kw})
+        ff.gradients(dy, dx=dx, dw_gate=dw, room=space)
+        return ff
+
+    try:
+        large = block(300)
+        others = {"rows": block(100), "d_hidden": block(300, f=320), "d_in": block(300, di=190), "type": block(300, dtype=F16),
+                  "act": block(300, act="gelu"), "p": block(300, p=0.3), "seed": block(300, seed=4), "stream id": block(300, stream_id=9)}
+        assert d.backward(large) != 0 and b"no forward pass" in d.L.b2c_last_error()
+        assert d.forward(large) == 0 and d.backward(large) == 0 and d.backward(large) == 0
+        for what, other in others.items():
+            emit(f"gradients with another {what}")
+            assert d.backward(other) != 0 and b"no forward pass" in d.L.b2c_last_error(), what
+        assert d.forward(others["rows"], train=0) == 0 and d.backward(large) == 0  # answers leave what is kept alone
+        wrong = nn.FfnArgs.from_buffer_copy(large.args)
+        wrong.act = 17
+        assert d.L.b2c_feed_forward(d.ptr, C.byref(wrong), 1, None) != 0
+        assert d.backward(large) != 0 and b"no forward pass" in d.L.b2c_last_error()  # the last pass to be kept was refused
+        assert d.forward(others["rows"]) == 0 and d.backward(others["rows"]) == 0
+    finally:
+        d.close()
     space.check()
