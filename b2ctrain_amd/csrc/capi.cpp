@@ -874,10 +874,10 @@ void b2c_dense_destroy(b2c_dense* d) { delete d; }
 
 extern "C++" {
 namespace {
-template <typename Args>
-const Args& given(const Args* a, const char* what) {
-  if (!a) throw std::runtime_error(std::string(what) + ": null argument");
-  return *a;
+template <typename T>
+T& given(T* p, const char* what) {
+  if (!p) throw std::runtime_error(std::string(what) + ": null argument");
+  return *p;
 }
 }  // namespace
 }
@@ -885,19 +885,19 @@ int b2c_dropout(const b2c_dropout_args* a, void* stream) {
   return guarded([&] { b2c::dropout(given(a, "dropout"), (hipStream_t)stream); });
 }
 int b2c_feed_forward(b2c_dense* d, const b2c_ffn_args* a, int train, void* stream) {
-  return guarded([&] { b2c::feed_forward(d->ctx, given(a, "feed_forward"), train != 0, (hipStream_t)stream); });
+  return guarded([&] { b2c::feed_forward(given(d, "feed_forward").ctx, given(a, "feed_forward"), train != 0, (hipStream_t)stream); });
 }
 int b2c_feed_forward_backward(b2c_dense* d, const b2c_ffn_grad_args* a, void* stream) {
-  return guarded([&] { b2c::feed_forward_backward(d->ctx, given(a, "feed_forward_backward"), (hipStream_t)stream); });
+  return guarded([&] { b2c::feed_forward_backward(given(d, "feed_forward_backward").ctx, given(a, "feed_forward_backward"), (hipStream_t)stream); });
 }
 int b2c_quantize_rows(const b2c_quantize_args* a, void* stream) {
   return guarded([&] { b2c::quantize_rows(given(a, "quantize_rows"), (hipStream_t)stream); });
 }
 int b2c_i8_linear(b2c_dense* d, const b2c_i8_linear_args* a, void* stream) {
-  return guarded([&] { b2c::i8_linear(d->ctx, given(a, "i8_linear"), (hipStream_t)stream); });
+  return guarded([&] { b2c::i8_linear(given(d, "i8_linear").ctx, given(a, "i8_linear"), (hipStream_t)stream); });
 }
 int b2c_i8_feed_forward(b2c_dense* d, const b2c_i8_ffn_args* a, void* stream) {
-  return guarded([&] { b2c::i8_feed_forward(d->ctx, given(a, "i8_feed_forward"), (hipStream_t)stream); });
+  return guarded([&] { b2c::i8_feed_forward(given(d, "i8_feed_forward").ctx, given(a, "i8_feed_forward"), (hipStream_t)stream); });
 }
 
 }  // extern "C"

@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 import torch
 
-from b2ctrain_amd import nn
+from b2ctrain_amd import _native, nn
 from tests.test_dense_host import ADDRESS, M, Room
 
 
@@ -60,3 +60,20 @@ def test_workspace_has_to_lie_on_the_gpu_and_be_large_enough():
     for room in (lambda n: torch.empty(n, dtype=torch.uint8), lambda n: Bytes(need - 1), lambda n: None, lambda n: bytearray(n)):
         with pytest.raises(ValueError, match="workspace"):
             linear(column(6), room)
+
+
+@pytest.mark.parametrize("entry,args", [("b2c_feed_forward", nn.FfnArgs), ("b2c_feed_forward_backward", nn.FfnGradArgs),
+                                        ("b2c_i8_linear", nn.I8LinearArgs), ("b2c_i8_feed_forward", nn.I8FfnArgs)])
+def test_a_null_handle_or_argument_is_an_error(entry, args):
+    L = _native.lib()
+    fn, p = getattr(L, entry), C.c_void_p
+    fn.argtypes = [p, p, C.c_int, p] if entry == "b2c_feed_forward" else [p, p, p]
+    more = (1, None) if entry == "b2c_feed_forward" else (None,)
+    L.b2c_dense_create.restype, L.b2c_dense_destroy.argtypes = p, [p]
+    d, some = L.b2c_dense_create(), args()
+    try:
+        for handle, a in ((None, C.addressof(some)), (d, None), (None, None)):
+            assert fn(handle, a, *more) != 0 and b"null" in L.b2c_last_error()
+    finally:
+        L.b2c_dense_destroy(d)
+        L.b2c_dense_destroy(None)
