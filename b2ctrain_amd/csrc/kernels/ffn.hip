@@ -135,7 +135,8 @@ struct ForwardPlan {
     if (a->saved) h = kept_h<T>(a);
     const bool in = direct(a->w_gate, a->ld_in, a->d_in) && direct(a->w_up, a->ld_in, a->d_in);
     const bool out = direct(a->w_down, a->ld_out, a->d_hidden), few = few_rows(M, in && out);
-    gate = choose({{M, fp}}, steps_of(a->d_in), true, few, a->saved ? 6 : 2);
+    const Way plain = choose({{M, fp}}, steps_of(a->d_in), true, few, 2), keeping = choose({{M, fp}}, steps_of(a->d_in), true, few, 6);
+    gate = a->saved ? keeping : plain;
     down = choose({{M, a->d_out}}, steps_of(a->d_hidden), false, few);
     x = {{(const T*)a->x, a->ldx}, M, a->d_in};
     wg = {{(const T*)a->w_gate, a->ld_in}, a->d_hidden, a->d_in};
@@ -147,7 +148,7 @@ struct ForwardPlan {
       wu.place(room, in);
       wd.place(room, out);
     }
-    sums = room.take<char>(std::max(gate.sums, down.sums));
+    sums = room.take<char>(std::max({plain.sums, keeping.sums, down.sums}));  // either call may follow the other in the same workspace
   }
 };
 

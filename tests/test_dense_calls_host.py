@@ -77,3 +77,13 @@ def test_a_null_handle_or_argument_is_an_error(entry, args):
     finally:
         L.b2c_dense_destroy(d)
         L.b2c_dense_destroy(None)
+
+
+@pytest.mark.parametrize("rows,di,f,do", [(1500, 2792, 7008, 2792), (3193, 1496, 5392, 48), (4545, 3336, 2320, 369), (5204, 3664, 128, 2832),
+                                          (86, 3949, 4311, 20), (40, 64, 96, 64), (3, 64, 96, 64)])
+def test_block_workspace_is_the_same_with_and_without_kept_values(rows, di, f, do):
+    """A call that answers may follow one that trains in the same workspace, and the other way round."""
+    def room(train):
+        return nn.FeedForward(M(rows, di), M(f, di), M(f, di), M(do, f), M(rows, do), train=train, room=Room()).args.workspace_bytes
+
+    assert room(False) == room(True)
