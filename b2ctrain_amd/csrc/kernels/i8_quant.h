@@ -18,14 +18,15 @@ struct RowScale {
   // x / scale rounded to nearest even twice, to single precision and to an integer, as two's complement in the low
   // byte. With the correctly rounded inverse y, q = x y and the remainder r = x - q scale (exact in one fused
   // operation), q + r y is the correctly rounded quotient (Markstein 1990): three operations in place of a division's ten.
-  // Adding 1.5 2^23 then leaves the integer in the low bits (the bits above the lowest byte are not cleared).
+  // Adding 1.5 2^23 then leaves the integer in the low bits (the bits above the lowest byte are not cleared). The scale of a row of
+  // subnormals may be rounded down so far that a quotient passes 127 (160 units in the last place have a scale of one): it is held there.
   __device__ __forceinline__ uint32_t operator()(float x) const {
     float q = 0.f;
     if (plain) {
       q = x * inverse;
       q = fmaf(fmaf(-q, scale, x), inverse, q);
     } else if (scale > 0.f) {
-      q = x / scale;
+      q = fminf(fmaxf(x / scale, -127.f), 127.f);
     }
     return __builtin_bit_cast(uint32_t, q + 12582912.f);
   }

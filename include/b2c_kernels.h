@@ -641,7 +641,8 @@ size_t b2c_ffn_grad_workspace_bytes(const b2c_ffn_grad_args* a);
 int b2c_hip_ffn_backward(const b2c_ffn_grad_args* a, hipStream_t stream);
 
 /* 8-bit rows: scale[i] = max |x[i][j]| / 127 and q[i][j] = x[i][j] / scale[i], rounded to nearest even, both in single
- * precision. A row of zeros gets scale 0; a row with an infinity or NaN gets scale NaN and zeros. Columns cols .. ldq - 1
+ * precision, q at most 127 in magnitude (which the quotient of a row of subnormals, whose scale is coarse, may exceed). A row of
+ * zeros gets scale 0, and so does one too small for a scale; a row with an infinity or NaN gets scale NaN and zeros. Columns cols .. ldq - 1
  * of q are set to 0 up to the next multiple of 16, those of the last row too. For weights, rows are output channels. */
 typedef struct b2c_quantize_args {
   int64_t rows, cols;

@@ -103,3 +103,42 @@ def test_a_handle_refuses_gradients_of_another_forward_pass():
     finally:
         d.close()
     space.check()
+
+
+def subnormal_rows(cols):
+    """Rows whose largest magnitude is some units of 2^-149, the smallest single-precision value: their scale is so coarse that the
+    quotient may pass 127."""
+    tops = [1, 63, 64, 100, 127, 128, 160, 190, 191, 500, 15811, 16065, 16066, 1 << 20]
+    g = np.random.default_rng(cols)
+    bits = (g.uniform(0, 1, (len(tops), cols)) * (np.array(tops)[:, None] + 1)).astype(np.uint32)
+    bits[:, 0] = tops
+    bits[:, -1] = tops
+    x = bits.view(np.float32)
+    x[:, -1] *= -1
+    return x
+
+
+@pytest.mark.parametrize("cols", [7, 64, 200, 1100, 5000])
+@pytest.mark.parametrize("copies", [1, 200])
+def test_quantize_rows_of_subnormals(cols, copies):
+    emit(f"quantize {copies} times 14 x {cols} subnormals")
+    x = np.tile(subnormal_rows(cols), (copies, 1))
+    h, q, s = U.Held(x, F32), U.Held(None, nn.I8, rows=len(x), cols=cols), U.Held(None, F32, rows=len(x), cols=1)
+    nn.QuantizeRows(h.matrix, q.matrix, s.matrix).run()
+    want, scale = U.quantised(x)  # held to -127 .. 127
+    assert np.array_equal(s.get()[:, 0], scale) and np.array_equal(q.get(), want)
+
+
+@pytest.mark.parametrize("rows,di,do", [(7, 64, 32), (14, 3000, 32), (70, 64, 32), (70, 200, 40)])
+def test_i8_linear_of_subnormals(rows, di, do):
+    """One layer's ways with a row: in the product, in registers, before the tiles. y = acc sx sw is off by its products in single
+    precision, the first of which may be subnormal: half of 2^-149, times sw."""
+    emit(f"i8 linear {rows} x {di}-{do} of subnormals")
+    x = np.resize(subnormal_rows(di)[::-1], (rows, di))
+    w, sw = np.random.default_rng(do).integers(-127, 128, (do, di)).astype(np.int8), np.float32(2.0 ** 100)
+    hx, hw, hs, y, space = U.Held(x, F32), U.Held(w, nn.I8), U.Held(np.full((do, 1), sw), F32), U.Held(None, F32, rows=rows, cols=do), U.Space()
+    nn.I8Linear(hx.matrix, hw.matrix, hs.matrix, y.matrix, room=space).run()
+    q, sx = U.quantised(x)
+    want = (q.astype(np.float64) @ w.T.astype(np.float64)) * sx[:, None].astype(np.float64) * float(sw)
+    close("y", y.get(), want, 4 * 2.0 ** -24 * abs(want) + 2.0 ** -150 * float(sw) * 1.001)
+    space.check()
