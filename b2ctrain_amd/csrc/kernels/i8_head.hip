@@ -128,8 +128,17 @@ __global__ __launch_bounds__(512) void head_kernel(b2c_i8_ffn_args a, const int8
         }
       }
     }
-    const RowScale rh(over_row(top));
-    const float sh = rh.scale * rx.scale;
+    top = over_row(top);
+    RowScale rh(top);
+    float sh = rh.scale * rx.scale;
+    if (!rh.plain && rh.scale > 0.f) {  // a row whose scale is too small for an inverse: the same 8 bits from 2^100 h
+#pragma unroll
+      for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) h[c][j] *= 0x1p100f;
+      rh = RowScale(__builtin_bit_cast(uint32_t, __builtin_bit_cast(float, top) * 0x1p100f));
+      sh = rh.scale * rx.scale * 0x1p-100f;
+    }
     i32x4 y[OT] = {};
 #pragma unroll
     for (int c = 0; c < NC; c++) {

@@ -31,7 +31,7 @@ struct RowScale {
     return __builtin_bit_cast(uint32_t, q + 12582912.f);
   }
   // The same for values that were computed in single precision themselves: one rounding of x inverse, which may fall to the
-  // other side where x / scale lies within 2^-17 of the middle of two integers.
+  // other side where x / scale lies within 2^-17 of the middle of two integers. Of a plain row, or one of zeros.
   __device__ __forceinline__ uint32_t near(float x) const { return __builtin_bit_cast(uint32_t, fmaf(x, inverse, 12582912.f)); }
 };
 __device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }

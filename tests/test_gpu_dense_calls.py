@@ -15,9 +15,9 @@ pytestmark = pytest.mark.gpu
 F32, F16, BF16 = nn.F32, nn.F16, nn.BF16
 
 
-def i8_block(x, ws, ss, name):
-    """y of the 8-bit block, and which values of h lie within single precision's rounding of the middle between two steps: each may
-    move y by one step of its row."""
+def i8_block(x, ws, ss, name, act_eps=2.0 ** -20):
+    """y of the 8-bit block, and how far it may move by values of h that lie within single precision's rounding of the middle between two
+    steps: each by one step of its row. act_eps: how far the activation may be off, beside 2^-20 of itself."""
     dense = lambda q, s, w, sw: (q.astype(np.float64) @ w.T.astype(np.float64)) * s[:, None].astype(np.float64) * sw[:, 0].astype(np.float64)  # noqa: E731
     q, sx = U.quantised(x)
     up = dense(q, sx, ws[1], ss[1])
@@ -26,7 +26,7 @@ def i8_block(x, ws, ss, name):
     step = top / 127
     safe = np.where(step > 0, step, 1)
     t = np.where(step > 0, h / safe, 0)
-    unsure = abs(t - np.floor(t) - 0.5) <= 2.0 ** -20 * (abs(h) + abs(up) + top) / safe
+    unsure = abs(t - np.floor(t) - 0.5) <= (2.0 ** -20 * (abs(h) + top) + act_eps * abs(up)) / safe
     want = (np.rint(t) @ ws[2].T.astype(np.float64)) * step * ss[2][:, 0].astype(np.float64)
     return want, (unsure @ abs(ws[2]).T.astype(np.float64)) * step * ss[2][:, 0]
 
@@ -141,4 +141,27 @@ def test_i8_linear_of_subnormals(rows, di, do):
     q, sx = U.quantised(x)
     want = (q.astype(np.float64) @ w.T.astype(np.float64)) * sx[:, None].astype(np.float64) * float(sw)
     close("y", y.get(), want, 4 * 2.0 ** -24 * abs(want) + 2.0 ** -150 * float(sw) * 1.001)
+    space.check()
+
+
+@pytest.mark.parametrize("rows,di,f,do", [(40, 64, 128, 64), (70, 100, 300, 72), (20, 64, 128, 64), (70, 200, 300, 72)])
+@pytest.mark.parametrize("name", ["silu", "relu"])
+@pytest.mark.parametrize("gate", [1e-28, 1e-31, 1e-33])
+def test_i8_block_with_tiny_inner_activations(rows, di, f, do, name, gate):
+    """h far below one, brought back by the down weights' scales: 8 bits of a row go by its own largest value, however small. Near
+    zero both activations are off by their relative error alone."""
+    emit(f"i8 block {rows} x {di}-{f}-{do} {name}, gate scales of {gate}")
+    g = np.random.default_rng(rows + di)
+    x = g.standard_normal((rows, di)).astype(np.float32)
+    x[5] = 0
+    ws = [g.integers(-127, 128, s).astype(np.int8) for s in ((f, di), (f, di), (do, f))]
+    ss = [(np.exp(g.uniform(-0.5, 0.5, (n, 1))) * k).astype(np.float32) for n, k in ((f, gate / 73), (f, 1 / 73), (do, 1e-3 / gate))]
+    hx, y, space = U.Held(x, F32), U.Held(None, F32, rows=rows, cols=do), U.Space()
+    hw, hs = [U.Held(w, nn.I8) for w in ws], [U.Held(s, F32) for s in ss]
+    nn.I8FeedForward(hx.matrix, hw[0].matrix, hs[0].matrix, hw[1].matrix, hs[1].matrix, hw[2].matrix, hs[2].matrix, y.matrix, act=name,
+                     room=space).run()
+    want, slack = i8_block(x, ws, ss, name, 0)
+    got = y.get()
+    assert (got[5] == 0).all()
+    close("y", got, want, 2.0 ** -18 * abs(want) + slack + 1e-30)
     space.check()
