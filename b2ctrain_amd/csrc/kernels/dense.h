@@ -278,6 +278,16 @@ struct ScaledGate {
   }
 };
 
+// ---- launches ----------------------------------------------------------------------------------------------
+
+// A dimension of a launch holds fewer than 2^32 threads; with more, only the remainder runs and nothing is reported. So many
+// workgroups of up to 512 threads go into two dimensions, where the last ones may have no work.
+constexpr int64_t kMostInRow = 1 << 22;
+inline dim3 grid_of(int64_t blocks) {
+  return blocks <= kMostInRow ? dim3((unsigned)blocks) : dim3((unsigned)kMostInRow, (unsigned)((blocks + kMostInRow - 1) / kMostInRow));
+}
+__device__ __forceinline__ uint32_t block_index() { return blockIdx.y * (uint32_t)kMostInRow + blockIdx.x; }
+
 // ---- host checks -------------------------------------------------------------------------------------------
 
 // A matrix that a call reads or writes: present, on its element's alignment, rows at least as far apart as wide.

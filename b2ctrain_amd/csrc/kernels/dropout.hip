@@ -10,7 +10,7 @@ namespace {
 // of 0.5 GiB reaches 5.3.
 template <typename T>
 __global__ __launch_bounds__(256) void flat_kernel(const T* x, const T* r, T* y, uint64_t n, Drop d) {
-  const uint64_t q = (uint64_t)blockIdx.x * 256 + threadIdx.x, e = q * 8;
+  const uint64_t q = (uint64_t)block_index() * 256 + threadIdx.x, e = q * 8;
   if (e >= n) return;
   Philox4 w{};
   if (d.threshold) w = philox(q, d.stream, d.seed);
@@ -44,7 +44,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void rows_kernel(const T* x, int64_t ldx, const T* r, int64_t ldr, T* y, int64_t ldy, uint64_t n,
                                                    uint32_t cols, Drop d) {
   const int lane = threadIdx.x & 63;
-  const uint64_t first = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 512;
+  const uint64_t first = ((uint64_t)block_index() * 4 + (threadIdx.x >> 6)) * 512;
   if (first >= n) return;
   uint32_t bits = 255;
   if (d.threshold) {
@@ -99,8 +99,8 @@ int launch(const b2c_dropout_args* a, const Drop& d, hipStream_t stream) {
   const bool flat = (a->rows == 1 || (a->ldx == a->cols && a->ldy == a->cols && (!a->residual || a->ldr == a->cols))) &&
                     on16(a->x) && on16(a->y) && on16(a->residual);
   const T *x = (const T*)a->x, *r = (const T*)a->residual;
-  if (flat) flat_kernel<T><<<dim3((unsigned)blocks), 256, 0, stream>>>(x, r, (T*)a->y, n, d);
-  else rows_kernel<T><<<dim3((unsigned)blocks), 256, 0, stream>>>(x, a->ldx, r, a->ldr, (T*)a->y, a->ldy, n, (uint32_t)a->cols, d);
+  if (flat) flat_kernel<T><<<grid_of((int64_t)blocks), 256, 0, stream>>>(x, r, (T*)a->y, n, d);
+  else rows_kernel<T><<<grid_of((int64_t)blocks), 256, 0, stream>>>(x, a->ldx, r, a->ldr, (T*)a->y, a->ldy, n, (uint32_t)a->cols, d);
   return hipGetLastError();
 }
 

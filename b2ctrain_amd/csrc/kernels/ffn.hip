@@ -41,6 +41,7 @@ template <typename T>
 struct Packs {
   Pack<T> of[5];
   int n = 0;
+  uint32_t blocks = 0;
   void add(const Side<T>& from, int64_t rows, int cols, T* to, int64_t pitch, const Drop& d) {
     const int64_t groups = up(cols, 8) / 8;
     of[n++] = {from, to, rows, pitch, cols, (uint32_t)groups, (uint32_t)(up(rows * groups, 256) / 256), d};
@@ -48,8 +49,9 @@ struct Packs {
 };
 template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(Packs<T> all) {
-  uint32_t block = blockIdx.x;
+  uint32_t block = block_index();
   int i = 0;
+  if (block >= all.blocks) return;
   while (block >= all.of[i].blocks) block -= all.of[i++].blocks;
   const Pack<T>& p = all.of[i];
   const int64_t t = (int64_t)block * 256 + threadIdx.x, m = t / p.groups;
@@ -73,7 +75,7 @@ __global__ __launch_bounds__(256) void pack_kernel(Packs<T> all) {
   *reinterpret_cast<vec<T, 8>*>(p.to + m * p.pitch + n) = v;
 }
 template <typename T>
-int make(const Packs<T>& all, hipStream_t stream) {
+int make(Packs<T>& all, hipStream_t stream) {
   int64_t blocks = 0;
   for (int i = 0; i < all.n; i++) {
     blocks += all.of[i].blocks;
@@ -81,7 +83,8 @@ int make(const Packs<T>& all, hipStream_t stream) {
   }
   if (blocks == 0) return hipSuccess;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-  pack_kernel<T><<<dim3((unsigned)blocks), 256, 0, stream>>>(all);
+  all.blocks = (uint32_t)blocks;
+  pack_kernel<T><<<grid_of(blocks), 256, 0, stream>>>(all);
   return hipGetLastError();
 }
 

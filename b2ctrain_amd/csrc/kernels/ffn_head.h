@@ -131,7 +131,7 @@ __global__ __launch_bounds__(WAVES * 64) void head_rows_kernel(HeadRows<T> a, co
   using F8 = vec<T, 8>;
   __shared__ __attribute__((aligned(1024))) F8 lds[2][N][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4;
-  const int64_t m0 = ((int64_t)blockIdx.x * WAVES + wave) * (16 * RT) + (lane & 15);
+  const int64_t m0 = ((int64_t)block_index() * WAVES + wave) * (16 * RT) + (lane & 15);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(char*)lds;
 
   auto start = [&](int c) {
@@ -439,8 +439,8 @@ template <typename T, int ACT, int USE, int KS>
 int head_rows(const HeadRows<T>& rows, const T* frags, int chunks, const RowsOut<T>& out, hipStream_t stream) {
   constexpr int RT = KS == 4 ? 1 : 2;
   const int64_t many = up(rows.M, 64 * RT) / (64 * RT), few = up(rows.M, 64) / 64;
-  if (RT == 1 || many < 768) head_rows_kernel<T, ACT, USE, KS, 1, 4><<<dim3((unsigned)few), 256, 0, stream>>>(rows, frags, chunks, out);
-  else head_rows_kernel<T, ACT, USE, KS, RT, 4><<<dim3((unsigned)many), 256, 0, stream>>>(rows, frags, chunks, out);
+  if (RT == 1 || many < 768) head_rows_kernel<T, ACT, USE, KS, 1, 4><<<grid_of(few), 256, 0, stream>>>(rows, frags, chunks, out);
+  else head_rows_kernel<T, ACT, USE, KS, RT, 4><<<grid_of(many), 256, 0, stream>>>(rows, frags, chunks, out);
   return hipGetLastError();
 }
 

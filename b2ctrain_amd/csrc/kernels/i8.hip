@@ -49,9 +49,11 @@ template <typename T, int THREADS, int HELD, typename With>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q,
                                                        int64_t ldq, float* scale, uint32_t own, With copies) {
   __shared__ uint32_t part[4];
+  const uint32_t block = block_index();
   if constexpr (std::is_same_v<With, Copies>) {
-    if (blockIdx.x >= own) {  // each with an index of its own: for a variable one the compiler puts them into scratch memory
-      const uint32_t b = blockIdx.x - own, b1 = copies.of[0].blocks, b2 = b1 + copies.of[1].blocks;
+    if (block >= own) {  // each with an index of its own: for a variable one the compiler puts them into scratch memory
+      const uint32_t b = block - own, b1 = copies.of[0].blocks, b2 = b1 + copies.of[1].blocks;
+      if (b >= copies.blocks) return;
       if (b < b1) copy_block(copies.of[0], b);
       else if (b < b2) copy_block(copies.of[1], b - b1);
       else copy_block(copies.of[2], b - b2);
@@ -59,7 +61,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t ldx, 
     }
   }
   const int t = threadIdx.x % THREADS;
-  const int64_t m = (int64_t)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
+  const int64_t m = (int64_t)block * (256 / THREADS) + threadIdx.x / THREADS;
   const bool there = m < rows;
   const T* row = x + (there ? m : 0) * ldx;
   auto load = [&](int64_t k) {
@@ -131,8 +133,8 @@ int quantize(const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int
     constexpr int N = decltype(threads)::value;
     const uint32_t own = (uint32_t)(up(rows, 256 / N) / (256 / N));
     constexpr int HELD = decltype(held)::value;
-    if (copies.blocks) quantize_kernel<T, N, HELD><<<dim3(own + copies.blocks), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale, own, copies);
-    else quantize_kernel<T, N, HELD><<<dim3(own), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale, own, Nothing{});
+    if (copies.blocks) quantize_kernel<T, N, HELD><<<grid_of((int64_t)own + copies.blocks), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale, own, copies);
+    else quantize_kernel<T, N, HELD><<<grid_of(own), 256, 0, stream>>>(x, ldx, rows, cols, q, ldq, scale, own, Nothing{});
     return hipGetLastError();
   };
   using std::integral_constant;

@@ -165,3 +165,86 @@ def test_i8_block_with_tiny_inner_activations(rows, di, f, do, name, gate):
     assert (got[5] == 0).all()
     close("y", got, want, 2.0 ** -18 * abs(want) + slack + 1e-30)
     space.check()
+
+
+class Raw:
+    """Device memory that is not filled, with windows of it to write and read."""
+
+    hip = None
+
+    def __init__(self, values, np_type):
+        Raw.hip = Raw.hip or C.CDLL("libamdhip64.so.7")  # the library's own copy
+        self.type, self.ptr = np.dtype(np_type), C.c_void_p()
+        self.check(self.hip.hipMalloc(C.byref(self.ptr), C.c_size_t(values * self.type.itemsize)))
+
+    @staticmethod
+    def check(rc):
+        assert rc == 0, f"hipError {rc}"
+
+    def at(self, first):
+        return C.c_void_p(self.ptr.value + first * self.type.itemsize)
+
+    def write(self, first, x):
+        x = np.ascontiguousarray(x, self.type)
+        self.check(self.hip.hipMemcpy(self.at(first), x.ctypes.data_as(C.c_void_p), C.c_size_t(x.nbytes), 1))
+
+    def read(self, first, n):
+        x = np.empty(n, self.type)
+        self.check(self.hip.hipMemcpy(x.ctypes.data_as(C.c_void_p), self.at(first), C.c_size_t(x.nbytes), 2))
+        return x
+
+    def free(self):
+        self.hip.hipFree(self.ptr)
+
+
+def test_quantize_rows_of_more_rows_than_a_launch_has_threads():
+    rows, n = (1 << 30) + 1003, 1000
+    emit(f"quantize {rows} x 1, 7 GB")
+    x, q, s = Raw(rows, np.float16), Raw(rows, np.int8), Raw(rows, np.float32)
+    try:
+        g = np.random.default_rng(1)
+        parts = {first: g.standard_normal((n, 1)).astype(np.float16) for first in (0, (1 << 30) - 500, rows - n)}
+        for first, v in parts.items():
+            x.write(first, v)
+        nn.QuantizeRows(nn.Matrix(x.ptr.value, rows, 1, 1, F16), nn.Matrix(q.ptr.value, rows, 1, 1, nn.I8), nn.Matrix(s.ptr.value, rows, 1, 1, F32)).run()
+        for first in (rows - n, 0):
+            want, scale = U.quantised(parts[first])
+            assert np.array_equal(q.read(first, n), want[:, 0]) and np.array_equal(s.read(first, n), scale), first
+    finally:
+        for m in (x, q, s):
+            m.free()
+
+
+@pytest.mark.parametrize("rows,cols,ld", [(1, (1 << 31) - 1, (1 << 31) - 1), ((1 << 24) + 1, 2049, 2049), ((1 << 24) + 1, 2049, 2050)])
+def test_dropout_of_more_values_than_a_launch_has_threads(rows, cols, ld):
+    """In place, windows at the start, around the value that the 2^32nd thread takes, and at the end."""
+    emit(f"dropout {rows} x {cols}, rows {ld} apart, {rows * ld / 2 ** 29:.0f} GiB")
+    p, seed, stream = 0.3, 11, 12
+    x = Raw(rows * ld, np.float16)
+    try:
+        places = sorted({0, min(rows // 2, (1 << 35) // cols), rows - 1})
+        parts = {m: np.random.default_rng(m).standard_normal(min(cols, 5000)).astype(np.float16) for m in places}
+        for m, v in parts.items():
+            x.write(m * ld + cols - len(v), v)
+        h = nn.Matrix(x.ptr.value, rows, cols, ld, F16)
+        nn.Dropout(h, h, p, seed, stream).run()
+        for m, v in parts.items():
+            e = m * cols + cols - len(v)
+            first = e // 8 * 8
+            want = U.value(v, F16) * window(first, e + len(v), p, seed, stream)[e - first:]
+            close(f"y of row {m}", U.value(x.read(m * ld + cols - len(v), len(v)), F16), want,
+                  U.UNIT[F16] * abs(want) + 3 * 2.0 ** -24 * abs(want) + 2.0 ** -25)
+    finally:
+        x.free()
+
+
+def window(first, end, p, seed, stream):
+    """Dropout's factors of values first .. end - 1, `first` a multiple of 8."""
+    at = np.arange(first // 8, -(-end // 8), dtype=np.uint64)
+    c = np.zeros((len(at), 4), np.uint64)
+    c[:, 0], c[:, 1] = at & np.uint64(0xFFFFFFFF), at >> np.uint64(32)
+    c[:, 2], c[:, 3] = stream & 0xFFFFFFFF, stream >> 32
+    w = U.philox(c, (seed & 0xFFFFFFFF, seed >> 32))
+    bits = np.stack([w & 0xFFFF, w >> 16], axis=2).reshape(-1)[:end - first]
+    t = U.threshold(p)
+    return np.where(bits >= t, 65536.0 / (65536 - t), 0.0)
