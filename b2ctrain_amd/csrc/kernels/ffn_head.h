@@ -1,4 +1,4 @@
-// The feed-forward block where its input and output are narrow (at most 128) and its rows many: a head over the splats
+// The feed-forward block where its input and output are narrow (at most 128) and its rows many (is_head): a head over the splats
 // of a scene. Written to memory and read back, the inner activations would be most of the traffic (g, u, h, dg, du of a
 // 64-256-64 head: 2.5 KB a row beside 128 bytes of x), so they never leave the registers: the forward pass and the two
 // halves of the backward pass each form g and u again from x. What bounds them then is the activation's arithmetic.
@@ -376,8 +376,14 @@ __global__ __launch_bounds__(256) void head_join_kernel(const float* sums, int64
 
 // ---- host --------------------------------------------------------------------------------------------------
 
-// Whether a block is such a head. Its rows are more than a few, since the weights are rearranged in each call.
-inline bool is_head(const b2c_ffn_args* a) { return a->rows > 32 && a->d_in <= 128 && a->d_out <= 128; }
+// Whether a block is such a head: narrow, and its rows, 64 to a workgroup, give every compute unit one, since a workgroup passes over
+// the whole hidden width by itself. Steps in microseconds, this way and by tiles through memory: 16384 rows of 64-512-64 69 and
+// 64, of 64-2048-64 167 and 236, of 128-2048-128 244 and 251; 4096 rows of 64-512-64 65 and 43, of 64-2048-64 147 and 68; 40 rows
+// of 96-8192-96 696 and 57; 32768 rows of 64-512-64 77 and 110. Up to 64 hidden units the two are alike for fewer rows (1024
+// rows of 64-64-64: 24 and 25), and this one keeps nothing between its passes; but the weights are rearranged in each call, which a few rows do not pay for.
+inline bool is_head(const b2c_ffn_args* a) {
+  return a->d_in <= 128 && a->d_out <= 128 && (a->rows >= 64 * 256 || (a->rows > 32 && a->d_hidden <= 64));
+}
 inline int head_steps(const b2c_ffn_args* a) {
   const int n = (int)(up(std::max(a->d_in, a->d_out), 32) / 32);
   return n == 3 ? 4 : n;

@@ -87,3 +87,13 @@ def test_block_workspace_is_the_same_with_and_without_kept_values(rows, di, f, d
         return nn.FeedForward(M(rows, di), M(f, di), M(f, di), M(do, f), M(rows, do), train=train, room=Room()).args.workspace_bytes
 
     assert room(False) == room(True)
+
+
+@pytest.mark.parametrize("rows,di,f,do,kept", [
+    (40, 96, 8192, 96, True), (33, 128, 1 << 20, 128, True), (2000, 128, 2048, 128, True), (8000, 64, 256, 64, True), (40, 96, 64, 96, False),
+    (16384, 96, 8192, 96, False), (1_000_000, 64, 256, 64, False), (1_000_000, 64, 256, 129, True), (1_000_000, 129, 256, 3, True),
+    (32, 64, 64, 64, True)])
+def test_a_block_is_a_head_where_its_rows_fill_the_device(rows, di, f, do, kept):
+    """A head keeps nothing for its backward pass. Its workgroups share out rows alone and each passes over the whole hidden width."""
+    a = nn.FfnArgs(rows=rows, d_in=di, d_hidden=f, d_out=do, dtype=nn.BF16)
+    assert (nn._lib().b2c_ffn_saved_bytes(C.byref(a)) > 0) == kept

@@ -8,7 +8,7 @@ import pytest
 from b2ctrain_amd import _native, nn
 from tests import dense_util as U
 from tests.gpu_harness import emit
-from tests.test_gpu_dense import close
+from tests.test_gpu_dense import check_block, close
 
 pytestmark = pytest.mark.gpu
 
@@ -248,3 +248,29 @@ def window(first, end, p, seed, stream):
     bits = np.stack([w & 0xFFFF, w >> 16], axis=2).reshape(-1)[:end - first]
     t = U.threshold(p)
     return np.where(bits >= t, 65536.0 / (65536 - t), 0.0)
+
+
+@pytest.mark.parametrize("sizes", [(16384, 33, 72, 24), (16399, 64, 256, 64), (17001, 128, 96, 16), (16384, 7, 200, 3), (16500, 61, 130, 128),
+                                   (33000, 32, 512, 32)])
+@pytest.mark.parametrize("dtype,name,p,residual,pad,shift", [(BF16, "silu", 0.0, False, 0, 0), (F16, "gelu", 0.2, True, 5, 1),
+                                                             (BF16, "relu", 0.1, True, 8, 0)])
+def test_heads(sizes, dtype, name, p, residual, pad, shift):
+    """Narrow blocks of as many rows as their own kernels are for."""
+    check_block(*sizes, dtype, name, p, residual, pad, shift)
+
+
+@pytest.mark.parametrize("sizes", [(98304 + 77, 24, 40, 16), (100_001, 64, 90, 48), (98304, 128, 33, 100)])
+def test_heads_of_two_row_tiles_a_wave(sizes):
+    check_block(*sizes, BF16, "silu", 0.1, True, 0, 0)
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("sizes", [(16384, 40, 72, 24), (16385, 100, 300, 64)])
+def test_heads_with_weight_gradients_in_single_precision(sizes, accumulate):
+    check_block(*sizes, BF16, "silu", 0.1, False, 0, 0, grad=F32, accumulate=accumulate)
+
+
+@pytest.mark.parametrize("sizes", [(40, 96, 8192, 96), (256, 128, 2048, 128), (2000, 64, 1030, 33), (100, 64, 64, 64), (65, 96, 65, 3)])
+@pytest.mark.parametrize("dtype,name", [(BF16, "silu"), (F16, "gelu")])
+def test_narrow_blocks_of_few_rows(sizes, dtype, name):
+    check_block(*sizes, dtype, name, 0.2, True, 0, 0)
