@@ -212,7 +212,7 @@ inline Way choose(std::initializer_list<Extent> jobs, int64_t steps, bool dual, 
 template <typename T, bool PT, bool QT, bool DUAL, bool TWO, int SIDE, typename Epi, int NJ>
 int launch_tiles(const Jobs<T, Epi, NJ>& jobs, int64_t first, int64_t count, int parts, hipStream_t stream) {
   if (count <= 0) return hipSuccess;
-  if (count * parts >= (int64_t)1 << 23) return hipErrorInvalidValue;  // of 512 threads; no device memory holds that much
+  if (count * parts * (SIDE == 64 ? 256 : 512) >= (int64_t)1 << 32) return hipErrorInvalidValue;  // no device memory holds that much
   const dim3 grid((unsigned)(count * parts));
   if constexpr (SIDE == 256)
     tile_kernel<T, PT, QT, DUAL, TWO, 2, 4, 128, 64, 2><<<grid, 512, 0, stream>>>(jobs, (uint32_t)first, (uint32_t)count, parts);
