@@ -27,7 +27,7 @@ __device__ __forceinline__ void copy_to_lds(const void* base, uint32_t offset, u
   const uint64_t b = reinterpret_cast<uint64_t>(base);
   const vec<uint32_t, 4> rsrc = {(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, kOutside, 0x00020000u};
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc)
-               : "memory");
+               : "m0", "memory");
 }
 
 template <typename T>
