@@ -87,6 +87,7 @@ __device__ __forceinline__ void put_as(int dtype, void* y, int64_t ldy, int64_t 
 template <int ACT, int KI, int NC>
 __global__ __launch_bounds__(512) void head_kernel(b2c_i8_ffn_args a, const int8_t* frags, int chunks) {
   constexpr int N = head_fragments(KI), OT = 4 * KI;
+  static_assert(NC >= KI);  // the loop over hidden units' scales covers the outputs'
   using A = vec<int8_t, 16>;
   __shared__ A w[NC * N][64];
   __shared__ f32x4 sg[NC * 16], su[NC * 16], sd[KI * 16];
@@ -97,8 +98,6 @@ __global__ __launch_bounds__(512) void head_kernel(b2c_i8_ffn_args a, const int8
     ((float*)su)[j] = j < a.d_hidden ? a.s_up[j] : 0.f;
     if (j < KI * 64) ((float*)sd)[j] = j < a.d_out ? a.s_down[j] : 0.f;
   }
-  if (NC < KI)
-    for (int j = NC * 64 + threadIdx.x; j < KI * 64; j += 512) ((float*)sd)[j] = j < a.d_out ? a.s_down[j] : 0.f;
   __syncthreads();
   const int64_t M = a.rows, tiles = (M + 15) / 16;
   for (int64_t tile = (int64_t)blockIdx.x * 8 + wave; tile < tiles; tile += (int64_t)gridDim.x * 8) {
