@@ -6,6 +6,8 @@ import pytest
 import torch
 
 from b2ctrain_amd import _native, nn
+from tests import dense_bounds as B
+from tests import dense_util as U
 from tests.test_dense_host import ADDRESS, M, Room
 
 
@@ -97,3 +99,20 @@ def test_a_block_is_a_head_where_its_rows_fill_the_device(rows, di, f, do, kept)
     """A head keeps nothing for its backward pass. Its workgroups share out rows alone and each passes over the whole hidden width."""
     a = nn.FfnArgs(rows=rows, d_in=di, d_hidden=f, d_out=do, dtype=nn.BF16)
     assert (nn._lib().b2c_ffn_saved_bytes(C.byref(a)) > 0) == kept
+
+
+@pytest.mark.parametrize("dtype,name", [(nn.BF16, "silu"), (nn.F16, "gelu")])
+def test_the_gradients_bound_sees_one_rounding_more(dtype, name):
+    """The roundings that the block makes stay within the bound; with g and u rounded too, some outputs of each kind do not."""
+    past = {k: 0 for k in ("dx", "dw_gate", "dw_up", "dw_down")}
+    for seed, sizes in enumerate(B.SINGLE * 4):
+        x, wg, wu, wd, dy = B.make(*sizes, dtype, seed)
+        m = U.mask(sizes[0], sizes[3], 0.2, 7, 5)
+        for kept in (False, True):
+            ref, bound = B.grads_bound(x, wg, wu, wd, name, dtype, dy, m, kept)
+            got = B.rounded_grads(x, wg, wu, wd, name, dtype, dy, m, kept)
+            more = B.rounded_grads(x, wg, wu, wd, name, dtype, dy, m, kept, inputs=True)
+            for k in past:
+                assert (abs(got[k] - ref[k]) <= bound[k]).all(), (sizes, k)
+                past[k] += (abs(more[k] - ref[k]) > bound[k]).sum()
+    assert all(past.values()), past

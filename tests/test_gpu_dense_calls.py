@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 from b2ctrain_amd import _native, nn
+from tests import dense_bounds as B
 from tests import dense_util as U
 from tests.gpu_harness import emit
 from tests.test_gpu_dense import check_block, close
@@ -274,3 +275,25 @@ def test_heads_with_weight_gradients_in_single_precision(sizes, accumulate):
 @pytest.mark.parametrize("dtype,name", [(BF16, "silu"), (F16, "gelu")])
 def test_narrow_blocks_of_few_rows(sizes, dtype, name):
     check_block(*sizes, dtype, name, 0.2, True, 0, 0)
+
+
+@pytest.mark.parametrize("sizes", B.SINGLE + [(16384, 40, 1, 24), (16384, 128, 1, 100), (40, 24, 1, 16), (40, 96, 1, 128)])
+@pytest.mark.parametrize("dtype,name", [(BF16, "silu"), (F16, "gelu"), (BF16, "relu")])
+@pytest.mark.parametrize("p", [0.0, 0.2])
+def test_gradients_have_no_other_roundings(sizes, dtype, name, p):
+    rows, di, f, do = sizes
+    emit(f"gradients of {rows} x {di}-{f}-{do} type {dtype} {name} p {p}")
+    x, wg, wu, wd, dy = B.make(*sizes, dtype, rows + f)
+    space, y = U.Space(), U.Held(None, dtype, rows=rows, cols=do)
+    h = [U.Held(v, dtype) for v in (x, wg, wu, wd, dy)]
+    ff = nn.FeedForward(*(v.matrix for v in h[:4]), y.matrix, act=name, p=p, seed=7, stream_id=5, train=True, room=space)
+    out = {k: U.Held(None, dtype, rows=a, cols=b) for k, a, b in (("dx", rows, di), ("dw_gate", f, di), ("dw_up", f, di), ("dw_down", do, f))}
+    ff.gradients(h[4].matrix, **{k: o.matrix for k, o in out.items()}, room=space)
+    ff.forward()
+    ff.backward()
+    m = U.mask(rows, do, p, 7, 5) if p else np.ones((rows, do))
+    kept = nn._lib().b2c_ffn_saved_bytes(C.byref(ff.args)) > 0
+    ref, bound = B.grads_bound(x, wg, wu, wd, name, dtype, dy, m, kept)
+    for k, o in out.items():
+        close(k, o.get(), ref[k], bound[k])
+    space.check()
