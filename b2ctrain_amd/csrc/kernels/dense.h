@@ -120,12 +120,13 @@ __device__ __forceinline__ void get(const T* base, int64_t ld, int64_t m, int n,
 // zeros, so that a later product may run over them.
 
 // h = act(g) u, and the factors of the backward pass: du = dh act(g), dg = dh u act'(g). act(g) at column n of `saved`,
-// u act'(g) at column fp + n, each rounded to T once; were g and u kept instead, the factors would hold two roundings more
-// (the gradients of a 8192 x 2048-5632 step: 3.5e-3 off in bf16, 2.9e-3 this way), and the backward pass would take act again.
+// u act'(g) at column fp + n, in single precision, since their products with dh are rounded for the matrix instructions anyway:
+// kept in T they left the gradients of a 8192 x 2048-5632 step 2.9e-3 off in bf16, where this way they are 2.3e-3 off, as y is; the
+// step takes 1551 us so, 1495 with them in T. Factors instead of g and u, so that the backward pass need not take act again.
 template <typename T, int ACT>
 struct GateOut {
   T* h;
-  T* saved;  // [m][2 fp] or null
+  float* saved;  // [m][2 fp] or null
   int64_t fp;
   int f;
   template <int W>
@@ -183,11 +184,11 @@ struct RowsOut {
   }
 };
 
-// dg and du from dh and the factors that the forward pass kept, rounded to T for the products that follow: relative errors of
+// dg and du from dh and the factors that the forward pass kept, rounded to T once for the products that follow: relative errors of
 // half a unit in the last place, independent from value to value, that average out in the sums.
 template <typename T>
 struct GateBack {
-  const T* saved;  // [m][2 fp]
+  const float* saved;  // [m][2 fp]
   T* dgu;          // [m][2 fp]: dg, then du
   int64_t fp;
   int f;

@@ -120,7 +120,7 @@ int64_t steps_of(int64_t k) { return up(k, 64) / 64; }
 // The inner activations that a forward pass keeps for the down weights' gradient: behind its factors.
 template <typename T>
 T* kept_h(const b2c_ffn_args* a) {
-  return (T*)a->saved + a->rows * 2 * up(a->d_hidden, 64);
+  return (T*)((float*)a->saved + a->rows * 2 * up(a->d_hidden, 64));
 }
 
 // What a forward pass needs beside its matrices.
@@ -138,7 +138,7 @@ struct ForwardPlan {
     if (a->saved) h = kept_h<T>(a);
     const bool in = direct(a->w_gate, a->ld_in, a->d_in) && direct(a->w_up, a->ld_in, a->d_in);
     const bool out = direct(a->w_down, a->ld_out, a->d_hidden), few = few_rows(M, in && out);
-    const Way plain = choose({{M, fp}}, steps_of(a->d_in), true, few, 2), keeping = choose({{M, fp}}, steps_of(a->d_in), true, few, 6);
+    const Way plain = choose({{M, fp}}, steps_of(a->d_in), true, few, 2), keeping = choose({{M, fp}}, steps_of(a->d_in), true, few, 10);
     gate = a->saved ? keeping : plain;
     down = choose({{M, a->d_out}}, steps_of(a->d_hidden), false, few);
     x = {{(const T*)a->x, a->ldx}, M, a->d_in};
@@ -163,7 +163,7 @@ int forward(const b2c_ffn_args* a, const Drop& d, hipStream_t stream) {
   Packs<T> packs;
   for (const Operand<T>* o : {&p.x, &p.wg, &p.wu, &p.wd}) o->add_to(packs);
   if ((rc = make(packs, stream))) return rc;
-  const GateOut<T, ACT> gate{p.h, (T*)a->saved, p.fp, a->d_hidden};
+  const GateOut<T, ACT> gate{p.h, (float*)a->saved, p.fp, a->d_hidden};
   Product<T> in{p.x.side(), p.wg.side(), {}, p.wu.side(), a->rows, p.fp, a->d_in, 0, a->rows, a->d_hidden};
   if ((rc = product<T, false, false, true, false>(in, p.gate, p.sums, gate, stream))) return rc;
   const RowsOut<T> out{(T*)a->y, a->ldy, (const T*)a->residual, a->ldr, a->d_out, d};
@@ -183,7 +183,7 @@ struct BackwardPlan {
     const int64_t M = a->rows;
     fp = up(a->d_hidden, 64);
     dgu = room.take<T>(M * 2 * fp);
-    back = choose({{M, fp}}, steps_of(a->d_out), false, false, 8);
+    back = choose({{M, fp}}, steps_of(a->d_out), false, false, 12);
     const Extent in{fp + a->d_hidden, a->d_in}, down{a->d_out, a->d_hidden};
     const int64_t k = steps_of(M);
     dw = b->dw_down && (b->dw_gate || b->dw_up) ? choose({in, down}, k, false, false)
@@ -223,7 +223,7 @@ int block_backward(const b2c_ffn_grad_args* b, const Drop& d, hipStream_t stream
     if ((rc = make(packs, stream))) return rc;
   }
   const Side<T> dz = p.dz.side(), x = p.x.side(), dgu{p.dgu, 2 * fp};
-  const GateBack<T> back{(const T*)a->saved, p.dgu, fp, a->d_hidden, scale};
+  const GateBack<T> back{(const float*)a->saved, p.dgu, fp, a->d_hidden, scale};
   const Product<T> dh{dz, p.wd.side(), {}, {}, M, fp, a->d_out, 0, M, a->d_hidden};
   if ((rc = product<T, true, false, false, false>(dh, p.back, p.sums, back, stream))) return rc;
   const bool f32 = b->grad_dtype == B2C_F32, add = b->accumulate != 0;
@@ -270,7 +270,7 @@ using namespace b2c::dev;
 
 extern "C" size_t b2c_ffn_saved_bytes(const b2c_ffn_args* a) {
   Drop d;
-  return sizes_ok(a, &d) && !is_head(a) ? (size_t)a->rows * 3 * up(a->d_hidden, 64) * 2 : 0;
+  return sizes_ok(a, &d) && !is_head(a) ? (size_t)a->rows * up(a->d_hidden, 64) * (2 * sizeof(float) + 2) : 0;
 }
 extern "C" size_t b2c_ffn_workspace_bytes(const b2c_ffn_args* a) {
   Drop d;

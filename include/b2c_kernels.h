@@ -590,8 +590,8 @@ typedef struct b2c_dropout_args {
 int b2c_hip_dropout(const b2c_dropout_args* a, hipStream_t stream);
 
 /* The gated feed-forward block: g = x w_gate^T, u = x w_up^T, h = act(g) u, y = residual + dropout(h w_down^T), dropout
- * as in b2c_hip_dropout over [rows][d_out]. h is rounded to dtype between the two products. With `saved` set, act(g),
- * u act'(g) and h are kept there (rounded to dtype) for the backward pass. rows at most 2^30, widths at most 2^20. */
+ * as in b2c_hip_dropout over [rows][d_out]. h is rounded to dtype between the two products. With `saved` set, act(g) and
+ * u act'(g) in single precision and h in dtype are kept there for the backward pass, which rounds dg and du to dtype. rows at most 2^30, widths at most 2^20. */
 typedef struct b2c_ffn_args {
   int64_t rows;
   int d_in, d_hidden, d_out;

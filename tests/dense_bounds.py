@@ -1,13 +1,12 @@
-"""How far the block's gradients may be off, term by term as they are formed: g and u stay in single precision, h is rounded once.
-A block that keeps values for its backward pass (`kept`) rounds act(g) and u act'(g), and then dg and du, their products with dh; one that
-does not rounds dg and du alone."""
+"""How far the block's gradients may be off, term by term as they are formed: g, u, act(g) and u act'(g) stay in single precision,
+h, dg and du are rounded once, for the products that take them."""
 import numpy as np
 
 from b2ctrain_amd import nn
 from tests import dense_util as U
 
 
-def grads_bound(x, wg, wu, wd, name, dtype, dy, m, kept):
+def grads_bound(x, wg, wu, wd, name, dtype, dy, m):
     """(the gradients in 64 bits, how far each value may be from them)."""
     e, b = U.UNIT[dtype], lambda n: (n + 8) * U.F32_SUM
     tiny = 2.0 ** -25 if dtype == nn.F16 else 2.0 ** -134  # half the distance of the type's subnormals
@@ -22,9 +21,8 @@ def grads_bound(x, wg, wu, wd, name, dtype, dy, m, kept):
     if name == "relu":  # a g within its error of zero may take either slope
         ed = ed + (abs(g) <= eg)
     eh = ea * (abs(u) + eu) + abs(a) * eu + e * abs(a * u) + tiny
-    roundings = 2 if kept else 1
-    edg = (abs(dh) + edh) * ((abs(u) + eu) * ed + eu * abs(d)) + edh * abs(u * d) + roundings * e * abs(dh * u * d) + tiny * (1 + kept * abs(dh))
-    edu = (abs(dh) + edh) * ea + edh * abs(a) + roundings * e * abs(dh * a) + tiny * (1 + kept * abs(dh))
+    edg = (abs(dh) + edh) * ((abs(u) + eu) * ed + eu * abs(d)) + edh * abs(u * d) + e * abs(dh * u * d) + tiny
+    edu = (abs(dh) + edh) * ea + edh * abs(a) + e * abs(dh * a) + tiny
     dg, du, h = dh * u * d, dh * a, a * u
     ref = U.block_grads(x, wg, wu, wd, name, dy, m)
     off = {"dx": edg @ abs(wg) + edu @ abs(wu) + b(2 * f) * (abs(dg) @ abs(wg) + abs(du) @ abs(wu)),
@@ -34,8 +32,9 @@ def grads_bound(x, wg, wu, wd, name, dtype, dy, m, kept):
     return ref, {k: off[k] * (1 + 4 * e) + e * (abs(ref[k]) + off[k]) + tiny for k in off}
 
 
-def rounded_grads(x, wg, wu, wd, name, dtype, dy, m, kept, inputs=False):
-    """The gradients with those roundings and 64 bits elsewhere; `inputs`: g and u are rounded first, as they would be if they were kept."""
+def rounded_grads(x, wg, wu, wd, name, dtype, dy, m, factors=False, inputs=False):
+    """The gradients with those roundings and 64 bits elsewhere; `factors`: act(g) and u act'(g) are rounded too, as they would be if they
+    were kept in 16 bits; `inputs`: g and u, likewise."""
     r = lambda v: U.rounded(v, dtype)  # noqa: E731
     g, u = x @ wg.T, x @ wu.T
     a0, _ = U.act(name, g)
@@ -45,7 +44,7 @@ def rounded_grads(x, wg, wu, wd, name, dtype, dy, m, kept, inputs=False):
         a0, _ = U.act(name, g)
         h = r(a0 * u)
     a, d = U.act(name, g)
-    fa, fb = (r(a), r(u * d)) if kept else (a, u * d)
+    fa, fb = (r(a), r(u * d)) if factors else (a, u * d)
     dz = dy * m
     dh = dz @ wd
     dg, du = r(dh * fb), r(dh * fa)

@@ -103,16 +103,17 @@ def test_a_block_is_a_head_where_its_rows_fill_the_device(rows, di, f, do, kept)
 
 @pytest.mark.parametrize("dtype,name", [(nn.BF16, "silu"), (nn.F16, "gelu")])
 def test_the_gradients_bound_sees_one_rounding_more(dtype, name):
-    """The roundings that the block makes stay within the bound; with g and u rounded too, some outputs of each kind do not."""
-    past = {k: 0 for k in ("dx", "dw_gate", "dw_up", "dw_down")}
+    """The roundings that the block makes stay within the bound; with g and u rounded too some outputs of each kind do not, with the
+    factors of dg and du some that come from those."""
+    past = {(k, what): 0 for k in ("dx", "dw_gate", "dw_up", "dw_down") for what in ("factors", "inputs") if (k, what) != ("dw_down", "factors")}
     for seed, sizes in enumerate(B.SINGLE * 4):
         x, wg, wu, wd, dy = B.make(*sizes, dtype, seed)
         m = U.mask(sizes[0], sizes[3], 0.2, 7, 5)
-        for kept in (False, True):
-            ref, bound = B.grads_bound(x, wg, wu, wd, name, dtype, dy, m, kept)
-            got = B.rounded_grads(x, wg, wu, wd, name, dtype, dy, m, kept)
-            more = B.rounded_grads(x, wg, wu, wd, name, dtype, dy, m, kept, inputs=True)
-            for k in past:
-                assert (abs(got[k] - ref[k]) <= bound[k]).all(), (sizes, k)
-                past[k] += (abs(more[k] - ref[k]) > bound[k]).sum()
+        ref, bound = B.grads_bound(x, wg, wu, wd, name, dtype, dy, m)
+        got = B.rounded_grads(x, wg, wu, wd, name, dtype, dy, m)
+        for k in ref:
+            assert (abs(got[k] - ref[k]) <= bound[k]).all(), (sizes, k)
+        for k, what in past:
+            more = B.rounded_grads(x, wg, wu, wd, name, dtype, dy, m, **{what: True})
+            past[k, what] += (abs(more[k] - ref[k]) > bound[k]).sum()
     assert all(past.values()), past

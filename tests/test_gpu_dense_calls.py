@@ -292,8 +292,7 @@ def test_gradients_have_no_other_roundings(sizes, dtype, name, p):
     ff.forward()
     ff.backward()
     m = U.mask(rows, do, p, 7, 5) if p else np.ones((rows, do))
-    kept = nn._lib().b2c_ffn_saved_bytes(C.byref(ff.args)) > 0
-    ref, bound = B.grads_bound(x, wg, wu, wd, name, dtype, dy, m, kept)
+    ref, bound = B.grads_bound(x, wg, wu, wd, name, dtype, dy, m)
     for k, o in out.items():
         close(k, o.get(), ref[k], bound[k])
     space.check()
