@@ -251,7 +251,7 @@ class FeedForward:
             raise ValueError("feed-forward: weight gradients are all of the weights' type, or all in single precision")
         if ws[0] and ws[1] and ws[0].ld != ws[1].ld:
             raise ValueError("feed-forward: dw_gate and dw_up have different distances between rows")
-        kind = types.pop() if types else t
+        kind = types.pop() if types else F32
         if accumulate and kind != F32:
             raise ValueError("feed-forward: gradients accumulate in single precision only")
         g = self.grad = FfnGradArgs(fwd=self.args, dy=dy.ptr, lddy=dy.ld, dx=dx.ptr if dx else None, lddx=dx.ld if dx else 0,

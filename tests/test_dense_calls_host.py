@@ -117,3 +117,10 @@ def test_the_gradients_bound_sees_one_rounding_more(dtype, name):
             more = B.rounded_grads(x, wg, wu, wd, name, dtype, dy, m, **{what: True})
             past[k, what] += (abs(more[k] - ref[k]) > bound[k]).sum()
     assert all(past.values()), past
+
+
+def test_accumulating_with_no_weight_gradient_wanted_is_taken():
+    """A loop that accumulates may pass through a block whose weights are frozen."""
+    f = nn.FeedForward(M(8, 16), M(32, 16), M(32, 16), M(24, 32), M(8, 24), train=True, room=Room())
+    f.gradients(M(8, 24), dx=M(8, 16), accumulate=True, room=Room())
+    assert f.grad.accumulate == 1 and f.grad.grad_dtype == nn.F32  # which is what the launcher takes with it

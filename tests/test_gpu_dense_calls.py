@@ -176,6 +176,10 @@ class Raw:
     def __init__(self, values, np_type):
         Raw.hip = Raw.hip or C.CDLL("libamdhip64.so.7")  # the library's own copy
         self.type, self.ptr = np.dtype(np_type), C.c_void_p()
+        free, total = C.c_size_t(), C.c_size_t()
+        self.check(self.hip.hipMemGetInfo(C.byref(free), C.byref(total)))
+        if free.value < values * self.type.itemsize + (1 << 30):
+            pytest.skip(f"needs {values * self.type.itemsize >> 30} GiB of device memory")
         self.check(self.hip.hipMalloc(C.byref(self.ptr), C.c_size_t(values * self.type.itemsize)))
 
     @staticmethod
