@@ -271,7 +271,8 @@ int b2c_train_step_adam(b2c_ctx* c, b2c_model* m, const b2c_view* v, const b2c_r
                         const b2c_loss_opts* lo, int mode, const b2c_adam_opts* a, b2c_step_times* times);
 
 /* ---- dense operators of a learned head (b2c/dense.h; the argument structs are b2c_kernels.h's) ----
- * A b2c_dense handle keeps one block's workspace, and between its passes what the backward pass needs: the workspace and saved
+ * A b2c_dense handle keeps one block's workspace, and between its passes what the backward pass needs (of the last call with
+ * train; gradients of another call's sizes, type, activation or mask are an error): the workspace and saved
  * fields of the structs are filled in here. stream: a hipStream_t (b2c_ctx_stream), NULL for the default stream. The calls
  * return before the work is done. Device memory is the caller's (b2c_device_upload). */
 typedef struct b2c_dense b2c_dense;
