@@ -101,6 +101,8 @@ def test_a_handle_refuses_gradients_of_another_forward_pass():
         assert d.L.b2c_feed_forward(d.ptr, C.byref(wrong), 1, None) != 0
         assert d.backward(large) != 0 and b"no forward pass" in d.L.b2c_last_error()  # the last pass to be kept was refused
         assert d.forward(others["rows"]) == 0 and d.backward(others["rows"]) == 0
+        plain, again = block(50, p=0.0), block(50, p=0.0, seed=8, stream_id=2)  # without dropout there is no mask to differ
+        assert d.forward(plain) == 0 and d.backward(again) == 0
     finally:
         d.close()
     space.check()
