@@ -130,10 +130,13 @@ EXPORTS = [
     "b2c_dataset_view_read", "b2c_dataset_view_upload", "b2c_dataset_points", "b2c_dataset_summary",
     # dense operators (nn.py)
     "b2c_dense_create", "b2c_dense_destroy", "b2c_dropout", "b2c_feed_forward", "b2c_feed_forward_backward",
-    "b2c_quantize_rows", "b2c_i8_linear", "b2c_i8_feed_forward",
+    "b2c_quantize_rows", "b2c_i8_linear", "b2c_i8_feed_forward", "b2c_block_norm", "b2c_block_norm_backward", "b2c_quantize4",
+    "b2c_q4_linear", "b2c_experts",
     "b2c_hip_dropout", "b2c_ffn_saved_bytes", "b2c_ffn_workspace_bytes", "b2c_hip_ffn_forward",
     "b2c_ffn_grad_workspace_bytes", "b2c_hip_ffn_backward", "b2c_hip_quantize_rows", "b2c_i8_linear_workspace_bytes",
-    "b2c_hip_i8_linear", "b2c_i8_ffn_workspace_bytes", "b2c_hip_i8_ffn",
+    "b2c_hip_i8_linear", "b2c_i8_ffn_workspace_bytes", "b2c_hip_i8_ffn", "b2c_hip_block_norm",
+    "b2c_block_norm_grad_workspace_bytes", "b2c_hip_block_norm_backward", "b2c_hip_quantize4", "b2c_q4_linear_workspace_bytes",
+    "b2c_hip_q4_linear", "b2c_experts_workspace_bytes", "b2c_hip_experts",
 ]
 
 _lib = None

@@ -60,4 +60,23 @@ void i8_feed_forward(DenseCtx& ctx, b2c_i8_ffn_args a, hipStream_t stream) {
   done(b2c_hip_i8_ffn(&a, stream), "i8_feed_forward");
 }
 
+void block_norm(const b2c_block_norm_args& a, hipStream_t stream) { done(b2c_hip_block_norm(&a, stream), "block_norm"); }
+
+void block_norm_backward(DenseCtx& ctx, b2c_block_norm_grad_args a, hipStream_t stream) {
+  give_workspace(ctx, a, b2c_block_norm_grad_workspace_bytes(&a), stream);
+  done(b2c_hip_block_norm_backward(&a, stream), "block_norm_backward");
+}
+
+void quantize4(const b2c_quantize4_args& a, hipStream_t stream) { done(b2c_hip_quantize4(&a, stream), "quantize4"); }
+
+void q4_linear(DenseCtx& ctx, b2c_q4_linear_args a, hipStream_t stream) {
+  give_workspace(ctx, a, b2c_q4_linear_workspace_bytes(&a), stream);
+  done(b2c_hip_q4_linear(&a, stream), "q4_linear");
+}
+
+void experts(DenseCtx& ctx, b2c_experts_args a, hipStream_t stream) {
+  give_workspace(ctx, a, b2c_experts_workspace_bytes(&a), stream);
+  done(b2c_hip_experts(&a, stream), "experts");
+}
+
 }  // namespace b2c

@@ -28,4 +28,15 @@ void quantize_rows(const b2c_quantize_args& a, hipStream_t stream);
 void i8_linear(DenseCtx& ctx, b2c_i8_linear_args a, hipStream_t stream);
 void i8_feed_forward(DenseCtx& ctx, b2c_i8_ffn_args a, hipStream_t stream);
 
+// The norms, gate and residual sum between two blocks, and their gradients.
+void block_norm(const b2c_block_norm_args& a, hipStream_t stream);
+void block_norm_backward(DenseCtx& ctx, b2c_block_norm_grad_args a, hipStream_t stream);
+
+// Groups of columns to 4 bits with a scale each, and products with weights held that way.
+void quantize4(const b2c_quantize4_args& a, hipStream_t stream);
+void q4_linear(DenseCtx& ctx, b2c_q4_linear_args a, hipStream_t stream);
+
+// A mixture-of-experts layer for a few tokens.
+void experts(DenseCtx& ctx, b2c_experts_args a, hipStream_t stream);
+
 }  // namespace b2c

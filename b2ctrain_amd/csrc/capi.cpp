@@ -899,6 +899,21 @@ int b2c_i8_linear(b2c_dense* d, const b2c_i8_linear_args* a, void* stream) {
 int b2c_i8_feed_forward(b2c_dense* d, const b2c_i8_ffn_args* a, void* stream) {
   return guarded([&] { b2c::i8_feed_forward(given(d, "i8_feed_forward").ctx, given(a, "i8_feed_forward"), (hipStream_t)stream); });
 }
+int b2c_block_norm(const b2c_block_norm_args* a, void* stream) {
+  return guarded([&] { b2c::block_norm(given(a, "block_norm"), (hipStream_t)stream); });
+}
+int b2c_block_norm_backward(b2c_dense* d, const b2c_block_norm_grad_args* a, void* stream) {
+  return guarded([&] { b2c::block_norm_backward(given(d, "block_norm_backward").ctx, given(a, "block_norm_backward"), (hipStream_t)stream); });
+}
+int b2c_quantize4(const b2c_quantize4_args* a, void* stream) {
+  return guarded([&] { b2c::quantize4(given(a, "quantize4"), (hipStream_t)stream); });
+}
+int b2c_q4_linear(b2c_dense* d, const b2c_q4_linear_args* a, void* stream) {
+  return guarded([&] { b2c::q4_linear(given(d, "q4_linear").ctx, given(a, "q4_linear"), (hipStream_t)stream); });
+}
+int b2c_experts(b2c_dense* d, const b2c_experts_args* a, void* stream) {
+  return guarded([&] { b2c::experts(given(d, "experts").ctx, given(a, "experts"), (hipStream_t)stream); });
+}
 
 }  // extern "C"
 

@@ -1,0 +1,560 @@
+// The norms, gate and residual sum between two blocks, and their gradients (b2c_hip_block_norm, b2c_hip_block_norm_backward).
+#include "dense.h"
+
+namespace b2c {
+namespace dev {
+namespace {
+
+// A team of LANES threads holds a row in registers, C pieces of sixteen bytes each, so that every matrix is read once, whatever
+// statistics the row needs: thread t has columns (c LANES + t) E .. + E - 1. Teams of up to 64 threads share a wave, larger ones are a
+// workgroup.
+template <int LANES>
+struct Team {
+  static constexpr int THREADS = LANES > 256 ? LANES : 256, TEAMS = THREADS / LANES, WAVES = THREADS / 64;
+  int flip = 0;
+
+  template <int CTRL>
+  static __device__ __forceinline__ float add_dpp(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+  }
+  // The sum over the team, to all of it. Every thread of a workgroup takes part. `room`: two rows of 16 values, used in turn, so that one
+  // barrier a sum is enough.
+  __device__ __forceinline__ float sum(float v, float (&room)[2][16]) {
+    if constexpr (LANES >= 2) v = add_dpp<0xB1>(v);   // quad_perm:[1,0,3,2]
+    if constexpr (LANES >= 4) v = add_dpp<0x4E>(v);   // quad_perm:[2,3,0,1]
+    if constexpr (LANES >= 8) v = add_dpp<0x141>(v);  // row_half_mirror
+    if constexpr (LANES >= 16) v = add_dpp<0x140>(v); // row_mirror
+    if constexpr (LANES >= 32) {
+      const uint32_t b = __builtin_bit_cast(uint32_t, v);
+      const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+      v = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+    }
+    if constexpr (LANES >= 64) {
+      const uint32_t b = __builtin_bit_cast(uint32_t, v);
+      const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+      v = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+    }
+    if constexpr (LANES > 64) {
+      if ((threadIdx.x & 63) == 0) room[flip][threadIdx.x >> 6] = v;
+      __syncthreads();
+      v = room[flip][0];
+#pragma unroll
+      for (int w = 1; w < WAVES; w++) v += room[flip][w];
+      flip ^= 1;
+    }
+    return v;
+  }
+};
+
+// E neighbouring values of a row as they are held in memory; zeros beyond the last column.
+template <int E, typename T>
+__device__ __forceinline__ vec<T, E> piece(const T* row, int n, int cols, bool there) {
+  vec<T, E> v{};
+  if (there && n + E <= cols) {
+    __builtin_memcpy(&v, row + n, sizeof(v));
+  } else if (there) {
+#pragma unroll
+    for (int j = 0; j < E; j++)
+      if (n + j < cols) v[j] = row[n + j];
+  }
+  return v;
+}
+template <int E, typename T>
+__device__ __forceinline__ void put_piece(T* row, int n, int cols, const float (&v)[E]) {
+  put<E>(row, 0, 0, n, cols, v);
+}
+// A norm's weights: ones without any, zeros beyond the last column.
+template <int E, typename T>
+__device__ __forceinline__ void weights(const void* w, bool f32, int n, int cols, float (&v)[E]) {
+#pragma unroll
+  for (int j = 0; j < E; j++) v[j] = n + j < cols ? 1.f : 0.f;
+  if (!w) return;
+  if (f32) get<E>((const float*)w, 0, 0, n, cols, v);
+  else get<E>((const T*)w, 0, 0, n, cols, v);
+}
+
+struct NormArgs {
+  int64_t rows;
+  int cols;
+  bool centre, post, sigmoid, w_f32;
+  float eps, scale, inv_cols;
+  const void *x, *r, *g, *w_post, *w_pre;
+  int64_t ldx, ldr, ldg;
+  uint32_t per_gate;
+  void *y, *n;
+  int64_t ldy, ldn;
+};
+
+// norm(v) in `u`; returns one over its size.
+template <int LANES, int C, int E>
+__device__ __forceinline__ float normalise(const NormArgs& a, Team<LANES>& team, float (&room)[2][16], int first, float (&u)[C][E]) {
+  if (a.centre) {
+    float s = 0;
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int j = 0; j < E; j++) s += u[c][j];
+    const float mean = team.sum(s, room) * a.inv_cols;
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int j = 0; j < E; j++) u[c][j] = first + c * LANES * E + j < a.cols ? u[c][j] - mean : 0.f;
+  }
+  float s = 0;
+#pragma unroll
+  for (int c = 0; c < C; c++)
+#pragma unroll
+    for (int j = 0; j < E; j++) s = fmaf(u[c][j], u[c][j], s);
+  const float size = rsqrtf(fmaf(team.sum(s, room), a.inv_cols, a.eps));
+#pragma unroll
+  for (int c = 0; c < C; c++)
+#pragma unroll
+    for (int j = 0; j < E; j++) u[c][j] *= size;
+  return size;
+}
+
+__device__ __forceinline__ float gate_of(bool sigmoid, float g) { return sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-g)) : g; }
+
+template <typename T, int LANES, int C>
+__global__ __launch_bounds__(Team<LANES>::THREADS) void norm_kernel(NormArgs a) {
+  constexpr int E = 16 / sizeof(T), TEAMS = Team<LANES>::TEAMS;
+  __shared__ float room[2][16];
+  Team<LANES> team;
+  const int first = (threadIdx.x % LANES) * E, mine = threadIdx.x / LANES;
+  float wa[C][E], wb[C][E];
+#pragma unroll
+  for (int c = 0; c < C; c++) {
+    weights<E, T>(a.w_post, a.w_f32, first + c * LANES * E, a.cols, wa[c]);
+    weights<E, T>(a.w_pre, a.w_f32, first + c * LANES * E, a.cols, wb[c]);
+  }
+  for (int64_t base = (int64_t)blockIdx.x * TEAMS; base < a.rows; base += (int64_t)gridDim.x * TEAMS) {
+    const int64_t m = base + mine;
+    const bool there = m < a.rows;
+    vec<T, E> x[C], r[C], g[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      const int n = first + c * LANES * E;
+      x[c] = piece<E>((const T*)a.x + m * a.ldx, n, a.cols, there && a.x);
+      r[c] = piece<E>((const T*)a.r + m * a.ldr, n, a.cols, there && a.r);
+      g[c] = piece<E>((const T*)a.g + (a.g ? (uint32_t)m / a.per_gate : 0) * a.ldg, n, a.cols, there && a.g);
+    }
+    float u[C][E];
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int j = 0; j < E; j++) u[c][j] = (float)x[c][j];
+    if (a.post) normalise<LANES, C, E>(a, team, room, first, u);
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+#pragma unroll
+      for (int j = 0; j < E; j++) {
+        const float gate = a.g ? gate_of(a.sigmoid, (float)g[c][j]) : 1.f;
+        u[c][j] = fmaf(a.scale * gate, u[c][j] * (a.post ? wa[c][j] : 1.f), (float)r[c][j]);
+        if (!a.x) u[c][j] = (float)r[c][j];
+        if (first + c * LANES * E + j >= a.cols) u[c][j] = 0.f;
+      }
+      if (there && a.y) put_piece<E>((T*)a.y + m * a.ldy, first + c * LANES * E, a.cols, u[c]);
+    }
+    if (!a.n) continue;
+    normalise<LANES, C, E>(a, team, room, first, u);
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+#pragma unroll
+      for (int j = 0; j < E; j++) u[c][j] *= wb[c][j];
+      if (there) put_piece<E>((T*)a.n + m * a.ldn, first + c * LANES * E, a.cols, u[c]);
+    }
+  }
+}
+
+// How the backward pass walks the rows: `groups` of `per` rows, each in `segments` of `rows`, one unit after the other in steps of the
+// grid. A gate row that several rows share is a group; else all rows are one.
+struct Walk {
+  uint32_t groups, per, segments, rows, blocks;
+};
+struct NormGradArgs {
+  NormArgs f;
+  Walk walk;
+  const void *dy, *dn;
+  int64_t lddy, lddn;
+  void *dx, *dr, *dg;
+  int64_t lddx, lddr, lddg;
+  float* w_parts;     // [blocks][2][cols]: of w_post, of w_pre; null: neither is wanted
+  float* gate_parts;  // [units][cols]; null: a unit is a group, and writes its sum itself
+  bool shared;        // the gate's gradient is summed over a unit's rows
+};
+
+// The sums of a workgroup's teams, which wave 0 (or, with one team, every thread) has afterwards. In a fixed order.
+template <int LANES, int C, int E>
+__device__ __forceinline__ void gather(float (&v)[C][E], float* lds) {
+  if constexpr (LANES <= 64) {
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int j = 0; j < E; j++)
+#pragma unroll
+        for (int o = LANES; o < 64; o *= 2) v[c][j] += __shfl_xor(v[c][j], o);
+    constexpr int W = LANES * C * E;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();
+    if (wave > 0 && lane < LANES) {
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int j = 0; j < E; j++) lds[(wave - 1) * W + (c * E + j) * LANES + lane] = v[c][j];
+    }
+    __syncthreads();
+    if (wave == 0 && lane < LANES) {
+#pragma unroll
+      for (int w = 0; w < 3; w++)
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+          for (int j = 0; j < E; j++) v[c][j] += lds[w * W + (c * E + j) * LANES + lane];
+    }
+  }
+}
+
+template <typename T, int LANES, int C>
+__global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGradArgs b) {
+  constexpr int E = 16 / sizeof(T), TEAMS = Team<LANES>::TEAMS;
+  __shared__ float room[2][16];
+  __shared__ float lds[LANES <= 64 ? 3 * LANES * C * E : 1];
+  const NormArgs& a = b.f;
+  Team<LANES> team;
+  const int first = (threadIdx.x % LANES) * E, mine = threadIdx.x / LANES;
+  const bool writes = LANES > 64 || threadIdx.x < LANES;  // what gather() leaves
+  float wa[C][E], wb[C][E], sa[C][E] = {}, sb[C][E] = {};
+#pragma unroll
+  for (int c = 0; c < C; c++) {
+    weights<E, T>(a.w_post, a.w_f32, first + c * LANES * E, a.cols, wa[c]);
+    weights<E, T>(a.w_pre, a.w_f32, first + c * LANES * E, a.cols, wb[c]);
+  }
+  const uint32_t units = b.walk.groups * b.walk.segments;
+  for (uint32_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const uint32_t group = unit / b.walk.segments, segment = unit - group * b.walk.segments;
+    const int64_t start = (int64_t)group * b.walk.per, last = start + b.walk.per < a.rows ? start + b.walk.per : a.rows;
+    const int64_t begin = start + (int64_t)segment * b.walk.rows, end = begin + b.walk.rows < last ? begin + b.walk.rows : last;
+    float sg[C][E] = {};
+    for (int64_t base = begin; base < end; base += TEAMS) {
+      const int64_t m = base + mine;
+      const bool there = m < end;
+      vec<T, E> x[C], r[C], g[C], dy[C], dn[C];
+#pragma unroll
+      for (int c = 0; c < C; c++) {
+        const int n = first + c * LANES * E;
+        x[c] = piece<E>((const T*)a.x + m * a.ldx, n, a.cols, there && a.x);
+        r[c] = piece<E>((const T*)a.r + m * a.ldr, n, a.cols, there && a.r);
+        g[c] = piece<E>((const T*)a.g + (a.g ? (uint32_t)m / a.per_gate : 0) * a.ldg, n, a.cols, there && a.g);
+        dy[c] = piece<E>((const T*)b.dy + m * b.lddy, n, a.cols, there && b.dy);
+        dn[c] = piece<E>((const T*)b.dn + m * b.lddn, n, a.cols, there && b.dn);
+      }
+      float u[C][E], gate[C][E], d[C][E];
+      float size_x = 1.f;
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+          u[c][j] = (float)x[c][j];
+          gate[c][j] = a.g ? gate_of(a.sigmoid, (float)g[c][j]) : 1.f;
+          d[c][j] = (float)dy[c][j];
+        }
+      if (a.post) size_x = normalise<LANES, C, E>(a, team, room, first, u);
+      if (b.dn) {
+        float v[C][E];
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+          for (int j = 0; j < E; j++) {
+            v[c][j] = a.x ? fmaf(a.scale * gate[c][j], u[c][j] * (a.post ? wa[c][j] : 1.f), (float)r[c][j]) : (float)r[c][j];
+            if (first + c * LANES * E + j >= a.cols) v[c][j] = 0.f;
+          }
+        const float size = normalise<LANES, C, E>(a, team, room, first, v);
+        float along = 0, mean = 0;
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+          for (int j = 0; j < E; j++) {
+            const float n = (float)dn[c][j];
+            if (there) sb[c][j] = fmaf(n, v[c][j], sb[c][j]);
+            along = fmaf(n * wb[c][j], v[c][j], along);
+            mean = fmaf(n, wb[c][j], mean);
+          }
+        along = team.sum(along, room) * a.inv_cols;
+        mean = a.centre ? team.sum(mean, room) * a.inv_cols : 0.f;
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+          for (int j = 0; j < E; j++)
+            d[c][j] = fmaf(size, fmaf(-v[c][j], along, fmaf((float)dn[c][j], wb[c][j], -mean)), d[c][j]);
+      }
+      if (b.dr && there) {
+#pragma unroll
+        for (int c = 0; c < C; c++) put_piece<E>((T*)b.dr + m * b.lddr, first + c * LANES * E, a.cols, d[c]);
+      }
+      if (!a.x) continue;
+      float dg[C][E];
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+          const float t = u[c][j] * (a.post ? wa[c][j] : 1.f);
+          dg[c][j] = a.scale * d[c][j] * t * (a.sigmoid ? gate[c][j] * (1.f - gate[c][j]) : 1.f);
+          if (there) sg[c][j] += dg[c][j];
+          d[c][j] *= a.scale * gate[c][j];
+        }
+      if (b.dg && !b.shared && there) {
+#pragma unroll
+        for (int c = 0; c < C; c++) put_piece<E>((T*)b.dg + m * b.lddg, first + c * LANES * E, a.cols, dg[c]);
+      }
+      if (a.post) {
+        float along = 0, mean = 0;
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+          for (int j = 0; j < E; j++) {
+            if (there) sa[c][j] = fmaf(d[c][j], u[c][j], sa[c][j]);
+            d[c][j] *= wa[c][j];
+            along = fmaf(d[c][j], u[c][j], along);
+            mean += d[c][j];
+          }
+        along = team.sum(along, room) * a.inv_cols;
+        mean = a.centre ? team.sum(mean, room) * a.inv_cols : 0.f;
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+          for (int j = 0; j < E; j++) d[c][j] = size_x * (fmaf(-u[c][j], along, d[c][j]) - mean);
+      }
+      if (b.dx && there) {
+#pragma unroll
+        for (int c = 0; c < C; c++) put_piece<E>((T*)b.dx + m * b.lddx, first + c * LANES * E, a.cols, d[c]);
+      }
+    }
+    if (b.shared) {
+      gather<LANES, C, E>(sg, lds);
+      if (writes) {
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+          const int n = first + c * LANES * E;
+          if (b.gate_parts) put_piece<E>(b.gate_parts + (int64_t)unit * a.cols, n, a.cols, sg[c]);
+          else put_piece<E>((T*)b.dg + (int64_t)group * b.lddg, n, a.cols, sg[c]);
+        }
+      }
+    }
+  }
+  if (!b.w_parts) return;
+  gather<LANES, C, E>(sa, lds);
+  gather<LANES, C, E>(sb, lds);
+  if (writes) {
+    float* to = b.w_parts + (int64_t)blockIdx.x * 2 * a.cols;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      put_piece<E>(to, first + c * LANES * E, a.cols, sa[c]);
+      put_piece<E>(to + a.cols, first + c * LANES * E, a.cols, sb[c]);
+    }
+  }
+}
+
+// out[job][n] = the sum of `parts` rows of single-precision sums, which lie `step` apart, in a fixed order: 32 columns a workgroup, a
+// thirty-second of the parts a thread. Jobs 0 and 1 are the weights, the others the gate's rows.
+struct JoinArgs {
+  const float *w_parts, *gate_parts;
+  int cols;
+  uint32_t tiles, w_count, g_count, w_jobs;
+  void *dw[2], *dg;
+  int64_t lddg;
+  bool w_f32, accumulate;
+};
+template <typename T>
+__global__ __launch_bounds__(1024) void norm_join_kernel(JoinArgs a) {
+  __shared__ float sums[32][33];
+  const uint32_t block = block_index(), job = block / a.tiles;
+  const int col = threadIdx.x & 31, part = threadIdx.x >> 5, n = (int)(block - job * a.tiles) * 32 + col;
+  const bool weight = job < a.w_jobs;
+  if (weight && !a.dw[job]) return;
+  if (!weight && !a.dg) return;
+  const uint32_t count = weight ? a.w_count : a.g_count;
+  const int64_t step = weight ? 2 * (int64_t)a.cols : a.cols;
+  const float* from = weight ? a.w_parts + job * (int64_t)a.cols : a.gate_parts + (int64_t)(job - a.w_jobs) * a.g_count * a.cols;
+  float s = 0;
+  if (n < a.cols)
+    for (uint32_t p = part; p < count; p += 32) s += from[p * step + n];
+  sums[part][col] = s;
+  __syncthreads();
+  if (part || n >= a.cols) return;
+#pragma unroll
+  for (int p = 1; p < 32; p++) s += sums[p][col];
+  if (!weight) {
+    ((T*)a.dg)[(int64_t)(job - a.w_jobs) * a.lddg + n] = (T)s;
+  } else if (a.w_f32) {
+    float* to = (float*)a.dw[job] + n;
+    *to = a.accumulate ? *to + s : s;
+  } else {
+    ((T*)a.dw[job])[n] = (T)s;
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------
+
+size_t size_of(int dtype) { return dtype == B2C_F32 ? 4 : 2; }
+
+bool sizes_ok(const b2c_block_norm_args* a) {
+  return a && a->rows >= 0 && a->rows <= (1 << 30) && a->cols >= 1 && a->cols <= 16384 && a->dtype >= B2C_F32 && a->dtype <= B2C_BF16 &&
+         (a->w_dtype == a->dtype || a->w_dtype == B2C_F32) && (a->kind == B2C_NORM_RMS || a->kind == B2C_NORM_LAYER) &&
+         (a->gate_act == B2C_GATE_NONE || a->gate_act == B2C_GATE_SIGMOID) && a->eps >= 0 && a->eps < __builtin_inff() &&
+         (a->x || a->residual) && (a->x || (!a->post && !a->gate)) && (!a->gate || a->rows_per_gate >= 1) && (a->post || !a->w_post);
+}
+bool inputs_ok(const b2c_block_norm_args* a) {
+  const size_t s = size_of(a->dtype), w = size_of(a->w_dtype);
+  return (!a->x || good(a->x, a->ldx, a->cols, s)) && (!a->residual || good(a->residual, a->ldr, a->cols, s)) &&
+         (!a->gate || good(a->gate, a->ldg, a->cols, s)) && reinterpret_cast<uintptr_t>(a->w_post) % w == 0 &&
+         reinterpret_cast<uintptr_t>(a->w_pre) % w == 0;
+}
+
+NormArgs to_device(const b2c_block_norm_args* a) {
+  const int64_t per = a->gate ? std::min<int64_t>(a->rows_per_gate, 1 << 30) : 1;
+  return {a->rows, a->cols, a->kind == B2C_NORM_LAYER, a->post != 0, a->gate && a->gate_act == B2C_GATE_SIGMOID, a->w_dtype == B2C_F32,
+          a->eps, a->scale, 1.f / (float)a->cols, a->x, a->residual, a->gate, a->w_post, a->w_pre, a->ldx, a->ldr, a->ldg, (uint32_t)per,
+          a->y, a->n, a->ldy, a->ldn};
+}
+
+// Calls f(lanes, pieces) with the team that a row of `cols` values takes.
+template <typename T, typename F>
+int with_team(int cols, F f) {
+  using std::integral_constant;
+  const int pieces = (int)(up(cols, 16 / sizeof(T)) * (int64_t)sizeof(T) / 16);
+  if (pieces <= 8) return f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+  if (pieces <= 16) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  if (pieces <= 32) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+  if (pieces <= 64) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  if (pieces <= 256) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  if (pieces <= 512) return f(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+  if (pieces <= 1024) return f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+  if (pieces <= 2048) return f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+  if constexpr (sizeof(T) == 4) return f(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+  return hipErrorInvalidValue;
+}
+
+template <typename T>
+int forward(const b2c_block_norm_args* a, hipStream_t stream) {
+  const NormArgs d = to_device(a);
+  return with_team<T>(a->cols, [&](auto lanes, auto pieces) -> int {
+    using L = Team<decltype(lanes)::value>;
+    const int64_t blocks = std::min<int64_t>(up(a->rows, L::TEAMS) / L::TEAMS, 256 * (2048 / L::THREADS));
+    norm_kernel<T, decltype(lanes)::value, decltype(pieces)::value><<<dim3((unsigned)blocks), L::THREADS, 0, stream>>>(d);
+    return hipGetLastError();
+  });
+}
+
+bool shared_gate(const b2c_block_norm_grad_args* b) { return b->dgate && b->fwd.rows_per_gate > 1; }
+
+struct NormGradPlan {
+  Walk walk;
+  float *w_parts = nullptr, *gate_parts = nullptr;
+  bool w, g;
+  NormGradPlan(const b2c_block_norm_grad_args* b, Room& room) {
+    const b2c_block_norm_args* a = &b->fwd;
+    const int64_t most = [&] {
+      int threads = 256, teams = 1;
+      auto look = [&](auto lanes, auto) -> int {
+        using L = Team<decltype(lanes)::value>;
+        threads = L::THREADS, teams = L::TEAMS;
+        return 0;
+      };
+      a->dtype == B2C_F32 ? with_team<float>(a->cols, look) : with_team<f16>(a->cols, look);
+      walk.rows = (uint32_t)teams;
+      return 256 * (1024 / threads);
+    }();
+    const int64_t teams = walk.rows, rows = std::max<int64_t>(a->rows, 1);
+    const bool shared = shared_gate(b);
+    const int64_t per = shared ? std::min(a->rows_per_gate, rows) : rows, groups = up(rows, per) / per;
+    const int64_t steps = up(per, teams) / teams, segments = std::max<int64_t>(1, std::min(steps, up(most, groups) / groups));
+    const int64_t each = up(up(per, segments) / segments, teams);
+    walk = {(uint32_t)groups, (uint32_t)per, (uint32_t)(up(per, each) / each), (uint32_t)each, 0};
+    walk.blocks = (uint32_t)std::min<int64_t>(most, groups * walk.segments);
+    w = (b->dw_post && a->post && a->x) || (b->dw_pre && b->dn);
+    g = shared && walk.segments > 1;
+    if (w) w_parts = room.take<float>((int64_t)walk.blocks * 2 * a->cols);
+    if (g) gate_parts = room.take<float>(groups * walk.segments * a->cols);
+  }
+};
+
+template <typename T>
+int backward(const b2c_block_norm_grad_args* b, hipStream_t stream) {
+  const b2c_block_norm_args* a = &b->fwd;
+  Room room{(char*)b->workspace};
+  const NormGradPlan p(b, room);
+  NormGradArgs d{to_device(a), p.walk, b->dy, b->dn, b->lddy, b->lddn, b->dx, b->dresidual, b->dgate, b->lddx, b->lddr, b->lddg,
+                 p.w_parts, p.gate_parts, shared_gate(b)};
+  int rc = with_team<T>(a->cols, [&](auto lanes, auto pieces) -> int {
+    constexpr int L = decltype(lanes)::value;
+    norm_back_kernel<T, L, decltype(pieces)::value><<<dim3(p.walk.blocks), Team<L>::THREADS, 0, stream>>>(d);
+    return hipGetLastError();
+  });
+  if (rc || (!p.w && !p.g)) return rc;
+  const uint32_t tiles = (uint32_t)(up(a->cols, 32) / 32);
+  JoinArgs j{p.w_parts, p.gate_parts, a->cols, tiles, p.walk.blocks, p.walk.segments, p.w ? 2u : 0u, {b->dw_post, b->dw_pre},
+             p.g ? b->dgate : nullptr, b->lddg, b->grad_dtype == B2C_F32, b->accumulate != 0};
+  const int64_t blocks = (int64_t)tiles * (j.w_jobs + (p.g ? p.walk.groups : 0));
+  norm_join_kernel<T><<<grid_of(blocks), 1024, 0, stream>>>(j);
+  return hipGetLastError();
+}
+
+// The weights' gradients of no rows.
+__global__ __launch_bounds__(256) void clear_kernel(void* a, void* b, int n, bool f32) {
+  const int i = (int)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  for (void* p : {a, b}) {
+    if (p && f32) ((float*)p)[i] = 0.f;
+    else if (p) ((uint16_t*)p)[i] = 0;
+  }
+}
+
+}  // namespace
+}  // namespace dev
+}  // namespace b2c
+
+using namespace b2c::dev;
+
+extern "C" int b2c_hip_block_norm(const b2c_block_norm_args* a, hipStream_t stream) {
+  if (!sizes_ok(a)) return hipErrorInvalidValue;
+  const size_t s = size_of(a->dtype);
+  if (a->rows == 0) return hipSuccess;
+  if (!inputs_ok(a) || (!a->y && !a->n) || (!a->x && a->y) || (a->y && !good(a->y, a->ldy, a->cols, s)) ||
+      (a->n && !good(a->n, a->ldn, a->cols, s)))
+    return hipErrorInvalidValue;
+  if (a->dtype == B2C_F32) return forward<float>(a, stream);
+  if (a->dtype == B2C_F16) return forward<f16>(a, stream);
+  return forward<bf16>(a, stream);
+}
+
+extern "C" size_t b2c_block_norm_grad_workspace_bytes(const b2c_block_norm_grad_args* b) {
+  if (!b || !sizes_ok(&b->fwd) || b->fwd.rows == 0) return 0;
+  Room room{nullptr};
+  NormGradPlan(b, room);
+  return room.used;
+}
+
+extern "C" int b2c_hip_block_norm_backward(const b2c_block_norm_grad_args* b, hipStream_t stream) {
+  if (!b || !sizes_ok(&b->fwd)) return hipErrorInvalidValue;
+  const b2c_block_norm_args* a = &b->fwd;
+  const size_t s = size_of(a->dtype), gs = size_of(b->grad_dtype);
+  if ((b->grad_dtype != a->w_dtype && b->grad_dtype != B2C_F32) || (b->accumulate && b->grad_dtype != B2C_F32) ||
+      (b->dw_post && (!a->x || !a->post)) || (b->dw_pre && !b->dn) || (b->dx && !a->x) || (b->dgate && !a->gate) ||
+      reinterpret_cast<uintptr_t>(b->dw_post) % gs || reinterpret_cast<uintptr_t>(b->dw_pre) % gs)
+    return hipErrorInvalidValue;
+  if (a->rows == 0) {
+    if (b->accumulate || (!b->dw_post && !b->dw_pre)) return hipSuccess;
+    clear_kernel<<<dim3((unsigned)(up(a->cols, 256) / 256)), 256, 0, stream>>>(b->dw_post, b->dw_pre, a->cols, gs == 4);
+    return hipGetLastError();
+  }
+  if (!inputs_ok(a) || (!b->dy && !b->dn) || (b->dy && !good(b->dy, b->lddy, a->cols, s)) || (b->dn && !good(b->dn, b->lddn, a->cols, s)) ||
+      (b->dx && !good(b->dx, b->lddx, a->cols, s)) || (b->dresidual && !good(b->dresidual, b->lddr, a->cols, s)) ||
+      (b->dgate && !good(b->dgate, b->lddg, a->cols, s)))
+    return hipErrorInvalidValue;
+  const size_t need = b2c_block_norm_grad_workspace_bytes(b);
+  if (need && (!b->workspace || reinterpret_cast<uintptr_t>(b->workspace) % 16 || b->workspace_bytes < need)) return hipErrorInvalidValue;
+  if (!b->dx && !b->dresidual && !b->dgate && !b->dw_post && !b->dw_pre) return hipSuccess;
+  if (a->dtype == B2C_F32) return backward<float>(b, stream);
+  if (a->dtype == B2C_F16) return backward<f16>(b, stream);
+  return backward<bf16>(b, stream);
+}

@@ -1,5 +1,6 @@
-"""Dense operators of a learned head over splats or tokens: the gated feed-forward block with its gradients, dropout, and
-products in 8-bit integers (include/b2c_kernels.h, "dense operators").
+"""Dense operators of a learned head over splats or tokens: the gated feed-forward block with its gradients, dropout, the norms
+between two blocks with their gradients, products in 8-bit integers and with 4-bit weights, and a mixture of experts for a few
+tokens (include/b2c_kernels.h, "dense operators").
 
 An operator is planned once for its matrices and then run on a HIP stream as often as wanted: the plan holds the
 launcher's argument struct, and allocates nothing but through `room`, a function that the caller gives (bytes -> an
@@ -25,10 +26,13 @@ import ctypes as C
 from b2ctrain_amd import _native
 
 F32, F16, BF16 = 0, 1, 2
-I8 = 3  # of a Matrix only
-SIZES = {F32: 4, F16: 2, BF16: 2, I8: 1}
-NAMES = {"float32": F32, "float16": F16, "bfloat16": BF16, "int8": I8}
+I8, U8, I32 = 3, 4, 5  # of a Matrix only
+SIZES = {F32: 4, F16: 2, BF16: 2, I8: 1, U8: 1, I32: 4}
+NAMES = {"float32": F32, "float16": F16, "bfloat16": BF16, "int8": I8, "uint8": U8, "int32": I32}
 ACTS = {"silu": 0, "gelu": 1, "relu": 2}
+NORMS = {"rms": 0, "layer": 1}
+GATES = {"none": 0, "sigmoid": 1}
+GROUPS = (32, 64, 128, 256)
 
 _i64, _int, _f32, _u64, _ptr, _size = C.c_int64, C.c_int, C.c_float, C.c_uint64, C.c_void_p, C.c_size_t
 
@@ -69,6 +73,39 @@ class I8FfnArgs(C.Structure):
                 ("workspace", _ptr), ("workspace_bytes", _size)]
 
 
+class BlockNormArgs(C.Structure):
+    _fields_ = [("rows", _i64), ("cols", _int), ("dtype", _int), ("w_dtype", _int), ("kind", _int), ("post", _int), ("gate_act", _int),
+                ("eps", _f32), ("scale", _f32), ("x", _ptr), ("ldx", _i64), ("residual", _ptr), ("ldr", _i64), ("gate", _ptr),
+                ("ldg", _i64), ("rows_per_gate", _i64), ("w_post", _ptr), ("w_pre", _ptr), ("y", _ptr), ("ldy", _i64), ("n", _ptr),
+                ("ldn", _i64)]
+
+
+class BlockNormGradArgs(C.Structure):
+    _fields_ = [("fwd", BlockNormArgs), ("dy", _ptr), ("lddy", _i64), ("dn", _ptr), ("lddn", _i64), ("dx", _ptr), ("lddx", _i64),
+                ("dresidual", _ptr), ("lddr", _i64), ("dgate", _ptr), ("lddg", _i64), ("grad_dtype", _int), ("accumulate", _int),
+                ("dw_post", _ptr), ("dw_pre", _ptr), ("workspace", _ptr), ("workspace_bytes", _size)]
+
+
+class Quantize4Args(C.Structure):
+    _fields_ = [("rows", _i64), ("cols", _int), ("group", _int), ("dtype", _int), ("scale_dtype", _int), ("x", _ptr), ("ldx", _i64),
+                ("q", _ptr), ("ldq", _i64), ("scale", _ptr), ("lds", _i64), ("zero", _ptr), ("ldz", _i64), ("values", _ptr),
+                ("ldv", _i64)]
+
+
+class Q4LinearArgs(C.Structure):
+    _fields_ = [("rows", _i64), ("d_in", _int), ("d_out", _int), ("group", _int), ("dtype", _int), ("x", _ptr), ("ldx", _i64),
+                ("w", _ptr), ("ldw", _i64), ("scale", _ptr), ("lds", _i64), ("zero", _ptr), ("ldz", _i64), ("y", _ptr), ("ldy", _i64),
+                ("workspace", _ptr), ("workspace_bytes", _size)]
+
+
+class ExpertsArgs(C.Structure):
+    _fields_ = [("rows", _i64), ("d_in", _int), ("d_hidden", _int), ("d_out", _int), ("experts", _int), ("top_k", _int),
+                ("dtype", _int), ("act", _int), ("normalize", _int), ("x", _ptr), ("ldx", _i64), ("w_router", _ptr),
+                ("ld_router", _i64), ("w_gate", _ptr), ("w_up", _ptr), ("ld_in", _i64), ("w_down", _ptr), ("ld_out", _i64),
+                ("residual", _ptr), ("ldr", _i64), ("y", _ptr), ("ldy", _i64), ("index", _ptr), ("ldi", _i64), ("weight", _ptr),
+                ("ldw", _i64), ("workspace", _ptr), ("workspace_bytes", _size)]
+
+
 _bound = False
 
 
@@ -77,12 +114,16 @@ def _lib():
     L = _native.lib()
     if not _bound:
         for name, args in (("dropout", DropoutArgs), ("ffn_forward", FfnArgs), ("ffn_backward", FfnGradArgs),
-                           ("quantize_rows", QuantizeArgs), ("i8_linear", I8LinearArgs), ("i8_ffn", I8FfnArgs)):
+                           ("quantize_rows", QuantizeArgs), ("i8_linear", I8LinearArgs), ("i8_ffn", I8FfnArgs),
+                           ("block_norm", BlockNormArgs), ("block_norm_backward", BlockNormGradArgs), ("quantize4", Quantize4Args),
+                           ("q4_linear", Q4LinearArgs), ("experts", ExpertsArgs)):
             fn = getattr(L, "b2c_hip_" + name)
             fn.argtypes, fn.restype = [C.POINTER(args), _ptr], _int
         for name, args in (("b2c_ffn_saved_bytes", FfnArgs), ("b2c_ffn_workspace_bytes", FfnArgs),
                            ("b2c_ffn_grad_workspace_bytes", FfnGradArgs), ("b2c_i8_linear_workspace_bytes", I8LinearArgs),
-                           ("b2c_i8_ffn_workspace_bytes", I8FfnArgs)):
+                           ("b2c_i8_ffn_workspace_bytes", I8FfnArgs),
+                           ("b2c_block_norm_grad_workspace_bytes", BlockNormGradArgs),
+                           ("b2c_q4_linear_workspace_bytes", Q4LinearArgs), ("b2c_experts_workspace_bytes", ExpertsArgs)):
             fn = getattr(L, name)
             fn.argtypes, fn.restype = [C.POINTER(args)], _size
         _bound = True
@@ -344,3 +385,207 @@ class I8FeedForward:
 
     def run(self, stream=0):
         _check(self._fn(self._ref, stream), "i8_ffn")
+
+
+def _weights(what, name, n, types):
+    """The pointer and type of a norm's n weights, which lie next to each other."""
+    if isinstance(what, Matrix):
+        m, fits = what, what.rows * what.cols == n and (what.rows <= 1 or what.ld == what.cols)
+    else:
+        try:
+            fits = tuple(what.shape) == (n,) and (n <= 1 or what.stride(0) == 1)
+            if getattr(what, "is_cuda", True) is False:
+                raise ValueError(f"{name}: is not on the GPU")
+            m = Matrix(what.data_ptr(), n, 1, 1, NAMES.get(str(what.dtype).replace("torch.", "")), keep=what)
+        except AttributeError:
+            raise ValueError(f"{name}: {n} values are wanted, got {type(what).__name__}") from None
+    if m.dtype not in types or not fits:
+        raise ValueError(f"{name}: {n} values next to each other are wanted, of the matrices' type or in single precision")
+    if not m.ptr:
+        raise ValueError(f"{name}: a null pointer")
+    return m
+
+
+class BlockNorm:
+    """Between two blocks: y = residual + scale act(gate) t with t = norm(x) w_post (`post`; else x itself), and n = norm(y) w_pre;
+    b2c_hip_block_norm. What is not given is left out: without x, n is the norm of the residual, without a residual it counts as
+    zeros, without n only y is formed. kind: rms or layer; gate_act: none or sigmoid. `gate` has a row for every `rows_per_gate` rows
+    (by default: one row for all, or one for each). The weights are of the matrices' type or in single precision, both the same. y may be
+    residual and n may be x, where no backward pass follows: that forms y again from x and residual."""
+
+    def __init__(self, x=None, residual=None, y=None, n=None, gate=None, rows_per_gate=None, gate_act="none", post=False, w_post=None,
+                 w_pre=None, kind="rms", eps=1e-6, scale=1.0):
+        L = _lib()
+        if x is None and residual is None:
+            raise ValueError("block norm: needs x or residual")
+        first = _floating(matrix(x if x is not None else residual, "x" if x is not None else "residual"), "x")
+        m, d, t = first.rows, first.cols, first.dtype
+        same = lambda what, name: matrix(what, name, m, d, t) if what is not None else None  # noqa: E731
+        x, r, y, n = same(x, "x"), same(residual, "residual"), same(y, "y"), same(n, "n")
+        if d > 16384:
+            raise ValueError(f"block norm: {d} columns, at most 16384")
+        if kind not in NORMS or gate_act not in GATES:
+            raise ValueError(f"block norm: kind {kind!r} of {', '.join(NORMS)}, gate_act {gate_act!r} of {', '.join(GATES)}")
+        if not 0.0 <= float(eps) < float("inf"):
+            raise ValueError(f"block norm: eps {eps}")
+        if x is None and (post or gate is not None or y is not None):
+            raise ValueError("block norm: `post`, a gate and y need x")
+        if w_post is not None and not post:
+            raise ValueError("block norm: w_post without `post`")
+        if w_pre is not None and n is None:
+            raise ValueError("block norm: w_pre without n")
+        if y is None and n is None:
+            raise ValueError("block norm: neither y nor n is wanted")
+        g = matrix(gate, "gate", None, d, t) if gate is not None else None
+        if g is not None:
+            if rows_per_gate is None:
+                if g.rows not in (1, m):
+                    raise ValueError("gate: rows_per_gate is needed")
+                rows_per_gate = 1 if g.rows == m else max(m, 1)
+            if rows_per_gate < 1 or g.rows < -(-m // rows_per_gate):
+                raise ValueError(f"gate: has {g.rows} rows for {m} rows, {rows_per_gate} to each")
+        elif rows_per_gate is not None:
+            raise ValueError("block norm: rows_per_gate without a gate")
+        ws = [_weights(w, name, d, (t, F32)) if w is not None else None for w, name in ((w_post, "w_post"), (w_pre, "w_pre"))]
+        types = {w.dtype for w in ws if w}
+        if len(types) > 1:
+            raise ValueError("block norm: w_post and w_pre have different types")
+        self._keep, self._shape, self._types = (x, r, g, ws, y, n), (m, d), (t, types.pop() if types else t)
+        self._post, self._gate_rows = bool(post), -(-m // rows_per_gate) if g is not None else 0
+        a = self.args = BlockNormArgs(rows=m, cols=d, dtype=t, w_dtype=self._types[1], kind=NORMS[kind], post=int(self._post),
+                                      gate_act=GATES[gate_act], eps=eps, scale=scale, rows_per_gate=rows_per_gate or 0)
+        for field, ld, v in (("x", "ldx", x), ("residual", "ldr", r), ("gate", "ldg", g), ("y", "ldy", y), ("n", "ldn", n)):
+            setattr(a, field, v.ptr if v else None)
+            setattr(a, ld, v.ld if v else 0)
+        a.w_post, a.w_pre = (w.ptr if w else None for w in ws)
+        self._ref, self._fwd, self._bwd = C.byref(a), L.b2c_hip_block_norm, L.b2c_hip_block_norm_backward
+        self.grad = None
+
+    def gradients(self, dy=None, dn=None, dx=None, dresidual=None, dgate=None, dw_post=None, dw_pre=None, accumulate=False, room=None):
+        """Plans backward(): the gradients of y and n in (either may be missing), and whichever outputs are given. Those of the weights
+        are of the weights' type, or in single precision, where `accumulate` adds to what they hold. dresidual may be dy and dx may be dn."""
+        m, d = self._shape
+        t, wt = self._types
+        x, r, gate = self._keep[:3]
+        if dy is None and dn is None:
+            raise ValueError("block norm: needs dy or dn")
+        if dn is None and dw_pre is not None:
+            raise ValueError("block norm: dw_pre without dn")
+        if x is None and dx is not None or gate is None and dgate is not None or not self._post and dw_post is not None:
+            raise ValueError("block norm: a gradient of what was not given")
+        same = lambda what, name: matrix(what, name, m, d, t) if what is not None else None  # noqa: E731
+        dy, dn, dx, dr = same(dy, "dy"), same(dn, "dn"), same(dx, "dx"), same(dresidual, "dresidual")
+        dg = matrix(dgate, "dgate", self._gate_rows, d, t) if dgate is not None else None
+        ws = [_weights(w, name, d, (wt, F32)) if w is not None else None for w, name in ((dw_post, "dw_post"), (dw_pre, "dw_pre"))]
+        types = {w.dtype for w in ws if w}
+        if len(types) > 1:
+            raise ValueError("block norm: dw_post and dw_pre have different types")
+        kind = types.pop() if types else F32
+        if accumulate and kind != F32:
+            raise ValueError("block norm: gradients accumulate in single precision only")
+        g = self.grad = BlockNormGradArgs(fwd=self.args, grad_dtype=kind, accumulate=int(bool(accumulate)))
+        for field, ld, v in (("dy", "lddy", dy), ("dn", "lddn", dn), ("dx", "lddx", dx), ("dresidual", "lddr", dr), ("dgate", "lddg", dg)):
+            setattr(g, field, v.ptr if v else None)
+            setattr(g, ld, v.ld if v else 0)
+        g.dw_post, g.dw_pre = (w.ptr if w else None for w in ws)
+        self._gref = C.byref(g)
+        g.workspace_bytes = _lib().b2c_block_norm_grad_workspace_bytes(self._gref)
+        b, g.workspace = _get_room(room, g.workspace_bytes, "block norm gradients")
+        self._gkeep = [dy, dn, dx, dr, dg, ws, b]
+
+    def forward(self, stream=0):
+        _check(self._fwd(self._ref, stream), "block norm")
+
+    def backward(self, stream=0):
+        if self.grad is None:
+            raise ValueError("block norm: plan gradients() first")
+        _check(self._bwd(self._gref, stream), "block norm gradients")
+
+
+def _group(group):
+    if group not in GROUPS:
+        raise ValueError(f"group of {group} columns: wanted one of {', '.join(map(str, GROUPS))}")
+    return group
+
+
+class QuantizeGroups:
+    """q, scale (and with `zero` zero points) = x in 4 bits, a scale for every `group` columns of a row; b2c_hip_quantize4. q is uint8,
+    two columns a byte, the even one in the low half; `scale` is in 16 bits. `values`: what the codes stand for, of x's type. For weights
+    [outputs, inputs], rows are channels."""
+
+    def __init__(self, x, q, scale, group, zero=None, values=None):
+        x = _floating(matrix(x, "x"), "x")
+        n = -(-x.cols // _group(group))
+        q = matrix(q, "q", x.rows, -(-x.cols // 2), U8)
+        s = _floating(matrix(scale, "scale", x.rows, n), "scale", (F16, BF16))
+        z = matrix(zero, "zero", x.rows, n, U8) if zero is not None else None
+        v = matrix(values, "values", x.rows, x.cols, x.dtype) if values is not None else None
+        self._keep = (x, q, s, z, v)
+        self.args = Quantize4Args(rows=x.rows, cols=x.cols, group=group, dtype=x.dtype, scale_dtype=s.dtype, x=x.ptr, ldx=x.ld, q=q.ptr,
+                                  ldq=q.ld, scale=s.ptr, lds=s.ld, zero=z.ptr if z else None, ldz=z.ld if z else 0,
+                                  values=v.ptr if v else None, ldv=v.ld if v else 0)
+        self._fn, self._ref = _lib().b2c_hip_quantize4, C.byref(self.args)
+
+    def run(self, stream=0):
+        _check(self._fn(self._ref, stream), "quantize4")
+
+
+class Q4Linear:
+    """y = x w' with w held in 4 bits as QuantizeGroups gives it, its scales of x's type; b2c_hip_q4_linear."""
+
+    def __init__(self, x, w, scale, y, group, zero=None, room=None):
+        L = _lib()
+        x = _floating(matrix(x, "x"), "x", (F16, BF16))
+        n = -(-x.cols // _group(group))
+        w = matrix(w, "w", None, -(-x.cols // 2), U8)
+        s = matrix(scale, "scale", w.rows, n, x.dtype)
+        z = matrix(zero, "zero", w.rows, n, U8) if zero is not None else None
+        y = matrix(y, "y", x.rows, w.rows, x.dtype)
+        a = self.args = Q4LinearArgs(rows=x.rows, d_in=x.cols, d_out=w.rows, group=group, dtype=x.dtype, x=x.ptr, ldx=x.ld, w=w.ptr,
+                                     ldw=w.ld, scale=s.ptr, lds=s.ld, zero=z.ptr if z else None, ldz=z.ld if z else 0, y=y.ptr, ldy=y.ld)
+        self._fn, self._ref = L.b2c_hip_q4_linear, C.byref(a)
+        a.workspace_bytes = L.b2c_q4_linear_workspace_bytes(self._ref)
+        b, a.workspace = _get_room(room, a.workspace_bytes, "q4_linear")
+        self._keep = (x, w, s, z, y, b)
+
+    def run(self, stream=0):
+        _check(self._fn(self._ref, stream), "q4_linear")
+
+
+class Experts:
+    """A mixture of experts for a few tokens: y = residual + the sum over a row's `top_k` experts of p w_down (act(w_gate x) * (w_up x)), p the
+    router's softmax, with `normalize` over the chosen ones alone; b2c_hip_experts. w_router is [experts, inputs]; w_gate and w_up hold one
+    expert's [hidden, inputs] after the other's as rows, w_down their [outputs, hidden]. index (int32) and weight (single precision),
+    [rows, top_k], take the choice, the largest first. y may be residual."""
+
+    def __init__(self, x, w_router, w_gate, w_up, w_down, y, top_k, act="silu", normalize=True, residual=None, index=None, weight=None,
+                 room=None):
+        L = _lib()
+        x = _floating(matrix(x, "x"), "x", (F16, BF16))
+        t, m = x.dtype, x.rows
+        wr = matrix(w_router, "w_router", None, x.cols, t)
+        g, u = matrix(w_gate, "w_gate", None, x.cols, t), matrix(w_up, "w_up", None, x.cols, t)
+        e = wr.rows
+        if not 1 <= e <= 1024 or not 1 <= top_k <= min(e, 64):
+            raise ValueError(f"experts: {top_k} of {e}; wanted 1 to 64 of at most 1024")
+        if g.rows < 1 or g.rows % e or u.rows != g.rows:
+            raise ValueError(f"experts: w_gate and w_up have {g.rows} and {u.rows} rows for {e} experts")
+        if g.ld != u.ld:
+            raise ValueError("experts: w_gate and w_up have different distances between rows")
+        y = matrix(y, "y", m, None, t)
+        d = matrix(w_down, "w_down", e * y.cols, g.rows // e, t)
+        r = matrix(residual, "residual", m, y.cols, t) if residual is not None else None
+        i = matrix(index, "index", m, top_k, I32) if index is not None else None
+        w = matrix(weight, "weight", m, top_k, F32) if weight is not None else None
+        a = self.args = ExpertsArgs(rows=m, d_in=x.cols, d_hidden=g.rows // e, d_out=y.cols, experts=e, top_k=top_k, dtype=t, act=_act(act),
+                                    normalize=int(bool(normalize)), x=x.ptr, ldx=x.ld, w_router=wr.ptr, ld_router=wr.ld, w_gate=g.ptr,
+                                    w_up=u.ptr, ld_in=g.ld, w_down=d.ptr, ld_out=d.ld, residual=r.ptr if r else None,
+                                    ldr=r.ld if r else 0, y=y.ptr, ldy=y.ld, index=i.ptr if i else None, ldi=i.ld if i else 0,
+                                    weight=w.ptr if w else None, ldw=w.ld if w else 0)
+        self._fn, self._ref = L.b2c_hip_experts, C.byref(a)
+        a.workspace_bytes = L.b2c_experts_workspace_bytes(self._ref)
+        b, a.workspace = _get_room(room, a.workspace_bytes, "experts")
+        self._keep = (x, wr, g, u, d, y, r, i, w, b)
+
+    def run(self, stream=0):
+        _check(self._fn(self._ref, stream), "experts")

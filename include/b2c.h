@@ -284,6 +284,11 @@ int b2c_feed_forward_backward(b2c_dense* d, const b2c_ffn_grad_args* a, void* st
 int b2c_quantize_rows(const b2c_quantize_args* a, void* stream);
 int b2c_i8_linear(b2c_dense* d, const b2c_i8_linear_args* a, void* stream);
 int b2c_i8_feed_forward(b2c_dense* d, const b2c_i8_ffn_args* a, void* stream);
+int b2c_block_norm(const b2c_block_norm_args* a, void* stream);
+int b2c_block_norm_backward(b2c_dense* d, const b2c_block_norm_grad_args* a, void* stream);
+int b2c_quantize4(const b2c_quantize4_args* a, void* stream);
+int b2c_q4_linear(b2c_dense* d, const b2c_q4_linear_args* a, void* stream);
+int b2c_experts(b2c_dense* d, const b2c_experts_args* a, void* stream);
 
 #ifdef __cplusplus
 }

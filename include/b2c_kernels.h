@@ -698,6 +698,151 @@ typedef struct b2c_i8_ffn_args {
 size_t b2c_i8_ffn_workspace_bytes(const b2c_i8_ffn_args* a);
 int b2c_hip_i8_ffn(const b2c_i8_ffn_args* a, hipStream_t stream);
 
+/* Between two blocks of a residual network: the norm after a block's output x, its gate, the residual scale and sum, and the
+ * norm before the next block:
+ *   t = norm(x) * w_post (or x itself without `post`);  y = residual + scale * act(gate) * t;  n = norm(y) * w_pre
+ * norm(v) = v / sqrt(mean v^2 + eps), or (v - mean v) / sqrt(mean (v - mean v)^2 + eps), over a row's columns. n is formed from y
+ * before y is rounded. Without x, y is the residual (no gate, no `post`) and n its norm. Statistics are held in single precision, in
+ * which squares overflow beyond 1.8e19. y may be residual and n may be x (same pointer and ld). rows at most 2^30, cols at most
+ * 16384. */
+enum { B2C_NORM_RMS = 0, B2C_NORM_LAYER = 1 };
+enum { B2C_GATE_NONE = 0, B2C_GATE_SIGMOID = 1 }; /* act(gate): the gate itself; 1 / (1 + e^-gate) */
+typedef struct b2c_block_norm_args {
+  int64_t rows;
+  int cols;
+  int dtype;            /* of every matrix: B2C_F32, B2C_F16 or B2C_BF16 */
+  int w_dtype;          /* of w_post and w_pre: dtype or B2C_F32 */
+  int kind, post, gate_act;
+  float eps;            /* >= 0 */
+  float scale;
+  const void* x;        /* [rows][cols] or NULL */
+  int64_t ldx;
+  const void* residual; /* [rows][cols]; NULL (where x is not): zeros */
+  int64_t ldr;
+  const void* gate;     /* [ceil(rows / rows_per_gate)][cols]: row i takes gate row i / rows_per_gate; NULL: ones */
+  int64_t ldg, rows_per_gate;
+  const void* w_post;   /* [cols] or NULL: ones */
+  const void* w_pre;    /* [cols] or NULL: ones */
+  void* y;              /* [rows][cols] or NULL: not written */
+  int64_t ldy;
+  void* n;              /* [rows][cols] or NULL: not formed */
+  int64_t ldn;
+} b2c_block_norm_args;
+int b2c_hip_block_norm(const b2c_block_norm_args* a, hipStream_t stream);
+
+/* Its gradients. `fwd` holds the forward call's arguments (y and n are not used): x, residual and gate as they were then, since y
+ * is formed again from them. Outputs that are NULL are not formed. dresidual may be dy and dx may be dn (same pointer and ld). The
+ * gate's gradient is summed over the rows that share a gate row. */
+typedef struct b2c_block_norm_grad_args {
+  b2c_block_norm_args fwd;
+  const void* dy;       /* [rows][cols], dtype, or NULL: zeros */
+  int64_t lddy;
+  const void* dn;       /* [rows][cols], dtype, or NULL: n had no part in what followed */
+  int64_t lddn;
+  void* dx;             /* [rows][cols], dtype */
+  int64_t lddx;
+  void* dresidual;      /* [rows][cols], dtype */
+  int64_t lddr;
+  void* dgate;          /* as gate */
+  int64_t lddg;
+  int grad_dtype;       /* of dw_post and dw_pre: w_dtype or B2C_F32 */
+  int accumulate;       /* add to dw_post and dw_pre (B2C_F32 only) instead of overwriting them */
+  void* dw_post;        /* [cols] */
+  void* dw_pre;         /* [cols] */
+  void* workspace;      /* b2c_block_norm_grad_workspace_bytes; not needed after the call */
+  size_t workspace_bytes;
+} b2c_block_norm_grad_args;
+size_t b2c_block_norm_grad_workspace_bytes(const b2c_block_norm_grad_args* a);
+int b2c_hip_block_norm_backward(const b2c_block_norm_grad_args* a, hipStream_t stream);
+
+/* 4 bits with a scale, and with `zero` a zero point, for every group of `group` columns of a row (the last group may be shorter):
+ *   without: scale = max |x| / 7, code = 8 + x / scale;  value = (code - 8) scale
+ *   with:    lo = min(x, 0), hi = max(x, 0), scale = (hi - lo) / 15, zero = -lo / scale, code = zero + x / scale;
+ *            value = (code - zero) scale
+ * The scale is formed in single precision and rounded to scale_dtype; quotients of that scale are rounded to single precision, then to
+ * the nearest integer (to even), zero and code to 0 .. 15. A group whose scale is zero gets the code of 0 throughout (8, or 0 with zero points); one
+ * with an infinity or NaN the scale NaN and those codes; a scale beyond scale_dtype's range becomes infinity, with those codes. Column
+ * 2 j is in the low half of byte j of q, column 2 j + 1 in the high half, which is 0 behind the last column of an odd row.
+ * `values`: what the codes stand for, formed in single precision, in dtype. rows at most 2^30, cols at most 2^20. */
+typedef struct b2c_quantize4_args {
+  int64_t rows;
+  int cols;
+  int group;            /* 32, 64, 128 or 256 */
+  int dtype;            /* of x and values: B2C_F32, B2C_F16 or B2C_BF16 */
+  int scale_dtype;      /* B2C_F16 or B2C_BF16 */
+  const void* x;        /* [rows][cols] */
+  int64_t ldx;
+  uint8_t* q;           /* [rows][(cols + 1) / 2] */
+  int64_t ldq;
+  void* scale;          /* [rows][ceil(cols / group)] */
+  int64_t lds;
+  uint8_t* zero;        /* as scale, or NULL */
+  int64_t ldz;
+  void* values;         /* [rows][cols] or NULL */
+  int64_t ldv;
+} b2c_quantize4_args;
+int b2c_hip_quantize4(const b2c_quantize4_args* a, hipStream_t stream);
+
+/* y = x w^T with w held as above: w[j][k] = (code - zero) scale, zero = 8 where there are none. With up to 32 rows each group's sum is
+ * formed from the codes and then scaled, with more w is rounded to dtype first. An infinity in a row of x may make its whole row of y NaN.
+ * rows at most 2^30, widths at most 2^20. */
+typedef struct b2c_q4_linear_args {
+  int64_t rows;
+  int d_in, d_out;
+  int group;            /* 32, 64, 128 or 256 */
+  int dtype;            /* of x, scale and y: B2C_F16 or B2C_BF16 */
+  const void* x;        /* [rows][d_in] */
+  int64_t ldx;
+  const uint8_t* w;     /* [d_out][(d_in + 1) / 2] */
+  int64_t ldw;          /* in bytes */
+  const void* scale;    /* [d_out][ceil(d_in / group)] */
+  int64_t lds;
+  const uint8_t* zero;  /* as scale, values 0 .. 15, or NULL */
+  int64_t ldz;
+  void* y;              /* [rows][d_out] */
+  int64_t ldy;
+  void* workspace;      /* b2c_q4_linear_workspace_bytes; not needed after the call */
+  size_t workspace_bytes;
+} b2c_q4_linear_args;
+size_t b2c_q4_linear_workspace_bytes(const b2c_q4_linear_args* a);
+int b2c_hip_q4_linear(const b2c_q4_linear_args* a, hipStream_t stream);
+
+/* A mixture-of-experts layer for a few tokens: l = x w_router^T; each row takes the `top_k` experts with the largest l (of equal ones
+ * the lowest index; a NaN counts as larger than any number), with weights p = softmax(l) over all experts, divided by the sum of the chosen
+ * ones' with `normalize`, and
+ *   y = residual + sum_j p_j w_down[e_j] (act(w_gate[e_j] x) * (w_up[e_j] x))
+ * The router's sums are held in 64 bits, so that the choice between experts that nearly agree does not depend on an order of
+ * summation; the other products' in 32, the inner activations rounded to dtype. A row with a NaN or an infinite largest l gets NaN weights. Rows go 1024 /
+ * top_k at a time, and the weights are read for each such lot. rows at most 2^20, widths at most 2^20, experts at most 1024, and all of a weight's
+ * rows (experts times width) less than 2^31. y may be residual (same pointer and ld). */
+typedef struct b2c_experts_args {
+  int64_t rows;
+  int d_in, d_hidden, d_out, experts, top_k;
+  int dtype, act;       /* dtype of every matrix but `weight`: B2C_F16 or B2C_BF16 */
+  int normalize;
+  const void* x;        /* [rows][d_in] */
+  int64_t ldx;
+  const void* w_router; /* [experts][d_in] */
+  int64_t ld_router;
+  const void* w_gate;   /* [experts * d_hidden][d_in]: one expert's rows after the other's */
+  const void* w_up;
+  int64_t ld_in;        /* of w_gate and w_up */
+  const void* w_down;   /* [experts * d_out][d_hidden] */
+  int64_t ld_out;
+  const void* residual; /* [rows][d_out] or NULL */
+  int64_t ldr;
+  void* y;              /* [rows][d_out] */
+  int64_t ldy;
+  int32_t* index;       /* [rows][top_k], largest first, or NULL: not written */
+  int64_t ldi;
+  float* weight;        /* [rows][top_k] or NULL: not written */
+  int64_t ldw;
+  void* workspace;      /* b2c_experts_workspace_bytes; not needed after the call */
+  size_t workspace_bytes;
+} b2c_experts_args;
+size_t b2c_experts_workspace_bytes(const b2c_experts_args* a);
+int b2c_hip_experts(const b2c_experts_args* a, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
