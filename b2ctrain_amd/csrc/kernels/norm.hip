@@ -46,16 +46,18 @@ struct Team {
   }
 };
 
-// E neighbouring values of a row as they are held in memory; zeros beyond the last column.
+// E neighbouring values of a row as they are held in memory; zeros beyond the last column, at whose place the last is read: loads without
+// conditions go out together.
 template <int E, typename T>
 __device__ __forceinline__ vec<T, E> piece(const T* row, int n, int cols, bool there) {
   vec<T, E> v{};
   if (there && n + E <= cols) {
     __builtin_memcpy(&v, row + n, sizeof(v));
-  } else if (there) {
+  } else if (there && n < cols) {
 #pragma unroll
-    for (int j = 0; j < E; j++)
-      if (n + j < cols) v[j] = row[n + j];
+    for (int j = 0; j < E; j++) v[j] = row[n + j < cols ? n + j : cols - 1];
+#pragma unroll
+    for (int j = 0; j < E; j++) v[j] = n + j < cols ? v[j] : (T)0.f;
   }
   return v;
 }

@@ -122,6 +122,14 @@ __device__ __forceinline__ vec<T, 8> codes(uint32_t w) {
   return __builtin_bit_cast(vec<T, 8>, v);
 }
 
+// The same in the order 0, 4, 1, 5, 2, 6, 3, 7, which takes seven operations in place of ten.
+template <typename T>
+__device__ __forceinline__ vec<uint32_t, 4> codes_apart(uint32_t w) {
+  using D = Codes<T>;
+  constexpr int down = std::is_same_v<T, bf16> ? 0 : 4;  // where the lowest bit of a code counts 1
+  return {D::two(w << down), D::two(down ? w : w >> 4), D::two(w >> (8 - down)), D::two(w >> (12 - down))};
+}
+
 template <typename T>
 struct Weights4 {
   const uint8_t* q;
@@ -133,18 +141,26 @@ struct Weights4 {
   int rows, cols, groups;
 };
 
-// Sixteen bytes of a row from byte b on; zeros beyond the row's last.
-__device__ __forceinline__ vec<uint32_t, 4> bytes16(const uint8_t* row, int b, int bytes, bool there) {
+// Sixteen bytes of a row from byte b on; zeros beyond the row's last, at whose place the last is read: loads without conditions go out
+// together, where one that waits for its condition holds up the next.
+__device__ __forceinline__ vec<uint32_t, 4> bytes16(const uint8_t* row, int b, int bytes) {
   vec<uint32_t, 4> v{};
-  if (!there || b >= bytes) return v;
   if (b + 16 <= bytes) {
     __builtin_memcpy(&v, row + b, 16);
   } else {
 #pragma unroll
     for (int j = 0; j < 16; j++)
-      if (b + j < bytes) v[j / 4] |= (uint32_t)row[b + j] << (j % 4 * 8);
+      v[j / 4] |= (b + j < bytes ? (uint32_t)row[b + j < bytes ? b + j : bytes - 1] : 0u) << (j % 4 * 8);
   }
   return v;
+}
+// Sixteen bytes moved down by n, zeros behind them.
+__device__ __forceinline__ vec<uint32_t, 4> moved_down(vec<uint32_t, 4> v, int n) {
+  uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+  if (n >= 8) lo = hi, hi = 0, n -= 8;
+  if (n >= 8) lo = 0;
+  else if (n > 0) lo = lo >> (8 * n) | hi << (64 - 8 * n), hi >>= 8 * n;
+  return {(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
 }
 // The four words that lanes l, l + 16, l + 32, l + 48 hold, turned: word i of lane 16 j + l becomes word j of lane 16 i + l.
 __device__ __forceinline__ void turn4(vec<uint32_t, 4>& v) {
@@ -152,103 +168,285 @@ __device__ __forceinline__ void turn4(vec<uint32_t, 4>& v) {
   const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
   v = {(uint32_t)c[0], (uint32_t)c[1], (uint32_t)d[0], (uint32_t)d[1]};
 }
+// N values of a row from i on; zeros beyond its last.
 template <typename E, int N>
-__device__ __forceinline__ vec<E, N> some(const E* row, int i, int count, bool there) {
+__device__ __forceinline__ vec<E, N> some(const E* row, int i, int count) {
   vec<E, N> v{};
-  if (!there) return v;
   if (i + N <= count) {
     __builtin_memcpy(&v, row + i, sizeof(E) * N);
   } else {
 #pragma unroll
     for (int j = 0; j < N; j++)
-      if (i + j < count) v[j] = row[i + j];
+      v[j] = row[i + j < count ? i + j : count - 1];
+#pragma unroll
+    for (int j = 0; j < N; j++) v[j] = i + j < count ? v[j] : (E)0;
   }
   return v;
 }
 
-// At most 16 MT rows of x. A workgroup takes 16 outputs, its eight waves every eighth run of 128 values of k: sixteen bytes of a row
-// a lane, turned so that each matrix instruction meets 32 neighbouring values of k, which are of one group. With c the code and B its
-// base, a group's sum is s (sum (B + c) x - (B + z) sum x), and sum x comes from the same instruction against ones, in the same lanes.
-// B is at most 128, so that the difference costs four bits of the 24 that the sums are held in. The eight sums meet in LDS and are
-// added in a fixed order.
-template <typename T, int GROUP, bool ZERO, int MT>
-__global__ __launch_bounds__(512) void q4_few_kernel(Weights4<T> w, Side<T> x, int64_t M, T* y, int64_t ldy) {
+// At most 16 MT rows of x. A workgroup takes 16 NT outputs, its eight waves every eighth run of 128 values of k: sixteen bytes of a row a
+// lane, turned so that each matrix instruction meets 32 neighbouring values of k, which are of one group. With c the code and B its base, a
+// group's sum is s (sum (B + c) x - (B + z) sum x), and sum x comes from the same instruction against ones, in the same lanes. B is at most
+// 128, so that the difference costs four bits of the 24 that the sums are held in. Rows beyond the last read the last one's values, which
+// nobody stores; in the run at the end of k (not the first: LONG) every load that would pass a row's end reads its last bytes, which are then
+// moved to their place, so that no load waits for a condition (7 rows of 2050-5001: 3 us less). The waves' sums meet in LDS and are added in a fixed order.
+template <typename T, int GROUP, bool ZERO, int MT, int NT, bool LONG>
+__global__ __launch_bounds__(512, 4) void q4_few_kernel(Weights4<T> w, int shift, Side<T> x, int M, T* y, int64_t ldy) {
   constexpr int NG = GROUP >= 128 ? 1 : 128 / GROUP, PER = 4 / NG;  // groups of a run, matrix instructions of a group
-  constexpr int U = 4;
-  __shared__ f32x4 sums[8][MT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, q4 = lane >> 4;
-  const int64_t n = (int64_t)blockIdx.x * 16 + row;
-  const bool there = n < w.rows;
-  const int K = w.cols, bytes = (K + 1) / 2;
-  const uint8_t* q = w.q + (there ? n : 0) * w.ldq;
-  const T* scale = w.scale + (there ? n : 0) * w.lds;
-  const uint8_t* zero = ZERO ? w.zero + (there ? n : 0) * w.ldz : nullptr;
+  constexpr int U = MT == 1 ? (NT == 1 ? 4 : 2) : (NT == 4 ? 1 : 2);  // runs in flight
+  __shared__ f32x4 sums[8][NT][MT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, q4 = lane >> 4;
+  const int n0 = (int)blockIdx.x * 16 * NT, rows = w.rows - n0;
+  const int K = w.cols, bytes = (K + 1) >> 1, whole = K >> 7, runs = (K + 127) >> 7;
+  const uint8_t* q = w.q + n0 * w.ldq;
+  const T* scale = w.scale + n0 * w.lds;
+  const uint8_t* zero = ZERO ? w.zero + n0 * w.ldz : nullptr;
+  uint32_t q_at[NT], s_at[NT], z_at[NT];
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    const uint32_t r = n * 16 + row < rows ? n * 16 + row : rows - 1;
+    q_at[n] = r * (uint32_t)w.ldq;
+    s_at[n] = r * (uint32_t)w.lds;
+    z_at[n] = ZERO ? r * (uint32_t)w.ldz : 0;
+  }
+  const T* px[MT];
+#pragma unroll
+  for (int t = 0; t < MT; t++) px[t] = x.p + (t * 16 + row < M ? t * 16 + row : M - 1) * x.ld;
   const T one = (T)1.f;
   const vec<T, 8> ones = {one, one, one, one, one, one, one, one};
   struct Run {
-    vec<uint32_t, 4> q;
-    vec<T, NG> s;
-    vec<uint8_t, NG> z;
+    vec<uint32_t, 4> q[NT];
+    vec<T, NG> s[NT];
+    vec<uint8_t, NG> z[NT];
+    vec<T, 8> x[MT][4];
   };
-  auto fetch = [&](int k0) {
-    Run r;
-    r.q = bytes16(q, k0 / 2 + q4 * 16, bytes, there && k0 < K);
-    r.s = some<T, NG>(scale, k0 / GROUP, w.groups, there && k0 < K);
-    if constexpr (ZERO) r.z = some<uint8_t, NG>(zero, k0 / GROUP, w.groups, there && k0 < K);
-    return r;
-  };
-  f32x4 total[MT] = {};
-  Run next[U];
+  auto fetch = [&](Run& r, int run) {
+    const int k = run * 128;
 #pragma unroll
-  for (int u = 0; u < U; u++) next[u] = fetch((u * 8 + wave) * 128);
-  for (int k0 = wave * 128; k0 < K; k0 += U * 1024) {
-    Run now[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) now[u] = next[u];
-    if (k0 + U * 1024 < K) {
-#pragma unroll
-      for (int u = 0; u < U; u++) next[u] = fetch(k0 + (U + u) * 1024);
+    for (int n = 0; n < NT; n++) {
+      __builtin_memcpy(&r.q[n], q + (q_at[n] + (uint32_t)(run * 64 + q4 * 16)), 16);
+      __builtin_memcpy(&r.s[n], scale + (s_at[n] + (uint32_t)(k >> shift)), sizeof(T) * NG);
+      if constexpr (ZERO) __builtin_memcpy(&r.z[n], zero + (z_at[n] + (uint32_t)(k >> shift)), NG);
     }
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int k = k0 + u * 1024;
-      if (k >= K) break;
-      turn4(now[u].q);
+    for (int t = 0; t < MT; t++)
 #pragma unroll
-      for (int g = 0; g < NG; g++) {
-        f32x4 acc[MT] = {}, sum[MT] = {};
+      for (int i = 0; i < 4; i++) __builtin_memcpy(&r.x[t][i], px[t] + k + i * 32 + q4 * 8, 16);
+  };
+  auto fetch_end = [&](Run& r) {  // the run in which a long k ends
+    const int k = whole * 128, b = whole * 64 + q4 * 16, at = b < bytes - 16 ? b : bytes - 16;
+    const int g = k >> shift, first = g < w.groups - NG ? g : w.groups - NG;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-          const vec<T, 8> p = codes<T>(now[u].q[g * PER + i]);
+    for (int n = 0; n < NT; n++) {
+      __builtin_memcpy(&r.q[n], q + (q_at[n] + (uint32_t)at), 16);
+      __builtin_memcpy(&r.s[n], scale + (s_at[n] + (uint32_t)first), sizeof(T) * NG);
+      if constexpr (ZERO) __builtin_memcpy(&r.z[n], zero + (z_at[n] + (uint32_t)first), NG);
+    }
 #pragma unroll
-          for (int t = 0; t < MT; t++) {
-            const int64_t m = t * 16 + row;
-            const int at = k + (g * PER + i) * 32 + q4 * 8;
-            const vec<T, 8> v = some<T, 8>(x.p + m * x.ld, at, K, m < M);
-            acc[t] = mfma(v, p, acc[t]);
-            sum[t] = mfma(v, ones, sum[t]);
-          }
+    for (int i = 0; i < 4; i++) {
+      const int j = k + i * 32 + q4 * 8, from = j < K - 8 ? j : K - 8;
+#pragma unroll
+      for (int t = 0; t < MT; t++) __builtin_memcpy(&r.x[t][i], px[t] + from, 16);
+    }
+  };
+  auto settle = [&](Run& r) {  // and everything of it to its place, zeros behind the last
+    const int k = whole * 128, b = whole * 64 + q4 * 16, g = k >> shift, off = g - (g < w.groups - NG ? g : w.groups - NG);
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      r.q[n] = moved_down(r.q[n], b - (bytes - 16));
+      vec<T, NG> s = r.s[n];
+      vec<uint8_t, NG> z = r.z[n];
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+        r.s[n][j] = (T)0.f;
+#pragma unroll
+        for (int i = 0; i < NG; i++)
+          if (j + off == i) r.s[n][j] = s[i], r.z[n][j] = z[i];
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        r.x[t][i] = __builtin_bit_cast(vec<T, 8>, moved_down(__builtin_bit_cast(vec<uint32_t, 4>, r.x[t][i]), 2 * (k + i * 32 + q4 * 8 - (K - 8))));
+  };
+  auto fetch_only = [&](Run& r) {  // the only run of a short k
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      r.q[n] = bytes16(q + q_at[n], q4 * 16, bytes);
+      r.s[n] = some<T, NG>(scale + s_at[n], 0, w.groups);
+      if constexpr (ZERO) r.z[n] = some<uint8_t, NG>(zero + z_at[n], 0, w.groups);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) r.x[t][i] = some<T, 8>(px[t], i * 32 + q4 * 8, K);
+  };
+  f32x4 total[NT][MT] = {};
+  auto multiply = [&](Run& r) {
+#pragma unroll
+    for (int n = 0; n < NT; n++) turn4(r.q[n]);
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+      f32x4 sum[MT] = {};
+#pragma unroll
+      for (int i = g * PER; i < (g + 1) * PER; i++)
+#pragma unroll
+        for (int t = 0; t < MT; t++) sum[t] = mfma(r.x[t][i], ones, sum[t]);
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        f32x4 acc[MT] = {};
+#pragma unroll
+        for (int i = g * PER; i < (g + 1) * PER; i++) {
+          const vec<T, 8> p = codes<T>(r.q[n][i]);
+#pragma unroll
+          for (int t = 0; t < MT; t++) acc[t] = mfma(r.x[t][i], p, acc[t]);
         }
-        const float s = (float)now[u].s[g], b = Codes<T>::BASE + (ZERO ? (float)now[u].z[g] : 8.f);
+        const float s = (float)r.s[n][g], b = Codes<T>::BASE + (ZERO ? (float)r.z[n][g] : 8.f);
 #pragma unroll
         for (int t = 0; t < MT; t++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) total[t][j] = fmaf(s, fmaf(-b, sum[t][j], acc[t][j]), total[t][j]);
+          for (int j = 0; j < 4; j++) total[n][t][j] = fmaf(s, fmaf(-b, sum[t][j], acc[t][j]), total[n][t][j]);
       }
+    }
+  };
+  if constexpr (LONG) {
+    if (whole < runs && wave == 0) {
+      Run r;
+      fetch_end(r);
+      settle(r);
+      multiply(r);
+    }
+    for (int run = wave + 7 & 7; run < whole; run += U * 8) {  // the first wave last, which has had the end
+      Run r[U];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (run + u * 8 < whole) fetch(r[u], run + u * 8);
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (run + u * 8 < whole) multiply(r[u]);
+    }
+  } else if (wave == 0) {
+    Run r;
+    fetch_only(r);
+    multiply(r);
+  }
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int t = 0; t < MT; t++) sums[wave][n][t][lane] = total[n][t];
+  __syncthreads();
+  if (wave >= NT * MT) return;
+  const int tn = wave % NT, tm = wave / NT, n = n0 + tn * 16 + row;
+  f32x4 v = sums[0][tn][tm][lane];
+#pragma unroll
+  for (int i = 1; i < 8; i++) v += sums[i][tn][tm][lane];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int m = tm * 16 + q4 * 4 + j;
+    if (m < M && n < w.rows) y[m * ldy + n] = (T)v[j];
+  }
+}
+
+// One row of x. Where a matrix instruction would multiply mostly nothing, a lane multiplies by pairs: 32 values of k of each of its
+// wave's four outputs at a time, sixteen bytes that are all of one group, against the same 32 of x, which wait in LDS with their sums, in
+// the order in which the codes come apart most cheaply. So a wave reads a kilobyte of a row at once, a slab of 2048 values, and two slabs of
+// four rows are on their way together. Where there are few outputs, `split` waves share four of them and take every split-th slab.
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c, bf16) {
+  using V = vec<bf16, 2>;
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, false);
+}
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c, f16) {
+  using V = vec<f16, 2>;
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, false);
+}
+template <typename T, bool ZERO>
+__global__ __launch_bounds__(256, 4) void q4_one_kernel(Weights4<T> w, int shift, const T* x, T* y, int split) {
+  constexpr int SLABS = 4, STEPS = 2;  // slabs of x in LDS; of weights on their way
+  __shared__ __attribute__((aligned(16))) vec<uint32_t, 4> held[SLABS * 256];
+  __shared__ float sums[SLABS * 64];
+  __shared__ float parts[4][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int K = w.cols, bytes = (K + 1) >> 1, slabs = (K + 2047) >> 11;
+  const int part = wave % split, n0 = ((int)blockIdx.x * (4 / split) + wave / split) * 4;
+  float total[4] = {};
+  struct Slab {
+    vec<uint32_t, 4> q[4];
+    T s[4];
+    uint8_t z[4];
+  };
+  auto fetch = [&](Slab& r, int slab) {
+    const int b = slab * 1024 + lane * 16, at = b < bytes - 16 ? b : bytes - 16;
+    const int k = slab * 2048 + lane * 32, g = (k < K ? k : K - 1) >> shift;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int64_t n = n0 + i < w.rows ? n0 + i : w.rows - 1;
+      __builtin_memcpy(&r.q[i], w.q + n * w.ldq + at, 16);
+      r.s[i] = w.scale[n * w.lds + g];
+      if constexpr (ZERO) r.z[i] = w.zero[n * w.ldz + g];
+    }
+  };
+  auto multiply = [&](Slab& r, int slab, int i0) {
+    if ((slab + 1) * 2048 > K) {  // k ends in this slab
+#pragma unroll
+      for (int i = 0; i < 4; i++) r.q[i] = moved_down(r.q[i], slab * 1024 + lane * 16 - (bytes - 16));
+    }
+    vec<uint32_t, 4> p[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) p[j] = held[i0 * 4 + (j ^ (i0 >> 2 & 3))];
+    const float sum = sums[i0];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      float acc[2] = {};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const vec<uint32_t, 4> c = codes_apart<T>(r.q[i][j]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e & 1] = dot2(c[e], p[j][e], acc[e & 1], T{});
+      }
+      const float b = Codes<T>::BASE + (ZERO ? (float)r.z[i] : 8.f);
+      total[i] = fmaf((float)r.s[i], fmaf(-b, sum, acc[0] + acc[1]), total[i]);
+    }
+  };
+  for (int base = 0; base < slabs; base += SLABS) {  // as much of x as LDS holds; `split` and STEPS divide it
+    if (base) __syncthreads();
+    for (int i = threadIdx.x; i < SLABS * 64; i += 256) {
+      const int k = base * 2048 + i * 32;
+      float s = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        vec<T, 8> v{};
+        if (k + j * 8 < K) v = some<T, 8>(x, k + j * 8, K);
+#pragma unroll
+        for (int e = 0; e < 8; e++) s += (float)v[e];
+        const vec<T, 8> apart = {v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
+        held[i * 4 + (j ^ (i >> 2 & 3))] = __builtin_bit_cast(vec<uint32_t, 4>, apart);  // turned: eight lanes' pieces in different banks
+      }
+      sums[i] = s;
+    }
+    __syncthreads();
+    const int end = slabs < base + SLABS ? slabs : base + SLABS;
+    for (int slab = base + part; slab < end; slab += STEPS * split) {
+      Slab r[STEPS];
+#pragma unroll
+      for (int u = 0; u < STEPS; u++)
+        if (slab + u * split < end) fetch(r[u], slab + u * split);
+#pragma unroll
+      for (int u = 0; u < STEPS; u++)
+        if (slab + u * split < end) multiply(r[u], slab + u * split, (slab + u * split - base) * 64 + lane);
     }
   }
 #pragma unroll
-  for (int t = 0; t < MT; t++) sums[wave][t][lane] = total[t];
-  __syncthreads();
-  if (wave >= MT) return;
-  f32x4 v = sums[0][wave][lane];
+  for (int i = 0; i < 4; i++) {
 #pragma unroll
-  for (int i = 1; i < 8; i++) v += sums[i][wave][lane];
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int64_t m = wave * 16 + q4 * 4 + j;
-    if (m < M && there) y[m * ldy + n] = (T)v[j];
+    for (int o = 32; o; o >>= 1) total[i] += __shfl_xor(total[i], o);
+    if (lane == i) parts[wave][i] = total[i];
   }
+  __syncthreads();
+  if (part || lane >= 4 || n0 + lane >= w.rows) return;
+  float v = parts[wave][lane];
+  for (int p = 1; p < split; p++) v += parts[wave + p][lane];
+  y[n0 + lane] = (T)v;
 }
 
 // The weights in T, for the tiles, and x where its rows have to be copied to ones that start on 16 bytes. (code - zero) scale is formed in
@@ -263,7 +461,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(Weights4<T> w, int shift, T
   const int n = (int)(t - m * groups) * 8;
   if (copies) {
     if (m >= M) return;
-    *reinterpret_cast<vec<T, 8>*>(x_to + m * pitch + n) = some<T, 8>(x.p + m * x.ld, n, w.cols, true);
+    *reinterpret_cast<vec<T, 8>*>(x_to + m * pitch + n) = some<T, 8>(x.p + m * x.ld, n, w.cols);
     return;
   }
   if (m >= w.rows) return;
@@ -342,30 +540,65 @@ struct Q4Plan {
   }
 };
 
+// One row takes a kernel of its own where its slabs are at least nine tenths full: 4096 -> 11264 9.6 us and 8192 -> 1024 5.1, by the kernel
+// for a few 12.1 and 8.4; 2600 -> 11264 9.2 and 7.8, and below one slab 1024 -> 1024 4.7 and 3.2. Its waves share outputs until there
+// are 2048 of them: 8192 -> 1024 takes 6.7, 5.5 and 5.0 us with one, two and four waves, 4096 -> 11264 9.7, 10.9 and 14.8.
+bool one_row(const b2c_q4_linear_args* a) {
+  const int64_t slabs = up(a->d_in, 2048) / 2048;
+  return a->rows == 1 && a->d_in >= 2048 && a->d_in * 10 >= slabs * 2048 * 9;
+}
+int split_of(const b2c_q4_linear_args* a) {
+  const int64_t slabs = up(a->d_in, 2048) / 2048;
+  int split = 1;
+  while (split < 4 && split * 2 <= slabs && (int64_t)split * a->d_out < 8192) split *= 2;
+  return split;
+}
+
 template <typename T>
 int linear(const b2c_q4_linear_args* a, hipStream_t stream) {
   const Weights4<T> w{a->w, a->ldw, (const T*)a->scale, a->lds, a->zero, a->ldz, a->d_out, a->d_in, groups_of(a->d_in, a->group)};
   Side<T> x{(const T*)a->x, a->ldx};
+  const int shift = a->group == 32 ? 5 : a->group == 64 ? 6 : a->group == 128 ? 7 : 8;
   if (a->rows <= kFewRows) {
-    const dim3 grid((unsigned)(up(a->d_out, 16) / 16));
-    return with_group(a->group, [&](auto group) -> int {
-      constexpr int G = decltype(group)::value;
-      auto run = [&](auto zero, auto tiles) {
-        q4_few_kernel<T, G, decltype(zero)::value, decltype(tiles)::value><<<grid, 512, 0, stream>>>(w, x, a->rows, (T*)a->y, a->ldy);
-      };
-      using One = std::integral_constant<int, 1>;
-      using Two = std::integral_constant<int, 2>;
-      if (a->zero) a->rows <= 16 ? run(std::true_type{}, One{}) : run(std::true_type{}, Two{});
-      else a->rows <= 16 ? run(std::false_type{}, One{}) : run(std::false_type{}, Two{});
+    using std::integral_constant;
+    if (one_row(a)) {
+      const int split = split_of(a);
+      const dim3 grid((unsigned)(up(a->d_out, 16 / split) / (16 / split)));
+      if (a->zero) q4_one_kernel<T, true><<<grid, 256, 0, stream>>>(w, shift, x.p, (T*)a->y, split);
+      else q4_one_kernel<T, false><<<grid, 256, 0, stream>>>(w, shift, x.p, (T*)a->y, split);
       return hipGetLastError();
-    });
+    }
+    auto run = [&](auto group, auto zero, auto rows, auto outputs, auto far) -> int {
+      constexpr int NT = decltype(outputs)::value;
+      q4_few_kernel<T, decltype(group)::value, decltype(zero)::value, decltype(rows)::value, NT, decltype(far)::value>
+          <<<dim3((unsigned)(up(a->d_out, 16 * NT) / (16 * NT))), 512, 0, stream>>>(w, shift, x, (int)a->rows, (T*)a->y, a->ldy);
+      return hipGetLastError();
+    };
+    auto with_rows = [&](auto group, auto zero) {
+      auto with_outputs = [&](auto rows) {
+        if (a->d_in < 128) return run(group, zero, rows, integral_constant<int, 1>{}, std::false_type{});
+        // One round of workgroups, one to a compute unit, with as few outputs each as that takes; but for three times sixteen of
+        // two row tiles, which spills. 16 rows of 4096 -> 4096, 8192 and 11264: 8.7, 11.4 and 13.9 us this way, 11.0, 14.0 and
+        // 16.2 with the next fewer or more outputs.
+        const int64_t tiles = up(a->d_out, 16) / 16;
+        if (tiles <= 256) return run(group, zero, rows, integral_constant<int, 1>{}, std::true_type{});
+        if (tiles <= 512) return run(group, zero, rows, integral_constant<int, 2>{}, std::true_type{});
+        if constexpr (decltype(rows)::value == 1)
+          if (tiles <= 768) return run(group, zero, rows, integral_constant<int, 3>{}, std::true_type{});
+        return run(group, zero, rows, integral_constant<int, 4>{}, std::true_type{});
+      };
+      return a->rows <= 16 ? with_outputs(integral_constant<int, 1>{}) : with_outputs(integral_constant<int, 2>{});
+    };
+    auto with_zero = [&](auto group) { return a->zero ? with_rows(group, std::true_type{}) : with_rows(group, std::false_type{}); };
+    if (a->group == 32) return with_zero(integral_constant<int, 32>{});
+    if (a->group == 64) return with_zero(integral_constant<int, 64>{});
+    return with_zero(integral_constant<int, 128>{});
   }
   Room room{(char*)a->workspace};
   const Q4Plan<T> p(a, room);
   const uint32_t pieces = (uint32_t)(up(a->d_in, 8) / 8);
   const int64_t own = up((int64_t)a->d_out * pieces, 256) / 256, copies = p.x ? up(a->rows * pieces, 256) / 256 : 0;
   if (own + copies > 0x7fffffff) return hipErrorInvalidValue;
-  const int shift = a->group == 32 ? 5 : a->group == 64 ? 6 : a->group == 128 ? 7 : 8;
   if (a->zero) unpack_kernel<T, true><<<grid_of(own + copies), 256, 0, stream>>>(w, shift, p.w, p.pitch, pieces, (uint32_t)own, x, a->rows, p.x);
   else unpack_kernel<T, false><<<grid_of(own + copies), 256, 0, stream>>>(w, shift, p.w, p.pitch, pieces, (uint32_t)own, x, a->rows, p.x);
   int rc = hipGetLastError();
