@@ -1,6 +1,6 @@
 // A mixture-of-experts layer for a few tokens (b2c_hip_experts): the router, the chosen experts' gate and up projections, their down
-// projections with the weighted sum, a launch each.
-#include "dense.h"
+// projections, and the weighted sum.
+#include "dense_rows.h"
 
 namespace b2c {
 namespace dev {
@@ -8,20 +8,6 @@ namespace {
 
 constexpr int kMostExperts = 1024, kMostChosen = 64;
 constexpr int kLot = 1024;  // pairs of a token and an expert that one set of launches carries out
-
-template <int N, typename T>
-__device__ __forceinline__ vec<T, N> run_of(const T* row, int k, int K, bool there) {
-  vec<T, N> v{};
-  if (!there || k >= K) return v;
-  if (k + N <= K) {
-    __builtin_memcpy(&v, row + k, sizeof(v));
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; j++)
-      if (k + j < K) v[j] = row[k + j];
-  }
-  return v;
-}
 
 // ---- the router --------------------------------------------------------------------------------------------
 
@@ -33,72 +19,234 @@ struct RouteArgs {
   int64_t ldi, ldw;
 };
 
-// A workgroup a token. Products of 16-bit floats are exact in 64 bits and their sums nearly so: two experts are told apart where the numbers
-// do it. An expert's place is how many are before it, so that the order takes no rounds of maxima.
-template <typename T>
+// x . w in 64 bits, by a wave, for AT rows of w that lie `step` apart; those from `left` on are not there. Products of 16-bit floats are exact in
+// 64 bits and their sums nearly so: two experts are told apart where the numbers do it.
+template <typename T, int AT>
+__device__ __forceinline__ void wide_dots(const T* x, const T* w, int64_t step, int left, int D, double (&s)[AT]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < AT; i++) s[i] = 0;
+  auto add = [&](auto read, int k) {
+    const vec<T, 8> v = read(x, k);
+    vec<T, 8> u[AT];
+#pragma unroll
+    for (int i = 0; i < AT; i++) u[i] = read(w + (i < left ? i : 0) * step, k);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const double d = (double)(float)v[j];
+#pragma unroll
+      for (int i = 0; i < AT; i++) s[i] = fma(d, (double)(float)u[i][j], s[i]);
+    }
+  };
+  const int whole = D / 512 * 512;
+#pragma unroll 4
+  for (int k = 0; k < whole; k += 512)
+    add([](const T* p, int k) {
+      vec<T, 8> v;
+      __builtin_memcpy(&v, p + k, 16);
+      return v;
+    }, k + lane * 8);
+  if (D < 8) {
+    if (lane == 0) add([D](const T* p, int k) { return some<T, 8>(p, k, D); }, 0);
+  } else if (whole < D) {
+    add([D](const T* p, int k) { return end8<T>(p, k, D); }, whole + lane * 8);
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < AT; i++) s[i] += __shfl_xor(s[i], o);
+}
+
+// Chooses among the logits of one token, which a workgroup of THREADS has in LDS: an expert's place is how many are before it, so that the
+// order takes no rounds of maxima.
+template <int MOST, int THREADS>
+struct Choice {
+  double logits[MOST];
+  uint64_t keys[MOST + 8];
+  int chosen[kMostChosen];
+  float parts[THREADS / 64], share[kMostChosen];
+  __device__ __forceinline__ void set(int e, double l) {
+    l += 0.0;  // no negative zero
+    const uint64_t b = l != l ? 0x7fffffffffffffffull : __builtin_bit_cast(uint64_t, l);
+    logits[e] = l;
+    keys[e] = b >> 63 ? ~b : b | 1ull << 63;  // in the order of the numbers, a NaN above them
+  }
+  // After a barrier; leaves `chosen` and `share`, behind one.
+  __device__ __forceinline__ void choose(const RouteArgs& a) {
+    const int t = threadIdx.x;
+    if (t < 8) keys[a.E + t] = 0;  // below every number
+    __syncthreads();
+    for (int e = t; e < a.E; e += THREADS) {
+      const uint64_t mine = keys[e];
+      int before = 0;
+      for (int i = 0; i < a.E; i += 8)
+#pragma unroll
+        for (int j = 0; j < 8; j++) before += keys[i + j] > mine || (keys[i + j] == mine && i + j < e);
+      if (before < a.K) chosen[before] = e;
+    }
+    __syncthreads();
+    const double top = logits[chosen[0]];
+    float all = 0;
+    if (a.normalize) {
+      for (int j = 0; j < a.K; j++) all += expf((float)(logits[chosen[j]] - top));
+    } else {
+      float s = 0;
+      for (int e = t; e < a.E; e += THREADS) s += expf((float)(logits[e] - top));
+#pragma unroll
+      for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+      if ((t & 63) == 0) parts[t >> 6] = s;
+      __syncthreads();
+      for (int i = 0; i < THREADS / 64; i++) all += parts[i];
+    }
+    if (t < a.K) share[t] = expf((float)(logits[chosen[t]] - top)) / all;
+    __syncthreads();
+  }
+  __device__ __forceinline__ void write(const RouteArgs& a, int64_t m) const {
+    const int t = threadIdx.x;
+    if (t >= a.K) return;
+    a.to[m * a.K + t] = chosen[t];
+    a.share[m * a.K + t] = share[t];
+    if (a.index) a.index[m * a.ldi + t] = chosen[t];
+    if (a.weight) a.weight[m * a.ldw + t] = share[t];
+  }
+};
+
+// A workgroup a token, AT experts of a wave at a time.
+template <typename T, int AT>
 __global__ __launch_bounds__(1024) void route_kernel(Side<T> x, Side<T> w, RouteArgs a) {
-  __shared__ double logits[kMostExperts];
-  __shared__ uint64_t keys[kMostExperts];
-  __shared__ int chosen[kMostChosen];
-  __shared__ float parts[16];
+  __shared__ Choice<kMostExperts, 1024> choice;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t m = blockIdx.x;
-  const T* row = x.p + m * x.ld;
-  constexpr int AT = 4;  // experts of a wave at a time
-  for (int e0 = wave; e0 < a.E; e0 += 16 * AT) {
-    double s[AT] = {};
-    for (int k = lane * 8; k < a.D; k += 512) {
-      const vec<T, 8> v = run_of<8>(row, k, a.D, true);
-      vec<T, 8> u[AT];
+  for (int e0 = wave * AT; e0 < a.E; e0 += 16 * AT) {
+    double s[AT];
+    wide_dots<T, AT>(x.p + m * x.ld, w.p + e0 * w.ld, w.ld, a.E - e0, a.D, s);
 #pragma unroll
-      for (int i = 0; i < AT; i++) u[i] = run_of<8>(w.p + (int64_t)(e0 + 16 * i) * w.ld, k, a.D, e0 + 16 * i < a.E);
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const double d = (double)(float)v[j];
-#pragma unroll
-        for (int i = 0; i < AT; i++) s[i] = fma(d, (double)(float)u[i][j], s[i]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < AT; i++) {
-#pragma unroll
-      for (int o = 32; o; o >>= 1) s[i] += __shfl_xor(s[i], o);
-      const int e = e0 + 16 * i;
-      if (lane == 0 && e < a.E) {
-        const double l = s[i] + 0.0;  // no negative zero
-        const uint64_t b = l != l ? 0x7fffffffffffffffull : __builtin_bit_cast(uint64_t, l);
-        logits[e] = l;
-        keys[e] = b >> 63 ? ~b : b | 1ull << 63;  // in the order of the numbers, a NaN above them
-      }
-    }
+    for (int i = 0; i < AT; i++)
+      if (lane == i && e0 + i < a.E) choice.set(e0 + i, s[i]);
   }
-  __syncthreads();
-  const int e = threadIdx.x;
-  if (e < a.E) {
-    const uint64_t mine = keys[e];
-    int before = 0;
-    for (int i = 0; i < a.E; i++) before += keys[i] > mine || (keys[i] == mine && i < e);
-    if (before < a.K) chosen[before] = e;
+  choice.choose(a);
+  choice.write(a, m);
+}
+
+// ---- one token ---------------------------------------------------------------------------------------------
+
+// The logits of one token by more than one workgroup; every workgroup of the kernel that follows chooses for itself.
+template <typename T>
+__global__ __launch_bounds__(256) void logits_kernel(const T* x, Side<T> w, int E, int D, double* logits) {
+  const int e = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (e >= E) return;
+  double s[1];
+  wide_dots<T, 1>(x, w.p + e * w.ld, 0, 1, D, s);
+  if ((threadIdx.x & 63) == 0) logits[e] = s[0];
+}
+
+constexpr int kChooseOften = 256;  // experts among which every workgroup of a launch may choose again
+
+// A row's slab of 512 values is a kilobyte, sixteen bytes a lane. Values begin .. end - 1 of four rows (a wave's) against those of x, SLABS slabs
+// at a time; each row's sum stays spread over the lanes. `end` is the rows' end K or a multiple of 512.
+template <typename T, int SLABS>
+__device__ __forceinline__ void four_rows(const T* const (&rows)[4], const T* x, int K, int begin, int end, float (&sum)[4]) {
+  const int lane = threadIdx.x & 63;
+  using V = vec<uint32_t, 4>;
+  auto add = [&](const V& w, const V& v, float& to) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) to = dot2(w[j], v[j], to, T{});
+  };
+  int k0 = begin;
+  for (; k0 + 512 <= end; k0 += SLABS * 512) {
+    V w[SLABS][4], v[SLABS];
+#pragma unroll
+    for (int s = 0; s < SLABS; s++)
+      if (k0 + s * 512 + 512 <= end) {
+        __builtin_memcpy(&v[s], x + k0 + s * 512 + lane * 8, 16);
+#pragma unroll
+        for (int i = 0; i < 4; i++) __builtin_memcpy(&w[s][i], rows[i] + k0 + s * 512 + lane * 8, 16);
+      }
+#pragma unroll
+    for (int s = 0; s < SLABS; s++)
+      if (k0 + s * 512 + 512 <= end)
+#pragma unroll
+        for (int i = 0; i < 4; i++) add(w[s][i], v[s], sum[i]);
   }
-  __syncthreads();
-  const double top = logits[chosen[0]];
-  float all = 0;
-  if (a.normalize) {
-    for (int j = 0; j < a.K; j++) all += expf((float)(logits[chosen[j]] - top));
+  const int k = begin + (end - begin) / 512 * 512;  // what a slab holds of the end
+  if (k >= end) return;
+  if (K < 8) {
+    if (lane == 0)
+#pragma unroll
+      for (int i = 0; i < 4; i++) add(__builtin_bit_cast(V, some<T, 8>(rows[i], 0, K)), __builtin_bit_cast(V, some<T, 8>(x, 0, K)), sum[i]);
+    return;
+  }
+  const V v = __builtin_bit_cast(V, end8<T>(x, k + lane * 8, K));
+#pragma unroll
+  for (int i = 0; i < 4; i++) add(__builtin_bit_cast(V, end8<T>(rows[i], k + lane * 8, K)), v, sum[i]);
+}
+__device__ __forceinline__ float over_wave(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// h[choice] = act(w_gate x) (w_up x): two hidden units a wave, eight a workgroup, so that a few experts' rows fill the device, and a wave's 16
+// kilobytes are on their way together.
+template <typename T, int ACT, bool CHOOSE>
+__global__ __launch_bounds__(256) void gate_up_one_kernel(const T* x, Side<T> wg, Side<T> wu, int F, const double* logits, T* h, int64_t hp, RouteArgs a) {
+  __shared__ Choice<CHOOSE ? kChooseOften : 1, 256> choice;
+  const int wave = threadIdx.x >> 6, slot = (int)blockIdx.y, n = (int)blockIdx.x * 8 + wave * 2;
+  int e;
+  if constexpr (CHOOSE) {
+    for (int i = threadIdx.x; i < a.E; i += 256) choice.set(i, logits[i]);
+    choice.choose(a);
+    e = choice.chosen[slot];
+    if (blockIdx.x == 0 && slot == 0) choice.write(a, 0);
   } else {
-    float s = e < a.E ? expf((float)(logits[e] - top)) : 0.f;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-    if (lane == 0) parts[wave] = s;
-    __syncthreads();
-    for (int i = 0; i < 16; i++) all += parts[i];
+    e = a.to[slot];
   }
-  if (e >= a.K) return;
-  const float p = expf((float)(logits[chosen[e]] - top)) / all;
-  a.to[m * a.K + e] = chosen[e];
-  a.share[m * a.K + e] = p;
-  if (a.index) a.index[m * a.ldi + e] = chosen[e];
-  if (a.weight) a.weight[m * a.ldw + e] = p;
+  if (n >= F) return;
+  const int64_t row = (int64_t)e * F + n;
+  const int next = n + 1 < F ? 1 : 0;
+  const T* const rows[4] = {wg.p + row * wg.ld, wg.p + (row + next) * wg.ld, wu.p + row * wu.ld, wu.p + (row + next) * wu.ld};
+  float sum[4] = {};
+  four_rows<T, 4>(rows, x, a.D, 0, a.D, sum);
+#pragma unroll
+  for (int i = 0; i < 4; i++) sum[i] = over_wave(sum[i]);
+  const int lane = threadIdx.x & 63;
+  if (lane <= next) h[slot * hp + n + lane] = (T)(act<ACT>(lane ? sum[1] : sum[0]) * (lane ? sum[3] : sum[2]));
+}
+
+// y = residual + the weighted sum over the choices of w_down h: four outputs a workgroup, its eight waves a choice each, or a part of one's k
+// where there are fewer.
+template <typename T>
+__global__ __launch_bounds__(512) void down_one_kernel(const T* h, int64_t hp, Side<T> w, int F, int O, const T* residual, T* y, RouteArgs a) {
+  __shared__ float sums[8][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = (int)blockIdx.x * 4;
+  int parts = 1;
+  while (parts * 2 * a.K <= 8 && parts * 1024 <= F) parts *= 2;
+  const int each = ((F + parts - 1) / parts + 511) / 512 * 512;
+  float total[4] = {};
+  for (int unit = wave; unit < a.K * parts; unit += 8) {
+    const int slot = unit / parts, begin = (unit - slot * parts) * each, end = begin + each < F ? begin + each : F;
+    const int e = a.to[slot];
+    const float p = a.share[slot];
+    const T* rows[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) rows[i] = w.p + ((int64_t)e * O + (n0 + i < O ? n0 + i : O - 1)) * w.ld;
+    float sum[4] = {};
+    four_rows<T, 2>(rows, h + slot * hp, F, begin, end, sum);
+#pragma unroll
+    for (int i = 0; i < 4; i++) total[i] = fmaf(p, sum[i], total[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float v = over_wave(total[i]);
+    if (lane == i) sums[wave][i] = v;
+  }
+  __syncthreads();
+  const int n = n0 + (int)threadIdx.x;
+  if (threadIdx.x >= 4 || n >= O) return;
+  float v = residual ? (float)residual[n] : 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) v += sums[i][threadIdx.x];
+  y[n] = (T)v;
 }
 
 // ---- who goes where ----------------------------------------------------------------------------------------
@@ -106,16 +254,11 @@ __global__ __launch_bounds__(1024) void route_kernel(Side<T> x, Side<T> w, Route
 // Which experts the pairs of a lot (token t's j-th choice is pair t K + j) name, as bits in LDS.
 struct Taken {
   uint32_t bits[kMostExperts / 32];
-  __device__ __forceinline__ void find(const int32_t* to, int pairs, int E) {
+  __device__ __forceinline__ void find(const int32_t* to, int pairs) {
     for (int i = threadIdx.x; i < kMostExperts / 32; i += blockDim.x) bits[i] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < pairs; i += blockDim.x) atomicOr(&bits[to[i] >> 5], 1u << (to[i] & 31));
     __syncthreads();
-  }
-  __device__ __forceinline__ int count(int E) const {
-    int n = 0;
-    for (int i = 0; i < (E + 31) / 32; i++) n += __builtin_popcount(bits[i]);
-    return n;
   }
   // The expert with `before` taken ones below it, or -1.
   __device__ __forceinline__ int at(int before, int E) const {
@@ -149,173 +292,182 @@ __device__ __forceinline__ int pairs_of(const int32_t* to, int pairs, int e, uin
 // ---- products ----------------------------------------------------------------------------------------------
 
 struct ExpertArgs {
-  int64_t rows;
-  int D, F, O, E, K;
-  int64_t hp;  // between rows of h
+  int pairs, K, E;   // of the lot, choices a token, experts
+  int cols, rows;    // of an expert's matrix
+  int shared;        // waves that share a tile's k: 1, 2, 4 or 8
   const int32_t* to;
-  const float* share;
 };
 
-// h[pair] = act(w_gate x) (w_up x) for one expert's pairs: 16 hidden units a workgroup, its eight waves every eighth run of 128 values of
-// k, 16 MT pairs at a time. The weights go from memory straight to the matrix instructions' registers.
-template <typename T, int ACT, int MT>
-__global__ __launch_bounds__(512) void gate_up_kernel(Side<T> x, Side<T> wg, Side<T> wu, T* h, ExpertArgs a) {
+// Products of an expert's rows with its pairs' vectors, PL = 2 of them with the same (gate and up) or one (down): 16 rows a tile, 16 MT pairs at
+// a time; `shared` waves take every shared-th run of 128 values of k of one. The weights go from memory straight to the matrix
+// instructions' registers, U runs of them at a time. Rows beyond the last read the last one's values, which nobody stores. LONG: K >= 8.
+template <typename T, int PL, int MT, bool LONG, typename In, typename Out>
+__device__ __forceinline__ void expert_product(const Side<T> (&w)[PL], const ExpertArgs& a, In in, Out out) {
+  constexpr int U = MT * PL == 1 ? 2 : 1;
   __shared__ Taken taken;
   __shared__ uint16_t list[kLot];
   __shared__ int count;
-  __shared__ f32x4 sums[8][2 * MT][64];
-  const int pairs = (int)a.rows * a.K, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, q4 = lane >> 4;
-  taken.find(a.to, pairs, a.E);
+  __shared__ f32x4 sums[8][PL * MT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, q4 = lane >> 4;
+  taken.find(a.to, a.pairs);
   const int e = taken.at((int)blockIdx.y, a.E);
   if (e < 0) return;
   if (wave == 0) {
-    const int n = pairs_of(a.to, pairs, e, list);
+    const int n = pairs_of(a.to, a.pairs, e, list);
     if (lane == 0) count = n;
   }
   __syncthreads();
-  const int n = (int)blockIdx.x * 16 + row, all = count;
-  const bool there = n < a.F;
-  const T* pg = wg.p + ((int64_t)e * a.F + (there ? n : 0)) * wg.ld;
-  const T* pu = wu.p + ((int64_t)e * a.F + (there ? n : 0)) * wu.ld;
+  const int all = count, K = a.cols, whole = K >> 7, runs = (K + 127) >> 7;
+  const int part = wave & (a.shared - 1), n0 = ((int)blockIdx.x * (8 / a.shared) + wave / a.shared) * 16;
+  const int left = a.rows - n0;  // none: the wave has no tile
+  const T* base[PL];
+  uint32_t at[PL];
+#pragma unroll
+  for (int d = 0; d < PL; d++) {
+    base[d] = w[d].p + ((int64_t)e * a.rows + (left > 0 ? n0 : 0)) * w[d].ld;
+    at[d] = (uint32_t)(left > 0 ? (row < left ? row : left - 1) : 0) * (uint32_t)w[d].ld;
+  }
   for (int first = 0; first < all; first += 16 * MT) {
     const T* px[MT];
-    bool has[MT];
 #pragma unroll
     for (int t = 0; t < MT; t++) {
       const int i = first + t * 16 + row;
-      has[t] = i < all;
-      px[t] = x.p + (int64_t)(has[t] ? list[i] / a.K : 0) * x.ld;
+      px[t] = in(list[i < all ? i : all - 1]);
     }
-    f32x4 acc[2][MT] = {};
-    using A = vec<T, 8>;
-    A g[2][4], u[2][4], v[2][MT][4];
-    auto fetch = [&](int b, int k0) {
+    struct Run {
+      vec<T, 8> w[PL][4], x[MT][4];
+    };
+    f32x4 acc[PL][MT] = {};
+    auto fetch = [&](Run& r, int run) {
 #pragma unroll
       for (int c = 0; c < 4; c++) {
-        const int k = k0 + (c * 4 + q4) * 8;
-        g[b][c] = run_of<8>(pg, k, a.D, there);
-        u[b][c] = run_of<8>(pu, k, a.D, there);
+        const int k = run * 128 + c * 32 + q4 * 8;
 #pragma unroll
-        for (int t = 0; t < MT; t++) v[b][t][c] = run_of<8>(px[t], k, a.D, has[t]);
+        for (int d = 0; d < PL; d++) __builtin_memcpy(&r.w[d][c], base[d] + (at[d] + (uint32_t)k), 16);
+#pragma unroll
+        for (int t = 0; t < MT; t++) __builtin_memcpy(&r.x[t][c], px[t] + k, 16);
       }
     };
-    auto multiply = [&](int b) {
+    auto fetch_end = [&](Run& r) {
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const int k = whole * 128 + c * 32 + q4 * 8;
+#pragma unroll
+        for (int d = 0; d < PL; d++) r.w[d][c] = end8<T>(base[d] + at[d], k, K);
+#pragma unroll
+        for (int t = 0; t < MT; t++) r.x[t][c] = end8<T>(px[t], k, K);
+      }
+    };
+    auto fetch_only = [&](Run& r) {  // a row shorter than a piece
+      r = {};
+      if (q4 == 0) {
+#pragma unroll
+        for (int d = 0; d < PL; d++) r.w[d][0] = some<T, 8>(base[d] + at[d], 0, K);
+#pragma unroll
+        for (int t = 0; t < MT; t++) r.x[t][0] = some<T, 8>(px[t], 0, K);
+      }
+    };
+    auto multiply = [&](const Run& r) {
 #pragma unroll
       for (int c = 0; c < 4; c++)
 #pragma unroll
-        for (int t = 0; t < MT; t++) {
-          acc[0][t] = mfma(g[b][c], v[b][t][c], acc[0][t]);
-          acc[1][t] = mfma(u[b][c], v[b][t][c], acc[1][t]);
-        }
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+          for (int d = 0; d < PL; d++) acc[d][t] = mfma(r.w[d][c], r.x[t][c], acc[d][t]);
     };
-    fetch(0, wave * 128);
-    for (int k0 = wave * 128; k0 < a.D; k0 += 2048) {
-      fetch(1, k0 + 1024);
-      multiply(0);
-      fetch(0, k0 + 2048);
-      multiply(1);
-    }
-    __syncthreads();
+    if (left > 0) {
+      if constexpr (LONG) {
+        if (whole < runs && part == 0) {
+          Run r;
+          fetch_end(r);
+          multiply(r);
+        }
+        for (int run = (part + a.shared - 1) & (a.shared - 1); run < whole; run += U * a.shared) {
+          Run r[U];
 #pragma unroll
-    for (int d = 0; d < 2; d++)
+          for (int u = 0; u < U; u++)
+            if (run + u * a.shared < whole) fetch(r[u], run + u * a.shared);
 #pragma unroll
-      for (int t = 0; t < MT; t++) sums[wave][d * MT + t][lane] = acc[d][t];
-    __syncthreads();
-    if (wave < MT) {
-      f32x4 s[2];
-#pragma unroll
-      for (int d = 0; d < 2; d++) {
-        s[d] = sums[0][d * MT + wave][lane];
-#pragma unroll
-        for (int i = 1; i < 8; i++) s[d] += sums[i][d * MT + wave][lane];
+          for (int u = 0; u < U; u++)
+            if (run + u * a.shared < whole) multiply(r[u]);
+        }
+      } else if (part == 0) {
+        Run r;
+        fetch_only(r);
+        multiply(r);
       }
-      const int i = first + wave * 16 + row, to = (int)blockIdx.x * 16 + q4 * 4;
-      if (i < all && to < a.F) {
-        float o[4];
+    }
+    if (a.shared > 1) {  // the sums of the waves that share a tile, in their order; wave i of them finishes pairs 16 i ..
+      if (first) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; j++) o[j] = act<ACT>(s[0][j]) * s[1][j];
-        put<4>(h, a.hp, list[i], to, a.F, o);
+      for (int d = 0; d < PL; d++)
+#pragma unroll
+        for (int t = 0; t < MT; t++) sums[wave][d * MT + t][lane] = acc[d][t];
+      __syncthreads();
+      if (part < MT) {
+        const int w0 = wave - part;
+#pragma unroll
+        for (int d = 0; d < PL; d++) {
+          f32x4 v = sums[w0][d * MT + part][lane];
+          for (int i = 1; i < a.shared; i++) v += sums[w0 + i][d * MT + part][lane];
+          acc[d][0] = v;
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+      if (a.shared > 1 && t > 0) break;
+      if (a.shared > 1 && part >= MT) break;
+      const int i = first + (a.shared > 1 ? part : t) * 16 + row;
+      if (i < all && q4 * 4 < left) {
+        float v[PL][4];
+#pragma unroll
+        for (int d = 0; d < PL; d++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) v[d][j] = acc[d][t][j];
+        out(list[i], n0 + q4 * 4, v);
       }
     }
   }
 }
 
-// y = residual + the weighted sum over a token's choices of w_down h: 16 outputs a workgroup, its sixteen waves an expert each, or a part of
-// one's k where there are fewer. Every pair's sums stand in LDS before they are added, in the order of the choices.
-template <typename T, int MT>
-__global__ __launch_bounds__(1024) void down_kernel(const T* h, Side<T> w, const T* residual, int64_t ldr, T* y, int64_t ldy, ExpertArgs a) {
-  __shared__ Taken taken;
-  __shared__ uint16_t lists[16][kLot];
-  __shared__ __attribute__((aligned(16))) float sums[kLot][16];
-  const int pairs = (int)a.rows * a.K, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, q4 = lane >> 4;
-  taken.find(a.to, pairs, a.E);
-  const int experts = taken.count(a.E), steps = (a.F + 127) / 128;
-  int parts = 16 / experts;  // of an expert's k
-  parts = parts < steps ? parts : steps;
-  parts = parts < kLot / pairs ? parts : kLot / pairs;
-  parts = parts < 1 ? 1 : parts;
-  const int n = (int)blockIdx.x * 16 + row;
-  const bool there = n < a.O;
-  for (int unit = wave; unit < experts * parts; unit += 16) {
-    const int i = unit / parts, part = unit - i * parts, e = taken.at(i, a.E);
-    uint16_t* list = lists[wave];
-    const int all = pairs_of(a.to, pairs, e, list);
-    const int begin = steps * part / parts, end = steps * (part + 1) / parts;
-    const T* p = w.p + ((int64_t)e * a.O + (there ? n : 0)) * w.ld;
-    for (int first = 0; first < all; first += 16 * MT) {
-      const T* ph[MT];
-      bool has[MT];
+// h[pair] = act(w_gate x) (w_up x)
+template <typename T, int ACT, int MT, bool LONG>
+__global__ __launch_bounds__(512, 4) void gate_up_kernel(Side<T> x, Side<T> wg, Side<T> wu, T* h, int64_t hp, ExpertArgs a) {
+  const Side<T> w[2] = {wg, wu};
+  expert_product<T, 2, MT, LONG>(
+      w, a, [&](int pair) { return x.p + (int64_t)(pair / a.K) * x.ld; },
+      [&](int pair, int n, const float (&v)[2][4]) {
+        float o[4];
 #pragma unroll
-      for (int t = 0; t < MT; t++) {
-        const int j = first + t * 16 + row;
-        has[t] = j < all;
-        ph[t] = h + (int64_t)(has[t] ? list[j] : 0) * a.hp;
-      }
-      f32x4 acc[MT] = {};
-      vec<T, 8> g[2][4], v[2][MT][4];
-      auto fetch = [&](int b, int step) {
+        for (int j = 0; j < 4; j++) o[j] = act<ACT>(v[0][j]) * v[1][j];
+        put<4>(h, hp, pair, n, a.rows, o);
+      });
+}
+// parts[pair] = w_down h
+template <typename T, int MT, bool LONG>
+__global__ __launch_bounds__(512, 4) void down_kernel(const T* h, int64_t hp, Side<T> wd, float* parts, int64_t pp, ExpertArgs a) {
+  const Side<T> w[1] = {wd};
+  expert_product<T, 1, MT, LONG>(
+      w, a, [&](int pair) { return h + pair * hp; },
+      [&](int pair, int n, const float (&v)[1][4]) { put<4>(parts, pp, pair, n, a.rows, v[0]); });
+}
+// y = residual + the weighted sum of a token's parts, in the order of its choices; four columns a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void combine_kernel(const float* parts, int64_t pp, const float* share, const T* residual, int64_t ldr, T* y,
+                                                      int64_t ldy, int K, int O) {
+  const int64_t m = blockIdx.y;
+  const int n = ((int)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (n >= O) return;
+  float v[4] = {};
+  if (residual) get<4>(residual, ldr, m, n, O, v);
+  for (int j = 0; j < K; j++) {
+    const f32x4 s = *reinterpret_cast<const f32x4*>(parts + (m * K + j) * pp + n);
+    const float p = share[m * K + j];
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          const int k = step * 128 + (c * 4 + q4) * 8;
-          g[b][c] = run_of<8>(p, k, a.F, there && step < end);
-#pragma unroll
-          for (int t = 0; t < MT; t++) v[b][t][c] = run_of<8>(ph[t], k, a.F, has[t] && step < end);
-        }
-      };
-      auto multiply = [&](int b) {
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-          for (int t = 0; t < MT; t++) acc[t] = mfma(g[b][c], v[b][t][c], acc[t]);
-      };
-      fetch(0, begin);
-      for (int s = begin; s < end; s += 2) {
-        fetch(1, s + 1);
-        multiply(0);
-        fetch(0, s + 2);
-        multiply(1);
-      }
-#pragma unroll
-      for (int t = 0; t < MT; t++) {
-        const int j = first + t * 16 + row;
-        if (j < all) *reinterpret_cast<f32x4*>(&sums[part * pairs + list[j]][q4 * 4]) = acc[t];
-      }
-    }
+    for (int i = 0; i < 4; i++) v[i] = fmaf(p, s[i], v[i]);
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < (int)a.rows * 16; i += 1024) {
-    const int64_t m = i >> 4;
-    const int c = i & 15, to = (int)blockIdx.x * 16 + c;
-    if (to >= a.O) continue;
-    float v = residual ? (float)residual[m * ldr + to] : 0.f;
-    for (int j = 0; j < a.K; j++) {
-      const int p = (int)m * a.K + j;
-      float s = 0;
-      for (int q = 0; q < parts; q++) s += sums[q * pairs + p][c];
-      v = fmaf(a.share[p], s, v);
-    }
-    y[m * ldy + to] = (T)v;
-  }
+  put<4>(y, ldy, m, n, O, v);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------
@@ -330,18 +482,51 @@ bool sizes_ok(const b2c_experts_args* a) {
 
 template <typename T>
 struct ExpertsPlan {
-  int64_t lot, hp;
+  int64_t lot, hp, pp;
   int32_t* to;
-  float* share;
+  float *share, *parts = nullptr;
+  double* logits = nullptr;
   T* h;
   ExpertsPlan(const b2c_experts_args* a, Room& room) {
     lot = std::min<int64_t>(a->rows, kLot / a->top_k);
     hp = up(a->d_hidden, 8);
+    pp = up(a->d_out, 4);
     to = room.take<int32_t>(lot * a->top_k);
     share = room.take<float>(lot * a->top_k);
     h = room.take<T>(lot * a->top_k * hp);
+    if (a->rows == 1) logits = room.take<double>(a->experts);
+    else parts = room.take<float>(lot * a->top_k * pp);
   }
 };
+
+template <typename T, int ACT>
+int one_token(const b2c_experts_args* a, const ExpertsPlan<T>& p, const RouteArgs& r, hipStream_t stream) {
+  const T *x = (const T*)a->x, *residual = (const T*)a->residual;
+  const Side<T> wr{(const T*)a->w_router, a->ld_router}, wg{(const T*)a->w_gate, a->ld_in}, wu{(const T*)a->w_up, a->ld_in},
+      wd{(const T*)a->w_down, a->ld_out};
+  const dim3 units((unsigned)(up(a->d_hidden, 8) / 8), (unsigned)a->top_k), outputs((unsigned)(up(a->d_out, 4) / 4));
+  int rc;
+  if (a->experts <= kChooseOften) {
+    logits_kernel<T><<<dim3((unsigned)(up(a->experts, 4) / 4)), 256, 0, stream>>>(x, wr, a->experts, a->d_in, p.logits);
+    if ((rc = hipGetLastError())) return rc;
+    gate_up_one_kernel<T, ACT, true><<<units, 256, 0, stream>>>(x, wg, wu, a->d_hidden, p.logits, p.h, p.hp, r);
+    if ((rc = hipGetLastError())) return rc;
+  } else {
+    route_kernel<T, 4><<<dim3(1), 1024, 0, stream>>>(Side<T>{x, a->ldx}, wr, r);
+    if ((rc = hipGetLastError())) return rc;
+    gate_up_one_kernel<T, ACT, false><<<units, 256, 0, stream>>>(x, wg, wu, a->d_hidden, p.logits, p.h, p.hp, r);
+    if ((rc = hipGetLastError())) return rc;
+  }
+  down_one_kernel<T><<<outputs, 512, 0, stream>>>(p.h, p.hp, wd, a->d_hidden, a->d_out, residual, (T*)a->y, r);
+  return hipGetLastError();
+}
+
+// Waves that share a tile's k: as many as it takes to fill the device four to a SIMD.
+int sharing(int64_t tiles, int cols) {
+  int n = 1;
+  while (n < 8 && tiles * n * 2 <= 4096 && n * 2 <= std::max(cols / 128, 1)) n *= 2;
+  return n;
+}
 
 template <typename T, int ACT>
 int run(const b2c_experts_args* a, hipStream_t stream) {
@@ -349,24 +534,44 @@ int run(const b2c_experts_args* a, hipStream_t stream) {
   const ExpertsPlan<T> p(a, room);
   const Side<T> wr{(const T*)a->w_router, a->ld_router}, wg{(const T*)a->w_gate, a->ld_in}, wu{(const T*)a->w_up, a->ld_in},
       wd{(const T*)a->w_down, a->ld_out};
+  const int K = a->top_k, E = a->experts;
   for (int64_t m = 0; m < a->rows; m += p.lot) {
     const int64_t rows = std::min(p.lot, a->rows - m);
     const Side<T> x{(const T*)a->x + m * a->ldx, a->ldx};
-    const RouteArgs r{a->d_in, a->experts, a->top_k, a->normalize != 0, p.to, a->index ? a->index + m * a->ldi : nullptr, p.share,
+    const RouteArgs r{a->d_in, E, K, a->normalize != 0, p.to, a->index ? a->index + m * a->ldi : nullptr, p.share,
                       a->weight ? a->weight + m * a->ldw : nullptr, a->ldi, a->ldw};
-    route_kernel<T><<<dim3((unsigned)rows), 1024, 0, stream>>>(x, wr, r);
+    if (a->rows == 1) return one_token<T, ACT>(a, p, r, stream);
+    if (E <= 16) route_kernel<T, 1><<<dim3((unsigned)rows), 1024, 0, stream>>>(x, wr, r);
+    else if (E <= 32) route_kernel<T, 2><<<dim3((unsigned)rows), 1024, 0, stream>>>(x, wr, r);
+    else route_kernel<T, 4><<<dim3((unsigned)rows), 1024, 0, stream>>>(x, wr, r);
     int rc = hipGetLastError();
     if (rc) return rc;
-    const ExpertArgs e{rows, a->d_in, a->d_hidden, a->d_out, a->experts, a->top_k, p.hp, p.to, p.share};
-    const dim3 grid((unsigned)(up(a->d_hidden, 16) / 16), (unsigned)std::min<int64_t>(rows * a->top_k, a->experts));
-    if (rows <= 16) gate_up_kernel<T, ACT, 1><<<grid, 512, 0, stream>>>(x, wg, wu, p.h, e);
-    else gate_up_kernel<T, ACT, 2><<<grid, 512, 0, stream>>>(x, wg, wu, p.h, e);
-    if ((rc = hipGetLastError())) return rc;
-    const T* residual = a->residual ? (const T*)a->residual + m * a->ldr : nullptr;
-    T* y = (T*)a->y + m * a->ldy;
-    const dim3 tiles((unsigned)(up(a->d_out, 16) / 16));
-    if (rows <= 16) down_kernel<T, 1><<<tiles, 1024, 0, stream>>>(p.h, wd, residual, a->ldr, y, a->ldy, e);
-    else down_kernel<T, 2><<<tiles, 1024, 0, stream>>>(p.h, wd, residual, a->ldr, y, a->ldy, e);
+    const int pairs = (int)rows * K;
+    const int64_t slots = std::min(pairs, E);
+    const bool two = pairs > 12 * E;  // pairs of an expert mostly pass one tile of 16
+    ExpertArgs up_args{pairs, K, E, a->d_in, a->d_hidden, 0, p.to}, down_args{pairs, K, E, a->d_hidden, a->d_out, 0, p.to};
+    auto launch = [&](ExpertArgs& args, auto with) -> int {
+      const int64_t tiles = up(args.rows, 16) / 16;
+      args.shared = sharing(tiles * slots, args.cols);
+      const dim3 grid((unsigned)(up(tiles * args.shared, 8) / 8), (unsigned)slots);
+      using One = std::integral_constant<int, 1>;
+      using Two = std::integral_constant<int, 2>;
+      if (args.cols < 8) with(grid, One{}, std::false_type{});
+      else if (two) with(grid, Two{}, std::true_type{});
+      else with(grid, One{}, std::true_type{});
+      return hipGetLastError();
+    };
+    rc = launch(up_args, [&](dim3 grid, auto mt, auto far) {
+      gate_up_kernel<T, ACT, decltype(mt)::value, decltype(far)::value><<<grid, 512, 0, stream>>>(x, wg, wu, p.h, p.hp, up_args);
+    });
+    if (rc) return rc;
+    rc = launch(down_args, [&](dim3 grid, auto mt, auto far) {
+      down_kernel<T, decltype(mt)::value, decltype(far)::value><<<grid, 512, 0, stream>>>(p.h, p.hp, wd, p.parts, p.pp, down_args);
+    });
+    if (rc) return rc;
+    const dim3 grid((unsigned)(up(a->d_out, 1024) / 1024), (unsigned)rows);
+    combine_kernel<T><<<grid, 256, 0, stream>>>(p.parts, p.pp, p.share, a->residual ? (const T*)a->residual + m * a->ldr : nullptr, a->ldr,
+                                                (T*)a->y + m * a->ldy, a->ldy, K, a->d_out);
     if ((rc = hipGetLastError())) return rc;
   }
   return hipSuccess;
@@ -397,7 +602,7 @@ extern "C" int b2c_hip_experts(const b2c_experts_args* a, hipStream_t stream) {
       !good(a->w_up, a->ld_in, a->d_in, 2) || !good(a->w_down, a->ld_out, a->d_hidden, 2) || !good(a->y, a->ldy, a->d_out, 2) ||
       (a->residual && !good(a->residual, a->ldr, a->d_out, 2)) || (a->index && !good(a->index, a->ldi, a->top_k, 4)) ||
       (a->weight && !good(a->weight, a->ldw, a->top_k, 4)) || !a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 ||
-      a->workspace_bytes < b2c_experts_workspace_bytes(a))
+      a->workspace_bytes < b2c_experts_workspace_bytes(a) || a->ld_in > kFarRows || a->ld_out > kFarRows)
     return hipErrorInvalidValue;
   return a->dtype == B2C_F16 ? run<f16>(a, stream) : run<bf16>(a, stream);
 }

@@ -1,6 +1,7 @@
 // Weights in 4 bits with a scale, and a zero point where there are any, for each group of columns (b2c_hip_quantize4,
 // b2c_hip_q4_linear).
 #include "dense_product.h"
+#include "dense_rows.h"
 
 namespace b2c {
 namespace dev {
@@ -154,36 +155,12 @@ __device__ __forceinline__ vec<uint32_t, 4> bytes16(const uint8_t* row, int b, i
   }
   return v;
 }
-// Sixteen bytes moved down by n, zeros behind them.
-__device__ __forceinline__ vec<uint32_t, 4> moved_down(vec<uint32_t, 4> v, int n) {
-  uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
-  if (n >= 8) lo = hi, hi = 0, n -= 8;
-  if (n >= 8) lo = 0;
-  else if (n > 0) lo = lo >> (8 * n) | hi << (64 - 8 * n), hi >>= 8 * n;
-  return {(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
-}
 // The four words that lanes l, l + 16, l + 32, l + 48 hold, turned: word i of lane 16 j + l becomes word j of lane 16 i + l.
 __device__ __forceinline__ void turn4(vec<uint32_t, 4>& v) {
   const auto a = __builtin_amdgcn_permlane32_swap(v[0], v[2], false, false), b = __builtin_amdgcn_permlane32_swap(v[1], v[3], false, false);
   const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
   v = {(uint32_t)c[0], (uint32_t)c[1], (uint32_t)d[0], (uint32_t)d[1]};
 }
-// N values of a row from i on; zeros beyond its last.
-template <typename E, int N>
-__device__ __forceinline__ vec<E, N> some(const E* row, int i, int count) {
-  vec<E, N> v{};
-  if (i + N <= count) {
-    __builtin_memcpy(&v, row + i, sizeof(E) * N);
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; j++)
-      v[j] = row[i + j < count ? i + j : count - 1];
-#pragma unroll
-    for (int j = 0; j < N; j++) v[j] = i + j < count ? v[j] : (E)0;
-  }
-  return v;
-}
-
 // At most 16 MT rows of x. A workgroup takes 16 NT outputs, its eight waves every eighth run of 128 values of k: sixteen bytes of a row a
 // lane, turned so that each matrix instruction meets 32 neighbouring values of k, which are of one group. With c the code and B its base, a
 // group's sum is s (sum (B + c) x - (B + z) sum x), and sum x comes from the same instruction against ones, in the same lanes. B is at most
@@ -352,14 +329,6 @@ __global__ __launch_bounds__(512, 4) void q4_few_kernel(Weights4<T> w, int shift
 // wave's four outputs at a time, sixteen bytes that are all of one group, against the same 32 of x, which wait in LDS with their sums, in
 // the order in which the codes come apart most cheaply. So a wave reads a kilobyte of a row at once, a slab of 2048 values, and two slabs of
 // four rows are on their way together. Where there are few outputs, `split` waves share four of them and take every split-th slab.
-__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c, bf16) {
-  using V = vec<bf16, 2>;
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, false);
-}
-__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c, f16) {
-  using V = vec<f16, 2>;
-  return __builtin_amdgcn_fdot2(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, false);
-}
 template <typename T, bool ZERO>
 __global__ __launch_bounds__(256, 4) void q4_one_kernel(Weights4<T> w, int shift, const T* x, T* y, int split) {
   constexpr int SLABS = 4, STEPS = 2;  // slabs of x in LDS; of weights on their way
@@ -643,6 +612,7 @@ extern "C" int b2c_hip_q4_linear(const b2c_q4_linear_args* a, hipStream_t stream
   const size_t need = b2c_q4_linear_workspace_bytes(a);
   if (!good(a->x, a->ldx, a->d_in, 2) || !good(a->w, a->ldw, (a->d_in + 1) / 2, 1) || !good(a->scale, a->lds, groups, 2) ||
       (a->zero && !good(a->zero, a->ldz, groups, 1)) || !good(a->y, a->ldy, a->d_out, 2) ||
+      a->ldw > kFarRows || a->lds > kFarRows || (a->zero && a->ldz > kFarRows) ||
       (need && (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_bytes < need)))
     return hipErrorInvalidValue;
   return a->dtype == B2C_F16 ? linear<f16>(a, stream) : linear<bf16>(a, stream);
