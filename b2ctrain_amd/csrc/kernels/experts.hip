@@ -2,6 +2,8 @@
 // projections, and the weighted sum.
 #include "dense_rows.h"
 
+#include <cmath>
+
 namespace b2c {
 namespace dev {
 namespace {
@@ -382,14 +384,21 @@ __device__ __forceinline__ void expert_product(const Side<T> (&w)[PL], const Exp
           fetch_end(r);
           multiply(r);
         }
-        for (int run = (part + a.shared - 1) & (a.shared - 1); run < whole; run += U * a.shared) {
+        // From a run on that differs from tile to tile, and around: rows are often a multiple of 4 KB apart, and waves that read the same
+        // columns of theirs at the same time ask the same channels of the memory (168 us for 148).
+        const int mine = (part + a.shared - 1) & (a.shared - 1), steps = whole > mine ? (whole - 1 - mine) / a.shared + 1 : 0;
+        const int start = steps ? (n0 >> 4) % steps : 0;
+        for (int i = 0; i < steps; i += U) {
           Run r[U];
 #pragma unroll
           for (int u = 0; u < U; u++)
-            if (run + u * a.shared < whole) fetch(r[u], run + u * a.shared);
+            if (i + u < steps) {
+              const int step = start + i + u;
+              fetch(r[u], mine + (step < steps ? step : step - steps) * a.shared);
+            }
 #pragma unroll
           for (int u = 0; u < U; u++)
-            if (run + u * a.shared < whole) multiply(r[u]);
+            if (i + u < steps) multiply(r[u]);
         }
       } else if (part == 0) {
         Run r;
@@ -521,11 +530,18 @@ int one_token(const b2c_experts_args* a, const ExpertsPlan<T>& p, const RouteArg
   return hipGetLastError();
 }
 
-// Waves that share a tile's k: as many as it takes to fill the device four to a SIMD.
-int sharing(int64_t tiles, int cols) {
-  int n = 1;
-  while (n < 8 && tiles * n * 2 <= 4096 && n * 2 <= std::max(cols / 128, 1)) n *= 2;
-  return n;
+// Waves that share a tile's k, from how many rounds of 4096 waves (four to a SIMD) the tiles of the experts that are expected to be met take:
+// 16 tokens, two of 16 experts of 2048-5632: gate and up take 182 us with one wave to a tile, 148, 158 and 201 with two, four and eight;
+// two tokens, eight of 64 of 2048-1024: 59, 33, 28 and 35.
+int sharing(double tiles, int cols) {
+  constexpr double more[] = {1, 1.07, 1.3, 1.45};
+  int best = 1;
+  double least = 1e30;
+  for (int i = 0; i < 4 && (i == 0 || cols >= 128 << i); i++) {
+    const double cost = std::ceil(tiles * (1 << i) / 4096) / (1 << i) * more[i];
+    if (cost < least) least = cost, best = 1 << i;
+  }
+  return best;
 }
 
 template <typename T, int ACT>
@@ -548,11 +564,12 @@ int run(const b2c_experts_args* a, hipStream_t stream) {
     if (rc) return rc;
     const int pairs = (int)rows * K;
     const int64_t slots = std::min(pairs, E);
+    const double met = std::max(1.0, E * (1 - std::pow(1 - (double)K / E, (double)rows)));  // experts, where any are as likely
     const bool two = pairs > 12 * E;  // pairs of an expert mostly pass one tile of 16
     ExpertArgs up_args{pairs, K, E, a->d_in, a->d_hidden, 0, p.to}, down_args{pairs, K, E, a->d_hidden, a->d_out, 0, p.to};
     auto launch = [&](ExpertArgs& args, auto with) -> int {
       const int64_t tiles = up(args.rows, 16) / 16;
-      args.shared = sharing(tiles * slots, args.cols);
+      args.shared = sharing((double)tiles * met, args.cols);
       const dim3 grid((unsigned)(up(tiles * args.shared, 8) / 8), (unsigned)slots);
       using One = std::integral_constant<int, 1>;
       using Two = std::integral_constant<int, 2>;

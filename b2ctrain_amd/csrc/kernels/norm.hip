@@ -217,7 +217,7 @@ __device__ __forceinline__ void gather(float (&v)[C][E], float* lds) {
 }
 
 template <typename T, int LANES, int C>
-__global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGradArgs b) {
+__global__ __launch_bounds__(Team<LANES>::THREADS, 4) void norm_back_kernel(NormGradArgs b) {
   constexpr int E = 16 / sizeof(T), TEAMS = Team<LANES>::TEAMS;
   __shared__ float room[2][16];
   __shared__ float lds[LANES <= 64 ? 3 * LANES * C * E : 1];
@@ -378,8 +378,17 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(JoinArgs a) {
   const int64_t step = weight ? 2 * (int64_t)a.cols : a.cols;
   const float* from = weight ? a.w_parts + job * (int64_t)a.cols : a.gate_parts + (int64_t)(job - a.w_jobs) * a.g_count * a.cols;
   float s = 0;
-  if (n < a.cols)
-    for (uint32_t p = part; p < count; p += 32) s += from[p * step + n];
+  if (n < a.cols) {
+    uint32_t p = part;
+    for (; p + 7 * 32 < count; p += 8 * 32) {  // eight loads on their way
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = from[(p + i * 32) * step + n];
+#pragma unroll
+      for (int i = 0; i < 8; i++) s += v[i];
+    }
+    for (; p < count; p += 32) s += from[p * step + n];
+  }
   sums[part][col] = s;
   __syncthreads();
   if (part || n >= a.cols) return;
