@@ -7,8 +7,6 @@ namespace b2c {
 namespace dev {
 namespace {
 
-constexpr int64_t kFewRows = 32;  // up to here the weights are multiplied as codes
-
 // ---- to 4 bits ---------------------------------------------------------------------------------------------
 
 // The largest of the values that N neighbouring lanes hold, to all of them.
@@ -168,9 +166,14 @@ __device__ __forceinline__ void turn4(vec<uint32_t, 4>& v) {
 // nobody stores; in the run at the end of k (not the first: LONG) every load that would pass a row's end reads its last bytes, which are then
 // moved to their place, so that no load waits for a condition (7 rows of 2050-5001: 3 us less). The waves' sums meet in LDS and are added in a fixed order.
 template <typename T, int GROUP, bool ZERO, int MT, int NT, bool LONG>
-__global__ __launch_bounds__(512, 4) void q4_few_kernel(Weights4<T> w, int shift, Side<T> x, int M, T* y, int64_t ldy) {
+__global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void q4_few_kernel(Weights4<T> w, int shift, Side<T> all, int64_t all_rows, T* all_y,
+                                                                      int64_t ldy) {
+  const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
+  const Side<T> x{all.p + m0 * all.ld, all.ld};
+  T* y = all_y + m0 * ldy;
+  const int M = all_rows - m0 < 16 * MT ? (int)(all_rows - m0) : 16 * MT;
   constexpr int NG = GROUP >= 128 ? 1 : 128 / GROUP, PER = 4 / NG;  // groups of a run, matrix instructions of a group
-  constexpr int U = MT == 1 ? (NT == 1 ? 4 : 2) : (NT == 4 ? 1 : 2);  // runs in flight
+  constexpr int U = MT == 4 ? 1 : MT == 1 ? (NT == 1 ? 4 : 2) : (NT == 4 ? 1 : 2);  // runs in flight
   __shared__ f32x4 sums[8][NT][MT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, q4 = lane >> 4;
   const int n0 = (int)blockIdx.x * 16 * NT, rows = w.rows - n0;
@@ -313,15 +316,16 @@ __global__ __launch_bounds__(512, 4) void q4_few_kernel(Weights4<T> w, int shift
 #pragma unroll
     for (int t = 0; t < MT; t++) sums[wave][n][t][lane] = total[n][t];
   __syncthreads();
-  if (wave >= NT * MT) return;
-  const int tn = wave % NT, tm = wave / NT, n = n0 + tn * 16 + row;
-  f32x4 v = sums[0][tn][tm][lane];
+  for (int tile = wave; tile < NT * MT; tile += 8) {
+    const int tn = tile % NT, tm = tile / NT, n = n0 + tn * 16 + row;
+    f32x4 v = sums[0][tn][tm][lane];
 #pragma unroll
-  for (int i = 1; i < 8; i++) v += sums[i][tn][tm][lane];
+    for (int i = 1; i < 8; i++) v += sums[i][tn][tm][lane];
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int m = tm * 16 + q4 * 4 + j;
-    if (m < M && n < w.rows) y[m * ldy + n] = (T)v[j];
+    for (int j = 0; j < 4; j++) {
+      const int m = tm * 16 + q4 * 4 + j;
+      if (m < M && n < w.rows) y[m * ldy + n] = (T)v[j];
+    }
   }
 }
 
@@ -493,6 +497,28 @@ bool direct(const b2c_q4_linear_args* a) {
   return reinterpret_cast<uintptr_t>(a->x) % 16 == 0 && a->ldx % 8 == 0 && a->d_in % 8 == 0 && a->ldx < ((int64_t)1 << 21);
 }
 
+// Outputs of a workgroup of the kernel for a few rows, in sixteens: one round of workgroups, one to a compute unit, with as few each as that
+// takes; but for three sixteens of more than one row tile, which spill. 16 rows of 4096 -> 4096, 8192 and 11264: 8.7, 11.4 and 13.9 us this
+// way, 11.0, 14.0 and 16.2 with the next fewer or more outputs.
+int outputs_of(const b2c_q4_linear_args* a) {
+  const int64_t tiles = up(a->d_out, 16) / 16;
+  if (a->d_in < 128 || tiles <= 256) return 1;
+  if (tiles <= 512) return 2;
+  return tiles <= 768 && a->rows <= 16 ? 3 : 4;
+}
+// Whether the weights are multiplied as codes: up to 32 rows; with more, 64 to a workgroup, where that takes less time than to unpack them for
+// the tiles. A workgroup reads all of its rows of x, and what a compute unit may have on its way from the die's cache bounds that: 64 rows of
+// 4096 -> 4096, 11264 and 1024 -> 8192 take 19, 27 and 8 us this way, 25, 45 and 17 by tiles; 128 of 4096 -> 4096 35 and 28.
+bool few(const b2c_q4_linear_args* a) {
+  if (a->rows <= 32) return true;
+  if (a->rows > 512) return false;
+  const int n = outputs_of(a);
+  const int64_t blocks = up(a->rows, 64) / 64 * (up(a->d_out, 16 * n) / (16 * n));
+  const double weights = (double)a->d_in * a->d_out;
+  const double codes = 3 + (double)(up(blocks, 256) / 256) * a->d_in * (0.0033 + 0.0007 * n);
+  return codes < 11 + weights * 0.55e-6 + weights * (double)a->rows * 2e-9;
+}
+
 template <typename T>
 struct Q4Plan {
   T *w = nullptr, *x = nullptr;
@@ -500,7 +526,7 @@ struct Q4Plan {
   Way way{};
   void* sums = nullptr;
   Q4Plan(const b2c_q4_linear_args* a, Room& room) {
-    if (a->rows <= kFewRows) return;
+    if (few(a)) return;
     pitch = up(a->d_in, 64);
     w = room.take<T>(a->d_out * pitch);
     if (!direct(a)) x = room.take<T>(a->rows * pitch);
@@ -528,7 +554,7 @@ int linear(const b2c_q4_linear_args* a, hipStream_t stream) {
   const Weights4<T> w{a->w, a->ldw, (const T*)a->scale, a->lds, a->zero, a->ldz, a->d_out, a->d_in, groups_of(a->d_in, a->group)};
   Side<T> x{(const T*)a->x, a->ldx};
   const int shift = a->group == 32 ? 5 : a->group == 64 ? 6 : a->group == 128 ? 7 : 8;
-  if (a->rows <= kFewRows) {
+  if (few(a)) {
     using std::integral_constant;
     if (one_row(a)) {
       const int split = split_of(a);
@@ -538,24 +564,23 @@ int linear(const b2c_q4_linear_args* a, hipStream_t stream) {
       return hipGetLastError();
     }
     auto run = [&](auto group, auto zero, auto rows, auto outputs, auto far) -> int {
-      constexpr int NT = decltype(outputs)::value;
-      q4_few_kernel<T, decltype(group)::value, decltype(zero)::value, decltype(rows)::value, NT, decltype(far)::value>
-          <<<dim3((unsigned)(up(a->d_out, 16 * NT) / (16 * NT))), 512, 0, stream>>>(w, shift, x, (int)a->rows, (T*)a->y, a->ldy);
+      constexpr int NT = decltype(outputs)::value, MT = decltype(rows)::value;
+      q4_few_kernel<T, decltype(group)::value, decltype(zero)::value, MT, NT, decltype(far)::value>
+          <<<dim3((unsigned)(up(a->d_out, 16 * NT) / (16 * NT)), (unsigned)(up(a->rows, 16 * MT) / (16 * MT))), 512, 0, stream>>>(
+              w, shift, x, a->rows, (T*)a->y, a->ldy);
       return hipGetLastError();
     };
     auto with_rows = [&](auto group, auto zero) {
       auto with_outputs = [&](auto rows) {
         if (a->d_in < 128) return run(group, zero, rows, integral_constant<int, 1>{}, std::false_type{});
-        // One round of workgroups, one to a compute unit, with as few outputs each as that takes; but for three times sixteen of
-        // two row tiles, which spills. 16 rows of 4096 -> 4096, 8192 and 11264: 8.7, 11.4 and 13.9 us this way, 11.0, 14.0 and
-        // 16.2 with the next fewer or more outputs.
-        const int64_t tiles = up(a->d_out, 16) / 16;
-        if (tiles <= 256) return run(group, zero, rows, integral_constant<int, 1>{}, std::true_type{});
-        if (tiles <= 512) return run(group, zero, rows, integral_constant<int, 2>{}, std::true_type{});
+        const int n = outputs_of(a);
+        if (n == 1) return run(group, zero, rows, integral_constant<int, 1>{}, std::true_type{});
+        if (n == 2) return run(group, zero, rows, integral_constant<int, 2>{}, std::true_type{});
         if constexpr (decltype(rows)::value == 1)
-          if (tiles <= 768) return run(group, zero, rows, integral_constant<int, 3>{}, std::true_type{});
+          if (n == 3) return run(group, zero, rows, integral_constant<int, 3>{}, std::true_type{});
         return run(group, zero, rows, integral_constant<int, 4>{}, std::true_type{});
       };
+      if (a->rows > 32) return with_outputs(integral_constant<int, 4>{});
       return a->rows <= 16 ? with_outputs(integral_constant<int, 1>{}) : with_outputs(integral_constant<int, 2>{});
     };
     auto with_zero = [&](auto group) { return a->zero ? with_rows(group, std::true_type{}) : with_rows(group, std::false_type{}); };

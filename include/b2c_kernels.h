@@ -783,8 +783,8 @@ typedef struct b2c_quantize4_args {
 } b2c_quantize4_args;
 int b2c_hip_quantize4(const b2c_quantize4_args* a, hipStream_t stream);
 
-/* y = x w^T with w held as above: w[j][k] = (code - zero) scale, zero = 8 where there are none. With up to 32 rows each group's sum is
- * formed from the codes and then scaled, with more w is rounded to dtype first. An infinity in a row of x may make its whole row of y NaN.
+/* y = x w^T with w held as above: w[j][k] = (code - zero) scale, zero = 8 where there are none. With few rows (up to 32, and up to 512
+ * where that is faster) each group's sum is formed from the codes and then scaled, with more w is rounded to dtype first. An infinity in a row of x may make its whole row of y NaN.
  * rows at most 2^30, widths at most 2^20. */
 typedef struct b2c_q4_linear_args {
   int64_t rows;

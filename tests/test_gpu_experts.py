@@ -166,5 +166,5 @@ def test_a_block_and_its_head(rows):
     close("y", y2.get(), *want["y"])
     c = n2.get()
     close("n", c, *want["n"])
-    close("head", y3.get(), *V.q4_linear(c, code, U.value(stored, BF16), zero, group, BF16, rows <= 32))
+    close("head", y3.get(), *V.q4_linear(c, code, U.value(stored, BF16), zero, group, BF16, True))
     space.check()
