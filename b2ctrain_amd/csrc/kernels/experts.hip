@@ -144,23 +144,27 @@ __global__ __launch_bounds__(256) void logits_kernel(const T* x, Side<T> w, int 
 
 constexpr int kChooseOften = 256;  // experts among which every workgroup of a launch may choose again
 
-// A row's slab of 512 values is a kilobyte, sixteen bytes a lane. Values begin .. end - 1 of four rows (a wave's) against those of x, SLABS slabs
-// at a time; each row's sum stays spread over the lanes. `end` is the rows' end K or a multiple of 512.
-template <typename T, int SLABS>
-__device__ __forceinline__ void four_rows(const T* const (&rows)[4], const T* x, int K, int begin, int end, float (&sum)[4]) {
+// A row's slab of 512 values is a kilobyte, sixteen bytes a lane. Values begin .. end - 1 of four rows (a wave's) against those of the sum of X
+// vectors that lie `next` apart, SLABS slabs at a time; each row's sum stays spread over the lanes. `end` is the rows' end K or a multiple
+// of 512.
+template <typename T, int SLABS, int X>
+__device__ __forceinline__ void four_rows(const T* const (&rows)[4], const T* x, int64_t next, int K, int begin, int end, float (&sum)[4]) {
   const int lane = threadIdx.x & 63;
   using V = vec<uint32_t, 4>;
-  auto add = [&](const V& w, const V& v, float& to) {
+  auto add = [&](const V& w, const V (&v)[X], float& to) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) to = dot2(w[j], v[j], to, T{});
+    for (int p = 0; p < X; p++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) to = dot2(w[j], v[p][j], to, T{});
   };
   int k0 = begin;
   for (; k0 + 512 <= end; k0 += SLABS * 512) {
-    V w[SLABS][4], v[SLABS];
+    V w[SLABS][4], v[SLABS][X];
 #pragma unroll
     for (int s = 0; s < SLABS; s++)
       if (k0 + s * 512 + 512 <= end) {
-        __builtin_memcpy(&v[s], x + k0 + s * 512 + lane * 8, 16);
+#pragma unroll
+        for (int p = 0; p < X; p++) __builtin_memcpy(&v[s][p], x + p * next + k0 + s * 512 + lane * 8, 16);
 #pragma unroll
         for (int i = 0; i < 4; i++) __builtin_memcpy(&w[s][i], rows[i] + k0 + s * 512 + lane * 8, 16);
       }
@@ -172,13 +176,17 @@ __device__ __forceinline__ void four_rows(const T* const (&rows)[4], const T* x,
   }
   const int k = begin + (end - begin) / 512 * 512;  // what a slab holds of the end
   if (k >= end) return;
+  V v[X];
   if (K < 8) {
-    if (lane == 0)
+    if (lane) return;
 #pragma unroll
-      for (int i = 0; i < 4; i++) add(__builtin_bit_cast(V, some<T, 8>(rows[i], 0, K)), __builtin_bit_cast(V, some<T, 8>(x, 0, K)), sum[i]);
+    for (int p = 0; p < X; p++) v[p] = __builtin_bit_cast(V, some<T, 8>(x + p * next, 0, K));
+#pragma unroll
+    for (int i = 0; i < 4; i++) add(__builtin_bit_cast(V, some<T, 8>(rows[i], 0, K)), v, sum[i]);
     return;
   }
-  const V v = __builtin_bit_cast(V, end8<T>(x, k + lane * 8, K));
+#pragma unroll
+  for (int p = 0; p < X; p++) v[p] = __builtin_bit_cast(V, end8<T>(x + p * next, k + lane * 8, K));
 #pragma unroll
   for (int i = 0; i < 4; i++) add(__builtin_bit_cast(V, end8<T>(rows[i], k + lane * 8, K)), v, sum[i]);
 }
@@ -188,7 +196,8 @@ __device__ __forceinline__ float over_wave(float v) {
   return v;
 }
 
-// h[choice] = act(w_gate x) (w_up x): two hidden units a wave, eight a workgroup, so that a few experts' rows fill the device, and a wave's 16
+// h[choice] = act(w_gate x) (w_up x), as a value of T and what it is off by, hp behind it: one rounding to T would leave y half as far off
+// again as its own does (2.5e-3 for 1.7e-3 in bf16), and the second product costs the down projection, which waits for memory, nothing. Two hidden units a wave, eight a workgroup, so that a few experts' rows fill the device, and a wave's 16
 // kilobytes are on their way together.
 template <typename T, int ACT, bool CHOOSE>
 __global__ __launch_bounds__(256) void gate_up_one_kernel(const T* x, Side<T> wg, Side<T> wu, int F, const double* logits, T* h, int64_t hp, RouteArgs a) {
@@ -208,11 +217,15 @@ __global__ __launch_bounds__(256) void gate_up_one_kernel(const T* x, Side<T> wg
   const int next = n + 1 < F ? 1 : 0;
   const T* const rows[4] = {wg.p + row * wg.ld, wg.p + (row + next) * wg.ld, wu.p + row * wu.ld, wu.p + (row + next) * wu.ld};
   float sum[4] = {};
-  four_rows<T, 4>(rows, x, a.D, 0, a.D, sum);
+  four_rows<T, 4, 1>(rows, x, 0, a.D, 0, a.D, sum);
 #pragma unroll
   for (int i = 0; i < 4; i++) sum[i] = over_wave(sum[i]);
   const int lane = threadIdx.x & 63;
-  if (lane <= next) h[slot * hp + n + lane] = (T)(act<ACT>(lane ? sum[1] : sum[0]) * (lane ? sum[3] : sum[2]));
+  if (lane > next) return;
+  const float v = act<ACT>(lane ? sum[1] : sum[0]) * (lane ? sum[3] : sum[2]);
+  T* to = h + slot * 2 * hp + n + lane;
+  to[0] = (T)v;
+  to[hp] = (T)(v - (float)(T)v);
 }
 
 // y = residual + the weighted sum over the choices of w_down h: four outputs a workgroup, its eight waves a choice each, or a part of one's k
@@ -233,7 +246,7 @@ __global__ __launch_bounds__(512) void down_one_kernel(const T* h, int64_t hp, S
 #pragma unroll
     for (int i = 0; i < 4; i++) rows[i] = w.p + ((int64_t)e * O + (n0 + i < O ? n0 + i : O - 1)) * w.ld;
     float sum[4] = {};
-    four_rows<T, 2>(rows, h + slot * hp, F, begin, end, sum);
+    four_rows<T, 2, 2>(rows, h + slot * 2 * hp, hp, F, begin, end, sum);
 #pragma unroll
     for (int i = 0; i < 4; i++) total[i] = fmaf(p, sum[i], total[i]);
   }
@@ -300,12 +313,14 @@ struct ExpertArgs {
   const int32_t* to;
 };
 
-// Products of an expert's rows with its pairs' vectors, PL = 2 of them with the same (gate and up) or one (down): 16 rows a tile, 16 MT pairs at
-// a time; `shared` waves take every shared-th run of 128 values of k of one. The weights go from memory straight to the matrix
-// instructions' registers, U runs of them at a time. Rows beyond the last read the last one's values, which nobody stores. LONG: K >= 8.
-template <typename T, int PL, int MT, bool LONG, typename In, typename Out>
-__device__ __forceinline__ void expert_product(const Side<T> (&w)[PL], const ExpertArgs& a, In in, Out out) {
-  constexpr int U = MT * PL == 1 ? 2 : 1;
+// Products of an expert's rows with its pairs' vectors, PL = 2 of them with the same (gate and up) or one (down): 16 rows a tile, 16 MT vectors
+// at a time. With HALVES a pair's vector is the sum of two that lie `next` apart; a matrix instruction's 16 columns are then eight pairs
+// twice, since an expert of few tokens has less than eight as a rule, and the two sums are added at the end (with two instructions for 16
+// pairs the down projection of 16 tokens, two of 16 of 2048-5632, took 92 us where it takes 80: it waits for what the die's cache gives). `shared` waves take every shared-th run
+// of 128 values of k of a tile. The weights go from memory straight to the matrix instructions' registers. Rows beyond the last read the
+// last one's values, which nobody stores. LONG: K >= 8.
+template <typename T, int PL, bool HALVES, int MT, bool LONG, typename In, typename Out>
+__device__ __forceinline__ void expert_product(const Side<T> (&w)[PL], int64_t next, const ExpertArgs& a, In in, Out out) {
   __shared__ Taken taken;
   __shared__ uint16_t list[kLot];
   __shared__ int count;
@@ -329,12 +344,14 @@ __device__ __forceinline__ void expert_product(const Side<T> (&w)[PL], const Exp
     base[d] = w[d].p + ((int64_t)e * a.rows + (left > 0 ? n0 : 0)) * w[d].ld;
     at[d] = (uint32_t)(left > 0 ? (row < left ? row : left - 1) : 0) * (uint32_t)w[d].ld;
   }
-  for (int first = 0; first < all; first += 16 * MT) {
+  constexpr int PAIRS = HALVES ? 8 : 16;  // of a tile
+  const int column = HALVES ? row & 7 : row;
+  for (int first = 0; first < all; first += PAIRS * MT) {
     const T* px[MT];
 #pragma unroll
     for (int t = 0; t < MT; t++) {
-      const int i = first + t * 16 + row;
-      px[t] = in(list[i < all ? i : all - 1]);
+      const int i = first + t * PAIRS + column;
+      px[t] = in(list[i < all ? i : all - 1]) + (HALVES ? (row >> 3) * next : 0);
     }
     struct Run {
       vec<T, 8> w[PL][4], x[MT][4];
@@ -388,17 +405,11 @@ __device__ __forceinline__ void expert_product(const Side<T> (&w)[PL], const Exp
         // columns of theirs at the same time ask the same channels of the memory (168 us for 148).
         const int mine = (part + a.shared - 1) & (a.shared - 1), steps = whole > mine ? (whole - 1 - mine) / a.shared + 1 : 0;
         const int start = steps ? (n0 >> 4) % steps : 0;
-        for (int i = 0; i < steps; i += U) {
-          Run r[U];
-#pragma unroll
-          for (int u = 0; u < U; u++)
-            if (i + u < steps) {
-              const int step = start + i + u;
-              fetch(r[u], mine + (step < steps ? step : step - steps) * a.shared);
-            }
-#pragma unroll
-          for (int u = 0; u < U; u++)
-            if (i + u < steps) multiply(r[u]);
+        for (int i = 0; i < steps; i++) {
+          Run r;
+          const int step = start + i;
+          fetch(r, mine + (step < steps ? step : step - steps) * a.shared);
+          multiply(r);
         }
       } else if (part == 0) {
         Run r;
@@ -406,59 +417,76 @@ __device__ __forceinline__ void expert_product(const Side<T> (&w)[PL], const Exp
         multiply(r);
       }
     }
-    if (a.shared > 1) {  // the sums of the waves that share a tile, in their order; wave i of them finishes pairs 16 i ..
-      if (first) __syncthreads();
-#pragma unroll
-      for (int d = 0; d < PL; d++)
-#pragma unroll
-        for (int t = 0; t < MT; t++) sums[wave][d * MT + t][lane] = acc[d][t];
-      __syncthreads();
-      if (part < MT) {
-        const int w0 = wave - part;
-#pragma unroll
-        for (int d = 0; d < PL; d++) {
-          f32x4 v = sums[w0][d * MT + part][lane];
-          for (int i = 1; i < a.shared; i++) v += sums[w0 + i][d * MT + part][lane];
-          acc[d][0] = v;
-        }
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < MT; t++) {
-      if (a.shared > 1 && t > 0) break;
-      if (a.shared > 1 && part >= MT) break;
-      const int i = first + (a.shared > 1 ? part : t) * 16 + row;
-      if (i < all && q4 * 4 < left) {
-        float v[PL][4];
+    auto finish = [&](int t, f32x4 (&v)[PL]) {
+      if constexpr (HALVES) {
 #pragma unroll
         for (int d = 0; d < PL; d++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) v[d][j] = acc[d][t][j];
-        out(list[i], n0 + q4 * 4, v);
+          for (int j = 0; j < 4; j++) {  // row_ror:8
+            const float mine = v[d][j];
+            v[d][j] = mine + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, mine), 0x128, 0xF, 0xF, true));
+          }
       }
+      const int i = first + t * PAIRS + column;
+      if (i >= all || q4 * 4 >= left || (HALVES && row >= 8)) return;
+      float o[PL][4];
+#pragma unroll
+      for (int d = 0; d < PL; d++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[d][j] = v[d][j];
+      out(list[i], n0 + q4 * 4, o);
+    };
+    if (a.shared == 1) {
+#pragma unroll
+      for (int t = 0; t < MT; t++) {
+        f32x4 v[PL];
+#pragma unroll
+        for (int d = 0; d < PL; d++) v[d] = acc[d][t];
+        finish(t, v);
+      }
+      continue;
+    }
+    // The sums of the waves that share a tile, in their order; each finishes every shared-th of its column tiles.
+    if (first) __syncthreads();
+#pragma unroll
+    for (int d = 0; d < PL; d++)
+#pragma unroll
+      for (int t = 0; t < MT; t++) sums[wave][d * MT + t][lane] = acc[d][t];
+    __syncthreads();
+    for (int t = part; t < MT; t += a.shared) {
+      f32x4 v[PL];
+#pragma unroll
+      for (int d = 0; d < PL; d++) {
+        v[d] = sums[wave - part][d * MT + t][lane];
+        for (int i = 1; i < a.shared; i++) v[d] += sums[wave - part + i][d * MT + t][lane];
+      }
+      finish(t, v);
     }
   }
 }
 
-// h[pair] = act(w_gate x) (w_up x)
+// h[pair] = act(w_gate x) (w_up x), as a value of T and what it is off by
 template <typename T, int ACT, int MT, bool LONG>
 __global__ __launch_bounds__(512, 4) void gate_up_kernel(Side<T> x, Side<T> wg, Side<T> wu, T* h, int64_t hp, ExpertArgs a) {
   const Side<T> w[2] = {wg, wu};
-  expert_product<T, 2, MT, LONG>(
-      w, a, [&](int pair) { return x.p + (int64_t)(pair / a.K) * x.ld; },
+  expert_product<T, 2, false, MT, LONG>(
+      w, 0, a, [&](int pair) { return x.p + (int64_t)(pair / a.K) * x.ld; },
       [&](int pair, int n, const float (&v)[2][4]) {
         float o[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) o[j] = act<ACT>(v[0][j]) * v[1][j];
-        put<4>(h, hp, pair, n, a.rows, o);
+        put<4>(h, 2 * hp, pair, n, a.rows, o);
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] -= (float)(T)o[j];
+        put<4>(h + hp, 2 * hp, pair, n, a.rows, o);
       });
 }
 // parts[pair] = w_down h
 template <typename T, int MT, bool LONG>
 __global__ __launch_bounds__(512, 4) void down_kernel(const T* h, int64_t hp, Side<T> wd, float* parts, int64_t pp, ExpertArgs a) {
   const Side<T> w[1] = {wd};
-  expert_product<T, 1, MT, LONG>(
-      w, a, [&](int pair) { return h + pair * hp; },
+  expert_product<T, 1, true, MT, LONG>(
+      w, hp, a, [&](int pair) { return h + pair * 2 * hp; },
       [&](int pair, int n, const float (&v)[1][4]) { put<4>(parts, pp, pair, n, a.rows, v[0]); });
 }
 // y = residual + the weighted sum of a token's parts, in the order of its choices; four columns a thread.
@@ -502,7 +530,7 @@ struct ExpertsPlan {
     pp = up(a->d_out, 4);
     to = room.take<int32_t>(lot * a->top_k);
     share = room.take<float>(lot * a->top_k);
-    h = room.take<T>(lot * a->top_k * hp);
+    h = room.take<T>(lot * a->top_k * 2 * hp);
     if (a->rows == 1) logits = room.take<double>(a->experts);
     else parts = room.take<float>(lot * a->top_k * pp);
   }
@@ -565,24 +593,26 @@ int run(const b2c_experts_args* a, hipStream_t stream) {
     const int pairs = (int)rows * K;
     const int64_t slots = std::min(pairs, E);
     const double met = std::max(1.0, E * (1 - std::pow(1 - (double)K / E, (double)rows)));  // experts, where any are as likely
-    const bool two = pairs > 12 * E;  // pairs of an expert mostly pass one tile of 16
     ExpertArgs up_args{pairs, K, E, a->d_in, a->d_hidden, 0, p.to}, down_args{pairs, K, E, a->d_hidden, a->d_out, 0, p.to};
-    auto launch = [&](ExpertArgs& args, auto with) -> int {
+    // One tile of columns, or as many as an expert's vectors, of which the down projection has two for each pair, mostly fill: 64 tokens, eight
+    // of 64 of 2048-1024: down 115, 89 and 107 us with one, two and four; 61 tokens, three of 10 of 1000-1365: 43, 32 and 27, and gate and up
+    // 24, 18 and 24.
+    auto launch = [&](ExpertArgs& args, double vectors, auto most, auto with) -> int {
       const int64_t tiles = up(args.rows, 16) / 16;
       args.shared = sharing((double)tiles * met, args.cols);
       const dim3 grid((unsigned)(up(tiles * args.shared, 8) / 8), (unsigned)slots);
-      using One = std::integral_constant<int, 1>;
-      using Two = std::integral_constant<int, 2>;
-      if (args.cols < 8) with(grid, One{}, std::false_type{});
-      else if (two) with(grid, Two{}, std::true_type{});
-      else with(grid, One{}, std::true_type{});
+      using std::integral_constant;
+      if (args.cols < 8) with(grid, integral_constant<int, 1>{}, std::false_type{});
+      else if (vectors <= 14) with(grid, integral_constant<int, 1>{}, std::true_type{});
+      else if (vectors <= 32 || decltype(most)::value == 2) with(grid, integral_constant<int, 2>{}, std::true_type{});
+      else with(grid, most, std::true_type{});
       return hipGetLastError();
     };
-    rc = launch(up_args, [&](dim3 grid, auto mt, auto far) {
+    rc = launch(up_args, pairs / met, std::integral_constant<int, 2>{}, [&](dim3 grid, auto mt, auto far) {
       gate_up_kernel<T, ACT, decltype(mt)::value, decltype(far)::value><<<grid, 512, 0, stream>>>(x, wg, wu, p.h, p.hp, up_args);
     });
     if (rc) return rc;
-    rc = launch(down_args, [&](dim3 grid, auto mt, auto far) {
+    rc = launch(down_args, 2 * pairs / met, std::integral_constant<int, 4>{}, [&](dim3 grid, auto mt, auto far) {
       down_kernel<T, decltype(mt)::value, decltype(far)::value><<<grid, 512, 0, stream>>>(p.h, p.hp, wd, p.parts, p.pp, down_args);
     });
     if (rc) return rc;
