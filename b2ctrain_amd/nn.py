@@ -508,6 +508,12 @@ def _group(group):
     return group
 
 
+def _near(*matrices):
+    for m in matrices:
+        if m is not None and m.ld > 1 << 25:
+            raise ValueError(f"rows {m.ld} values apart: at most {1 << 25} for weights here")
+
+
 class QuantizeGroups:
     """q, scale (and with `zero` zero points) = x in 4 bits, a scale for every `group` columns of a row; b2c_hip_quantize4. q is uint8,
     two columns a byte, the even one in the low half; `scale` is in 16 bits. `values`: what the codes stand for, of x's type. For weights
@@ -541,6 +547,7 @@ class Q4Linear:
         s = matrix(scale, "scale", w.rows, n, x.dtype)
         z = matrix(zero, "zero", w.rows, n, U8) if zero is not None else None
         y = matrix(y, "y", x.rows, w.rows, x.dtype)
+        _near(w, s, z)
         a = self.args = Q4LinearArgs(rows=x.rows, d_in=x.cols, d_out=w.rows, group=group, dtype=x.dtype, x=x.ptr, ldx=x.ld, w=w.ptr,
                                      ldw=w.ld, scale=s.ptr, lds=s.ld, zero=z.ptr if z else None, ldz=z.ld if z else 0, y=y.ptr, ldy=y.ld)
         self._fn, self._ref = L.b2c_hip_q4_linear, C.byref(a)
@@ -575,6 +582,7 @@ class Experts:
         y = matrix(y, "y", m, None, t)
         d = matrix(w_down, "w_down", e * y.cols, g.rows // e, t)
         r = matrix(residual, "residual", m, y.cols, t) if residual is not None else None
+        _near(g, d)
         i = matrix(index, "index", m, top_k, I32) if index is not None else None
         w = matrix(weight, "weight", m, top_k, F32) if weight is not None else None
         a = self.args = ExpertsArgs(rows=m, d_in=x.cols, d_hidden=g.rows // e, d_out=y.cols, experts=e, top_k=top_k, dtype=t, act=_act(act),

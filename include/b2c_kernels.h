@@ -784,8 +784,9 @@ typedef struct b2c_quantize4_args {
 int b2c_hip_quantize4(const b2c_quantize4_args* a, hipStream_t stream);
 
 /* y = x w^T with w held as above: w[j][k] = (code - zero) scale, zero = 8 where there are none. With few rows (up to 32, and up to 512
- * where that is faster) each group's sum is formed from the codes and then scaled, with more w is rounded to dtype first. An infinity in a row of x may make its whole row of y NaN.
- * rows at most 2^30, widths at most 2^20. */
+ * where that is faster) each group's sum is formed from the codes and then scaled, with more w is rounded to dtype first. Those
+ * sums hold up to 144 times the values of x: where that passes single precision's range, and with an infinity in x, a row of y becomes NaN.
+ * rows at most 2^30, widths at most 2^20; rows of w, scale and zero lie at most 2^25 apart. */
 typedef struct b2c_q4_linear_args {
   int64_t rows;
   int d_in, d_out;
@@ -815,7 +816,7 @@ int b2c_hip_q4_linear(const b2c_q4_linear_args* a, hipStream_t stream);
  * summation; the other products' in 32; the inner activations enter theirs as two values of dtype, the
  * second what the first is off by, so that they lose less than a sum in 32 bits does. A row with a NaN or an infinite largest l gets NaN weights. Rows go 1024 /
  * top_k at a time, and the weights are read for each such lot. rows at most 2^20, widths at most 2^20, experts at most 1024, and all of a weight's
- * rows (experts times width) less than 2^31. y may be residual (same pointer and ld). */
+ * rows (experts times width) less than 2^31; rows of w_gate, w_up and w_down lie at most 2^25 apart. y may be residual (same pointer and ld). */
 typedef struct b2c_experts_args {
   int64_t rows;
   int d_in, d_hidden, d_out, experts, top_k;
