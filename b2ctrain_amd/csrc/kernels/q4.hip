@@ -69,15 +69,25 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
   const S held = (S)(top < 0x7f800000u ? reach : __builtin_nanf(""));
   const float scale = (float)held;
   const bool fine = scale > 0.f && scale < __builtin_inff();
-  const float zero = !ZERO ? 8.f : fine ? fminf(fmaxf(rintf(-lo / scale), 0.f), 15.f) : 0.f;
+  // x / scale, correctly rounded: with the correctly rounded inverse y, q = x y and its remainder x - q scale (exact in one fused operation),
+  // q + remainder y is it (Markstein 1990), three operations in place of a division's ten, where nothing under- or overflows. With divisions
+  // the arithmetic takes longer than the memory: 47 us for 11264 x 4096.
+  const bool plain = scale > 1e-30f && scale < 1e30f;
+  const float inverse = plain ? 1.f / scale : 0.f;
+  auto over = [&](float v) {
+    if (!plain) return v / scale;
+    const float q = v * inverse;
+    return fmaf(fmaf(-q, scale, v), inverse, q);
+  };
+  const float zero = !ZERO ? 8.f : fine ? fminf(fmaxf(rintf(over(-lo)), 0.f), 15.f) : 0.f;
   if (!there || n >= a.cols) return;
   uint32_t word = 0;
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    const float code = fine ? fminf(fmaxf(rintf(x[j] / scale) + zero, 0.f), 15.f) : zero;
+    const float code = fine ? __builtin_amdgcn_fmed3f(rintf(over(x[j])) + zero, 0.f, 15.f) : zero;
     v[j] = (code - zero) * scale;
-    if (n + j < a.cols) word |= (uint32_t)code << (4 * j);
+    word |= (uint32_t)(n + j < a.cols ? code : 0.f) << (4 * j);
   }
   uint8_t* q = a.q + m * a.ldq + piece * 4;
   if (n + 8 <= a.cols) {
