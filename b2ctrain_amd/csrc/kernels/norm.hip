@@ -263,11 +263,21 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
   Team<LANES> team;
   const int first = (threadIdx.x % LANES) * E, mine = threadIdx.x / LANES;
   const bool writes = LANES > 64 || threadIdx.x < LANES;  // what gather() leaves
+  // The largest teams have 128 registers a thread, which the row itself takes. Their weights are read again for each row, and the sums of
+  // the weights' gradients stay in LDS, each thread's own, where that is faster (us with it and without, plain norms: bf16 2048 x 8192 81
+  // and 93, 2000 x 6000 66 and 79, 1000 x 16384 145 and 191; f32 600 x 16384 163 and 184; but bf16 2000 x 5001 83 and 70, f32 2048 x 8192
+  // 110 and 100, 2048 x 4096 45 and 41).
+  constexpr bool WIDE = LANES == 1024 && (E == 8 ? END == WHOLE || C > 1 : C > 2);
+  __shared__ float held[2][WIDE ? C * E * LANES : 1];
   float wa[C][E], wb[C][E], sa[C][E] = {}, sb[C][E] = {};
+  if constexpr (WIDE) {
+    for (int i = 0; i < C * E; i++) held[0][i * LANES + threadIdx.x] = held[1][i * LANES + threadIdx.x] = 0.f;
+  } else {
 #pragma unroll
-  for (int c = 0; c < C; c++) {
-    weights<E, T>(a.w_post, a.w_f32, first + c * LANES * E, a.cols, wa[c]);
-    weights<E, T>(a.w_pre, a.w_f32, first + c * LANES * E, a.cols, wb[c]);
+    for (int c = 0; c < C; c++) {
+      weights<E, T>(a.w_post, a.w_f32, first + c * LANES * E, a.cols, wa[c]);
+      weights<E, T>(a.w_pre, a.w_f32, first + c * LANES * E, a.cols, wb[c]);
+    }
   }
   const uint32_t units = b.walk.groups * b.walk.segments;
   struct Raw {
@@ -320,6 +330,10 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
           d[c][j] = (float)w.dy[c][j];
         }
       if (a.post) size_x = normalise<LANES, C, E>(a, team, room, first, u);
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int c = 0; c < C; c++) weights<E, T>(a.w_post, a.w_f32, first + c * LANES * E, a.cols, wa[c]);
+      }
       float gate[C][E];
 #pragma unroll
       for (int c = 0; c < C; c++)
@@ -332,13 +346,18 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
 #pragma unroll
           for (int j = 0; j < E; j++) v[c][j] = fmaf(a.scale * gate[c][j], u[c][j] * wa[c][j], (float)w.r[c][j]);
         const float size = normalise<LANES, C, E>(a, team, room, first, v);
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int c = 0; c < C; c++) weights<E, T>(a.w_pre, a.w_f32, first + c * LANES * E, a.cols, wb[c]);
+        }
         float along = 0, mean = 0;
 #pragma unroll
         for (int c = 0; c < C; c++)
 #pragma unroll
           for (int j = 0; j < E; j++) {
             const float n = (float)w.dn[c][j];
-            sb[c][j] = fmaf(n, v[c][j], sb[c][j]);
+            float& sum = WIDE ? held[1][WIDE ? (c * E + j) * LANES + threadIdx.x : 0] : sb[c][j];
+            sum = fmaf(n, v[c][j], sum);
             along = fmaf(n * wb[c][j], v[c][j], along);
             mean = fmaf(n, wb[c][j], mean);
           }
@@ -384,7 +403,8 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
         for (int c = 0; c < C; c++)
 #pragma unroll
           for (int j = 0; j < E; j++) {
-            sa[c][j] = fmaf(d[c][j], u[c][j], sa[c][j]);
+            float& sum = WIDE ? held[0][WIDE ? (c * E + j) * LANES + threadIdx.x : 0] : sa[c][j];
+            sum = fmaf(d[c][j], u[c][j], sum);
             d[c][j] *= wa[c][j];
             along = fmaf(d[c][j], u[c][j], along);
             mean += d[c][j];
@@ -414,6 +434,15 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
     }
   }
   if (!b.w_parts) return;
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int j = 0; j < E; j++) {
+        sa[c][j] = held[0][(c * E + j) * LANES + threadIdx.x];
+        sb[c][j] = held[1][(c * E + j) * LANES + threadIdx.x];
+      }
+  }
   gather<LANES, C, E>(sa, lds);
   gather<LANES, C, E>(sb, lds);
   if (writes) {
