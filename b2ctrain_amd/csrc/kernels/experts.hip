@@ -142,6 +142,14 @@ __global__ __launch_bounds__(256) void logits_kernel(const T* x, Side<T> w, int 
   if ((threadIdx.x & 63) == 0) logits[e] = s[0];
 }
 
+// An inner activation as a value of T and what that is off by. The first stays within T's largest, so that the second takes what is beyond.
+template <typename T>
+__device__ __forceinline__ void halves(float v, T& first, T& second) {
+  constexpr float most = std::is_same_v<T, f16> ? 65504.f : 0x1.fep127f;
+  first = (T)__builtin_amdgcn_fmed3f(v, -most, most);
+  second = (T)(v - (float)first);
+}
+
 constexpr int kChooseOften = 256;  // experts among which every workgroup of a launch may choose again
 
 // A row's slab of 512 values is a kilobyte, sixteen bytes a lane. Values begin .. end - 1 of four rows (a wave's) against those of the sum of X
@@ -224,8 +232,7 @@ __global__ __launch_bounds__(256) void gate_up_one_kernel(const T* x, Side<T> wg
   if (lane > next) return;
   const float v = act<ACT>(lane ? sum[1] : sum[0]) * (lane ? sum[3] : sum[2]);
   T* to = h + slot * 2 * hp + n + lane;
-  to[0] = (T)v;
-  to[hp] = (T)(v - (float)(T)v);
+  halves(v, to[0], to[hp]);
 }
 
 // y = residual + the weighted sum over the choices of w_down h: four outputs a workgroup, its eight waves a choice each, or a part of one's k
@@ -472,13 +479,15 @@ __global__ __launch_bounds__(512, 4) void gate_up_kernel(Side<T> x, Side<T> wg, 
   expert_product<T, 2, false, MT, LONG>(
       w, 0, a, [&](int pair) { return x.p + (int64_t)(pair / a.K) * x.ld; },
       [&](int pair, int n, const float (&v)[2][4]) {
-        float o[4];
+        float o[4], rest[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) o[j] = act<ACT>(v[0][j]) * v[1][j];
+        for (int j = 0; j < 4; j++) {
+          T first, second;
+          halves(act<ACT>(v[0][j]) * v[1][j], first, second);
+          o[j] = (float)first, rest[j] = (float)second;
+        }
         put<4>(h, 2 * hp, pair, n, a.rows, o);
-#pragma unroll
-        for (int j = 0; j < 4; j++) o[j] -= (float)(T)o[j];
-        put<4>(h + hp, 2 * hp, pair, n, a.rows, o);
+        put<4>(h + hp, 2 * hp, pair, n, a.rows, rest);
       });
 }
 // parts[pair] = w_down h

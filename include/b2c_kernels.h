@@ -814,7 +814,7 @@ int b2c_hip_q4_linear(const b2c_q4_linear_args* a, hipStream_t stream);
  *   y = residual + sum_j p_j w_down[e_j] (act(w_gate[e_j] x) * (w_up[e_j] x))
  * The router's sums are held in 64 bits, so that the choice between experts that nearly agree does not depend on an order of
  * summation; the other products' in 32; the inner activations enter theirs as two values of dtype, the
- * second what the first is off by, so that they lose less than a sum in 32 bits does. A row with a NaN or an infinite largest l gets NaN weights. Rows go 1024 /
+ * second what the first is off by, so that they lose less than a sum in 32 bits does; beyond twice dtype's largest value they are infinite. A row with a NaN or an infinite largest l gets NaN weights. Rows go 1024 /
  * top_k at a time, and the weights are read for each such lot. rows at most 2^20, widths at most 2^20, experts at most 1024, and all of a weight's
  * rows (experts times width) less than 2^31; rows of w_gate, w_up and w_down lie at most 2^25 apart. y may be residual (same pointer and ld). */
 typedef struct b2c_experts_args {

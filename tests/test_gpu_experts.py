@@ -128,6 +128,26 @@ def test_tokens_without_numbers_leave_the_others_alone():
         assert np.isnan(got[6]).all() and np.isnan(weight.get()[6]).all()
 
 
+@pytest.mark.parametrize("rows", [1, 5])
+def test_subnormal_weights(rows):
+    """Which count like any others, and so do the second halves of inner activations, subnormal as a rule."""
+    check(rows, 64, 48, 40, 4, 2, F16, name="relu",
+          values=lambda v: {"wd": np.random.default_rng(6).integers(-1000, 1001, v["wd"].shape) * 2.0 ** -24, "wg": v["wg"] * 30, "wu": v["wu"] * 30})
+
+
+@pytest.mark.parametrize("rows", [1, 5])
+def test_inner_activations_beyond_the_type(rows):
+    """Up to twice float16's largest value they are held as well as others."""
+    def values(v):
+        # one column of x is 100, and a hidden unit's weights of it give 200 x 250 to 280 x 420: 50000 to 117600
+        x, wg, wu = v["x"], 0 * v["wg"], 0 * v["wu"]
+        x[:, 0] = 100
+        g = np.random.default_rng(7)
+        wg[:, 0], wu[:, 0] = 2 + 0.8 * g.random(len(wg)), 2.5 + 1.7 * g.random(len(wu))
+        return {"x": x, "wr": np.where(np.arange(64) > 0, v["wr"], 0), "wg": wg, "wu": wu, "wd": v["wd"] * 2.0 ** -10}
+    check(rows, 64, 48, 40, 4, 2, F16, name="relu", values=values)
+
+
 def test_no_rows():
     s = U.Held(np.ones((8, 8)), BF16)
     none = lambda c: nn.Matrix(s.matrix.ptr, 0, c, c, BF16)  # noqa: E731

@@ -141,6 +141,12 @@ def test_linear_of_rows_all_of_one_sign(rows):
         linear(rows, 4096, 40, 128, False, dtype, x=U.rounded(1 + g.random((rows, 4096)), dtype))
 
 
+@pytest.mark.parametrize("rows,k", [(1, 4096), (1, 500), (9, 512), (40, 512), (600, 300)])
+def test_linear_of_subnormal_values(rows, k):
+    """Which count like any others."""
+    linear(rows, k, 40, 64, True, F16, x=np.random.default_rng(5).integers(-1000, 1001, (rows, k)) * 2.0 ** -24)
+
+
 @pytest.mark.parametrize("rows,k,n", [(700, 600, 1100), (1300, 2048, 2048), (129, 4096, 520)])
 def test_linear_larger(rows, k, n):
     linear(rows, k, n, 128, True, BF16)
