@@ -760,9 +760,9 @@ int b2c_hip_block_norm_backward(const b2c_block_norm_grad_args* a, hipStream_t s
  *   with:    lo = min(x, 0), hi = max(x, 0), scale = (hi - lo) / 15, zero = -lo / scale, code = zero + x / scale;
  *            value = (code - zero) scale
  * The scale is formed in single precision and rounded to scale_dtype; quotients of that scale are rounded to single precision, then to
- * the nearest integer (to even), zero and code to 0 .. 15. A group whose scale is zero gets the code of 0 throughout (8, or 0 with zero points); one
- * with an infinity or NaN the scale NaN and those codes; a scale beyond scale_dtype's range becomes infinity, with those codes. Column
- * 2 j is in the low half of byte j of q, column 2 j + 1 in the high half, which is 0 behind the last column of an odd row.
+ * the nearest integer (to even), zero and code to 0 .. 15. A group whose scale is zero gets the code of 0 throughout (8, or 0 with zero
+ * points); one with an infinity or NaN the scale NaN and those codes; a scale beyond scale_dtype's range becomes infinity, with those
+ * codes. Column 2 j is in the low half of byte j of q, column 2 j + 1 in the high half, which is 0 behind the last column of an odd row.
  * `values`: what the codes stand for, formed in single precision, in dtype. rows at most 2^30, cols at most 2^20. */
 typedef struct b2c_quantize4_args {
   int64_t rows;
@@ -813,10 +813,11 @@ int b2c_hip_q4_linear(const b2c_q4_linear_args* a, hipStream_t stream);
  * ones' with `normalize`, and
  *   y = residual + sum_j p_j w_down[e_j] (act(w_gate[e_j] x) * (w_up[e_j] x))
  * The router's sums are held in 64 bits, so that the choice between experts that nearly agree does not depend on an order of
- * summation; the other products' in 32; the inner activations enter theirs as two values of dtype, the
- * second what the first is off by, so that they lose less than a sum in 32 bits does; beyond twice dtype's largest value they are infinite. A row with a NaN or an infinite largest l gets NaN weights. Rows go 1024 /
- * top_k at a time, and the weights are read for each such lot. rows at most 2^20, widths at most 2^20, experts at most 1024, and all of a weight's
- * rows (experts times width) less than 2^31; rows of w_gate, w_up and w_down lie at most 2^25 apart. y may be residual (same pointer and ld). */
+ * summation; the other products' in 32. The inner activations enter theirs as two values of dtype, the second what the first is off by:
+ * together off by 2^-18 of their value in bf16, 2^-24 in f16 (or 2^-25, where that is more); beyond twice dtype's largest value they are
+ * infinite. A row with a NaN or an infinite largest l gets NaN weights. Rows go 1024 / top_k at a time, and the weights are read for each
+ * such lot. rows at most 2^20, widths at most 2^20, experts at most 1024, top_k at most 64, and all of a weight's rows (experts times
+ * width) less than 2^31; rows of w_gate, w_up and w_down lie at most 2^25 apart. y may be residual (same pointer and ld). */
 typedef struct b2c_experts_args {
   int64_t rows;
   int d_in, d_hidden, d_out, experts, top_k;
