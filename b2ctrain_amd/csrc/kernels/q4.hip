@@ -438,36 +438,56 @@ __global__ __launch_bounds__(256, 4) void q4_one_kernel(Weights4<T> w, int shift
 }
 
 // The weights in T, for the tiles, and x where its rows have to be copied to ones that start on 16 bytes. (code - zero) scale is formed in
-// single precision and rounded once. Eight values a thread. Bound by memory: 4096-11264 (116 MB) 27 to 30 us, 4 TB/s.
-template <typename T, bool ZERO>
+// single precision and rounded once. A thread takes AT pieces of eight values, whose loads are on their way together. Bound by memory:
+// 4096-11264 (116 MB) 25.5 us, 4.5 TB/s.
+template <typename T, bool ZERO, int AT>
 __global__ __launch_bounds__(256) void unpack_kernel(Weights4<T> w, int shift, T* to, int64_t pitch, uint32_t groups, uint32_t own,
                                                      Side<T> x, int64_t M, T* x_to) {
   uint32_t block = block_index();
   const bool copies = block >= own;
   if (copies) block -= own;
-  const int64_t t = (int64_t)block * 256 + threadIdx.x, m = t / groups;
-  const int n = (int)(t - m * groups) * 8;
+  const int64_t first = (int64_t)block * (256 * AT) + threadIdx.x, m0 = first / groups;
+  const uint32_t start = (uint32_t)(first - m0 * groups);
   if (copies) {
-    if (m >= M) return;
-    *reinterpret_cast<vec<T, 8>*>(x_to + m * pitch + n) = some<T, 8>(x.p + m * x.ld, n, w.cols);
+#pragma unroll
+    for (int i = 0; i < AT; i++) {
+      const uint32_t at = start + i * 256, down = i ? at / groups : 0;
+      const int64_t m = m0 + down;
+      const int n = (int)(at - down * groups) * 8;
+      if (m < M) *reinterpret_cast<vec<T, 8>*>(x_to + m * pitch + n) = some<T, 8>(x.p + m * x.ld, n, w.cols);
+    }
     return;
   }
-  if (m >= w.rows) return;
-  uint32_t word = 0;
-  const uint8_t* q = w.q + m * w.ldq + n / 2;
-  if (n + 8 <= w.cols) {
-    __builtin_memcpy(&word, q, 4);
-  } else {
+  uint32_t word[AT];
+  float s[AT], z[AT];
+  int64_t to_at[AT];
+  int left[AT];
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (n + 2 * j < w.cols) word |= (uint32_t)q[j] << (8 * j);
+  for (int i = 0; i < AT; i++) {
+    const uint32_t at = start + i * 256, down = i ? at / groups : 0;
+    const bool there = m0 + down < w.rows;
+    const int64_t m = there ? m0 + down : w.rows - 1;
+    const int n = (int)(at - down * groups) * 8, g = n >> shift;
+    const uint8_t* q = w.q + m * w.ldq + n / 2;
+    word[i] = 0;
+    if (n + 8 <= w.cols) {
+      __builtin_memcpy(&word[i], q, 4);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (n + 2 * j < w.cols) word[i] |= (uint32_t)q[j] << (8 * j);
+    }
+    s[i] = (float)w.scale[m * w.lds + g], z[i] = ZERO ? (float)w.zero[m * w.ldz + g] : 8.f;
+    to_at[i] = m * pitch + n;
+    left[i] = there ? w.cols - n : 0;
   }
-  const int g = n >> shift;
-  const float s = (float)w.scale[m * w.lds + g], z = ZERO ? (float)w.zero[m * w.ldz + g] : 8.f;
-  vec<T, 8> v;
 #pragma unroll
-  for (int j = 0; j < 8; j++) v[j] = n + j < w.cols ? (T)(((float)(word >> (4 * j) & 15) - z) * s) : (T)0.f;
-  *reinterpret_cast<vec<T, 8>*>(to + m * pitch + n) = v;
+  for (int i = 0; i < AT; i++) {
+    vec<T, 8> v;
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = j < left[i] ? (T)(((float)(word[i] >> (4 * j) & 15) - z[i]) * s[i]) : (T)0.f;
+    if (left[i] > 0) *reinterpret_cast<vec<T, 8>*>(to + to_at[i]) = v;
+  }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------
@@ -606,11 +626,19 @@ int linear(const b2c_q4_linear_args* a, hipStream_t stream) {
   Room room{(char*)a->workspace};
   const Q4Plan<T> p(a, room);
   const uint32_t pieces = (uint32_t)(up(a->d_in, 8) / 8);
-  const int64_t own = up((int64_t)a->d_out * pieces, 256) / 256, copies = p.x ? up(a->rows * pieces, 256) / 256 : 0;
-  if (own + copies > 0x7fffffff) return hipErrorInvalidValue;
-  if (a->zero) unpack_kernel<T, true><<<grid_of(own + copies), 256, 0, stream>>>(w, shift, p.w, p.pitch, pieces, (uint32_t)own, x, a->rows, p.x);
-  else unpack_kernel<T, false><<<grid_of(own + copies), 256, 0, stream>>>(w, shift, p.w, p.pitch, pieces, (uint32_t)own, x, a->rows, p.x);
-  int rc = hipGetLastError();
+  auto unpack = [&](auto zero, auto at) -> int {
+    const int64_t block = 256 * at.value, own = up((int64_t)a->d_out * pieces, block) / block, copies = p.x ? up(a->rows * pieces, block) / block : 0;
+    if (own + copies > 0x7fffffff) return hipErrorInvalidValue;
+    unpack_kernel<T, zero.value, at.value>
+        <<<grid_of(own + copies), 256, 0, stream>>>(w, shift, p.w, p.pitch, pieces, (uint32_t)own, x, a->rows, p.x);
+    return hipGetLastError();
+  };
+  // Four pieces a thread where that leaves workgroups enough: 4096-11264 25.5 us, 30 with one; 1000-1000 5.1 and 4.0, 2050-5001 9.9 and 9.0.
+  auto with_zero = [&](auto zero) {
+    if ((int64_t)a->d_out * pieces >= 1 << 21) return unpack(zero, std::integral_constant<int, 4>{});
+    return unpack(zero, std::integral_constant<int, 1>{});
+  };
+  const int rc = a->zero ? with_zero(std::true_type{}) : with_zero(std::false_type{});
   if (rc) return rc;
   if (p.x) x = {p.x, p.pitch};
   const RowsOut<T> out{(T*)a->y, a->ldy, nullptr, 0, a->d_out, {}};

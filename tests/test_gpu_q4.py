@@ -147,7 +147,7 @@ def test_linear_of_subnormal_values(rows, k):
     linear(rows, k, 40, 64, True, F16, x=np.random.default_rng(5).integers(-1000, 1001, (rows, k)) * 2.0 ** -24)
 
 
-@pytest.mark.parametrize("rows,k,n", [(700, 600, 1100), (1300, 2048, 2048), (129, 4096, 520)])
+@pytest.mark.parametrize("rows,k,n", [(700, 600, 1100), (1300, 2048, 2048), (129, 4096, 520), (513, 4090, 4110)])
 def test_linear_larger(rows, k, n):
     linear(rows, k, n, 128, True, BF16)
 
