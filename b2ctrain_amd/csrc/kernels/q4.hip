@@ -439,7 +439,8 @@ __global__ __launch_bounds__(256, 4) void q4_one_kernel(Weights4<T> w, int shift
 
 // The weights in T, for the tiles, and x where its rows have to be copied to ones that start on 16 bytes. (code - zero) scale is formed in
 // single precision and rounded once. A thread takes AT pieces of eight values, whose loads are on their way together. Bound by memory:
-// 4096-11264 (116 MB) 25.5 us, 4.5 TB/s.
+// 4096-11264 (116 MB) 25.5 us, 4.5 TB/s. Workgroups from `own` on copy rows of x, of which there are M: none where x is read in place, and
+// none for the workgroups that a launch of more than 2^22 has too many.
 template <typename T, bool ZERO, int AT>
 __global__ __launch_bounds__(256) void unpack_kernel(Weights4<T> w, int shift, T* to, int64_t pitch, uint32_t groups, uint32_t own,
                                                      Side<T> x, int64_t M, T* x_to) {
@@ -630,7 +631,7 @@ int linear(const b2c_q4_linear_args* a, hipStream_t stream) {
     const int64_t block = 256 * at.value, own = up((int64_t)a->d_out * pieces, block) / block, copies = p.x ? up(a->rows * pieces, block) / block : 0;
     if (own + copies > 0x7fffffff) return hipErrorInvalidValue;
     unpack_kernel<T, zero.value, at.value>
-        <<<grid_of(own + copies), 256, 0, stream>>>(w, shift, p.w, p.pitch, pieces, (uint32_t)own, x, a->rows, p.x);
+        <<<grid_of(own + copies), 256, 0, stream>>>(w, shift, p.w, p.pitch, pieces, (uint32_t)own, x, p.x ? a->rows : 0, p.x);
     return hipGetLastError();
   };
   // Four pieces a thread where that leaves workgroups enough: 4096-11264 25.5 us, 30 with one; 1000-1000 5.1 and 4.0, 2050-5001 9.9 and 9.0.

@@ -1,0 +1,46 @@
+"""Products with 4-bit weights where the size, the range or the precision is at its limit."""
+import numpy as np
+import pytest
+
+from b2ctrain_amd import nn
+from tests.gpu_harness import emit
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = nn.F32, nn.F16, nn.BF16
+
+
+def test_more_than_four_million_workgroups_of_weights():
+    """Weights whose unpacking takes just more workgroups than one dimension of a launch holds, so that a launch has some without work,
+    while x is read in place and there is nothing to copy: 17 GB of codes, 69 GB of workspace. Outputs picked from all over."""
+    torch = pytest.importorskip("torch")
+    rows, k, n, group = 513, 1 << 20, 32776, 256
+    blocks = n * (k // 8) // 1024
+    assert blocks > 1 << 22 and rows > 512
+    if torch.cuda.mem_get_info()[0] < 110e9:
+        pytest.skip("110 GB of device memory are wanted")
+    emit(f"q4 linear {rows} x {k}-{n}, {blocks} workgroups")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(rows, k, generator=g, device="cuda").bfloat16()
+    q = torch.randint(0, 256, (n, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    s = (torch.rand(n, k // group, generator=g, device="cuda") / 4096).bfloat16()
+    y = torch.full((rows, n), float("nan"), device="cuda", dtype=torch.bfloat16)
+    p = nn.Q4Linear(x, q, s, y, group, room=lambda size: torch.empty(size, dtype=torch.uint8, device="cuda"))
+    try:
+        p.run(torch.cuda.current_stream().cuda_stream)
+        at = torch.cat([torch.arange(0, n, 1171, device="cuda"), torch.arange(n - 9, n, device="cuda")])
+        wide = x.double()
+        assert bool(torch.isfinite(y).all())
+        for i in at.split(8):
+            code = torch.stack([q[i] & 15, q[i] >> 4], 2).reshape(len(i), k).double() - 8
+            w = code * s[i].double().repeat_interleave(group, 1)
+            got, want = y[:, i].double(), wide @ w.T
+            # w may be rounded to bfloat16, sums of k products in single precision are off by k 2^-24 of their magnitudes at most, y is rounded
+            size = wide.abs() @ w.abs().T
+            bound = (2.0 ** -8 + (k + 8) * 2.0 ** -24) * size
+            # and by no more than a few standard deviations of roundings that know nothing of each other
+            several = 8 * 2.0 ** -8 * torch.sqrt(wide.pow(2) @ w.pow(2).T) + 2.0 ** -7 * want.abs()
+            assert bool(((got - want).abs() <= torch.minimum(bound, several)).all()), f"outputs {i.tolist()}"
+    finally:
+        del p, x, q, s, y
+        torch.cuda.empty_cache()
