@@ -37,6 +37,13 @@ struct Parts {
   }
 };
 
+// The same of a product with scales (GroupScales).
+template <typename P, int N>
+struct WithScales : P {
+  static constexpr int GROUPS = N;
+  GroupScales scales;
+};
+
 // Adds the parts in their order and finishes them with the product's epilogue, eight columns a thread.
 template <typename T, bool DUAL, int ROWS, int COLS, typename S, typename Epi, int NJ>
 __global__ __launch_bounds__(256) void join_kernel(Jobs<T, Epi, NJ> jobs, uint32_t first, uint32_t count, int parts, S* sums) {
@@ -179,12 +186,12 @@ inline double tile_time(int tile, int64_t n, double steps) {
 
 // The cheapest way for products of these extents, `steps` long. Tiles beyond the last full round of compute units, or all of them
 // where there are too few, may be split over k, for a write and a read of their sums at 5 TB/s. `moved`: bytes that the
-// epilogue reads and writes for each value of out; several tiles in a compute unit hide a little of them.
-inline Way choose(std::initializer_list<Extent> jobs, int64_t steps, bool dual, bool few, int moved = 2) {
+// epilogue reads and writes for each value of out; several tiles in a compute unit hide a little of them. `largest`: the largest tile.
+inline Way choose(std::initializer_list<Extent> jobs, int64_t steps, bool dual, bool few, int moved = 2, int largest = TILE_256) {
   if (few) return {FEW_ROWS, 0, 0, 1, 0};
   Way best{TILE_64, 0, 0, 1, 0};
   double least = 1e30;
-  for (int t = 0; t < 3; t++) {
+  for (int t = largest; t < 3; t++) {
     const int64_t side = t == TILE_256 ? 256 : t == TILE_128 ? 128 : 64, cols = dual ? side / 2 : side;
     const int64_t full = t == TILE_256 ? 256 : t == TILE_128 ? 512 : 1280;
     int64_t count = 0;
@@ -240,11 +247,14 @@ int run_tiles(Jobs<T, Epi, NJ>& jobs, const Way& way, void* sums, hipStream_t st
   int rc = launch_tiles<T, PT, QT, DUAL, TWO, SIDE>(jobs, 0, way.whole, 1, stream);
   if (rc || way.rest == 0) return rc;
   using S = std::conditional_t<std::is_same_v<T, int8_t>, int, float>;
-  using P = Parts<S, SIDE, COLS, DUAL ? 2 : 1>;
+  constexpr int GROUPS = groups_of_step<Epi>();
+  using Sums = Parts<S, SIDE, COLS, DUAL ? 2 : 1>;
+  using P = std::conditional_t<GROUPS == 0, Sums, WithScales<Sums, GROUPS>>;
   Jobs<T, P, NJ> parts{};
   for (int j = 0; j < NJ; j++) {
     parts.product[j] = jobs.product[j];
-    parts.epi[j] = P{(S*)sums};
+    parts.epi[j] = P{{(S*)sums}};
+    if constexpr (GROUPS > 0) parts.epi[j].scales = jobs.epi[j].scales;
     parts.tiles_m[j] = jobs.tiles_m[j];
     parts.tiles_n[j] = jobs.tiles_n[j];
   }
@@ -269,7 +279,9 @@ int products(Jobs<T, Epi, NJ>& jobs, const Way& way, void* sums, hipStream_t str
       return hipGetLastError();
     }
   }
-  if (way.tile == TILE_256) return run_tiles<T, PT, QT, DUAL, TWO, 256>(jobs, way, sums, stream);
+  if constexpr (groups_of_step<Epi>() == 0) {
+    if (way.tile == TILE_256) return run_tiles<T, PT, QT, DUAL, TWO, 256>(jobs, way, sums, stream);
+  }
   if (way.tile == TILE_128) return run_tiles<T, PT, QT, DUAL, TWO, 128>(jobs, way, sums, stream);
   return run_tiles<T, PT, QT, DUAL, TWO, 64>(jobs, way, sums, stream);
 }

@@ -437,16 +437,28 @@ __global__ __launch_bounds__(256, 4) void q4_one_kernel(Weights4<T> w, int shift
   y[n0 + lane] = (T)v;
 }
 
-// The weights in T, for the tiles, and x where its rows have to be copied to ones that start on 16 bytes. (code - zero) scale is formed in
-// single precision and rounded once. A thread takes AT pieces of eight values, whose loads are on their way together. Bound by memory:
-// 4096-11264 (116 MB) 25.5 us, 4.5 TB/s. Workgroups from `own` on copy rows of x, of which there are M: none where x is read in place, and
-// none for the workgroups that a launch of more than 2^22 has too many.
+// What the whole numbers code - zero count in the tiles' weights, a power of two, so that 16 bits hold them exactly: as little as keeps the sum
+// of a group's 256 products with the largest value of T, up to 15 each, in single precision's range.
+template <typename T>
+constexpr float kWhole = std::is_same_v<T, bf16> ? 0x1p-12f : 1.f;
+
+// The weights less their scales in T, for the tiles, their scales in single precision and turned, one group's next to each other, and x where
+// its rows have to be copied to ones that start on 16 bytes: `own`, the next `scaling` and all other workgroups. There are M rows of x to copy:
+// none where x is read in place, and none for the workgroups that a launch of more than 2^22 has too many. A thread takes AT pieces of eight
+// values, whose loads are on their way together. Bound by memory: 4096-11264 (116 MB) 25.5 us, 4.5 TB/s.
 template <typename T, bool ZERO, int AT>
-__global__ __launch_bounds__(256) void unpack_kernel(Weights4<T> w, int shift, T* to, int64_t pitch, uint32_t groups, uint32_t own,
-                                                     Side<T> x, int64_t M, T* x_to) {
+__global__ __launch_bounds__(256) void unpack_kernel(Weights4<T> w, int shift, T* to, int64_t pitch, float* scale_to, uint32_t scale_pitch,
+                                                     uint32_t groups, uint32_t own, uint32_t scaling, Side<T> x, int64_t M, T* x_to) {
   uint32_t block = block_index();
+  if (block >= own && block - own < scaling) {
+    const int64_t first = (int64_t)(block - own) * 256, g0 = first / scale_pitch;
+    const uint32_t at = (uint32_t)(first - g0 * scale_pitch) + threadIdx.x, down = at / scale_pitch;
+    const int64_t g = g0 + down, m = at - down * scale_pitch;
+    if (g < w.groups && m < w.rows) scale_to[g * scale_pitch + m] = (float)w.scale[m * w.lds + g];
+    return;
+  }
   const bool copies = block >= own;
-  if (copies) block -= own;
+  if (copies) block -= own + scaling;
   const int64_t first = (int64_t)block * (256 * AT) + threadIdx.x, m0 = first / groups;
   const uint32_t start = (uint32_t)(first - m0 * groups);
   if (copies) {
@@ -460,7 +472,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(Weights4<T> w, int shift, T
     return;
   }
   uint32_t word[AT];
-  float s[AT], z[AT];
+  float z[AT];
   int64_t to_at[AT];
   int left[AT];
 #pragma unroll
@@ -468,7 +480,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(Weights4<T> w, int shift, T
     const uint32_t at = start + i * 256, down = i ? at / groups : 0;
     const bool there = m0 + down < w.rows;
     const int64_t m = there ? m0 + down : w.rows - 1;
-    const int n = (int)(at - down * groups) * 8, g = n >> shift;
+    const int n = (int)(at - down * groups) * 8;
     const uint8_t* q = w.q + m * w.ldq + n / 2;
     word[i] = 0;
     if (n + 8 <= w.cols) {
@@ -478,7 +490,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(Weights4<T> w, int shift, T
       for (int j = 0; j < 4; j++)
         if (n + 2 * j < w.cols) word[i] |= (uint32_t)q[j] << (8 * j);
     }
-    s[i] = (float)w.scale[m * w.lds + g], z[i] = ZERO ? (float)w.zero[m * w.ldz + g] : 8.f;
+    z[i] = ZERO ? (float)w.zero[m * w.ldz + (n >> shift)] : 8.f;
     to_at[i] = m * pitch + n;
     left[i] = there ? w.cols - n : 0;
   }
@@ -486,10 +498,27 @@ __global__ __launch_bounds__(256) void unpack_kernel(Weights4<T> w, int shift, T
   for (int i = 0; i < AT; i++) {
     vec<T, 8> v;
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = j < left[i] ? (T)(((float)(word[i] >> (4 * j) & 15) - z[i]) * s[i]) : (T)0.f;
+    for (int j = 0; j < 8; j++) v[j] = j < left[i] ? (T)(((float)(word[i] >> (4 * j) & 15) - z[i]) * kWhole<T>) : (T)0.f;
     if (left[i] > 0) *reinterpret_cast<vec<T, 8>*>(to + to_at[i]) = v;
   }
 }
+
+// y from the tiles' sums
+template <typename T, int N>
+struct Q4Out {
+  static constexpr int GROUPS = N;
+  GroupScales scales;
+  T* y;
+  int64_t ldy;
+  int cols;
+  template <int W>
+  __device__ __forceinline__ void operator()(uint32_t, int64_t m, int n, const float (&acc)[W]) const {
+    float v[W];
+#pragma unroll
+    for (int j = 0; j < W; j++) v[j] = acc[j] * (1.f / kWhole<T>);
+    put<W>(y, ldy, m, n, cols, v);
+  }
+};
 
 // ---- host --------------------------------------------------------------------------------------------------
 
@@ -543,8 +572,9 @@ int outputs_of(const b2c_q4_linear_args* a) {
   return tiles <= 768 && a->rows <= 16 ? 3 : 4;
 }
 // Whether the weights are multiplied as codes: up to 32 rows; with more, 64 to a workgroup, where that takes less time than to unpack them for
-// the tiles. A workgroup reads all of its rows of x, and what a compute unit may have on its way from the die's cache bounds that: 64 rows of
-// 4096 -> 4096, 11264 and 1024 -> 8192 take 19, 27 and 8 us this way, 25, 45 and 17 by tiles; 128 of 4096 -> 4096 35 and 28.
+// the tiles, from 64 products timed both ways. A workgroup reads all of its rows of x, and what a compute unit may have on its way from the
+// die's cache bounds that: 128 rows of 1024 -> 8192 and 256 of 2048 -> 2048 and 1024 -> 8192 take 13, 20 and 24 us this way, 18, 27 and 29 by
+// tiles; but 128 of 4096 -> 4096 35 and 31, 256 of 4096 -> 11264 78 and 62, 512 of 2048 -> 2048 36 and 28.
 bool few(const b2c_q4_linear_args* a) {
   if (a->rows <= 32) return true;
   if (a->rows > 512) return false;
@@ -552,21 +582,24 @@ bool few(const b2c_q4_linear_args* a) {
   const int64_t blocks = up(a->rows, 64) / 64 * (up(a->d_out, 16 * n) / (16 * n));
   const double weights = (double)a->d_in * a->d_out;
   const double codes = 3 + (double)(up(blocks, 256) / 256) * a->d_in * (0.0033 + 0.0007 * n);
-  return codes < 11 + weights * 0.55e-6 + weights * (double)a->rows * 2e-9;
+  return codes < 19 + weights * 0.45e-6 + weights * (double)a->rows * 2e-9;
 }
 
 template <typename T>
 struct Q4Plan {
   T *w = nullptr, *x = nullptr;
-  int64_t pitch = 0;
+  float* scales = nullptr;
+  int64_t pitch = 0, scale_pitch = 0;
   Way way{};
   void* sums = nullptr;
   Q4Plan(const b2c_q4_linear_args* a, Room& room) {
     if (few(a)) return;
     pitch = up(a->d_in, 64);
     w = room.take<T>(a->d_out * pitch);
+    scale_pitch = up(a->d_out, 128);
+    scales = room.take<float>(groups_of(a->d_in, a->group) * scale_pitch);
     if (!direct(a)) x = room.take<T>(a->rows * pitch);
-    way = choose({{a->rows, a->d_out}}, pitch / 64, false, false);
+    way = choose({{a->rows, a->d_out}}, pitch / 64, false, false, 2, TILE_128);
     sums = room.take<char>(way.sums);
   }
 };
@@ -629,9 +662,11 @@ int linear(const b2c_q4_linear_args* a, hipStream_t stream) {
   const uint32_t pieces = (uint32_t)(up(a->d_in, 8) / 8);
   auto unpack = [&](auto zero, auto at) -> int {
     const int64_t block = 256 * at.value, own = up((int64_t)a->d_out * pieces, block) / block, copies = p.x ? up(a->rows * pieces, block) / block : 0;
-    if (own + copies > 0x7fffffff) return hipErrorInvalidValue;
+    const int64_t scaling = up(w.groups * p.scale_pitch, 256) / 256;
+    if (own + scaling + copies > 0x7fffffff) return hipErrorInvalidValue;
     unpack_kernel<T, zero.value, at.value>
-        <<<grid_of(own + copies), 256, 0, stream>>>(w, shift, p.w, p.pitch, pieces, (uint32_t)own, x, p.x ? a->rows : 0, p.x);
+        <<<grid_of(own + scaling + copies), 256, 0, stream>>>(w, shift, p.w, p.pitch, p.scales, (uint32_t)p.scale_pitch, pieces,
+                                                              (uint32_t)own, (uint32_t)scaling, x, p.x ? a->rows : 0, p.x);
     return hipGetLastError();
   };
   // Four pieces a thread where that leaves workgroups enough: 4096-11264 25.5 us, 30 with one; 1000-1000 5.1 and 4.0, 2050-5001 9.9 and 9.0.
@@ -642,9 +677,12 @@ int linear(const b2c_q4_linear_args* a, hipStream_t stream) {
   const int rc = a->zero ? with_zero(std::true_type{}) : with_zero(std::false_type{});
   if (rc) return rc;
   if (p.x) x = {p.x, p.pitch};
-  const RowsOut<T> out{(T*)a->y, a->ldy, nullptr, 0, a->d_out, {}};
   const Product<T> product_of{x, {p.w, p.pitch}, {}, {}, a->rows, a->d_out, a->d_in, 0, a->rows, a->d_out};
-  return product<T, false, false, false, false>(product_of, p.way, p.sums, out, stream);
+  const GroupScales scales{p.scales, p.scale_pitch, shift};
+  auto tiles = [&](auto groups) {
+    return product<T, false, false, false, false>(product_of, p.way, p.sums, Q4Out<T, groups.value>{scales, (T*)a->y, a->ldy, a->d_out}, stream);
+  };
+  return a->group == 32 ? tiles(std::integral_constant<int, 2>{}) : tiles(std::integral_constant<int, 1>{});
 }
 
 }  // namespace

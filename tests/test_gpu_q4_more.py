@@ -3,7 +3,11 @@ import numpy as np
 import pytest
 
 from b2ctrain_amd import nn
+from tests import dense_util as U
+from tests import more_util as V
+from tests import precision as P
 from tests.gpu_harness import emit
+from tests.test_gpu_q4 import Bytes
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +48,18 @@ def test_more_than_four_million_workgroups_of_weights():
     finally:
         del p, x, q, s, y
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows", [1, 5, 17, 32, 33, 64, 200, 520, 700])
+@pytest.mark.parametrize("k,n", [(4096, 600), (2050, 1040), (515, 900), (128, 2048)])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True), (256, False)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_products_are_as_exact_as_their_outputs(rows, k, n, group, zeros, dtype):
+    """Whatever the number of rows: weights of whole numbers and scales are nowhere rounded to 16 bits."""
+    emit(f"q4 linear {rows} x {k}-{n} by {group} zeros {zeros} type {dtype}")
+    x, code, scale, zero, w = P.weights4(rows, k, n, group, zeros, dtype)
+    hx, hs, hw, hz, y = U.Held(x, dtype), U.Held(scale, dtype), Bytes(V.packed(code)), Bytes(zero), U.Held(None, dtype, rows=rows, cols=n)
+    space = U.Space()
+    nn.Q4Linear(hx.matrix, hw.matrix, hs.matrix, y.matrix, group, zero=hz.matrix if zeros else None, room=space).run()
+    assert P.excess(y.get(), x @ w.T, dtype) < (P.MOST if rows * n > 2000 else 1.2)
+    space.check()
