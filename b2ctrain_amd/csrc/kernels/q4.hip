@@ -109,19 +109,20 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
 
 // ---- products ----------------------------------------------------------------------------------------------
 
-// A code c of 4 bits becomes the 16-bit float BASE + c by taking its place among the mantissa's bits of BASE, two to a register: no
-// conversion. The eight codes of a word, in their order.
+// A code c of 4 bits becomes the 16-bit float (BASE + c) UNIT by taking its place among the mantissa's bits of BASE UNIT, two to a register: no
+// conversion. UNIT is a power of two small enough that a group's sum of up to 128 (BASE + c) x, c up to 15, stays within single precision's
+// range whatever numbers x holds. The eight codes of a word, in their order.
 template <typename T>
 struct Codes;
 template <>
 struct Codes<bf16> {
-  static constexpr float BASE = 128.f;  // 0x4300: the lowest mantissa bit counts 1
-  static __device__ __forceinline__ uint32_t two(uint32_t t) { return (t & 0x000f000fu) | 0x43004300u; }
+  static constexpr float BASE = 128.f, UNIT = 0x1p-15f;  // 0x3b80: the lowest mantissa bit counts 1 UNIT
+  static __device__ __forceinline__ uint32_t two(uint32_t t) { return (t & 0x000f000fu) | 0x3b803b80u; }
   static __device__ __forceinline__ uint32_t spread(uint32_t a) { return a << 12 | a; }
 };
 template <>
 struct Codes<f16> {
-  static constexpr float BASE = 64.f;  // 0x5400: bit 4 counts 1
+  static constexpr float BASE = 64.f, UNIT = 1.f;  // 0x5400: bit 4 counts 1
   static __device__ __forceinline__ uint32_t two(uint32_t t) { return (t & 0x00f000f0u) | 0x54005400u; }
   static __device__ __forceinline__ uint32_t spread(uint32_t a) { return a << 16 | a << 4; }
 };
@@ -173,7 +174,8 @@ __device__ __forceinline__ void turn4(vec<uint32_t, 4>& v) {
 }
 // At most 16 MT rows of x. A workgroup takes 16 NT outputs, its eight waves every eighth run of 128 values of k: sixteen bytes of a row a
 // lane, turned so that each matrix instruction meets 32 neighbouring values of k, which are of one group. With c the code and B its base, a
-// group's sum is s (sum (B + c) x - (B + z) sum x), and sum x comes from the same instruction against ones, in the same lanes. B is at most
+// group's sum is s (sum (B + c) x - (B + z) sum x), and sum x comes from the same instruction against ones, in the same lanes, all of it in
+// units of UNIT. B is at most
 // 128, so that the difference costs four bits of the 24 that the sums are held in. Rows beyond the last read the last one's values, which
 // nobody stores; in the run at the end of k (not the first: LONG) every load that would pass a row's end reads its last bytes, which are then
 // moved to their place, so that no load waits for a condition (7 rows of 2050-5001: 3 us less). The waves' sums meet in LDS and are added
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void q4_few_kernel(Weights4<T
   const T* px[MT];
 #pragma unroll
   for (int t = 0; t < MT; t++) px[t] = x.p + (t * 16 + row < M ? t * 16 + row : M - 1) * x.ld;
-  const T one = (T)1.f;
+  const T one = (T)Codes<T>::UNIT;
   const vec<T, 8> ones = {one, one, one, one, one, one, one, one};
   struct Run {
     vec<uint32_t, 4> q[NT];
@@ -338,7 +340,7 @@ __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void q4_few_kernel(Weights4<T
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const int m = tm * 16 + q4 * 4 + j;
-      if (m < M && n < w.rows) y[m * ldy + n] = (T)v[j];
+      if (m < M && n < w.rows) y[m * ldy + n] = (T)(v[j] * (1.f / Codes<T>::UNIT));
     }
   }
 }
@@ -406,7 +408,7 @@ __global__ __launch_bounds__(256, 4) void q4_one_kernel(Weights4<T> w, int shift
         vec<T, 8> v{};
         if (k + j * 8 < K) v = some<T, 8>(x, k + j * 8, K);
 #pragma unroll
-        for (int e = 0; e < 8; e++) s += (float)v[e];
+        for (int e = 0; e < 8; e++) s = fmaf((float)v[e], Codes<T>::UNIT, s);
         const vec<T, 8> apart = {v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
         held[i * 4 + (j ^ (i >> 2 & 3))] = __builtin_bit_cast(vec<uint32_t, 4>, apart);  // turned: eight lanes' pieces in different banks
       }
@@ -434,7 +436,7 @@ __global__ __launch_bounds__(256, 4) void q4_one_kernel(Weights4<T> w, int shift
   if (part || lane >= 4 || n0 + lane >= w.rows) return;
   float v = parts[wave][lane];
   for (int p = 1; p < split; p++) v += parts[wave + p][lane];
-  y[n0 + lane] = (T)v;
+  y[n0 + lane] = (T)(v * (1.f / Codes<T>::UNIT));
 }
 
 // What the whole numbers code - zero count in the tiles' weights, a power of two, so that 16 bits hold them exactly: as little as keeps the sum

@@ -784,9 +784,8 @@ typedef struct b2c_quantize4_args {
 int b2c_hip_quantize4(const b2c_quantize4_args* a, hipStream_t stream);
 
 /* y = x w^T with w held as above: w[j][k] = (code - zero) scale, zero = 8 where there are none. Each group's sum is formed from whole
- * numbers, which 16 bits hold exactly, and then scaled, in single precision, so that y is off by hardly more than its own rounding. With few
- * rows (up to 32, and up to 512 where that is faster) the whole numbers are the codes, and their sums hold up to 144 times the values of x:
- * where that passes single precision's range, and with an infinity in x, a row of y becomes NaN.
+ * numbers, which 16 bits hold exactly, and then scaled, in single precision, so that y is off by hardly more than its own rounding, whatever
+ * finite values x holds. A row of x with an infinity or NaN in it gives a row of y of infinities and NaN.
  * rows at most 2^30, widths at most 2^20; rows of w, scale and zero lie at most 2^25 apart. */
 typedef struct b2c_q4_linear_args {
   int64_t rows;

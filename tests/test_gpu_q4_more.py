@@ -7,6 +7,7 @@ from tests import dense_util as U
 from tests import more_util as V
 from tests import precision as P
 from tests.gpu_harness import emit
+from tests.test_gpu_dense import close
 from tests.test_gpu_q4 import Bytes
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +64,61 @@ def test_products_are_as_exact_as_their_outputs(rows, k, n, group, zeros, dtype)
     nn.Q4Linear(hx.matrix, hw.matrix, hs.matrix, y.matrix, group, zero=hz.matrix if zeros else None, room=space).run()
     assert P.excess(y.get(), x @ w.T, dtype) < (P.MOST if rows * n > 2000 else 1.2)
     space.check()
+
+
+def product(x, dtype, group, zeros, n=70, size=1.0, seed=3):
+    """y of x and weights of about `size` each, those weights' codes, scales and zero points, and whether x goes by codes."""
+    g = np.random.default_rng(seed)
+    rows, k = x.shape
+    code, m = g.integers(0, 16, (n, k)).astype(np.uint8), V.groups(k, group)
+    scale = U.rounded((0.5 + g.random((n, m))) * size, dtype)
+    zero = g.integers(0, 16, (n, m)).astype(np.uint8) if zeros else np.full((n, m), 8, np.uint8)
+    hx, hs, hw, hz, y = U.Held(x, dtype), U.Held(scale, dtype), Bytes(V.packed(code)), Bytes(zero), U.Held(None, dtype, rows=rows, cols=n)
+    p = nn.Q4Linear(hx.matrix, hw.matrix, hs.matrix, y.matrix, group, zero=hz.matrix if zeros else None, room=U.Space())
+    p.run()
+    return y.get(), code, scale, zero, p.args.workspace_bytes == 0
+
+
+@pytest.mark.parametrize("rows", [1, 5, 20, 40, 600])
+@pytest.mark.parametrize("k", [40, 300, 2048, 4100])
+@pytest.mark.parametrize("group,zeros", [(32, True), (128, False), (256, True)])
+@pytest.mark.parametrize("dtype,largest", [(BF16, 3.3e38), (F16, 65504.0)])
+def test_the_largest_values(rows, k, group, zeros, dtype, largest):
+    """Any number of x, where y is one, whatever the number of rows."""
+    emit(f"q4 linear {rows} x {k}, values of {largest}")
+    g = np.random.default_rng(rows + k)
+    x = U.rounded(g.uniform(0.5, 1, (rows, k)) * np.where(g.random((rows, k)) < 0.5, -largest, largest), dtype)
+    x[rows // 2] = abs(x[rows // 2])  # and of one sign
+    y, code, scale, zero, few = product(x, dtype, group, zeros, size=2.0 ** -10 / k)
+    close("y", y, *V.q4_linear(x, code, scale, zero, group, dtype, few))
+
+
+@pytest.mark.parametrize("rows", [1, 5, 20, 40, 600])
+@pytest.mark.parametrize("k", [40, 300, 2048, 4100])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_rows_with_infinities_or_nan(rows, k, dtype):
+    """No number of such a row of y, and the others as without."""
+    emit(f"q4 linear {rows} x {k}, not finite")
+    g = np.random.default_rng(rows + k)
+    x = U.rounded(g.standard_normal((rows, k)), dtype)
+    clean, code, scale, zero, few = product(x, dtype, 64, True, size=k ** -0.5)
+    close("y", clean, *V.q4_linear(x, code, scale, zero, 64, dtype, few))
+    bad, at = sorted({0, rows // 2}), int(g.integers(k))
+    for value in (np.inf, -np.inf, np.nan):
+        for m in bad:
+            x[m, at] = value
+        y = product(x, dtype, 64, True, size=k ** -0.5)[0]
+        assert not np.isfinite(y[bad]).any()
+        others = np.setdiff1d(np.arange(rows), bad)
+        assert np.array_equal(y[others], clean[others])
+
+
+@pytest.mark.parametrize("rows", [1, 5, 20, 40, 600])
+@pytest.mark.parametrize("k", [300, 4100])
+def test_the_smallest_normal_values(rows, k):
+    """bfloat16 down to 2^-126, by weights that make y of it about 1."""
+    g = np.random.default_rng(rows + k)
+    x = U.rounded(g.standard_normal((rows, k)) * 2.0 ** -123, BF16)
+    x[abs(x) < 2.0 ** -126] = 2.0 ** -126
+    y, code, scale, zero, few = product(x, BF16, 64, True, size=2.0 ** 110)
+    close("y", y, *V.q4_linear(x, code, scale, zero, 64, BF16, few))
