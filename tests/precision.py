@@ -30,3 +30,18 @@ def weights4(rows, k, n, group, zeros, dtype):
     zero = g.integers(5, 11, (n, m)).astype(np.uint8) if zeros else np.full((n, m), 8, np.uint8)
     wide = lambda v: np.repeat(v, group, axis=1)[:, :k].astype(np.float64)  # noqa: E731
     return x, code, scale, zero, (code - wide(zero)) * wide(scale)
+
+
+def experts(v, k, name, held=lambda h: h):
+    """y of the experts; `held`: how the inner activations are."""
+    e = len(v["wr"])
+    f, o = len(v["wg"]) // e, len(v["wd"]) // e
+    index, share = V.route(v["x"], v["wr"], k, True)
+    y = np.zeros((len(v["x"]), o))
+    for i in range(e):
+        at, slot = np.nonzero(index == i)
+        if len(at):
+            of = lambda w, n: v[w][i * n:(i + 1) * n].T  # noqa: E731
+            h = U.act(name, v["x"][at] @ of("wg", f))[0] * (v["x"][at] @ of("wu", f))
+            y[at] += share[at, slot][:, None] * (held(h) @ of("wd", o))
+    return y
