@@ -814,7 +814,8 @@ int b2c_hip_q4_linear(const b2c_q4_linear_args* a, hipStream_t stream);
  *   y = residual + sum_j p_j w_down[e_j] (act(w_gate[e_j] x) * (w_up[e_j] x))
  * The router's sums are held in 64 bits, so that the choice between experts that nearly agree does not depend on an order of
  * summation; the other products' in 32. The inner activations enter theirs as two values of dtype, the second what the first is off by:
- * together off by 2^-18 of their value in bf16, 2^-24 in f16 (or 2^-25, where that is more); beyond twice dtype's largest value they are
+ * together off by at most 2^-17 of their value in bf16, 2^-23 in f16 (or by 2^-25, where that is more). Beyond dtype's largest value the first
+ * stays there, and the second is rounded to its own 8 or 11 bits: off by up to 2^-9.5 and 2^-12.5 of the sum; beyond twice the largest they are
  * infinite. A row with a NaN or an infinite largest l gets NaN weights. Rows go 1024 / top_k at a time, and the weights are read for each
  * such lot. rows at most 2^20, widths at most 2^20, experts at most 1024, top_k at most 64, and all of a weight's rows (experts times
  * width) less than 2^31; rows of w_gate, w_up and w_down lie at most 2^25 apart. y may be residual (same pointer and ld). */
