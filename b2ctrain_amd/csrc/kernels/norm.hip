@@ -106,7 +106,7 @@ struct NormArgs {
   int64_t rows;
   int cols;
   bool centre, post, sigmoid, w_f32;
-  float eps, scale, inv_cols;
+  float eps, scale, inv_cols, part, of_parts;  // part: a power of two of at most one over the columns; of_parts part = inv_cols
   const void *x, *r, *g, *w_post, *w_pre;
   int64_t ldx, ldr, ldg;
   uint32_t per_gate;
@@ -114,32 +114,62 @@ struct NormArgs {
   int64_t ldy, ldn;
 };
 
-// norm(v) in `u`; returns one over its size.
-template <int LANES, int C, int E>
+// norm(v) in `u`; returns one over its size. The sums for a mean are of the values times `part`, so that they stay in range as the row does.
+// Rows whose squares pass single precision's range, and small ones with next to no eps, are multiplied by a power of two and summed again: TIGHT
+// in a loop, whose code stands once, else behind a branch. The loop keeps the largest teams' gradients from spilling (with the branch bf16
+// 2000 x 5001 takes 113 us, 64 with the loop, f32 2048 x 8192 113 and 94), and costs others time (forward a million rows of 64 99 and 105).
+template <bool TIGHT, int LANES, int C, int E>
 __device__ __forceinline__ float normalise(const NormArgs& a, Team<LANES>& team, float (&room)[2][16], int first, float (&u)[C][E]) {
   if (a.centre) {
     float s = 0;
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
-      for (int j = 0; j < E; j++) s += u[c][j];
-    const float mean = team.sum(s, room) * a.inv_cols;
+      for (int j = 0; j < E; j++) s = fmaf(u[c][j], a.part, s);
+    const float mean = team.sum(s, room) * a.of_parts;
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
       for (int j = 0; j < E; j++) u[c][j] = first + c * LANES * E + j < a.cols ? u[c][j] - mean : 0.f;
   }
-  float s = 0;
+  auto squares = [&] {
+    float s = 0;
 #pragma unroll
-  for (int c = 0; c < C; c++)
+    for (int c = 0; c < C; c++)
 #pragma unroll
-    for (int j = 0; j < E; j++) s = fmaf(u[c][j], u[c][j], s);
-  const float size = rsqrtf(fmaf(team.sum(s, room), a.inv_cols, a.eps));
+      for (int j = 0; j < E; j++) s = fmaf(u[c][j], u[c][j], s);
+    return team.sum(s, room);
+  };
+  auto times = [&](float by) {
 #pragma unroll
-  for (int c = 0; c < C; c++)
+    for (int c = 0; c < C; c++)
 #pragma unroll
-    for (int j = 0; j < E; j++) u[c][j] *= size;
-  return size;
+      for (int j = 0; j < E; j++) u[c][j] *= by;
+  };
+  float s, by = 1.f, eps = a.eps;
+  auto beyond = [&] { return !(s < __builtin_inff()) || (s < 0x1p-96f && eps < 0x1p-80f); };  // the whole team's answer
+  auto scale = [&] {
+    by = s < 1.f ? 0x1p100f : 0x1p-72f;
+    eps = eps * by * by;
+    times(by);
+  };
+  if constexpr (TIGHT) {
+#pragma unroll 1
+    for (;;) {
+      s = squares();
+      if (by != 1.f || !beyond()) break;
+      scale();
+    }
+  } else {
+    s = squares();
+    if (beyond()) {
+      scale();
+      s = squares();
+    }
+  }
+  const float size = rsqrtf(fmaf(s, a.inv_cols, eps));
+  times(size);
+  return size * by;
 }
 
 // A row's pieces, where the matrix is given.
@@ -185,7 +215,7 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_kernel(NormArgs a) 
     for (int c = 0; c < C; c++)
 #pragma unroll
       for (int j = 0; j < E; j++) u[c][j] = (float)x[c][j];
-    if (a.post) normalise<LANES, C, E>(a, team, room, first, u);
+    if (a.post) normalise<false>(a, team, room, first, u);
 #pragma unroll
     for (int c = 0; c < C; c++) {
 #pragma unroll
@@ -196,7 +226,7 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_kernel(NormArgs a) 
       if (a.y) put_piece<E, END>((T*)a.y + m * a.ldy, first + c * LANES * E, a.cols, there, u[c]);
     }
     if (!a.n) continue;
-    normalise<LANES, C, E>(a, team, room, first, u);
+    normalise<false>(a, team, room, first, u);
 #pragma unroll
     for (int c = 0; c < C; c++) {
 #pragma unroll
@@ -270,11 +300,10 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
   Team<LANES> team;
   const int first = (threadIdx.x % LANES) * E, mine = threadIdx.x / LANES;
   const bool writes = LANES > 64 || threadIdx.x < LANES;  // what gather() leaves
-  // The largest teams have 128 registers a thread, which the row itself takes. Their weights are read again for each row, and the sums of
-  // the weights' gradients stay in LDS, each thread's own, where that is faster (us with it and without, plain norms: bf16 2048 x 8192 81
-  // and 93, 2000 x 6000 66 and 79, 1000 x 16384 145 and 191; f32 600 x 16384 163 and 184; but bf16 2000 x 5001 83 and 70, f32 2048 x 8192
-  // 110 and 100, 2048 x 4096 45 and 41).
-  constexpr bool WIDE = LANES == 1024 && (E == 8 ? END == WHOLE || C > 1 : C > 2);
+  // The largest teams have 128 registers a thread. Where it holds sixteen of a row's values, they take all of them: the weights are read again
+  // for each row, and the sums of their gradients stay in LDS, each thread's own (us so and in registers: bf16 1000 x 16384 139 and 176, f32
+  // 600 x 16384 136 and 152; with eight values bf16 2048 x 8192 72 and 63, 2000 x 5001 73 and 64, f32 2048 x 8192 101 and 93).
+  constexpr bool WIDE = C * E > 8;
   __shared__ float held[2][WIDE ? C * E * LANES : 1];
   float wa[C][E], wb[C][E], sa[C][E] = {}, sb[C][E] = {};
   if constexpr (WIDE) {
@@ -336,7 +365,7 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
           u[c][j] = (float)w.x[c][j];
           d[c][j] = (float)w.dy[c][j];
         }
-      if (a.post) size_x = normalise<LANES, C, E>(a, team, room, first, u);
+      if (a.post) size_x = normalise<LANES == 1024>(a, team, room, first, u);
       if constexpr (WIDE) {
 #pragma unroll
         for (int c = 0; c < C; c++) weights<E, T>(a.w_post, a.w_f32, first + c * LANES * E, a.cols, wa[c]);
@@ -352,7 +381,7 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
         for (int c = 0; c < C; c++)
 #pragma unroll
           for (int j = 0; j < E; j++) v[c][j] = fmaf(a.scale * gate[c][j], u[c][j] * wa[c][j], (float)w.r[c][j]);
-        const float size = normalise<LANES, C, E>(a, team, room, first, v);
+        const float size = normalise<LANES == 1024>(a, team, room, first, v);
         if constexpr (WIDE) {
 #pragma unroll
           for (int c = 0; c < C; c++) weights<E, T>(a.w_pre, a.w_f32, first + c * LANES * E, a.cols, wb[c]);
@@ -530,8 +559,10 @@ bool inputs_ok(const b2c_block_norm_args* a) {
 
 NormArgs to_device(const b2c_block_norm_args* a) {
   const int64_t per = a->gate ? std::min<int64_t>(a->rows_per_gate, 1 << 30) : 1;
+  float part = 1.f;
+  while (part * (float)a->cols > 1.f) part *= 0.5f;
   return {a->rows, a->cols, a->kind == B2C_NORM_LAYER, a->post != 0, a->gate && a->gate_act == B2C_GATE_SIGMOID, a->w_dtype == B2C_F32,
-          a->eps, a->x ? a->scale : 0.f, 1.f / (float)a->cols, a->x, a->residual, a->gate, a->w_post, a->w_pre, a->ldx, a->ldr, a->ldg, (uint32_t)per,
+          a->eps, a->x ? a->scale : 0.f, 1.f / (float)a->cols, part, 1.f / (part * (float)a->cols), a->x, a->residual, a->gate, a->w_post, a->w_pre, a->ldx, a->ldr, a->ldg, (uint32_t)per,
           a->y, a->n, a->ldy, a->ldn};
 }
 

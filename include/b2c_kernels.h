@@ -702,9 +702,9 @@ int b2c_hip_i8_ffn(const b2c_i8_ffn_args* a, hipStream_t stream);
  * norm before the next block:
  *   t = norm(x) * w_post (or x itself without `post`);  y = residual + scale * act(gate) * t;  n = norm(y) * w_pre
  * norm(v) = v / sqrt(mean v^2 + eps), or (v - mean v) / sqrt(mean (v - mean v)^2 + eps), over a row's columns. n is formed from y
- * before y is rounded. Without x, y is the residual (no gate, no `post`) and n its norm. Statistics are held in single precision, in
- * which squares overflow beyond 1.8e19. y may be residual and n may be x (same pointer and ld). rows at most 2^30, cols at most
- * 16384. */
+ * before y is rounded. Without x, y is the residual (no gate, no `post`) and n its norm. Statistics are held in single precision; a
+ * finite row has its norm whatever its size (of a layer norm, as long as its differences from the mean are finite). y may be residual
+ * and n may be x (same pointer and ld). rows at most 2^30, cols at most 16384. */
 enum { B2C_NORM_RMS = 0, B2C_NORM_LAYER = 1 };
 enum { B2C_GATE_NONE = 0, B2C_GATE_SIGMOID = 1 }; /* act(gate): the gate itself; 1 / (1 + e^-gate) */
 typedef struct b2c_block_norm_args {

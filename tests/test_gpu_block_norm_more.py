@@ -90,3 +90,47 @@ def test_wide_rows_that_end_inside_a_piece(d, dtype):
 @pytest.mark.parametrize("per", [0, 13, 350])
 def test_more_wide_rows_than_workgroups(d, dtype, per):
     check(700, d, dtype, F32, per=per, act="sigmoid" if per else "none")
+
+
+def norms_of(u, dtype, kind, eps, gate=None):
+    """norm(u) and its gradient of dn, on the GPU and in 64 bits."""
+    rows, d = u.shape
+    g = np.random.default_rng(rows + d)
+    dn = U.rounded(g.standard_normal((rows, d)), dtype)
+    hx, hn, n, dx = U.Held(u, dtype), U.Held(dn, dtype), U.Held(None, dtype, rows=rows, cols=d), U.Held(None, dtype, rows=rows, cols=d)
+    p = nn.BlockNorm(residual=hx.matrix, n=n.matrix, kind=kind, eps=eps)
+    p.gradients(dn=hn.matrix, dresidual=dx.matrix, room=U.Space())
+    p.forward()
+    p.backward()
+    mean = lambda v: v.mean(axis=1, keepdims=True)  # noqa: E731
+    c = u - mean(u) if kind == "layer" else u
+    size = 1 / np.sqrt(mean(c * c) + float(np.float32(eps)))
+    v = c * size
+    back = dn - v * mean(dn * v) - (mean(dn) if kind == "layer" else 0)
+    return (n.get(), v), (dx.get(), size * back, size * (abs(dn) + abs(v) + 1))
+
+
+@pytest.mark.parametrize("d", [3, 33, 64, 200, 520, 1500, 4096, 5001, 16384])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("size", [1e17, 1.7e19, 3e19, 1e25, 3e37])
+def test_rows_whose_squares_pass_the_range(d, dtype, kind, size):
+    """A finite row has its norm, whatever its size, and the gradients that go with it."""
+    emit(f"norm of rows of {d} values of about {size}, type {dtype} {kind}")
+    u = U.rounded(np.random.default_rng(d).standard_normal((40, d)) * size * np.logspace(-0.4, 0.4, 40)[:, None], dtype)
+    u[7] = U.rounded(np.random.default_rng(1).standard_normal(d), dtype)  # and an ordinary row among them
+    u[9], u[9, d // 2] = 0, u[10, 0]
+    (n, v), (dx, back, terms) = norms_of(u, dtype, kind, 1e-6)
+    # statistics to 2^-18 of themselves at most, at the widths here, outputs rounded once; a layer norm's differences are of rounded means
+    close("n", n, v, U.UNIT[dtype] * abs(v) + 2.0 ** -18 * (abs(v) + 1))
+    close("dresidual", dx, back, U.UNIT[dtype] * abs(back) + 2.0 ** -16 * terms + 2.0 ** -133)
+
+
+@pytest.mark.parametrize("d", [3, 64, 520, 4096, 5001])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [1e-12, 1e-19, 1e-24, 1e-36])
+def test_small_rows_without_eps(d, dtype, size):
+    emit(f"norm of rows of {d} values of about {size}, type {dtype}")
+    u = U.rounded(np.random.default_rng(d).standard_normal((40, d)) * size, dtype)
+    (n, v), _ = norms_of(u, dtype, "rms", 0.0)
+    close("n", n, v, U.UNIT[dtype] * abs(v) + 2.0 ** -18 * (abs(v) + 1))
