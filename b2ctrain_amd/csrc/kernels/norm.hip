@@ -179,7 +179,25 @@ __device__ __forceinline__ void read(vec<T, E> (&v)[C], const void* p, int64_t a
 #pragma unroll
   for (int c = 0; c < C; c++) v[c] = piece<E, END>((const T*)p + at, first + c * LANES * E, cols);
 }
-__device__ __forceinline__ float gate_of(bool sigmoid, float g) { return sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-g)) : g; }
+// act(gate). Of 16-bit gates by the hardware's approximations, which are off by 2^-22, and by |g| 2^-24 for the exponential's argument.
+template <typename T>
+__device__ __forceinline__ float act_of(bool sigmoid, float g) {
+  if (!sigmoid) return g;
+  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-g));
+  return __builtin_amdgcn_rcpf(1.f + __expf(-g));
+}
+// A gate as the gradients keep it: itself, or, of a sigmoid, the smaller of it and what it is short of one, with a sign bit where that is the
+// second, so that neither cancels in its slope, their product.
+template <typename T>
+__device__ __forceinline__ float kept_gate(bool sigmoid, float g) {
+  if (!sigmoid) return g;
+  const float small = act_of<T>(true, -fabsf(g));
+  return g < 0.f ? small : -small;
+}
+__device__ __forceinline__ float gate_of(bool sigmoid, float kept) {
+  return sigmoid && __builtin_bit_cast(int, kept) < 0 ? 1.f + kept : kept;
+}
+__device__ __forceinline__ float slope_of(bool sigmoid, float kept) { return sigmoid ? fabsf(kept) * (1.f - fabsf(kept)) : 1.f; }
 
 // Both norms of a row from registers: t = u / size(u), y = r + scale gate t w_post, n = y / size(y) w_pre, with y as it was before it was
 // rounded; the sums of layer norms are of differences from the mean, in a second pass over registers. Bound by memory: 8192 rows of 4096
@@ -220,7 +238,7 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_kernel(NormArgs a) 
     for (int c = 0; c < C; c++) {
 #pragma unroll
       for (int j = 0; j < E; j++) {
-        const float gate = a.g ? gate_of(a.sigmoid, (float)g[c][j]) : 1.f;
+        const float gate = a.g ? act_of<T>(a.sigmoid, (float)g[c][j]) : 1.f;
         u[c][j] = fmaf(a.scale * gate, u[c][j] * wa[c][j], (float)r[c][j]);  // without x: the residual, since u is 0
       }
       if (a.y) put_piece<E, END>((T*)a.y + m * a.ldy, first + c * LANES * E, a.cols, there, u[c]);
@@ -374,13 +392,13 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
 #pragma unroll
       for (int c = 0; c < C; c++)
 #pragma unroll
-        for (int j = 0; j < E; j++) gate[c][j] = a.g ? gate_of(a.sigmoid, (float)w.g[c][j]) : 1.f;
+        for (int j = 0; j < E; j++) gate[c][j] = a.g ? kept_gate<T>(a.sigmoid, (float)w.g[c][j]) : 1.f;
       if (b.dn) {
         float v[C][E];
 #pragma unroll
         for (int c = 0; c < C; c++)
 #pragma unroll
-          for (int j = 0; j < E; j++) v[c][j] = fmaf(a.scale * gate[c][j], u[c][j] * wa[c][j], (float)w.r[c][j]);
+          for (int j = 0; j < E; j++) v[c][j] = fmaf(a.scale * gate_of(a.sigmoid, gate[c][j]), u[c][j] * wa[c][j], (float)w.r[c][j]);
         const float size = normalise<LANES == 1024>(a, team, room, first, v);
         if constexpr (WIDE) {
 #pragma unroll
@@ -415,10 +433,7 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
 #pragma unroll
         for (int c = 0; c < C; c++)
 #pragma unroll
-          for (int j = 0; j < E; j++) {
-            dg[c][j] = a.scale * d[c][j] * (u[c][j] * wa[c][j]);
-            if (a.sigmoid) dg[c][j] *= gate[c][j] * (1.f - gate[c][j]);
-          }
+          for (int j = 0; j < E; j++) dg[c][j] = a.scale * d[c][j] * (u[c][j] * wa[c][j]) * slope_of(a.sigmoid, gate[c][j]);
 #pragma unroll
         for (int c = 0; c < C; c++) {
           if (b.shared) {
@@ -432,7 +447,11 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
 #pragma unroll
       for (int c = 0; c < C; c++)
 #pragma unroll
-        for (int j = 0; j < E; j++) d[c][j] *= a.scale * gate[c][j];
+        for (int j = 0; j < E; j++) {
+          float kept = gate[c][j];
+          asm("" : "+v"(kept));  // formed again: the compiler would hold the gate from its first use on, beside what it is kept as
+          d[c][j] *= a.scale * gate_of(a.sigmoid, kept);
+        }
       if (a.post) {
         float along = 0, mean = 0;
 #pragma unroll

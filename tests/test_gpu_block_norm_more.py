@@ -134,3 +134,29 @@ def test_small_rows_without_eps(d, dtype, size):
     u = U.rounded(np.random.default_rng(d).standard_normal((40, d)) * size, dtype)
     (n, v), _ = norms_of(u, dtype, "rms", 0.0)
     close("n", n, v, U.UNIT[dtype] * abs(v) + 2.0 ** -18 * (abs(v) + 1))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("per", [1, 64])
+def test_sigmoids_far_from_zero(dtype, per):
+    """A gate of 1 / (1 + e^-g) and its slope keep their relative precision on both sides, down to the type's smallest normal values."""
+    rows, d = 64, 200
+    g = np.random.default_rng(per)
+    most = {BF16: 80, F16: 9, F32: 80}[dtype]
+    gate, x, dy = (U.rounded(v, dtype) for v in (g.uniform(-most, most, (rows // per, d)), g.uniform(1, 2, (rows, d)), g.uniform(1, 2, (rows, d))))
+    h = {k: U.Held(v, dtype) for k, v in (("x", x), ("gate", gate), ("dy", dy))}
+    y, dg = U.Held(None, dtype, rows=rows, cols=d), U.Held(None, dtype, rows=rows // per, cols=d)
+    p = nn.BlockNorm(x=h["x"].matrix, gate=h["gate"].matrix, rows_per_gate=per, gate_act="sigmoid", y=y.matrix, scale=0.5)
+    p.gradients(dy=h["dy"].matrix, dgate=dg.matrix, room=U.Space())
+    p.forward()
+    p.backward()
+    raw = np.repeat(gate, per, axis=0)
+    s, rest = 1 / (1 + np.exp(-raw)), 1 / (1 + np.exp(raw))
+    # In single precision: an exponential, a sum, a quotient, each within two units, and up to four products; sums of 64 rows six or more
+    # additions of terms of one sign. In 16 bits the exponential's argument is rounded too, and the quotient is an approximation.
+    off = (32 + (2 * abs(raw) + 32) * (dtype != F32)) * 2.0 ** -24 * np.ones_like(raw)
+    want = 0.5 * s * x
+    close("y", y.get(), want, (U.UNIT[dtype] + off) * want * 1.01)
+    terms = 0.5 * dy * x * s * rest
+    want = terms.reshape(-1, per, d).sum(axis=1)
+    close("dgate", dg.get(), want, (U.UNIT[dtype] + (off + 64 * 2.0 ** -24).max(axis=0)) * want * 1.01 + 2.0 ** -25 * (dtype == F16))
