@@ -225,8 +225,7 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_kernel(NormArgs a) 
     for (int c = 0; c < C; c++) {
       settle<E, END>(x[c], first + c * LANES * E, a.cols, true);
       settle<E, END>(r[c], first + c * LANES * E, a.cols, true);
-      if constexpr (END == RAGGED)
-        if (a.g) settle<E, END>(g[c], first + c * LANES * E, a.cols, true);
+      if (END != RAGGED || a.g) settle<E, END>(g[c], first + c * LANES * E, a.cols, true);  // an infinity times no x would be a NaN
     }
     float u[C][E];
 #pragma unroll
@@ -369,8 +368,7 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
         const int n = first + c * LANES * E;
         settle<E, END>(w.x[c], n, a.cols, true);
         settle<E, END>(w.r[c], n, a.cols, true);
-        if constexpr (END == RAGGED)
-          if (a.g) settle<E, END>(w.g[c], n, a.cols, true);
+        if (END != RAGGED || a.g) settle<E, END>(w.g[c], n, a.cols, true);
         settle<E, END>(w.dy[c], n, a.cols, there);
         settle<E, END>(w.dn[c], n, a.cols, there);
       }

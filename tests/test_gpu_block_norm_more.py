@@ -160,3 +160,29 @@ def test_sigmoids_far_from_zero(dtype, per):
     terms = 0.5 * dy * x * s * rest
     want = terms.reshape(-1, per, d).sum(axis=1)
     close("dgate", dg.get(), want, (U.UNIT[dtype] + (off + 64 * 2.0 ** -24).max(axis=0)) * want * 1.01 + 2.0 ** -25 * (dtype == F16))
+
+
+@pytest.mark.parametrize("d", [3, 8, 24, 45, 64, 200, 600, 1000, 2048, 2500, 5000, 5001, 9000, 16384])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("post", [False, True])
+def test_an_infinite_gate_makes_a_row_infinitely_large(d, dtype, post):
+    """As an infinity in x does: the other values of its norm are zeros, in every width."""
+    rows = 9
+    g = np.random.default_rng(d)
+    x, gate = (U.rounded(g.uniform(1, 2, (rows, d)), dtype) for _ in range(2))
+    at = {2: 0, 5: d // 2, 7: d - 1}
+    clean = gate.copy()
+    for m, c in at.items():
+        gate[m, c] = np.inf
+    y, n = U.Held(None, dtype, rows=rows, cols=d), U.Held(None, dtype, rows=rows, cols=d)
+    for v in (clean, gate):
+        nn.BlockNorm(x=U.Held(x, dtype).matrix, gate=U.Held(v, dtype).matrix, rows_per_gate=1, post=post, y=y.matrix, n=n.matrix).forward()
+        if v is clean:
+            want = y.get(), n.get()
+    y, n = y.get(), n.get()
+    for m, c in at.items():
+        others = np.arange(d) != c
+        assert y[m, c] == np.inf and np.array_equal(y[m, others], want[0][m, others])
+        assert np.isnan(n[m, c]) and not n[m, others].any()
+    rest = [m for m in range(rows) if m not in at]
+    assert np.array_equal(y[rest], want[0][rest]) and np.array_equal(n[rest], want[1][rest])
