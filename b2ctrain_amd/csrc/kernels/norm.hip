@@ -565,11 +565,11 @@ bool sizes_ok(const b2c_block_norm_args* a) {
   return a && a->rows >= 0 && a->rows <= (1 << 30) && a->cols >= 1 && a->cols <= 16384 && a->dtype >= B2C_F32 && a->dtype <= B2C_BF16 &&
          (a->w_dtype == a->dtype || a->w_dtype == B2C_F32) && (a->kind == B2C_NORM_RMS || a->kind == B2C_NORM_LAYER) &&
          (a->gate_act == B2C_GATE_NONE || a->gate_act == B2C_GATE_SIGMOID) && a->eps >= 0 && a->eps < __builtin_inff() &&
-         (a->x || a->residual) && (a->x || (!a->post && !a->gate)) && (!a->gate || a->rows_per_gate >= 1) && (a->post || !a->w_post);
+         (!a->gate || a->rows_per_gate >= 1) && (a->post || !a->w_post);
 }
-bool inputs_ok(const b2c_block_norm_args* a) {
+bool inputs_ok(const b2c_block_norm_args* a) {  // of some rows: those of none have no address
   const size_t s = size_of(a->dtype), w = size_of(a->w_dtype);
-  return (!a->x || good(a->x, a->ldx, a->cols, s)) && (!a->residual || good(a->residual, a->ldr, a->cols, s)) &&
+  return (a->x || a->residual) && (a->x || (!a->post && !a->gate)) && (!a->x || good(a->x, a->ldx, a->cols, s)) && (!a->residual || good(a->residual, a->ldr, a->cols, s)) &&
          (!a->gate || good(a->gate, a->ldg, a->cols, s)) && reinterpret_cast<uintptr_t>(a->w_post) % w == 0 &&
          reinterpret_cast<uintptr_t>(a->w_pre) % w == 0;
 }
@@ -727,8 +727,7 @@ extern "C" int b2c_hip_block_norm_backward(const b2c_block_norm_grad_args* b, hi
   if (!b || !sizes_ok(&b->fwd)) return hipErrorInvalidValue;
   const b2c_block_norm_args* a = &b->fwd;
   const size_t s = size_of(a->dtype), gs = size_of(b->grad_dtype);
-  if ((b->grad_dtype != a->w_dtype && b->grad_dtype != B2C_F32) || (b->accumulate && b->grad_dtype != B2C_F32) ||
-      (b->dw_post && (!a->x || !a->post)) || (b->dw_pre && !b->dn) || (b->dx && !a->x) || (b->dgate && !a->gate) ||
+  if ((b->grad_dtype != a->w_dtype && b->grad_dtype != B2C_F32) || (b->accumulate && b->grad_dtype != B2C_F32) || (b->dw_post && !a->post) ||
       reinterpret_cast<uintptr_t>(b->dw_post) % gs || reinterpret_cast<uintptr_t>(b->dw_pre) % gs)
     return hipErrorInvalidValue;
   if (a->rows == 0) {
@@ -736,7 +735,7 @@ extern "C" int b2c_hip_block_norm_backward(const b2c_block_norm_grad_args* b, hi
     clear_kernel<<<dim3((unsigned)(up(a->cols, 256) / 256)), 256, 0, stream>>>(b->dw_post, b->dw_pre, a->cols, gs == 4);
     return hipGetLastError();
   }
-  if (!inputs_ok(a) || (!b->dy && !b->dn) || (b->dy && !good(b->dy, b->lddy, a->cols, s)) || (b->dn && !good(b->dn, b->lddn, a->cols, s)) ||
+  if (!inputs_ok(a) || (b->dw_post && !a->x) || (b->dw_pre && !b->dn) || (b->dx && !a->x) || (b->dgate && !a->gate) || (!b->dy && !b->dn) || (b->dy && !good(b->dy, b->lddy, a->cols, s)) || (b->dn && !good(b->dn, b->lddn, a->cols, s)) ||
       (b->dx && !good(b->dx, b->lddx, a->cols, s)) || (b->dresidual && !good(b->dresidual, b->lddr, a->cols, s)) ||
       (b->dgate && !good(b->dgate, b->lddg, a->cols, s)))
     return hipErrorInvalidValue;

@@ -186,3 +186,16 @@ def test_an_infinite_gate_makes_a_row_infinitely_large(d, dtype, post):
         assert np.isnan(n[m, c]) and not n[m, others].any()
     rest = [m for m in range(rows) if m not in at]
     assert np.array_equal(y[rest], want[0][rest]) and np.array_equal(n[rest], want[1][rest])
+
+
+def test_tensors_of_no_rows():
+    """An empty batch's tensors have no address; the weights' gradients of it are zeros, or stay as they are."""
+    torch = pytest.importorskip("torch")
+    none = lambda: torch.empty(0, 40, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    w, dw = (torch.ones(40, dtype=torch.float32, device="cuda") for _ in range(2))
+    p = nn.BlockNorm(x=none(), residual=none(), y=none(), n=none(), post=True, w_post=w, w_pre=w)
+    p.forward(torch.cuda.current_stream().cuda_stream)
+    for accumulate in (True, False):
+        p.gradients(dy=none(), dn=none(), dx=none(), dresidual=none(), dw_post=dw, dw_pre=dw.clone(), accumulate=accumulate)
+        p.backward(torch.cuda.current_stream().cuda_stream)
+        assert dw.tolist() == [float(accumulate)] * 40
