@@ -188,14 +188,13 @@ def test_an_infinite_gate_makes_a_row_infinitely_large(d, dtype, post):
     assert np.array_equal(y[rest], want[0][rest]) and np.array_equal(n[rest], want[1][rest])
 
 
-def test_tensors_of_no_rows():
-    """An empty batch's tensors have no address; the weights' gradients of it are zeros, or stay as they are."""
-    torch = pytest.importorskip("torch")
-    none = lambda: torch.empty(0, 40, dtype=torch.bfloat16, device="cuda")  # noqa: E731
-    w, dw = (torch.ones(40, dtype=torch.float32, device="cuda") for _ in range(2))
-    p = nn.BlockNorm(x=none(), residual=none(), y=none(), n=none(), post=True, w_post=w, w_pre=w)
-    p.forward(torch.cuda.current_stream().cuda_stream)
+def test_batches_of_no_rows():
+    """An empty batch's matrices have no address; the weights' gradients of it are zeros, or stay as they are."""
+    none = lambda: nn.Matrix(0, 0, 40, 40, BF16)  # noqa: E731
+    w, dw = U.Held(np.ones((1, 40)), F32), [U.Held(np.ones((1, 40)), F32) for _ in range(2)]
+    p = nn.BlockNorm(x=none(), residual=none(), y=none(), n=none(), post=True, w_post=w.matrix, w_pre=w.matrix)
+    p.forward()
     for accumulate in (True, False):
-        p.gradients(dy=none(), dn=none(), dx=none(), dresidual=none(), dw_post=dw, dw_pre=dw.clone(), accumulate=accumulate)
-        p.backward(torch.cuda.current_stream().cuda_stream)
-        assert dw.tolist() == [float(accumulate)] * 40
+        p.gradients(dy=none(), dn=none(), dx=none(), dresidual=none(), dw_post=dw[0].matrix, dw_pre=dw[1].matrix, accumulate=accumulate)
+        p.backward()
+        assert all(np.array_equal(v.get(), np.full((1, 40), float(accumulate))) for v in dw)
