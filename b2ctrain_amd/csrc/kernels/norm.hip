@@ -116,8 +116,8 @@ struct NormArgs {
 
 // norm(v) in `u`; returns one over its size. The sums for a mean are of the values times `part`, so that they stay in range as the row does.
 // Rows whose squares pass single precision's range, and small ones with next to no eps, are multiplied by a power of two and summed again: TIGHT
-// in a loop, whose code stands once, else behind a branch. The loop keeps the largest teams' gradients from spilling (with the branch bf16
-// 2000 x 5001 takes 113 us, 64 with the loop, f32 2048 x 8192 113 and 94), and costs others time (forward a million rows of 64 99 and 105).
+// in a loop, whose code stands once, else behind a branch. The loop keeps the largest teams' gradients from spilling (bf16 2048 x 8192 takes
+// 82 us with the branch, 53 with the loop, 1000 x 16384 153 and 120), and costs others time (forward a million rows of 64 99 and 105).
 template <bool TIGHT, int LANES, int C, int E>
 __device__ __forceinline__ float normalise(const NormArgs& a, Team<LANES>& team, float (&room)[2][16], int first, float (&u)[C][E]) {
   if (a.centre) {
@@ -318,8 +318,8 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
   const int first = (threadIdx.x % LANES) * E, mine = threadIdx.x / LANES;
   const bool writes = LANES > 64 || threadIdx.x < LANES;  // what gather() leaves
   // The largest teams have 128 registers a thread. Where it holds sixteen of a row's values, they take all of them: the weights are read again
-  // for each row, and the sums of their gradients stay in LDS, each thread's own (us so and in registers: bf16 1000 x 16384 139 and 176, f32
-  // 600 x 16384 136 and 152; with eight values bf16 2048 x 8192 72 and 63, 2000 x 5001 73 and 64, f32 2048 x 8192 101 and 93).
+  // for each row, and the sums of their gradients stay in LDS, each thread's own (us so and in registers: bf16 1000 x 16384 120 and 155, f32
+  // 600 x 16384 122 and 143; with eight values bf16 2048 x 8192 64 and 53, 2000 x 5001 60 and 57, f32 2048 x 8192 101 and 94).
   constexpr bool WIDE = C * E > 8;
   __shared__ float held[2][WIDE ? C * E * LANES : 1];
   float wa[C][E], wb[C][E], sa[C][E] = {}, sb[C][E] = {};
@@ -508,7 +508,7 @@ __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGra
   }
 }
 
-// out[job][n] = the sum of `parts` rows of single-precision sums, which lie `step` apart, in a fixed order: 32 columns a workgroup, a
+// out[job][n] = the sum of `parts` rows of single-precision sums, which lie `step` apart, in 64 bits and a fixed order: 32 columns a workgroup, a
 // thirty-second of the parts a thread. Jobs 0 and 1 are the weights, the others the gate's rows. Adding in a launch of its own keeps the
 // order, which atomics would not; it takes 5 us for 256 workgroups' sums of 4096 columns (8 MB), most of it the launch and two round trips.
 struct JoinArgs {
@@ -521,7 +521,7 @@ struct JoinArgs {
 };
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_join_kernel(JoinArgs a) {
-  __shared__ float sums[32][33];
+  __shared__ double sums[32][33];
   const uint32_t block = block_index(), job = block / a.tiles;
   const int col = threadIdx.x & 31, part = threadIdx.x >> 5, n = (int)(block - job * a.tiles) * 32 + col;
   const bool weight = job < a.w_jobs;
@@ -530,7 +530,7 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(JoinArgs a) {
   const uint32_t count = weight ? a.w_count : a.g_count;
   const int64_t step = weight ? 2 * (int64_t)a.cols : a.cols;
   const float* from = weight ? a.w_parts + job * (int64_t)a.cols : a.gate_parts + (int64_t)(job - a.w_jobs) * a.g_count * a.cols;
-  float s = 0;
+  double s = 0;
   if (n < a.cols) {
     uint32_t p = part;
     for (; p + 7 * 32 < count; p += 8 * 32) {  // eight loads on their way
@@ -548,12 +548,12 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(JoinArgs a) {
 #pragma unroll
   for (int p = 1; p < 32; p++) s += sums[p][col];
   if (!weight) {
-    ((T*)a.dg)[(int64_t)(job - a.w_jobs) * a.lddg + n] = (T)s;
+    ((T*)a.dg)[(int64_t)(job - a.w_jobs) * a.lddg + n] = (T)(float)s;
   } else if (a.w_f32) {
     float* to = (float*)a.dw[job] + n;
-    *to = a.accumulate ? *to + s : s;
+    *to = (float)(a.accumulate ? *to + s : s);
   } else {
-    ((T*)a.dw[job])[n] = (T)s;
+    ((T*)a.dw[job])[n] = (T)(float)s;
   }
 }
 

@@ -732,8 +732,8 @@ int b2c_hip_block_norm(const b2c_block_norm_args* a, hipStream_t stream);
 
 /* Its gradients. `fwd` holds the forward call's arguments (y and n are not used): x, residual and gate as they were then, since y
  * is formed again from them. Outputs that are NULL are not formed. dresidual may be dy and dx may be dn (same pointer and ld). The
- * gate's gradient is summed over the rows that share a gate row; it and the weights' in single precision, in an order that depends on
- * the sizes alone. */
+ * gate's gradient is summed over the rows that share a gate row; it and the weights' in single precision over a workgroup's rows and in
+ * 64 bits over workgroups, in an order that depends on the sizes alone. */
 typedef struct b2c_block_norm_grad_args {
   b2c_block_norm_args fwd;
   const void* dy;       /* [rows][cols], dtype, or NULL: zeros */

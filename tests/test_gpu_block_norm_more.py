@@ -4,6 +4,8 @@ import pytest
 
 from b2ctrain_amd import nn
 from tests import dense_util as U
+from tests import more_util as V
+from tests import precision as P
 from tests.gpu_harness import emit
 from tests.test_gpu_block_norm import check
 from tests.test_gpu_dense import close
@@ -198,3 +200,25 @@ def test_batches_of_no_rows():
         p.gradients(dy=none(), dn=none(), dx=none(), dresidual=none(), dw_post=dw[0].matrix, dw_pre=dw[1].matrix, accumulate=accumulate)
         p.backward()
         assert all(np.array_equal(v.get(), np.full((1, 40), float(accumulate))) for v in dw)
+
+
+@pytest.mark.parametrize("rows,d,per", [(1037, 1000, 61), (300, 4096, 0), (5000, 300, 5000), (700, 8192, 350)])
+def test_sums_over_rows_are_as_exact_as_their_terms(rows, d, per):
+    """In single precision. A term has five roundings or so, each 2^-24 / sqrt 3 on the average, and the sum's own is a sixth: 8.4e-8 of it, where
+    terms have either sign. To add a thousand workgroups' sums in single precision would bring another 1.4e-7."""
+    emit(f"block norm {rows} x {d} per {per}: precision of the sums")
+    g = np.random.default_rng(rows)
+    q = lambda k, n=rows, add=0.0: U.rounded(g.standard_normal((n, d)) * k + add, F32)  # noqa: E731
+    x, r, dy, dn, w_post, w_pre = q(0.5), q(2.0), q(0.1), q(0.1), q(0.2, 1, 1.0), q(0.2, 1, 1.0)
+    gate = q(1.0, -(-rows // per)) if per else None
+    h = [U.Held(v, F32) for v in (x, r, dy, dn, w_post, w_pre)]
+    n, dw = U.Held(None, F32, rows=rows, cols=d), [U.Held(None, F32, rows=1, cols=d) for _ in range(2)]
+    dg = U.Held(None, F32, rows=len(gate), cols=d) if per else None
+    p = nn.BlockNorm(x=h[0].matrix, residual=h[1].matrix, n=n.matrix, gate=U.Held(gate, F32).matrix if per else None, rows_per_gate=per or None,
+                     post=True, w_post=h[4].matrix, w_pre=h[5].matrix, scale=0.5)
+    p.gradients(dy=h[2].matrix, dn=h[3].matrix, dgate=dg.matrix if per else None, dw_post=dw[0].matrix, dw_pre=dw[1].matrix, room=U.Space())
+    p.backward()
+    want = V.block_norm(F32, F32, x=x, r=r, gate=gate, per=per or 1, post=True, w_post=w_post[0], w_pre=w_pre[0], scale=0.5, dy=dy, dn=dn)
+    for k, got in (("dw_post", dw[0].get()[0]), ("dw_pre", dw[1].get()[0]), ("dgate", dg.get() if per else None)):
+        if got is not None:
+            assert P.rms(got - want[k][0]) / P.rms(want[k][0]) < 1.25e-7, k
