@@ -152,7 +152,8 @@ __device__ __forceinline__ int find(const J& jobs, uint32_t t, uint32_t& tm, uin
 // A product whose P has a scale for every row and group of 2^shift values of k: out[m][n] = sum_g scale[g][n] sum_(k in g) Q[m][k] P[n][k],
 // so that P may hold whole numbers, which 16 bits hold exactly. Such a product's epilogue has a member `scales`. Each group's sum is added to
 // the whole one when the group ends, in a second set of accumulators, for which tiles of 256x256 have no registers. The scales come to LDS
-// beside the step's values. 2048 x 4096-11264 with 4-bit weights takes 205 us with groups of 128, 0.92 PFLOP/s, 230 with groups of 32.
+// beside the step's values. 2048 x 4096-11264 takes 187 us with groups of 128, 214 with groups of 32, and 171 without scales in
+// tiles of 256x256.
 struct GroupScales {
   const float* p;  // [ceil(K / 2^shift)][pitch], pitch a multiple of the tile's width
   int64_t pitch;

@@ -201,7 +201,7 @@ __device__ __forceinline__ float slope_of(bool sigmoid, float kept) { return sig
 
 // Both norms of a row from registers: t = u / size(u), y = r + scale gate t w_post, n = y / size(y) w_pre, with y as it was before it was
 // rounded; the sums of layer norms are of differences from the mean, in a second pass over registers. Bound by memory: 8192 rows of 4096
-// with a gate a row (bf16, 336 MB) take 67 us, 5.0 TB/s, a million rows of 64 (512 MB) 93 us, 5.5 TB/s, one row of 4096 2.8 us.
+// with a gate a row (bf16, 336 MB) take 63 to 66 us, 5.1 TB/s, a million rows of 64 (512 MB) 92 us, 5.5 TB/s, one row of 4096 2.8 us.
 template <typename T, int E, int LANES, int C, int END>
 __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_kernel(NormArgs a) {
   constexpr int TEAMS = Team<LANES>::TEAMS;
@@ -306,7 +306,7 @@ __device__ __forceinline__ void gather(float (&v)[C][E], float* lds) {
 // arithmetic that memory hides and cost the forward pass a write where y is not wanted. A thread sums its columns' weight gradients over
 // all rows of its workgroup, in registers. A row's values are on their way while the one before is at work (AHEAD) where a compute unit
 // has one workgroup, whose waves wait for each other at every sum. Bound by memory: 8192 rows of 4096 with a gate a row
-// (bf16, 537 MB) take 108 us, 5.0 TB/s; a million rows of 64 (768 MB) 168 to 185 us, 4.4 TB/s, VALU 59%.
+// (bf16, 537 MB) take 114 us, 4.7 TB/s; a million rows of 64 (768 MB) 168 to 178 us, 4.5 TB/s, VALU 73%.
 template <typename T, int E, int LANES, int C, int END>
 __global__ __launch_bounds__(Team<LANES>::THREADS) void norm_back_kernel(NormGradArgs b) {
   constexpr bool AHEAD = LANES > 64 && LANES <= 512;
