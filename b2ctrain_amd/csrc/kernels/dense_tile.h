@@ -175,8 +175,8 @@ constexpr int least_waves(int waves, int stages) {
 // Tiles first .. first + count - 1 of the jobs, each in `parts` parts of its k: workgroup part count + slot. The epilogue is
 // told the workgroup too.
 template <typename T, bool PT, bool QT, bool DUAL, bool TWO, int WAVES_M, int WAVES_N, int WM, int WN, int STAGES, typename Epi, int NJ>
-__global__ __launch_bounds__(WAVES_M* WAVES_N * 64, least_waves<Epi>(WAVES_M * WAVES_N, STAGES)) void tile_kernel(Jobs<T, Epi, NJ> jobs, uint32_t first, uint32_t count,
-                                                                     int parts) {
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64, least_waves<Epi>(WAVES_M * WAVES_N, STAGES)) void tile_kernel(
+    Jobs<T, Epi, NJ> jobs, uint32_t first, uint32_t count, int parts) {
   constexpr int THREADS = WAVES_M * WAVES_N * 64, BM = WAVES_M * WM, BN = WAVES_N * WN;
   constexpr bool AHEAD = WAVES_M * WAVES_N == 8;
   constexpr int MT = WM / 16, NT = WN / 16, COLS = DUAL ? BN / 2 : BN;  // columns of out in a tile

@@ -569,7 +569,8 @@ bool sizes_ok(const b2c_block_norm_args* a) {
 }
 bool inputs_ok(const b2c_block_norm_args* a) {  // of some rows: those of none have no address
   const size_t s = size_of(a->dtype), w = size_of(a->w_dtype);
-  return (a->x || a->residual) && (a->x || (!a->post && !a->gate)) && (!a->x || good(a->x, a->ldx, a->cols, s)) && (!a->residual || good(a->residual, a->ldr, a->cols, s)) &&
+  return (a->x || a->residual) && (a->x || (!a->post && !a->gate)) && (!a->x || good(a->x, a->ldx, a->cols, s)) &&
+         (!a->residual || good(a->residual, a->ldr, a->cols, s)) &&
          (!a->gate || good(a->gate, a->ldg, a->cols, s)) && reinterpret_cast<uintptr_t>(a->w_post) % w == 0 &&
          reinterpret_cast<uintptr_t>(a->w_pre) % w == 0;
 }
@@ -579,8 +580,8 @@ NormArgs to_device(const b2c_block_norm_args* a) {
   float part = 1.f;
   while (part * (float)a->cols > 1.f) part *= 0.5f;
   return {a->rows, a->cols, a->kind == B2C_NORM_LAYER, a->post != 0, a->gate && a->gate_act == B2C_GATE_SIGMOID, a->w_dtype == B2C_F32,
-          a->eps, a->x ? a->scale : 0.f, 1.f / (float)a->cols, part, 1.f / (part * (float)a->cols), a->x, a->residual, a->gate, a->w_post, a->w_pre, a->ldx, a->ldr, a->ldg, (uint32_t)per,
-          a->y, a->n, a->ldy, a->ldn};
+          a->eps, a->x ? a->scale : 0.f, 1.f / (float)a->cols, part, 1.f / (part * (float)a->cols), a->x, a->residual, a->gate, a->w_post,
+          a->w_pre, a->ldx, a->ldr, a->ldg, (uint32_t)per, a->y, a->n, a->ldy, a->ldn};
 }
 
 // Calls f(lanes, pieces) with the team that a row of `cols` values takes, E to a piece.
@@ -735,7 +736,8 @@ extern "C" int b2c_hip_block_norm_backward(const b2c_block_norm_grad_args* b, hi
     clear_kernel<<<dim3((unsigned)(up(a->cols, 256) / 256)), 256, 0, stream>>>(b->dw_post, b->dw_pre, a->cols, gs == 4);
     return hipGetLastError();
   }
-  if (!inputs_ok(a) || (b->dw_post && !a->x) || (b->dw_pre && !b->dn) || (b->dx && !a->x) || (b->dgate && !a->gate) || (!b->dy && !b->dn) || (b->dy && !good(b->dy, b->lddy, a->cols, s)) || (b->dn && !good(b->dn, b->lddn, a->cols, s)) ||
+  if (!inputs_ok(a) || (b->dw_post && !a->x) || (b->dw_pre && !b->dn) || (b->dx && !a->x) || (b->dgate && !a->gate) ||
+      (!b->dy && !b->dn) || (b->dy && !good(b->dy, b->lddy, a->cols, s)) || (b->dn && !good(b->dn, b->lddn, a->cols, s)) ||
       (b->dx && !good(b->dx, b->lddx, a->cols, s)) || (b->dresidual && !good(b->dresidual, b->lddr, a->cols, s)) ||
       (b->dgate && !good(b->dgate, b->lddg, a->cols, s)))
     return hipErrorInvalidValue;

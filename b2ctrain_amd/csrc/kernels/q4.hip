@@ -175,12 +175,12 @@ __device__ __forceinline__ void turn4(vec<uint32_t, 4>& v) {
 // At most 16 MT rows of x. A workgroup takes 16 NT outputs, its eight waves every eighth run of 128 values of k: sixteen bytes of a row a
 // lane, turned so that each matrix instruction meets 32 neighbouring values of k, which are of one group. With c the code and B its base, a
 // group's sum is s (sum (B + c) x - (B + z) sum x), and sum x comes from the same instruction against ones, in the same lanes, all of it in
-// units of UNIT. B is at most
-// 128, so that the difference costs four bits of the 24 that the sums are held in. Rows beyond the last read the last one's values, which
-// nobody stores; in the run at the end of k (not the first: LONG) every load that would pass a row's end reads its last bytes, which are then
-// moved to their place, so that no load waits for a condition (7 rows of 2050-5001: 3 us less). The waves' sums meet in LDS and are added
-// in a fixed order. Bound by the latency of two to four round trips where there are few runs: 7 rows of 2050-5001 (f16, by 32, zero points; 6
-// MB) take 10.1 us, 9.7 with rows on even bytes and 6.3 on sixteen; of 2048 9.0, 8.5 and 5.8; 16 of 4096-11264 13.9.
+// units of UNIT. B is at most 128, so that the difference costs four bits of the 24 that the sums are held in. Rows beyond the last read
+// the last one's values, which nobody stores; in the run at the end of k (not the first: LONG) every load that would pass a row's end reads
+// its last bytes, which are then moved to their place, so that no load waits for a condition (7 rows of 2050-5001: 3 us less). The waves'
+// sums meet in LDS and are added in a fixed order. Bound by the latency of two to four round trips where there are few runs: 7 rows of
+// 2050-5001 (f16, by 32, zero points; 6 MB) take 10.1 us, 9.7 with rows on even bytes and 6.3 on sixteen; of 2048 9.0, 8.5 and 5.8; 16 of
+// 4096-11264 13.9.
 template <typename T, int GROUP, bool ZERO, int MT, int NT, bool LONG>
 __global__ __launch_bounds__(512, MT == 4 ? 2 : 4) void q4_few_kernel(Weights4<T> w, int shift, Side<T> all, int64_t all_rows, T* all_y,
                                                                       int64_t ldy) {

@@ -9,7 +9,7 @@ from tests import precision as P
 from tests.gpu_harness import emit
 from tests.test_gpu_dense import close
 from tests.test_gpu_dense_calls import Raw
-from tests.test_gpu_q4 import Bytes
+from tests.test_gpu_q4 import Bytes, linear
 
 pytestmark = pytest.mark.gpu
 
@@ -131,3 +131,12 @@ def test_the_smallest_normal_values(rows, k):
     x[abs(x) < 2.0 ** -126] = 2.0 ** -126
     y, code, scale, zero, few = product(x, BF16, 64, True, size=2.0 ** 110)
     close("y", y, *V.q4_linear(x, code, scale, zero, 64, BF16, few))
+
+
+@pytest.mark.parametrize("k,n", [(1, 1), (7, 3), (33, 17), (64, 65), (97, 129), (515, 50), (1000, 333), (4128, 200)])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (8, 0), (5, 1)])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True), (256, False)])
+def test_many_rows_of_every_width(k, n, pad, shift, group, zeros):
+    """By tiles: steps that end inside a group, groups that end inside a step, parts of k, x in place and copied."""
+    for dtype in (BF16, F16):
+        linear(513 + n, k, n, group, zeros, dtype, pad, shift)
